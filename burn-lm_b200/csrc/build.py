@@ -45,6 +45,7 @@ MODULES = {
     "attention_sigmoid": ["attention_sigmoid.cu"],
     "attention_quads": ["attention_quads.cu"],
     "attention_latent": ["attention_latent.cu"],
+    "attention_q8": ["attention_q8.cu"],
     "gemm": ["gemm_f32.cu"],
     "gemv": ["gemv.cu"],
     "gemm_tc": ["gemm_tc.cu"],

@@ -199,6 +199,13 @@ _protos = {
         "blm_latent_attention_blocks": [c_int, c_int, c_int],
         "blm_sigmoid_gate": [c_void_p, c_int, c_void_p, c_int, c_longlong, c_void_p, c_int, c_int, c_int, c_void_p],
     },
+    "attention_q8": {
+        "blm_rope_append_q8": [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p,
+                               c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
+        "blm_q8_values": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
+        "blm_attention_q8": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                             c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p],
+    },
     "moe": {
         "blm_moe_route": [c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
                           c_int, c_int, c_void_p],
@@ -1982,3 +1989,158 @@ def pass_entry(resid, delta, embedded, step):
         raise KernelError("pass_entry: resid, delta and embedded [N, D], step [D]")
     _call("stream_ops", "blm_pass_entry", _ptr(resid), _ptr(delta), _code(delta.dtype) if delta is not None else F32, _ptr(embedded),
           _ptr(step), n, d, _stream())
+
+
+# -- a cache line in 8 bits ------------------------------------------------------------------------------------------------------
+def q8_line_bytes(head_dim: int) -> int:
+    """Bytes of one kv head in a page of a cache line in 8 bits: its keys, and its values with the lanes filled up to 32."""
+    return PAGE * (head_dim + -(-head_dim // 32) * 32)
+
+
+def q8_pool(n_pages: int, n_kv: int, head_dim: int, device):
+    """(pool int8 [n_pages, n_kv, q8_line_bytes(head_dim)], scales float32 [n_pages, n_kv, 2]) of a cache line whose complete blocks of
+    PAGE positions are kept in 8 bits: keys and values of a block are whole numbers times one scale per kv head for the keys and one
+    for the values.  How the numbers lie in a page is the kernels' own affair: rope_append_q8 fills pages, attention_q8 reads them,
+    q8_values gives the numbers, q8_write takes them."""
+    if not 16 <= head_dim <= 256 or head_dim % 16:
+        raise KernelError(f"q8_pool: heads of {head_dim} lanes (multiples of 16 from 16 to 256)")
+    return (torch.zeros((n_pages, n_kv, q8_line_bytes(head_dim)), dtype=torch.int8, device=device),
+            torch.zeros((n_pages, n_kv, 2), dtype=torch.float32, device=device))
+
+
+def _q8_line(what, pool, scales, n_kv, head_dim):
+    if (pool.dtype != torch.int8 or pool.dim() != 3 or tuple(pool.shape[1:]) != (n_kv, q8_line_bytes(head_dim)) or scales.dtype != torch.float32
+            or tuple(scales.shape) != (pool.shape[0], n_kv, 2)):
+        raise KernelError(f"{what}: pool int8 [pages, {n_kv}, {q8_line_bytes(head_dim)}] and scales float32 [pages, {n_kv}, 2], as q8_pool gives them")
+
+
+def _on_current(what, *tensors):
+    """The tensors' device is the current one: kernels are launched on its current stream."""
+    now = _current_device() if _current_device is not None else torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != now:
+            raise KernelError(f"{what}: a tensor on {t.device} while the current device is cuda:{now}")
+
+
+def _aligned(what, *tensors):
+    for t in tensors:
+        if t is not None and t.data_ptr() % 16:
+            raise KernelError(f"{what}: tensors must begin at multiples of 16 bytes")
+
+
+_q8_places: dict = {}
+
+
+def _q8_value_places(head_dim: int, device):
+    """Where the value of (position, lane) lies among a page's bytes of one kv head's values: int64 [PAGE, head_dim]."""
+    key = (head_dim, device)
+    at = _q8_places.get(key)
+    if at is None:
+        k, d = torch.arange(PAGE)[:, None], torch.arange(head_dim)[None, :]
+        per = head_dim // 8
+        g, n = d // per, d % per
+        padded = -(-head_dim // 32) * 32
+        at = (k // 16) * 16 * padded + (n // 4) * 512 + (4 * g + k // 4 % 4) * 16 + n % 4 * 4 + k % 4
+        at = _q8_places[key] = at.to(device)
+    return at
+
+
+def q8_write(pool, scales, pages, keys, key_scales, values, value_scales) -> None:
+    """Puts whole blocks into a cache line in 8 bits (a saved conversation, say): pages int [P]; keys and values int8
+    [P, n_kv, PAGE, head_dim]; their scales [P, n_kv].  Plain tensor operations, on any device."""
+    p, n_kv, page, head_dim = keys.shape
+    _q8_line("q8_write", pool, scales, n_kv, head_dim)
+    if (page != PAGE or keys.dtype != torch.int8 or values.dtype != torch.int8 or values.shape != keys.shape or pages.numel() != p
+            or tuple(key_scales.shape) != (p, n_kv) or tuple(value_scales.shape) != (p, n_kv)):
+        raise KernelError(f"q8_write: keys and values int8 [P, kv heads, {PAGE}, head_dim], scales [P, kv heads], a page for each")
+    line = torch.zeros((p, n_kv, pool.shape[2]), dtype=torch.int8, device=pool.device)
+    line[:, :, : PAGE * head_dim] = keys.reshape(p, n_kv, -1)
+    line[:, :, PAGE * head_dim:][:, :, _q8_value_places(head_dim, pool.device).reshape(-1)] = values.reshape(p, n_kv, -1)
+    at = pages.to(torch.int64)
+    pool[at] = line
+    scales[at] = torch.stack([key_scales, value_scales], dim=2).to(torch.float32)
+
+
+def q8_values(pool, scales, pages, head_dim, dtype=torch.float32):
+    """The numbers that pages of a cache line in 8 bits stand for: [P, 2, n_kv, PAGE, head_dim] (keys, then values) in `dtype`
+    (float32 or bfloat16, each rounded once) for `pages` int32 [P] on the device.  A page number outside the pool leaves its entry zero."""
+    n_pages, n_kv = pool.shape[:2]
+    _q8_line("q8_values", pool, scales, n_kv, head_dim)
+    if pages.dtype != torch.int32:
+        raise KernelError("q8_values: pages must be int32")
+    _need_cuda(pool, scales, pages)
+    _on_current("q8_values", pool, scales, pages)
+    out = torch.zeros((pages.numel(), 2, n_kv, PAGE, head_dim), dtype=dtype, device=pool.device)
+    _call("attention_q8", "blm_q8_values", _ptr(pool), _ptr(scales), _ptr(pages), _ptr(out), _code(dtype), pages.numel(), n_kv, head_dim, n_pages,
+          _stream())
+    return out
+
+
+def _q8_step(what, step, block_table, tail, n_kv, head_dim, dtype):
+    for t in (step.cu_seqlens, step.slot_of_seq, step.start_pos, block_table):
+        if t.dtype != torch.int32:
+            raise KernelError(f"{what}: cu_seqlens, slot_of_seq, start_pos and the block table are int32")
+    if block_table.dim() != 2 or tail.dtype != dtype or tail.dim() != 5 or tuple(tail.shape) != (block_table.shape[0], 2, n_kv, PAGE, head_dim):
+        raise KernelError(f"{what}: block_table [slots, pages] and tail [slots, 2, {n_kv}, {PAGE}, {head_dim}] in the projection's dtype")
+
+
+def rope_append_q8(qkv, out, step, pool, scales, tail, block_table, inv_freq, rotary_dim, pairs, n_heads, n_kv, head_dim, table=None,
+                   turn_scale=1.0):
+    """rope_append for a cache line in 8 bits (q8_pool): rotates q and k of the step's tokens by their positions into `out` (which also
+    gets v, and may be `qkv` itself), and appends k and v to the line.  qkv and out [N, (n_heads + 2 n_kv) * head_dim], float32 or bfloat16.
+
+    A block of PAGE positions that the step completes goes into its page: 8-bit whole numbers x with |x| <= 127 and a float32 scale
+    per kv head for its keys and one for its values, the largest magnitude / 127 (0 for a block of zeros; a block that holds an
+    infinity or a NaN reads as NaN).  The rows of a block that is still unfinished after the step go to `tail`
+    [slots, 2, n_kv, PAGE, head_dim] (keys, values; rows 0 .. length % PAGE of a slot), in qkv's dtype.  Rows of no sequence (behind
+    the last of step.cu_seqlens) are left alone, in `out` too.
+
+    Returns `old` for attention_q8: None when every sequence brings at most one token (step.max_q_len 1), else the rows of the
+    unfinished blocks that the step found, [n_seqs, 2, n_kv, PAGE, head_dim], since the tail may hold the next block's by then.
+    A step of one token a sequence may be run again with the same or another token before the sequence goes on; one of several
+    tokens may not where it completes a block and leaves another unfinished.
+    `pairs`, `table`, `turn_scale`: as for rope_append."""
+    if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv) * head_dim or out.shape != qkv.shape or out.dtype != qkv.dtype:
+        raise KernelError("rope_append_q8: qkv and out [N, (heads + 2 kv heads) * head_dim] of one dtype")
+    _q8_line("rope_append_q8", pool, scales, n_kv, head_dim)
+    _q8_step("rope_append_q8", step, block_table, tail, n_kv, head_dim, qkv.dtype)
+    if rotary_dim and (inv_freq is None or inv_freq.dtype != torch.float64 or inv_freq.numel() != rotary_dim // 2):
+        raise KernelError("rope_append_q8: inv_freq must be float64 [rotary_dim / 2]")
+    if table is not None and (table.dtype != torch.float32 or tuple(table.shape[1:]) != (rotary_dim // 2, 2)):
+        raise KernelError("rope_append_q8: table must be float32 [positions, rotary_dim / 2, 2]")
+    _need_cuda(qkv, out, pool, scales, tail, block_table, inv_freq, table, step.cu_seqlens, step.slot_of_seq, step.start_pos)
+    _on_current("rope_append_q8", qkv, out, pool, scales, tail, block_table)
+    _aligned("rope_append_q8", qkv, out, pool, tail, table)
+    old = None
+    if step.max_q_len > 1:
+        old = torch.empty((step.n_seqs, 2, n_kv, PAGE, head_dim), dtype=qkv.dtype, device=qkv.device)
+    _call("attention_q8", "blm_rope_append_q8", _ptr(qkv), _ptr(out), _code(qkv.dtype), _ptr(step.cu_seqlens), _ptr(step.slot_of_seq),
+          _ptr(step.start_pos), _ptr(block_table), block_table.shape[1], _ptr(inv_freq), rotary_dim, int(pairs), _ptr(table),
+          table.shape[0] if table is not None else 0, turn_scale, _ptr(pool), _ptr(scales), _ptr(tail), _ptr(old), step.n_seqs,
+          step.max_q_len, n_heads, n_kv, head_dim, pool.shape[0], _stream())
+    return old
+
+
+def attention_q8(rotated, step, pool, scales, tail, old, block_table, out, n_heads, n_kv, head_dim, scale, window=0):
+    """Causal grouped-query attention of the step's tokens over a cache line in 8 bits, after rope_append_q8: `rotated` is what that
+    wrote (q, k and v of the step's tokens, [N, (n_heads + 2 n_kv) * head_dim]) and `old` what it returned.  The query at position p
+    sees the keys 0 .. p (the last `window` of them when window > 0): those of earlier blocks of PAGE positions in 8 bits, those of its
+    own block unrounded, from the step's rows and, before them, from `old` (steps of one token a sequence: from `tail`).  So the result
+    depends on the tokens, not on how they were cut into steps.  Scores, softmax and sums are fp32; out [N, n_heads * head_dim] in
+    rotated's dtype.  Rows of no sequence are left as they are."""
+    n = rotated.shape[0]
+    if rotated.dim() != 2 or rotated.shape[1] != (n_heads + 2 * n_kv) * head_dim or tuple(out.shape) != (n, n_heads * head_dim) or out.dtype != rotated.dtype:
+        raise KernelError("attention_q8: rotated [N, (heads + 2 kv heads) * head_dim] and out [N, heads * head_dim] of one dtype")
+    _q8_line("attention_q8", pool, scales, n_kv, head_dim)
+    _q8_step("attention_q8", step, block_table, tail, n_kv, head_dim, rotated.dtype)
+    if window < 0:
+        raise KernelError(f"attention_q8: a window of {window} keys")
+    if step.max_q_len > 1 and (old is None or old.dtype != rotated.dtype or tuple(old.shape) != (step.n_seqs, 2, n_kv, PAGE, head_dim)):
+        raise KernelError("attention_q8: a step of several tokens a sequence needs what rope_append_q8 returned")
+    _need_cuda(rotated, pool, scales, tail, old, block_table, out, step.cu_seqlens, step.slot_of_seq, step.start_pos)
+    _on_current("attention_q8", rotated, pool, scales, tail, old, block_table, out)
+    _aligned("attention_q8", rotated, pool, tail, old, out)
+    found = tail if step.max_q_len <= 1 else old
+    _call("attention_q8", "blm_attention_q8", _ptr(rotated), _ptr(pool), _ptr(scales), _ptr(found), 1 if step.max_q_len <= 1 else 0,
+          _code(rotated.dtype), _ptr(block_table), block_table.shape[1], _ptr(step.cu_seqlens), _ptr(step.slot_of_seq), _ptr(step.start_pos),
+          _ptr(out), n, step.n_seqs, n_heads, n_kv, head_dim, pool.shape[0], int(window or 0), scale, _stream())
