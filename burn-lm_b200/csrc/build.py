@@ -50,6 +50,7 @@ MODULES = {
     "gemv": ["gemv.cu"],
     "gemm_tc": ["gemm_tc.cu"],
     "gemm_sk": ["gemm_sk.cu"],
+    "gemm_q4": ["gemm_q4.cu"],
     "sampling": ["sampling.cu"],
     "runtime": ["runtime.cu"],
 }

@@ -257,6 +257,9 @@ _protos = {
         "blm_gemm_sk_supported": [c_int, c_int, c_int],
         "blm_gemm_sk_squares_row": [],
     },
+    "gemm_q4": {
+        "blm_gemm_q4": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p],
+    },
     "sampling": {
         "blm_argmax": [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                        c_void_p, c_void_p, c_int, c_void_p],
@@ -2144,3 +2147,146 @@ def attention_q8(rotated, step, pool, scales, tail, old, block_table, out, n_hea
     _call("attention_q8", "blm_attention_q8", _ptr(rotated), _ptr(pool), _ptr(scales), _ptr(found), 1 if step.max_q_len <= 1 else 0,
           _code(rotated.dtype), _ptr(block_table), block_table.shape[1], _ptr(step.cu_seqlens), _ptr(step.slot_of_seq), _ptr(step.start_pos),
           _ptr(out), n, step.n_seqs, n_heads, n_kv, head_dim, pool.shape[0], int(window or 0), scale, _stream())
+
+
+# -- weights in 4 bits -----------------------------------------------------------------------------------------------------------
+Q4_GROUPS = (32, 64, 128)     # places of K that share a scale
+_Q4_STRETCH = 256             # places of K that a warp of the product's kernels loads together
+
+
+class Q4Weight:
+    """A weight [out_features, in_features] in 4 bits, as pack_q4 and quantize_q4 make it: whole numbers of -8 .. 7 in the order in which
+    the kernels read them, and bfloat16 scales [rows filled up to 16, groups filled up to 256 places]."""
+
+    def __init__(self, packed, scales, out_features, in_features, group):
+        self.packed, self.scales = packed, scales
+        self.out_features, self.in_features, self.group = out_features, in_features, group
+
+    @property
+    def device(self):
+        return self.packed.device
+
+    def bytes(self) -> int:
+        return self.packed.numel() + 2 * self.scales.numel()
+
+
+def _five_bits(x):
+    """float32 rounded to five significant bits (to nearest, ties to even)."""
+    bits = x.contiguous().view(torch.int32)
+    return ((bits + 0x3ffff + ((bits >> 19) & 1)) & ~0x7ffff).view(torch.float32)
+
+
+def _q4_order(device):
+    """For the eight nibbles of each of a tile's 128 words, (row, place) of the 16 x 64 tile: int64 [32, 4, 8] twice."""
+    lane, s, nibble = torch.arange(32)[:, None, None], torch.arange(4)[None, :, None], torch.arange(8)[None, None, :]
+    pair, high = nibble % 4, nibble // 4
+    row = lane // 4 + 8 * (pair % 2)
+    place = 32 * (s // 2) + 8 * (lane % 4) + 4 * (s % 2) + 2 * (pair // 2) + high
+    full = torch.zeros((32, 4, 8), dtype=torch.int64)
+    return (row + full).to(device), (place + full).to(device)
+
+
+def pack_q4(values, scales, group) -> Q4Weight:
+    """A weight in 4 bits from its numbers: values [M, K] whole numbers of -8 .. 7 (any integer type), scales [M, ceil(K / group)] of
+    five significant bits at most; the weight is scales[m, k // group] * values[m, k].  Plain tensor operations, on any device."""
+    if group not in Q4_GROUPS:
+        raise KernelError(f"pack_q4: groups of {group} places; {Q4_GROUPS} are known")
+    if values.dim() != 2 or values.is_floating_point() or values.numel() == 0 or tuple(scales.shape) != (values.shape[0], -(-values.shape[1] // group)):
+        raise KernelError("pack_q4: values [M, K] whole numbers and scales [M, ceil(K / group)]")
+    m, k = values.shape
+    if int(values.min()) < -8 or int(values.max()) > 7:
+        raise KernelError("pack_q4: values are whole numbers of -8 .. 7")
+    s = scales.to(torch.float32)
+    if not torch.equal(_five_bits(s), s) or not torch.isfinite(s).all():
+        raise KernelError("pack_q4: scales are finite and have five significant bits at most")
+    tiles, k_tiles = -(-m // 16), -(-k // 64)
+    stretches = -(-k_tiles * 64 // _Q4_STRETCH)
+    packed_scales = torch.zeros((tiles * 16, stretches * (_Q4_STRETCH // group)), dtype=torch.bfloat16, device=values.device)
+    packed_scales[:m, : s.shape[1]] = s
+    row, place = _q4_order(values.device)
+    packed = torch.empty((tiles, k_tiles, 512), dtype=torch.uint8, device=values.device)
+    for t0 in range(0, tiles, 256):                      # some tiles at a time: an embedding's table would fill the memory
+        t1 = min(tiles, t0 + 256)
+        u = torch.full(((t1 - t0) * 16, k_tiles * 64), 8, dtype=torch.uint8, device=values.device)
+        part = values[t0 * 16: min(m, t1 * 16)]
+        u[: part.shape[0], :k] = (part + 8).to(torch.uint8)
+        u = u.view(t1 - t0, 16, k_tiles, 64).permute(0, 2, 1, 3)[:, :, row, place]          # [tiles, k tiles, 32, 4, 8]
+        packed[t0:t1] = (u[..., 0::2] | (u[..., 1::2] << 4)).reshape(t1 - t0, k_tiles, 512)
+    return Q4Weight(packed, packed_scales, m, k, group)
+
+
+def quantize_q4(w, group=64) -> Q4Weight:
+    """A weight [M, K] (float32 or bfloat16) rounded to 4 bits.  Of each row's groups of `group` places, the number of largest magnitude
+    (the negative one on a tie) becomes -8 times the scale, rounded to five significant bits; the others the nearest whole numbers of
+    -8 .. 7 times it.  A group of zeros has scale 0.  Plain tensor operations, on any device."""
+    if group not in Q4_GROUPS:
+        raise KernelError(f"quantize_q4: groups of {group} places; {Q4_GROUPS} are known")
+    if w.dim() != 2 or w.dtype not in (torch.float32, torch.bfloat16) or w.numel() == 0:
+        raise KernelError("quantize_q4: a weight [M, K] in float32 or bfloat16")
+    m, k = w.shape
+    groups = -(-k // group)
+    values, scales = torch.empty((m, k), dtype=torch.int8, device=w.device), torch.empty((m, groups), dtype=torch.float32, device=w.device)
+    for r in range(0, m, 4096):
+        x = torch.zeros((min(m, r + 4096) - r, groups * group), dtype=torch.float32, device=w.device)
+        x[:, :k] = w[r: r + 4096]
+        x = x.view(-1, groups, group)
+        lo, hi = x.amin(dim=2), x.amax(dim=2)
+        s = _five_bits(torch.where(hi > -lo, hi, lo) / -8.0)
+        s = torch.where(s.abs() < 2.0 ** -110, torch.zeros_like(s), s)          # (so that a scale times a whole number is no denormal number)
+        if not torch.isfinite(s).all():
+            raise KernelError("quantize_q4: the weight holds an infinity or a NaN")
+        safe = torch.where(s == 0, torch.ones_like(s), s)
+        v = torch.where((s == 0)[..., None], torch.zeros_like(x), torch.round(x / safe[..., None]).clamp(-8, 7))
+        values[r: r + 4096] = v.to(torch.int8).view(x.shape[0], -1)[:, :k]
+        scales[r: r + 4096] = s
+    return pack_q4(values, scales, group)
+
+
+def q4_values(w) -> torch.Tensor:
+    """The bfloat16 weight [out_features, in_features] that a weight in 4 bits stands for, exactly.  Plain tensor operations, on any device."""
+    tiles, k_tiles = w.packed.shape[:2]
+    row, place = _q4_order(w.device)
+    out = torch.empty((tiles * 16, k_tiles * 64), dtype=torch.bfloat16, device=w.device)
+    for t0 in range(0, tiles, 256):
+        p = w.packed[t0: t0 + 256].view(-1, k_tiles, 32, 4, 4)
+        n = torch.stack([p & 15, p >> 4], dim=-1).reshape(p.shape[0], k_tiles, 32, 4, 8)
+        tile = torch.empty((p.shape[0], k_tiles, 16, 64), dtype=torch.bfloat16, device=w.device)
+        tile[:, :, row, place] = n.to(torch.bfloat16) - 8
+        s = w.scales[t0 * 16: (t0 + p.shape[0]) * 16].repeat_interleave(w.group, dim=1)[:, : k_tiles * 64]
+        out[t0 * 16: (t0 + p.shape[0]) * 16] = tile.permute(0, 2, 1, 3).reshape(-1, k_tiles * 64) * s
+    return out[: w.out_features, : w.in_features].contiguous()
+
+
+Q4_STORE, Q4_ADD, Q4_GATED = 0, 1, 2
+
+
+def product_q4(w, x, out=None, add_into=None, swiglu=False):
+    """x [N, K] (bfloat16) times a weight in 4 bits (Q4Weight) transposed: whole numbers on the tensor cores, scales on float32 sums.
+
+    Ends, one at a time: `out` [N, M] bfloat16 or float32; `add_into` (float32 [N, M]) += the product; `swiglu`: the weight's rows
+    come in tiles of GATE_TILE gate rows followed by the up rows of the same outputs and out [N, M / 2] = silu(gate) * up, in
+    bfloat16 or float32.  x, out and add_into may be column ranges of wider tensors; x's rows begin at multiples of 16 bytes, or are
+    copied first."""
+    n, k, m = x.shape[0], w.in_features, w.out_features
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] != k or (k > 1 and x.stride(1) != 1):
+        raise KernelError(f"product_q4: x is bfloat16 [N, {k}] with unit stride along its rows")
+    y = out if add_into is None else add_into
+    if add_into is not None:
+        if out is not None or swiglu or add_into.dtype != torch.float32:
+            raise KernelError("product_q4: add_into is float32 [N, M], alone")
+    elif out is None or out.dtype not in (torch.bfloat16, torch.float32):
+        raise KernelError("product_q4: out is bfloat16 or float32")
+    if swiglu and m % (2 * GATE_TILE):
+        raise KernelError(f"product_q4: gated rows come in tiles of {2 * GATE_TILE}, the weight has {m}")
+    if tuple(y.shape) != (n, m // 2 if swiglu else m) or (y.shape[1] > 1 and y.stride(1) != 1):
+        raise KernelError("product_q4: the result is [N, M] (gated: [N, M / 2]) with unit stride along its rows")
+    if not (x.is_cuda and y.is_cuda and w.packed.is_cuda):
+        raise KernelError("burn-lm_b200 kernels run on a CUDA device only; got a CPU tensor")
+    _on_current("product_q4", x, y, w.packed)
+    if k % 8 or x.stride(0) % 8 or x.data_ptr() % 16:
+        wide = torch.zeros((n, -(-k // 64) * 64), dtype=torch.bfloat16, device=x.device)
+        wide[:, :k] = x
+        x, k = wide, wide.shape[1]
+    _call("gemm_q4", "blm_gemm_q4", _ptr(w.packed), _ptr(w.scales), w.scales.shape[1], w.group, _ptr(x), x.stride(0), _ptr(y), y.stride(0),
+          1 if y.dtype == torch.float32 else 0, Q4_ADD if add_into is not None else (Q4_GATED if swiglu else Q4_STORE), n, m, k, _stream())
+    return y
