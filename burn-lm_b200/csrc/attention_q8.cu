@@ -12,10 +12,13 @@
 // copied to `old` (one entry a sequence of the step) before the tail takes the last block's, and attention reads the step's own
 // rows from the rotated projection and the rows before them from `old`.  Steps of one token a sequence read the tail itself.
 //
-// Layout of a kv head's part of a page: keys [64][D] bytes, then values so that the decode kernel's tensor-core fragments are
-// 16-byte pieces: for keys 16 w + 4 t + e and lanes d = g (D / 8) + n the byte at
+// Layout of a kv head's part of a page: keys [64][D] bytes; then values so that the decode kernel's tensor-core fragments are 16-byte
+// pieces: for keys 16 w + 4 t + e and lanes d = g (D / 8) + n the byte at
 //     w (16 Dp) + (n / 4) 512 + (4 g + t) 16 + (n % 4) 4 + e,     Dp = D rounded up to a multiple of 32:
-// thread (g, t) of a warp finds four lanes of four keys in 16 bytes.
+// thread (g, t) of a warp finds four lanes of four keys in 16 bytes; then 16 bytes whose first eight are the two scales, so that one
+// copy brings all a block needs.  A byte holds q + 128: behind the byte 0x64 it is the half-precision number 1024 + 128 + q, so that
+// one byte permutation makes two numbers.
+#include <cuda_fp16.h>
 #include <math.h>
 
 #include "common.cuh"
@@ -27,7 +30,9 @@ constexpr int kPage = 64;
 enum { PAIRS_HALVES = 0, PAIRS_INTERLEAVED = 1, PAIRS_TILED = 2 };
 
 __host__ __device__ constexpr int padded(int hd) { return (hd + 31) / 32 * 32; }
-__host__ __device__ constexpr int line_bytes(int hd) { return kPage * (hd + padded(hd)); }       // of one kv head in a page
+__host__ __device__ constexpr int number_bytes(int hd) { return kPage * (hd + padded(hd)); }     // of one kv head in a page
+__host__ __device__ constexpr int line_bytes(int hd) { return number_bytes(hd) + 16; }             // ... and its scales
+__device__ __forceinline__ const float2* scales_of(const void* line, int hd) { return reinterpret_cast<const float2*>((const signed char*)line + number_bytes(hd)); }
 
 // where the word of the values of keys k .. k + 3 (k a multiple of 4) and lane d lies, from the start of the values
 __device__ __forceinline__ int value_word(int k, int d, int hd) {
@@ -91,7 +96,6 @@ struct AppendArgs {
     float turn_scale;
     int rot, pairing;
     signed char* pool;           // [pages][n_kv][line_bytes]
-    float* scales;               // [pages][n_kv][2]
     void* tail;                  // [slots][2][n_kv][64][hd]
     void* old;                   // [n_seqs][2][n_kv][64][hd], or null when every sequence brings one token
     int n_heads, n_kv, hd, n_pages;
@@ -111,10 +115,10 @@ __device__ __forceinline__ void turn(float& x, float& y, float2 cs) {
 }
 
 // Unit u of a row (16 lanes, one thread): rotates it when it belongs to a query or key and lies among the rotated lanes, writes it
-// to `dst` and, where given, to `dst2` and `dst3`.  VEC: the rotated lanes are a multiple of 16, so that a unit is eight pairs in
+// to `dst` and, where given, to `dst2`.  VEC: the rotated lanes are a multiple of 16, so that a unit is eight pairs in
 // two pieces of eight lanes; otherwise lane by lane.
 template <typename T, bool VEC>
-__device__ __forceinline__ void unit(const AppendArgs& a, const T* src, T* dst, T* dst2, T* dst3, int u, int pos, bool rotates) {
+__device__ __forceinline__ void unit(const AppendArgs& a, const T* src, T* dst, T* dst2, int u, int pos, bool rotates) {
     const int rot = rotates ? a.rot : 0;
     if (VEC || rot == 0) {
         const bool turns = u < rot / 16;
@@ -151,7 +155,6 @@ __device__ __forceinline__ void unit(const AppendArgs& a, const T* src, T* dst, 
         store8(dst + la, x);
         store8(dst + lb, y);
         if (dst2) { store8(dst2 + la, x); store8(dst2 + lb, y); }
-        if (dst3) { store8(dst3 + la, x); store8(dst3 + lb, y); }
         return;
     }
     // any even number of rotated lanes: pairs 8 u .. 8 u + 7 and, of the lanes that stand still, eight at a time and their next eight
@@ -159,7 +162,6 @@ __device__ __forceinline__ void unit(const AppendArgs& a, const T* src, T* dst, 
         const T t = from_f32<T>(v);
         dst[d] = t;
         if (dst2) dst2[d] = t;
-        if (dst3) dst3[d] = t;
     };
     for (int i = 8 * u; i < 8 * u + 8; ++i) {
         if (i < rot / 2) {
@@ -175,15 +177,16 @@ __device__ __forceinline__ void unit(const AppendArgs& a, const T* src, T* dst, 
     }
 }
 
-// Stores a complete block of one kv head's keys (VALUES: values): rows(key) gives a row's address.  All 128 threads.
-template <typename T, bool VALUES, typename Rows>
-__device__ void store_block(const AppendArgs& a, Rows rows, int page, int kvh, float* red) {
+constexpr int kAppendThreads = 256;
+// Stores a complete block of one kv head's keys or values from its rows in shared memory, `ld` apart.  All 256 threads.
+template <typename T>
+__device__ void store_block(const AppendArgs& a, const T* rows, int ld, bool value, int page, int kvh, float* red) {
     if (page < 0) return;                                // (uniform)
     const int hd = a.hd, pieces = hd / 8, tid = threadIdx.x;
     unsigned top = 0;                                    // of the magnitudes' bits: infinities and NaN stand above every number
-    for (int i = tid; i < kPage * pieces; i += 128) {
+    for (int i = tid; i < kPage * pieces; i += kAppendThreads) {
         float x[8];
-        load_n<8>(rows(i / pieces) + (i % pieces) * 8, x);
+        load_n<8>(rows + i / pieces * ld + i % pieces * 8, x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
     }
@@ -191,77 +194,75 @@ __device__ void store_block(const AppendArgs& a, Rows rows, int page, int kvh, f
     __syncthreads();                                     // (red is free, whatever used it before)
     if ((tid & 31) == 0) red[tid >> 5] = __uint_as_float(top);
     __syncthreads();
-    top = max(max(__float_as_uint(red[0]), __float_as_uint(red[1])), max(__float_as_uint(red[2]), __float_as_uint(red[3])));
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / 32; ++w) top = max(top, __float_as_uint(red[w]));
     const float scale = __fdiv_rn(__uint_as_float(top), 127.0f);
-    auto eight = [&](float x) -> unsigned {
-        const int q = scale == 0.f ? 0 : __float2int_rn(__fdiv_rn(x, scale));
-        return (unsigned)max(-127, min(127, q)) & 0xffu;
+    auto eight = [&](float v) -> unsigned {
+        const int q = scale == 0.f ? 0 : __float2int_rn(__fdiv_rn(v, scale));
+        return (unsigned)(max(-127, min(127, q)) + 128);
     };
     signed char* line = a.pool + ((size_t)page * a.n_kv + kvh) * line_bytes(hd);
-    if (tid == 0) a.scales[((size_t)page * a.n_kv + kvh) * 2 + (VALUES ? 1 : 0)] = scale;
-    if (!VALUES) {
-        for (int i = tid; i < kPage * pieces; i += 128) {
-            const int key = i / pieces, c = i % pieces;
-            float x[8];
-            load_n<8>(rows(key) + c * 8, x);
-            uint2 w;
-            w.x = eight(x[0]) | eight(x[1]) << 8 | eight(x[2]) << 16 | eight(x[3]) << 24;
-            w.y = eight(x[4]) | eight(x[5]) << 8 | eight(x[6]) << 16 | eight(x[7]) << 24;
-            *reinterpret_cast<uint2*>(line + key * hd + c * 8) = w;
+    if (tid == 0) reinterpret_cast<float*>(line + number_bytes(hd))[value ? 1 : 0] = scale;
+    // four lanes of four keys a thread: a word of each key, or of each lane
+    for (int i = tid; i < 4 * hd; i += kAppendThreads) {
+        const int key = i / (hd / 4) * 4, d = i % (hd / 4) * 4;
+        unsigned q[4][4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const T* x = rows + (key + r) * ld + d;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[r][e] = eight(to_f32(x[e]));
         }
-    } else {
-        signed char* values = line + kPage * hd;
-        for (int i = tid; i < 16 * pieces; i += 128) {
-            const int key = (i / pieces) * 4, c = i % pieces;
-            unsigned w[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = 0u;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float x[8];
-                load_n<8>(rows(key + j) + c * 8, x);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] |= eight(x[e]) << (8 * j);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) *reinterpret_cast<unsigned*>(values + value_word(key, c * 8 + e, hd)) = w[e];
+        for (int e = 0; e < 4; ++e) {
+            if (value) *reinterpret_cast<unsigned*>(line + kPage * hd + value_word(key, d + e, hd)) = q[0][e] | q[1][e] << 8 | q[2][e] << 16 | q[3][e] << 24;
+            else *reinterpret_cast<unsigned*>(line + (key + e) * hd + d) = q[e][0] | q[e][1] << 8 | q[e][2] << 16 | q[e][3] << 24;
         }
     }
 }
+// Rows of hd numbers, 16 bytes a thread.
+template <typename T>
+__device__ __forceinline__ void copy_rows(const T* src, T* dst, int ld, T* dst2, int n, int hd) {
+    constexpr int V = Vec<T>::n;
+    for (int i = threadIdx.x; i < n * (hd / V); i += kAppendThreads) {
+        const int r = i / (hd / V), c = i % (hd / V) * V;
+        const uint4 v = *reinterpret_cast<const uint4*>(src + (size_t)r * hd + c);
+        if (dst) *reinterpret_cast<uint4*>(dst + r * ld + c) = v;
+        if (dst2) *reinterpret_cast<uint4*>(dst2 + (size_t)r * hd + c) = v;
+    }
+}
 
-// Steps of one token a sequence: a block is (kv head, sequence) and has that head's queries, its key and its value.  Bound by its
-// launch; the rare block that completes a page reads the tail's 63 rows and stores them.
+// Steps of one token a sequence: a block is (kv head, sequence, 0: that head's queries and its key, 1: its value).  Bound by its launch
+// and the few loads that wait for one another; the block that completes a page reads the tail's 63 rows and stores them.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(128) append_token_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads) append_token_kernel(const AppendArgs a) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    T* own = reinterpret_cast<T*>(smem_raw);             // [2][hd]: the new key and value
-    float* red = reinterpret_cast<float*>(own + 2 * a.hd);
+    T* rows = reinterpret_cast<T*>(smem_raw);            // [64][hd + 16 bytes], of a block that is completed
+    const int ld = a.hd + 16 / (int)sizeof(T);
+    float* red = reinterpret_cast<float*>(rows + kPage * ld);
+    pdl_launch_dependents();
     pdl_wait();
-    const int kvh = blockIdx.x, seq = blockIdx.y, tok = a.cu_seqlens[seq];
-    if (a.cu_seqlens[seq + 1] == tok) return;
+    const int kvh = blockIdx.x, seq = blockIdx.y, tok = a.cu_seqlens[seq], next = a.cu_seqlens[seq + 1];
     const int pos = a.start_pos[seq], slot = a.slot_of_seq[seq], at = pos % kPage;
-    const bool completes = at == kPage - 1;
-    const int group = a.n_heads / a.n_kv, units = a.hd / 16, width = a.n_heads + 2 * a.n_kv;
-    const T* src = reinterpret_cast<const T*>(a.qkv) + (size_t)tok * width * a.hd;
-    T* dst = reinterpret_cast<T*>(a.out) + (size_t)tok * width * a.hd;
-    T* tail = reinterpret_cast<T*>(a.tail) + ((size_t)slot * 2 * a.n_kv + kvh) * kPage * a.hd;     // the keys' rows of this head
-    const size_t to_values = (size_t)a.n_kv * kPage * a.hd;
-    for (int i = threadIdx.x; i < (group + 2) * units; i += 128) {
-        const int r = i / units, u = i % units;          // the group's queries, the key, the value
+    if (next == tok) return;
+    const bool completes = at == kPage - 1, value = blockIdx.z == 1;
+    const int page = completes ? page_of(a.block_table, a.table_stride, slot, pos / kPage, a.n_pages) : -1;
+    const int group = a.n_heads / a.n_kv, units = a.hd / 16, width = a.n_heads + 2 * a.n_kv, hd = a.hd;
+    const T* src = reinterpret_cast<const T*>(a.qkv) + (size_t)tok * width * hd;
+    T* dst = reinterpret_cast<T*>(a.out) + (size_t)tok * width * hd;
+    T* tail = reinterpret_cast<T*>(a.tail) + (((size_t)slot * 2 + (value ? 1 : 0)) * a.n_kv + kvh) * kPage * hd;
+    if (completes) copy_rows<T>(tail, rows, ld, nullptr, kPage - 1, hd);
+    const int first = value ? group + 1 : 0, count = value ? 1 : group + 1;
+    for (int i = threadIdx.x; i < count * units; i += kAppendThreads) {
+        const int r = first + i / units, u = i % units;  // the group's queries, the key, the value
         const int head = r < group ? kvh * group + r : (r == group ? a.n_heads + kvh : a.n_heads + a.n_kv + kvh);
         T* keep = nullptr;
-        if (r >= group) keep = completes ? own + (r - group) * a.hd : tail + (r == group ? 0 : to_values) + (size_t)at * a.hd;
-        unit<T, VEC>(a, src + (size_t)head * a.hd, dst + (size_t)head * a.hd, keep, nullptr, u, pos, r <= group);
+        if (r >= group) keep = completes ? rows + at * ld : tail + (size_t)at * hd;
+        unit<T, VEC>(a, src + (size_t)head * hd, dst + (size_t)head * hd, keep, u, pos, r <= group);
     }
     if (!completes) return;
     __syncthreads();
-    const int page = page_of(a.block_table, a.table_stride, slot, pos / kPage, a.n_pages);
-    const T* kt = tail;
-    const T* vt = tail + to_values;
-    const T* mine = own;
-    const int hd = a.hd;
-    store_block<T, false>(a, [=](int key) { return key == kPage - 1 ? mine : kt + (size_t)key * hd; }, page, kvh, red);
-    store_block<T, true>(a, [=](int key) { return key == kPage - 1 ? mine + hd : vt + (size_t)key * hd; }, page, kvh, red);
+    store_block<T>(a, rows, ld, value, page, kvh, red);
 }
 
 // Steps of several tokens: a block is (64-position block x of the sequence's new tokens, head of q, k or v, sequence).  Bound by the
@@ -269,11 +270,12 @@ __global__ void __launch_bounds__(128) append_token_kernel(const AppendArgs a) {
 // that the step found in the tail and the rows of its last, unfinished block belong to one thread block (x = 0), which reads the
 // tail before it writes it.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(128) append_prompt_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads) append_prompt_kernel(const AppendArgs a) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     T* rows = reinterpret_cast<T*>(smem_raw);            // [64][hd + 16 bytes]
     const int hd = a.hd, ld = hd + 16 / (int)sizeof(T), units = hd / 16, width = a.n_heads + 2 * a.n_kv;
     float* red = reinterpret_cast<float*>(rows + kPage * ld);
+    pdl_launch_dependents();
     pdl_wait();
     const int seq = blockIdx.z, head = blockIdx.y, tok0 = a.cu_seqlens[seq], n = a.cu_seqlens[seq + 1] - tok0;
     if (n <= 0) return;
@@ -291,31 +293,23 @@ __global__ void __launch_bounds__(128) append_prompt_kernel(const AppendArgs a) 
     for (;;) {
         const int p0 = b * kPage, lo = max(start, p0), hi = min(end, p0 + kPage);
         const bool complete = hi == p0 + kPage;
-        for (int i = threadIdx.x; i < (hi - lo) * units; i += 128) {
+        for (int i = threadIdx.x; i < (hi - lo) * units; i += kAppendThreads) {
             const int pos = lo + i / units;
             const size_t at = ((size_t)(tok0 + pos - start) * width + head) * hd;
             T* keep = nullptr;
             if (!query) keep = complete ? rows + (pos - p0) * ld : tail + (size_t)(pos - p0) * hd;
-            unit<T, VEC>(a, qkv + at, out + at, keep, nullptr, i % units, pos, !value);
+            unit<T, VEC>(a, qkv + at, out + at, keep, i % units, pos, !value);
         }
         if (query) return;
         if (b == first && start > p0) {
             // the rows found in the tail: to `old`, and to the block that is being completed
             T* old = reinterpret_cast<T*>(a.old) + (((size_t)seq * 2 + (value ? 1 : 0)) * a.n_kv + kvh) * kPage * hd;
-            constexpr int V = Vec<T>::n;
-            for (int i = threadIdx.x; i < (start - p0) * (hd / V); i += 128) {
-                const int r = i / (hd / V), c = (i % (hd / V)) * V;
-                const uint4 v = *reinterpret_cast<const uint4*>(tail + (size_t)r * hd + c);
-                *reinterpret_cast<uint4*>(old + (size_t)r * hd + c) = v;
-                if (complete) *reinterpret_cast<uint4*>(rows + r * ld + c) = v;
-            }
+            copy_rows<T>(tail, complete ? rows : nullptr, ld, old, start - p0, hd);
         }
         if (complete) {
             __syncthreads();
             const int page = page_of(a.block_table, a.table_stride, slot, b, a.n_pages);
-            const T* r = rows;
-            if (value) store_block<T, true>(a, [=](int key) { return r + key * ld; }, page, kvh, red);
-            else store_block<T, false>(a, [=](int key) { return r + key * ld; }, page, kvh, red);
+            store_block<T>(a, rows, ld, value, page, kvh, red);
         }
         if (b != first || last == first || !last_open) return;
         __syncthreads();                                  // the tail's rows have been read
@@ -324,27 +318,39 @@ __global__ void __launch_bounds__(128) append_prompt_kernel(const AppendArgs a) 
 }
 
 // ---- pages as the numbers they stand for ----------------------------------------------------------------------------------
+// A thread has four lanes of four keys: four words of keys, four of values.
 template <typename T>
-__global__ void __launch_bounds__(128) values_kernel(const signed char* __restrict__ pool, const float* __restrict__ scales, const int* __restrict__ pages,
-                                                     T* __restrict__ out, int n_kv, int hd, int n_pages) {
-    const int i = blockIdx.x, kvh = blockIdx.y, page = pages[i];
-    if (page < 0 || page >= n_pages) return;
-    const signed char* line = pool + ((size_t)page * n_kv + kvh) * line_bytes(hd);
-    const float ks = scales[((size_t)page * n_kv + kvh) * 2], vs = scales[((size_t)page * n_kv + kvh) * 2 + 1];
-    T* ko = out + ((size_t)i * 2 * n_kv + kvh) * kPage * hd;
-    T* vo = ko + (size_t)n_kv * kPage * hd;
-    for (int j = threadIdx.x; j < kPage * hd; j += 128) {
-        const int key = j / hd, d = j % hd;
-        ko[j] = from_f32<T>(line[j] * ks);
-        vo[j] = from_f32<T>(line[kPage * hd + value_word(key & ~3, d, hd) + (key & 3)] * vs);
+__global__ void __launch_bounds__(256) values_kernel(const signed char* __restrict__ pool, const int* __restrict__ pages, T* __restrict__ out, int n_kv, int hd,
+                                                     int n_pages) {
+    const int kvh = blockIdx.y, page = pages[blockIdx.x], i = blockIdx.z * 256 + threadIdx.x;
+    if (i >= 4 * hd) return;
+    const int key = i / (hd / 4) * 4, d = i % (hd / 4) * 4;
+    const signed char* line = pool + ((size_t)max(page, 0) * n_kv + kvh) * line_bytes(hd);
+    const bool is = page >= 0 && page < n_pages;
+    const float2 scale = is ? *scales_of(line, hd) : make_float2(0.f, 0.f);
+    unsigned k[4] = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u}, v[4] = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+    if (is) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            k[e] = *reinterpret_cast<const unsigned*>(line + (key + e) * hd + d);
+            v[e] = *reinterpret_cast<const unsigned*>(line + kPage * hd + value_word(key, d + e, hd));
+        }
     }
+    T* ko = out + (((size_t)blockIdx.x * 2 * n_kv + kvh) * kPage + key) * hd + d;
+    T* vo = ko + (size_t)n_kv * kPage * hd;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+            ko[e * hd + f] = from_f32<T>((float)((int)(k[e] >> (8 * f) & 0xffu) - 128) * scale.x);
+            vo[e * hd + f] = from_f32<T>((float)((int)(v[f] >> (8 * e) & 0xffu) - 128) * scale.y);
+        }
 }
 
 // ---- attention -------------------------------------------------------------------------------------------------------------
 struct AttendArgs {
     const void* rotated;         // [N, n_heads + 2 n_kv, hd]: the append's output
     const signed char* pool;
-    const float* scales;
     const void* found;           // rows of the unfinished blocks: the tail (by slot), or `old` (by sequence)
     int found_by_slot;
     const int* block_table;
@@ -397,8 +403,9 @@ __global__ void __launch_bounds__(kGeneralWarps * 32) attend_general_kernel(cons
             const int page = page_of(a.block_table, a.table_stride, slot, b, a.n_pages);
             if (page < 0) continue;
             line = a.pool + ((size_t)page * a.n_kv + kvh) * line_bytes(hd);
-            ks = a.scales[((size_t)page * a.n_kv + kvh) * 2];
-            vs = a.scales[((size_t)page * a.n_kv + kvh) * 2 + 1];
+            const float2 scale = *scales_of(line, hd);
+            ks = scale.x;
+            vs = scale.y;
         }
         float s = -INFINITY;
         if (seen) {
@@ -415,9 +422,9 @@ __global__ void __launch_bounds__(kGeneralWarps * 32) attend_general_kernel(cons
                 const signed char* kr = line + (key % kPage) * hd;
                 for (int d = 0; d < hd; d += 16) {
                     const int4 w = *reinterpret_cast<const int4*>(kr + d);
-                    const signed char* x = reinterpret_cast<const signed char*>(&w);
+                    const unsigned char* x = reinterpret_cast<const unsigned char*>(&w);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) sum = fmaf(q[d + e], (float)x[e], sum);
+                    for (int e = 0; e < 16; ++e) sum = fmaf(q[d + e], (float)((int)x[e] - 128), sum);
                 }
                 sum *= ks;
             }
@@ -449,8 +456,11 @@ __global__ void __launch_bounds__(kGeneralWarps * 32) attend_general_kernel(cons
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (lane + 32 * i < hd) {
-                        const char4 v = *reinterpret_cast<const char4*>(line + kPage * hd + value_word(k, lane + 32 * i, hd));
-                        acc[i] = fmaf(w[0], (float)v.x, fmaf(w[1], (float)v.y, fmaf(w[2], (float)v.z, fmaf(w[3], (float)v.w, acc[i]))));
+                        const uchar4 v = *reinterpret_cast<const uchar4*>(line + kPage * hd + value_word(k, lane + 32 * i, hd));
+                        acc[i] = fmaf(w[0], (float)((int)v.x - 128), acc[i]);
+                        acc[i] = fmaf(w[1], (float)((int)v.y - 128), acc[i]);
+                        acc[i] = fmaf(w[2], (float)((int)v.z - 128), acc[i]);
+                        acc[i] = fmaf(w[3], (float)((int)v.w - 128), acc[i]);
                     }
             }
         }
@@ -470,19 +480,519 @@ __global__ void __launch_bounds__(kGeneralWarps * 32) attend_general_kernel(cons
     }
 }
 
+// ---- single tokens -----------------------------------------------------------------------------------------------------------
+// One new token a sequence, bfloat16, heads of 64 or 128 lanes: a block owns (share of the sequence's pages, up to eight query heads
+// of a kv head, sequence).  Its producer warp streams the pages into a ring in shared memory, one bulk copy of 8 or 16 KB each (keys,
+// values and scales of the kv head), completion on mbarriers; eight consumer warps, WPP of them to a page, form scores and sums with
+// the query heads as rows of 16-row tensor-core tiles.  What bounds it, beside the memory, is the instructions that turn bytes into
+// operands, so:
+//   * a thread reads its bytes as 16-byte pieces that hold its fragments, and everything is in half precision: a byte behind 0x64 is
+//     1024 + 128 + q exactly, one permutation for two numbers;
+//   * of the keys the 1152 is not taken off: a score's sum starts at -1152 times the sum of its query, which is exact in what it takes
+//     off and costs 2^-23 of 1152 |q| a step in 32-bit sums (1e-6 of the largest score the block's keys could have);
+//   * the queries are multiplied by a power of two that brings their largest lane to 16 .. 32 (bfloat16 numbers above 2^-18 of it stay
+//     exact), the scores divided by it again;
+//   * the values' scale rides in the exponent: p' = 2^(score + log2 vs - m), with the maximum m taken of that sum, is at most 1, its
+//     product with the whole numbers needs no scale, and the sum of the probabilities gets p' / vs.  p' is rounded to half precision
+//     times 2^12 (11 bits from the largest down to 2^-26 of it).
+// Warps keep their own running maximum, sum and output and merge at the end; shares of a sequence meet in a second kernel.  The own
+// block's keys, unrounded, are read straight from the tail and the step's rows by the first four warps of the last share, in bfloat16,
+// while the first pages are on their way.  Waits are bounded; one that runs out leaves a code in the status word.
+struct TokenArgs {
+    AttendArgs a;
+    float* part_acc;             // [N, n_heads, n_splits, hd]
+    float* part_ml;              // [N, n_heads, n_splits, 2]: maximum (base 2) and sum
+    int n_splits, head_tiles, heads_a_tile, pages_per_split, n_stages;
+    int* status;
+};
+enum { Q8_TIMEOUT_PAGE = 51, Q8_TIMEOUT_FREE = 52 };
+constexpr unsigned kSpinLimit = 1u << 22;
+
+__device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(unsigned long long* bar, unsigned count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(unsigned long long* bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(unsigned long long* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait(unsigned long long* bar, unsigned parity) {
+    const unsigned addr = smem_u32(bar);
+    for (unsigned spin = 0; spin < kSpinLimit; ++spin) {
+        unsigned done;
+        asm volatile(
+            "{\n.reg .pred p;\n"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+            "selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(done)
+            : "r"(addr), "r"(parity)
+            : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+// rows 8 .. 15 of A are zero
+__device__ __forceinline__ void mma_bf16(float (&c)[4], unsigned a0, unsigned a2, unsigned b0, unsigned b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_half(float (&c)[4], unsigned a0, unsigned a2, unsigned b0, unsigned b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1));
+}
+// Bytes LO and LO + 1 of a word as two half-precision numbers, 1152 too large, and without that.
+template <int LO>
+__device__ __forceinline__ unsigned biased_two(unsigned word) { return __byte_perm(word, 0x64u, LO == 0 ? 0x4140 : 0x4342); }
+template <int LO>
+__device__ __forceinline__ unsigned two_of(unsigned word) {
+    const unsigned p = biased_two<LO>(word);
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&p), __float2half2_rn(1152.f));
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ unsigned pack_half(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ float ex2(float x) {          // 2^x (x = -inf gives 0)
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// How many of the n_splits shares of a sequence work: one per `pages_per_split` pages of 8-bit blocks.
+__host__ __device__ inline int active_splits(int n_pages, int n_splits, int pages_per_split) {
+    const int want = (n_pages + pages_per_split - 1) / pages_per_split;
+    return want < 1 ? 1 : (want > n_splits ? n_splits : want);
+}
+
+constexpr float kPShift = 12.f;          // probabilities are kept times 2^12
+constexpr int kTokenWarps = 8;           // consumers of a block
+
+// What a warp knows of its rows: thread (g, t) has head g of the tile.
+template <int HD>
+struct TokenState {
+    float o[HD / 8][4], m, l;
+    // a new maximum `top` of the thread's scores of row g (their own, or any of the row): moves the reference and gives what is to be
+    // added to a score in the exponent
+    __device__ __forceinline__ float refer(float top) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float now = fmaxf(m, top), ref = now == -INFINITY ? 0.f : now;
+        const float alpha = ex2(m - ref);
+        m = now;
+        if (__any_sync(0xffffffffu, alpha != 1.f)) {
+            l *= alpha;
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n) {
+                o[n][0] *= alpha;
+                o[n][1] *= alpha;
+            }
+        }
+        return kPShift - ref;
+    }
+};
+
+template <int HD, int WPP>
+__global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(const TokenArgs ta) {
+    constexpr int WARPS = kTokenWarps, NG = WARPS / WPP, CH = 4 / WPP;   // groups of warps, 16-key chunks of a page that a warp has
+    constexpr int KS = HD / 16, PIECES = HD / 64;                        // PIECES: 16-byte pieces of a key row in a thread
+    constexpr unsigned STAGE = line_bytes(HD);
+    const AttendArgs& a = ta.a;
+    const int S = ta.n_stages;                                           // a multiple of NG: a stage always serves the same group
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    unsigned char* ring = smem_raw;                                      // [S][keys, values, scales]
+    float* sm_acc = reinterpret_cast<float*>(ring);                      // [WARPS][8][HD], when the ring has been read
+    float* sm_m = reinterpret_cast<float*>(ring + (size_t)S * STAGE);
+    float* sm_l = sm_m + WARPS * 8;
+    unsigned long long* full = reinterpret_cast<unsigned long long*>(sm_l + WARPS * 8);
+    unsigned long long* empty = full + S;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int split = blockIdx.x, kvh = blockIdx.y / ta.head_tiles, tile = blockIdx.y % ta.head_tiles, seq = blockIdx.z;
+    const int group = a.n_heads / a.n_kv, head0 = kvh * group + tile * ta.heads_a_tile, G = min(ta.heads_a_tile, group - tile * ta.heads_a_tile);
+    pdl_launch_dependents();
+    if (tid == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(full + s, 1);
+            mbar_init(empty + s, WPP);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    pdl_wait();
+    const int tok = a.cu_seqlens[seq], next = a.cu_seqlens[seq + 1], pos = a.start_pos[seq], slot = a.slot_of_seq[seq];
+    const int key_lo = a.window > 0 ? max(0, pos + 1 - a.window) : 0, mine = pos / kPage;
+    const int pg_first = key_lo / kPage, n_pg = max(0, mine - pg_first);          // blocks in 8 bits
+    const int active = active_splits(n_pg, ta.n_splits, ta.pages_per_split);
+    if (next <= tok || split >= active) return;          // (the whole block; the kernel that merges computes the same number)
+    const int per = (n_pg + active - 1) / active;
+    const int pg_lo = pg_first + split * per, pg_hi = min(pg_first + n_pg, pg_lo + per);
+    __syncthreads();
+
+    if (warp == WARPS) {
+        // ---- producer: page numbers 32 at a time, copies by lane 0 ----
+        int s = -1, i = 0;
+        unsigned phase = 0;
+        bool failed = false;
+        for (int base = pg_lo; base < pg_hi; base += 32) {
+            const int n = min(32, pg_hi - base);
+            const int my_page = lane < n ? page_of(a.block_table, a.table_stride, slot, base + lane, a.n_pages) : -1;
+            for (int j = 0; j < n; ++j) {
+                const int page = __shfl_sync(0xffffffffu, my_page, j);
+                if (lane != 0 || failed) continue;
+                if (++s == S) { s = 0; phase ^= 1; }
+                if (i >= S && !mbar_wait(empty + s, phase ^ 1)) {
+                    atomicCAS(ta.status, 0, Q8_TIMEOUT_FREE);
+                    failed = true;
+                    continue;
+                }
+                ++i;
+                // (a page that the pool does not have: page 0's bytes; the consumers know as well)
+                mbar_expect_tx(full + s, STAGE);
+                bulk_copy(ring + (size_t)s * STAGE, a.pool + ((size_t)max(page, 0) * a.n_kv + kvh) * STAGE, STAGE, full + s);
+            }
+        }
+        // every copy has landed before the ring is used otherwise or the block ends, whatever became of the consumers
+        if (lane == 0)
+            for (int k = max(0, i - S); k < i; ++k) mbar_wait(full + k % S, (k / S) & 1);
+    } else {
+        // Q as the A operand: thread t's lanes of a row are t HD / 4 .. + HD / 4, four of them a step of K
+        const int width = a.n_heads + 2 * a.n_kv;
+        const __nv_bfloat16* rows = reinterpret_cast<const __nv_bfloat16*>(a.rotated) + (size_t)tok * width * HD;
+        unsigned qf[KS][2];
+        {
+            const uint4* q = reinterpret_cast<const uint4*>(rows + (size_t)(head0 + min(g, G - 1)) * HD + t * (HD / 4));
+#pragma unroll
+            for (int i = 0; i < KS / 2; ++i) {
+                const uint4 v = g < G ? q[i] : make_uint4(0u, 0u, 0u, 0u);
+                qf[2 * i][0] = v.x; qf[2 * i][1] = v.y; qf[2 * i + 1][0] = v.z; qf[2 * i + 1][1] = v.w;
+            }
+        }
+        TokenState<HD> st;
+        st.m = -INFINITY;
+        st.l = 0.f;
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st.o[n][e] = 0.f;
+
+        if (split == active - 1 && warp < 4 && warp * 16 <= pos % kPage) {
+            // ---- the own block: 16 of its rows, unrounded ----
+            const __nv_bfloat16* found = reinterpret_cast<const __nv_bfloat16*>(a.found) + ((size_t)slot * 2 * a.n_kv + kvh) * kPage * HD;
+            auto row = [&](int k, int which) -> const __nv_bfloat16* {            // k of the own block, at most pos
+                if (mine * kPage + k == pos) return rows + (size_t)(a.n_heads + which * a.n_kv + kvh) * HD;
+                return found + ((size_t)which * a.n_kv * kPage + k) * HD;
+            };
+            const int own_lo = max(0, key_lo - mine * kPage), own_hi = pos % kPage;      // the keys seen
+            float sc[2][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                const int k = warp * 16 + 4 * (g >> 1) + 2 * i + (g & 1);
+                const bool seen = k <= own_hi && k >= own_lo;
+                const uint4* kr = reinterpret_cast<const uint4*>(row(min(k, own_hi), 0) + t * (HD / 4));
+#pragma unroll
+                for (int j = 0; j < KS / 2; ++j) {
+                    const uint4 v = seen ? kr[j] : make_uint4(0u, 0u, 0u, 0u);
+                    mma_bf16(c, qf[2 * j][0], qf[2 * j][1], v.x, v.y);
+                    mma_bf16(c, qf[2 * j + 1][0], qf[2 * j + 1][1], v.z, v.w);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int key = warp * 16 + 4 * t + 2 * i + e;
+                    sc[i][e] = key <= own_hi && key >= own_lo ? c[e] * a.scale_log2e : -INFINITY;
+                }
+            }
+            const float shift = st.refer(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])));
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    sc[i][e] = ex2(sc[i][e] + shift);
+                    st.l += sc[i][e];
+                }
+            const unsigned p01 = pack_bf16(sc[0][0], sc[0][1]), p23 = pack_bf16(sc[1][0], sc[1][1]);
+            // lanes g HD / 8 .. + HD / 8 of the thread's four keys
+#pragma unroll
+            for (int j = 0; j < HD / 64; ++j) {
+                uint4 v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int key = warp * 16 + 4 * t + e;
+                    const bool seen = key <= own_hi && key >= own_lo;
+                    v[e] = seen ? reinterpret_cast<const uint4*>(row(min(key, own_hi), 1) + g * (HD / 8))[j] : make_uint4(0u, 0u, 0u, 0u);
+                }
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    const unsigned w0 = n < 2 ? v[0].x : n < 4 ? v[0].y : n < 6 ? v[0].z : v[0].w, w1 = n < 2 ? v[1].x : n < 4 ? v[1].y : n < 6 ? v[1].z : v[1].w;
+                    const unsigned w2 = n < 2 ? v[2].x : n < 4 ? v[2].y : n < 6 ? v[2].z : v[2].w, w3 = n < 2 ? v[3].x : n < 4 ? v[3].y : n < 6 ? v[3].z : v[3].w;
+                    mma_bf16(st.o[8 * j + n], p01, p23, __byte_perm(w0, w1, n & 1 ? 0x7632 : 0x5410), __byte_perm(w2, w3, n & 1 ? 0x7632 : 0x5410));
+                }
+            }
+        }
+
+        // the queries in half precision: times a power of two that brings the row's largest lane to 16 .. 32
+        float start, to_log2;
+        {
+            float q[KS][4], top = 0.f, sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    q[k][2 * h] = __uint_as_float(qf[k][h] << 16);
+                    q[k][2 * h + 1] = __uint_as_float(qf[k][h] & 0xffff0000u);
+                    top = fmaxf(top, fmaxf(fabsf(q[k][2 * h]), fabsf(q[k][2 * h + 1])));
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int exponent = (int)(__float_as_uint(top) >> 23);               // 0: zero or next to it; 255: an infinity
+            const int by = exponent == 0 || exponent == 255 ? 127 : min(254, max(1, 258 - exponent));
+            const float factor = __uint_as_float((unsigned)by << 23);
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const __half2 v = __floats2half2_rn(q[k][2 * h] * factor, q[k][2 * h + 1] * factor);
+                    qf[k][h] = *reinterpret_cast<const unsigned*>(&v);
+                    const float2 f = __half22float2(v);
+                    sum += f.x + f.y;
+                }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            start = -1152.f * sum;
+            to_log2 = a.scale_log2e / factor;
+        }
+
+        // ---- the pages: this warp's group takes every NG-th, the warp CH chunks of 16 keys of each ----
+        const int grp = warp / WPP, part = warp % WPP;
+        int s = grp - NG;
+        unsigned phase = 0;
+        for (int pg = pg_lo + grp; pg < pg_hi; pg += NG) {
+            s += NG;
+            if (s >= S) { s -= S; phase ^= 1; }
+            const bool none = page_of(a.block_table, a.table_stride, slot, pg, a.n_pages) < 0;
+            if (!mbar_wait(full + s, phase)) {
+                if (lane == 0) atomicCAS(ta.status, 0, Q8_TIMEOUT_PAGE);
+                break;
+            }
+            const unsigned char* keys = ring + (size_t)s * STAGE;
+            const unsigned char* values = keys + kPage * HD;
+            const float2 scale = *scales_of(keys, HD);
+            // (a block whose values are all next to zero: any scale will do; a NaN stays one)
+            const float vs = scale.y < 0x1p-100f ? 0x1p-100f : scale.y, lv = __log2f(vs);
+            const float factor = to_log2 * scale.x;
+            float sc[CH][2][2];
+            float top = -INFINITY;
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float c[4] = {start, start, 0.f, 0.f};
+                    const int k = (part * CH + ch) * 16 + 4 * (g >> 1) + 2 * i + (g & 1);
+                    const uint4* kr = reinterpret_cast<const uint4*>(keys + k * HD + t * (HD / 4));
+                    uint4 v[PIECES];
+                    // (with two pieces a thread, odd rows read theirs in the other order: no two threads of a phase meet in a bank)
+#pragma unroll
+                    for (int j = 0; j < PIECES; ++j) v[j] = kr[PIECES == 1 ? 0 : j ^ (g & 1)];
+                    if (PIECES == 2 && (g & 1)) { const uint4 x = v[0]; v[0] = v[PIECES - 1]; v[PIECES - 1] = x; }
+#pragma unroll
+                    for (int j = 0; j < PIECES; ++j) {
+                        const unsigned w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) mma_half(c, qf[4 * j + x][0], qf[4 * j + x][1], biased_two<0>(w[x]), biased_two<2>(w[x]));
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        sc[ch][i][e] = fmaf(c[e], factor, lv);
+                        if (pg == pg_first && pg * kPage + (part * CH + ch) * 16 + 4 * t + 2 * i + e < key_lo) sc[ch][i][e] = -INFINITY;      // the window's edge
+                        top = fmaxf(top, sc[ch][i][e]);
+                    }
+                }
+            if (!none) {
+                const float shift = st.refer(top);
+                float sum = 0.f;
+                const float to_sum = 1.f / vs;
+                const uint4* vr = reinterpret_cast<const uint4*>(values + part * CH * (16 * HD)) + lane;
+#pragma unroll
+                for (int ch = 0; ch < CH; ++ch) {
+                    float p[2][2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            p[i][e] = ex2(sc[ch][i][e] + shift);
+                            sum += p[i][e];
+                        }
+                    const unsigned p01 = pack_half(p[0][0], p[0][1]), p23 = pack_half(p[1][0], p[1][1]);
+#pragma unroll
+                    for (int j = 0; j < HD / 32; ++j) {
+                        const uint4 v = vr[(ch * (HD / 32) + j) * 32];
+                        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) mma_half(st.o[4 * j + x], p01, p23, two_of<0>(w[x]), two_of<2>(w[x]));
+                    }
+                }
+                st.l = fmaf(sum, to_sum, st.l);          // this lane's share
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + s);
+        }
+        st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
+        st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
+        if (t == 0) { sm_m[warp * 8 + g] = st.m; sm_l[warp * 8 + g] = st.l; }
+        // the ring is free when all consumers and the producer are here (named barrier: all threads of the block)
+        asm volatile("bar.sync 1, %0;\n" ::"r"((WARPS + 1) * 32) : "memory");
+        // lanes 2 t HD / 8 + n and (2 t + 1) HD / 8 + n of row g
+#pragma unroll
+        for (int n = 0; n < HD / 8; n += 4) {
+            *reinterpret_cast<float4*>(sm_acc + (warp * 8 + g) * HD + 2 * t * (HD / 8) + n) = make_float4(st.o[n][0], st.o[n + 1][0], st.o[n + 2][0], st.o[n + 3][0]);
+            *reinterpret_cast<float4*>(sm_acc + (warp * 8 + g) * HD + (2 * t + 1) * (HD / 8) + n) = make_float4(st.o[n][1], st.o[n + 1][1], st.o[n + 2][1], st.o[n + 3][1]);
+        }
+    }
+    if (warp == WARPS) asm volatile("bar.sync 1, %0;\n" ::"r"((WARPS + 1) * 32) : "memory");
+    __syncthreads();
+    for (int i = tid; i < G * HD; i += blockDim.x) {
+        const int h = i / HD, d = i % HD;
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, sm_m[w * 8 + h]);
+        const float ref = m == -INFINITY ? 0.f : m;
+        float l = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = ex2(sm_m[w * 8 + h] - ref);
+            l += sm_l[w * 8 + h] * f;
+            o += sm_acc[(w * 8 + h) * HD + d] * f;
+        }
+        const size_t row = (size_t)tok * a.n_heads + head0 + h;
+        if (active == 1) {
+            reinterpret_cast<__nv_bfloat16*>(a.out)[row * HD + d] = __float2bfloat16_rn(o / l);
+        } else {
+            const size_t part = row * ta.n_splits + split;
+            ta.part_acc[part * HD + d] = o;
+            if (d == 0) { ta.part_ml[part * 2] = m; ta.part_ml[part * 2 + 1] = l; }
+        }
+    }
+}
+
+// Merges the shares: a block per (sequence, head); 512 / HD groups of threads take shares in turn, four lanes a thread.
+template <int HD>
+__global__ void __launch_bounds__(128) merge_kernel(const TokenArgs ta) {
+    constexpr int LANES = HD / 4, GROUPS = 128 / LANES;
+    const AttendArgs& a = ta.a;
+    __shared__ float weight[64];
+    __shared__ float2 red[2];
+    __shared__ float4 sums[128];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tid = threadIdx.x, head = blockIdx.x, seq = blockIdx.y, tok = a.cu_seqlens[seq], next = a.cu_seqlens[seq + 1], pos = a.start_pos[seq];
+    const int key_lo = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+    const int active = active_splits(max(0, pos / kPage - key_lo / kPage), ta.n_splits, ta.pages_per_split);
+    if (next <= tok || active == 1) return;              // written by the block itself
+    const size_t row = (size_t)tok * a.n_heads + head;
+    const float4* acc = reinterpret_cast<const float4*>(ta.part_acc + row * ta.n_splits * HD) + tid % LANES;
+    if (tid < 64) {                                      // two warps: maximum and sum of up to 64 shares
+        const float2 x = tid < active ? reinterpret_cast<const float2*>(ta.part_ml)[row * ta.n_splits + tid] : make_float2(-INFINITY, 0.f);
+        const float m = warp_max(x.x), ref = m == -INFINITY ? 0.f : m;
+        const float w = ex2(x.x - ref), l = warp_sum(x.y * w);
+        weight[tid] = w;
+        if (tid % 32 == 0) red[tid / 32] = make_float2(m, l);
+    }
+    __syncthreads();
+    const float m = fmaxf(red[0].x, red[1].x), ref = m == -INFINITY ? 0.f : m;
+    const float f0 = ex2(red[0].x - ref), f1 = ex2(red[1].x - ref), l = red[0].y * f0 + red[1].y * f1;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int z = tid / LANES; z < active; z += GROUPS) {
+        const float w = weight[z] * (z < 32 ? f0 : f1);
+        const float4 v = acc[(size_t)z * LANES];
+        o.x = fmaf(v.x, w, o.x); o.y = fmaf(v.y, w, o.y); o.z = fmaf(v.z, w, o.z); o.w = fmaf(v.w, w, o.w);
+    }
+    sums[tid] = o;
+    __syncthreads();
+    if (tid >= LANES) return;
+#pragma unroll
+    for (int i = 1; i < GROUPS; ++i) {
+        const float4 v = sums[i * LANES + tid];
+        o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+    }
+    const float by = 1.f / l;
+    uint2 w;
+    w.x = pack_bf16(o.x * by, o.y * by);
+    w.y = pack_bf16(o.z * by, o.w * by);
+    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + row * HD + tid * 4) = w;
+}
+
+// The plan of a step of single tokens, the same for the caller that provides the scratch and for the launch.
+struct TokenPlan { int splits, pages_per_split, stages, wpp, head_tiles, heads_a_tile; };
+static TokenPlan plan_tokens(int n_seqs, int n_heads, int n_kv, int hd, int max_kv_len, int window) {
+    TokenPlan p;
+    const int group = n_heads / n_kv, sms = blm_sm_count();
+    p.head_tiles = (group + 7) / 8;
+    p.heads_a_tile = (group + p.head_tiles - 1) / p.head_tiles;
+    int pages = (max_kv_len + kPage - 1) / kPage;
+    if (window > 0 && pages > window / kPage + 2) pages = window / kPage + 2;
+    if (pages < 1) pages = 1;
+    const int rows = n_seqs * n_kv * p.head_tiles;       // blocks of an unsplit step
+    // Walks of more than 8 pages are cut, as far as that fills the SMs about twice.
+    const int by_length = (pages + 7) / 8, to_fill = (2 * sms + rows - 1) / rows;
+    p.splits = by_length < to_fill ? by_length : to_fill;
+    if (p.splits > 64) p.splits = 64;
+    if (p.splits < 1) p.splits = 1;
+    const int blocks = rows * p.splits, each = (pages + p.splits - 1) / p.splits;
+    p.pages_per_split = blocks > 2 * sms ? each : 1;
+    p.wpp = 2;
+    const int groups = kTokenWarps / p.wpp;
+    p.stages = (hd == 64 ? 8 : 4) / groups * groups;
+    return p;
+}
+
+template <int HD, int WPP>
+static int launch_tokens_as(const TokenArgs& ta, cudaStream_t stream) {
+    const dim3 grid(ta.n_splits, ta.a.n_kv * ta.head_tiles, ta.a.n_seqs);
+    const size_t smem = (size_t)ta.n_stages * (line_bytes(HD) + 16) + (size_t)kTokenWarps * 8 * 2 * 4;
+    static bool opted_in[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !opted_in[dev]) {
+        if (cudaFuncSetAttribute(attend_token_kernel<HD, WPP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024) != cudaSuccess)
+            return blm_fail(BLM_CUDA_ERROR, "attention_q8: %s", cudaGetErrorString(cudaGetLastError()));
+        if (dev >= 0 && dev < 64) opted_in[dev] = true;
+    }
+    blm_launch_dependent(attend_token_kernel<HD, WPP>, grid, dim3((kTokenWarps + 1) * 32), smem, stream, ta);
+    if (ta.n_splits > 1) blm_launch_dependent(merge_kernel<HD>, dim3(ta.a.n_heads, ta.a.n_seqs), dim3(128), 0, stream, ta);
+    return blm_check_launch("attention_q8");
+}
+// bfloat16 steps of single tokens with heads of 64 or 128 lanes
+static bool tokens_take(int dtype, int hd, int max_q_len, int n_seqs, int n_kv, int n_heads) {
+    return dtype == BLM_BF16 && (hd == 64 || hd == 128) && max_q_len == 1 && n_seqs <= 65535 && (n_heads / n_kv + 7) / 8 * n_kv <= 65535;
+}
+
 template <typename T, bool VEC>
 static int launch_append(const AppendArgs& a, int n_seqs, int max_q_len, cudaStream_t stream) {
+    const size_t smem = (size_t)kPage * (a.hd + 16 / sizeof(T)) * sizeof(T) + kAppendThreads / 32 * sizeof(float);
+    const void* kernel = max_q_len == 1 ? (const void*)append_token_kernel<T, VEC> : (const void*)append_prompt_kernel<T, VEC>;
+    if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+        return blm_fail(BLM_CUDA_ERROR, "rope_append_q8: %s", cudaGetErrorString(cudaGetLastError()));
     if (max_q_len == 1) {
-        const size_t smem = 2 * a.hd * sizeof(T) + 4 * sizeof(float);
-        blm_launch_dependent(append_token_kernel<T, VEC>, dim3(a.n_kv, n_seqs), dim3(128), smem, stream, a);
+        blm_launch_dependent(append_token_kernel<T, VEC>, dim3(a.n_kv, n_seqs, 2), dim3(kAppendThreads), smem, stream, a);
     } else {
-        const size_t smem = (size_t)kPage * (a.hd + 16 / sizeof(T)) * sizeof(T) + 4 * sizeof(float);
-        if (smem > 48 * 1024 &&
-            cudaFuncSetAttribute(append_prompt_kernel<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-            return blm_fail(BLM_CUDA_ERROR, "rope_append_q8: no room for a block's rows");
         // a run of max_q_len tokens touches this many blocks at most, wherever it begins
         const dim3 grid((max_q_len + kPage - 2) / kPage + 1, a.n_heads + 2 * a.n_kv, n_seqs);
-        blm_launch_dependent(append_prompt_kernel<T, VEC>, grid, dim3(128), smem, stream, a);
+        blm_launch_dependent(append_prompt_kernel<T, VEC>, grid, dim3(kAppendThreads), smem, stream, a);
     }
     return blm_check_launch("rope_append_q8");
 }
@@ -490,7 +1000,7 @@ static int launch_append(const AppendArgs& a, int n_seqs, int max_q_len, cudaStr
 
 BLM_API int blm_rope_append_q8(const void* qkv, void* out, int dtype, const int* cu_seqlens, const int* slot_of_seq, const int* start_pos,
                                const int* block_table, int table_stride, const double* inv_freq, int rot, int pairing, const float* table,
-                               int table_len, float turn_scale, void* pool, float* scales, void* tail, void* old, int n_seqs, int max_q_len,
+                               int table_len, float turn_scale, void* pool, void* tail, void* old, int n_seqs, int max_q_len,
                                int n_heads, int n_kv, int hd, int n_pages, cudaStream_t stream) {
     using namespace q8;
     if (n_seqs == 0 || max_q_len == 0) return BLM_OK;
@@ -502,35 +1012,49 @@ BLM_API int blm_rope_append_q8(const void* qkv, void* out, int dtype, const int*
     BLM_REQUIRE(n_seqs <= 65535 && n_heads + 2 * n_kv <= 65535, "rope_append_q8: %d sequences, %d heads (at most 65535 of either)", n_seqs, n_heads + 2 * n_kv);
     BLM_REQUIRE(dtype == BLM_F32 || dtype == BLM_BF16, "rope_append_q8: dtype %d", dtype);
     const AppendArgs a{qkv, out, cu_seqlens, slot_of_seq, start_pos, block_table, table_stride, inv_freq, (const float2*)table, table ? table_len : 0,
-                       turn_scale, rot, pairing, (signed char*)pool, scales, tail, old, n_heads, n_kv, hd, n_pages};
+                       turn_scale, rot, pairing, (signed char*)pool, tail, old, n_heads, n_kv, hd, n_pages};
     const bool vec = rot % 16 == 0;
     if (dtype == BLM_F32) return vec ? launch_append<float, true>(a, n_seqs, max_q_len, stream) : launch_append<float, false>(a, n_seqs, max_q_len, stream);
     return vec ? launch_append<__nv_bfloat16, true>(a, n_seqs, max_q_len, stream) : launch_append<__nv_bfloat16, false>(a, n_seqs, max_q_len, stream);
 }
 
-BLM_API int blm_q8_values(const void* pool, const float* scales, const int* pages, void* out, int dtype, int n, int n_kv, int hd, int n_pages,
-                          cudaStream_t stream) {
+BLM_API int blm_q8_values(const void* pool, const int* pages, void* out, int dtype, int n, int n_kv, int hd, int n_pages, cudaStream_t stream) {
     using namespace q8;
     if (n == 0) return BLM_OK;
     BLM_REQUIRE(hd >= 16 && hd <= 256 && hd % 16 == 0 && n_kv <= 65535, "q8_values: %d heads of %d lanes", n_kv, hd);
-    const dim3 grid(n, n_kv);
-    if (dtype == BLM_F32) values_kernel<<<grid, 128, 0, stream>>>((const signed char*)pool, scales, pages, (float*)out, n_kv, hd, n_pages);
-    else if (dtype == BLM_BF16) values_kernel<<<grid, 128, 0, stream>>>((const signed char*)pool, scales, pages, (__nv_bfloat16*)out, n_kv, hd, n_pages);
+    const dim3 grid(n, n_kv, (4 * hd + 255) / 256);
+    if (dtype == BLM_F32) values_kernel<<<grid, 256, 0, stream>>>((const signed char*)pool, pages, (float*)out, n_kv, hd, n_pages);
+    else if (dtype == BLM_BF16) values_kernel<<<grid, 256, 0, stream>>>((const signed char*)pool, pages, (__nv_bfloat16*)out, n_kv, hd, n_pages);
     else return blm_fail(BLM_BAD_ARGUMENT, "q8_values: dtype %d", dtype);
     return blm_check_launch("q8_values");
 }
 
-BLM_API int blm_attention_q8(const void* rotated, const void* pool, const float* scales, const void* found, int found_by_slot, int dtype,
+// Over how many shares a step cuts its sequences: what the scratch holds is n_tokens * n_heads * shares * (hd + 2) float32 when there are
+// several, which a second kernel merges.
+BLM_API int blm_attention_q8_splits(int dtype, int n_seqs, int max_q_len, int max_kv_len, int n_heads, int n_kv, int hd, int window) {
+    using namespace q8;
+    if (n_seqs < 1 || n_kv < 1 || n_heads < n_kv || !tokens_take(dtype, hd, max_q_len, n_seqs, n_kv, n_heads)) return 1;
+    return plan_tokens(n_seqs, n_heads, n_kv, hd, max_kv_len, window).splits;
+}
+
+BLM_API int blm_attention_q8(const void* rotated, const void* pool, const void* found, int found_by_slot, int dtype,
                              const int* block_table, int table_stride, const int* cu_seqlens, const int* slot_of_seq, const int* start_pos,
-                             void* out, int n_tokens, int n_seqs, int n_heads, int n_kv, int hd, int n_pages, int window, float scale,
-                             cudaStream_t stream) {
+                             void* out, int n_tokens, int n_seqs, int n_heads, int n_kv, int hd, int n_pages, int window, float scale, int max_q_len,
+                             int max_kv_len, float* scratch, int splits, int* status, cudaStream_t stream) {
     using namespace q8;
     if (n_tokens == 0 || n_seqs == 0) return BLM_OK;
     BLM_REQUIRE(hd >= 16 && hd <= 256 && hd % 16 == 0, "attention_q8: heads of %d lanes (multiples of 16 from 16 to 256)", hd);
     BLM_REQUIRE(n_kv > 0 && n_heads % n_kv == 0, "attention_q8: %d heads do not divide into %d kv heads", n_heads, n_kv);
     BLM_REQUIRE((long long)n_tokens * n_heads < (1ll << 31), "attention_q8: %d tokens of %d heads in one step", n_tokens, n_heads);
-    const AttendArgs a{rotated, (const signed char*)pool, scales, found, found_by_slot, block_table, table_stride, cu_seqlens, slot_of_seq, start_pos,
+    const AttendArgs a{rotated, (const signed char*)pool, found, found_by_slot, block_table, table_stride, cu_seqlens, slot_of_seq, start_pos,
                        out, n_seqs, n_heads, n_kv, hd, n_pages, window, scale * 1.4426950408889634f};
+    if (tokens_take(dtype, hd, max_q_len, n_seqs, n_kv, n_heads)) {
+        const TokenPlan p = plan_tokens(n_seqs, n_heads, n_kv, hd, max_kv_len, window);
+        BLM_REQUIRE(p.splits == splits && (splits == 1 || scratch != nullptr), "attention_q8: scratch for %d shares, the step has %d", splits, p.splits);
+        const TokenArgs ta{a, scratch, scratch ? scratch + (size_t)n_tokens * n_heads * splits * hd : nullptr, p.splits, p.head_tiles, p.heads_a_tile,
+                           p.pages_per_split, p.stages, status};
+        return hd == 64 ? launch_tokens_as<64, 2>(ta, stream) : launch_tokens_as<128, 2>(ta, stream);
+    }
     const dim3 grid(n_heads * n_tokens);
     if (dtype == BLM_F32) blm_launch_dependent(attend_general_kernel<float>, grid, dim3(kGeneralWarps * 32), 0, stream, a);
     else if (dtype == BLM_BF16) blm_launch_dependent(attend_general_kernel<__nv_bfloat16>, grid, dim3(kGeneralWarps * 32), 0, stream, a);

@@ -201,10 +201,11 @@ _protos = {
     },
     "attention_q8": {
         "blm_rope_append_q8": [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p,
-                               c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
-        "blm_q8_values": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
-        "blm_attention_q8": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
-                             c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p],
+                               c_int, c_float, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
+        "blm_q8_values": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
+        "blm_attention_q8": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                             c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
+        "blm_attention_q8_splits": [c_int] * 8,
     },
     "moe": {
         "blm_moe_route": [c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
@@ -1117,7 +1118,8 @@ _WAITS = {
     35: "prompt attention: the probabilities were not written", 36: "prompt attention: the product with the values did not arrive",
     37: "prompt attention: the producer waited in vain for a free stage",
     41: "gemm_sk: the tensor-core thread waited in vain for a stage", 42: "gemm_sk: the producer waited in vain for a free stage",
-    43: "gemm_sk: the epilogue waited in vain for the accumulator"}
+    43: "gemm_sk: the epilogue waited in vain for the accumulator",
+    51: "attention over 8 bits: a consumer waited in vain for a page", 52: "attention over 8 bits: the producer waited in vain for a free stage"}
 
 
 def check_status(device) -> None:
@@ -1996,39 +1998,51 @@ def pass_entry(resid, delta, embedded, step):
 
 # -- a cache line in 8 bits ------------------------------------------------------------------------------------------------------
 def q8_line_bytes(head_dim: int) -> int:
-    """Bytes of one kv head in a page of a cache line in 8 bits: its keys, and its values with the lanes filled up to 32."""
-    return PAGE * (head_dim + -(-head_dim // 32) * 32)
+    """Bytes of one kv head in a page of a cache line in 8 bits: its keys, its values with the lanes filled up to 32, its two scales
+    (filled up to 16 bytes)."""
+    return PAGE * (head_dim + -(-head_dim // 32) * 32) + 16
 
 
 def q8_pool(n_pages: int, n_kv: int, head_dim: int, device):
-    """(pool int8 [n_pages, n_kv, q8_line_bytes(head_dim)], scales float32 [n_pages, n_kv, 2]) of a cache line whose complete blocks of
-    PAGE positions are kept in 8 bits: keys and values of a block are whole numbers times one scale per kv head for the keys and one
-    for the values.  How the numbers lie in a page is the kernels' own affair: rope_append_q8 fills pages, attention_q8 reads them,
-    q8_values gives the numbers, q8_write takes them."""
+    """(pool int8 [n_pages, n_kv, q8_line_bytes(head_dim)], scales float32 [n_pages, n_kv, 2], a view into it) of a cache line whose
+    complete blocks of PAGE positions are kept in 8 bits: keys and values of a block are whole numbers times one scale per kv head for
+    the keys and one for the values.  How the numbers lie in a page is the kernels' own affair: rope_append_q8 fills pages, attention_q8
+    reads them, q8_values gives the numbers, q8_write takes them."""
     if not 16 <= head_dim <= 256 or head_dim % 16:
         raise KernelError(f"q8_pool: heads of {head_dim} lanes (multiples of 16 from 16 to 256)")
-    return (torch.zeros((n_pages, n_kv, q8_line_bytes(head_dim)), dtype=torch.int8, device=device),
-            torch.zeros((n_pages, n_kv, 2), dtype=torch.float32, device=device))
+    pool = torch.zeros((n_pages, n_kv, q8_line_bytes(head_dim)), dtype=torch.int8, device=device)
+    return pool, pool.view(torch.float32)[:, :, -4:-2]
 
 
 def _q8_line(what, pool, scales, n_kv, head_dim):
-    if (pool.dtype != torch.int8 or pool.dim() != 3 or tuple(pool.shape[1:]) != (n_kv, q8_line_bytes(head_dim)) or scales.dtype != torch.float32
-            or tuple(scales.shape) != (pool.shape[0], n_kv, 2)):
-        raise KernelError(f"{what}: pool int8 [pages, {n_kv}, {q8_line_bytes(head_dim)}] and scales float32 [pages, {n_kv}, 2], as q8_pool gives them")
+    line = q8_line_bytes(head_dim)
+    if (pool.dtype is not torch.int8 or pool.dim() != 3 or pool.shape[1] != n_kv or pool.shape[2] != line or scales.dtype is not torch.float32
+            or scales.shape != (pool.shape[0], n_kv, 2) or scales.data_ptr() != pool.data_ptr() + line - 16 or scales.stride() != (n_kv * line // 4, line // 4, 1)):
+        raise KernelError(f"{what}: pool int8 [pages, {n_kv}, {line}] and scales float32 [pages, {n_kv}, 2], as q8_pool gives them")
 
 
-def _on_current(what, *tensors):
-    """The tensors' device is the current one: kernels are launched on its current stream."""
-    now = _current_device() if _current_device is not None else torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != now:
-            raise KernelError(f"{what}: a tensor on {t.device} while the current device is cuda:{now}")
-
-
-def _aligned(what, *tensors):
-    for t in tensors:
-        if t is not None and t.data_ptr() % 16:
-            raise KernelError(f"{what}: tensors must begin at multiples of 16 bytes")
+def _launch_ptrs(what, tensors, anywhere=()):
+    """The addresses of the tensors (None: 0), which must be contiguous and lie on the current device (kernels are launched on its
+    current stream); those of `tensors` begin at multiples of 16 bytes, those of `anywhere` where they like."""
+    now, out, odd = None, [], 15
+    for t in (*tensors, Ellipsis, *anywhere):
+        if t is Ellipsis:
+            odd = 0
+            continue
+        if t is None:
+            out.append(0)
+            continue
+        device, ptr = t.get_device(), t.data_ptr()
+        if device != now:
+            if device < 0:
+                raise KernelError("burn-lm_b200 kernels run on a CUDA device only; got a CPU tensor")
+            now = _current_device() if _current_device is not None else torch.cuda.current_device()
+            if device != now:
+                raise KernelError(f"{what}: a tensor on cuda:{device} while the current device is cuda:{now}")
+        if ptr & odd or not t.is_contiguous():
+            raise KernelError(f"{what}: tensors must be contiguous and begin at multiples of 16 bytes")
+        out.append(ptr)
+    return out
 
 
 _q8_places: dict = {}
@@ -2056,9 +2070,9 @@ def q8_write(pool, scales, pages, keys, key_scales, values, value_scales) -> Non
     if (page != PAGE or keys.dtype != torch.int8 or values.dtype != torch.int8 or values.shape != keys.shape or pages.numel() != p
             or tuple(key_scales.shape) != (p, n_kv) or tuple(value_scales.shape) != (p, n_kv)):
         raise KernelError(f"q8_write: keys and values int8 [P, kv heads, {PAGE}, head_dim], scales [P, kv heads], a page for each")
-    line = torch.zeros((p, n_kv, pool.shape[2]), dtype=torch.int8, device=pool.device)
-    line[:, :, : PAGE * head_dim] = keys.reshape(p, n_kv, -1)
-    line[:, :, PAGE * head_dim:][:, :, _q8_value_places(head_dim, pool.device).reshape(-1)] = values.reshape(p, n_kv, -1)
+    line = torch.full((p, n_kv, pool.shape[2]), -128, dtype=torch.int8, device=pool.device)      # a byte holds the number + 128
+    line[:, :, : PAGE * head_dim] = (keys ^ -128).reshape(p, n_kv, -1)
+    line[:, :, PAGE * head_dim:][:, :, _q8_value_places(head_dim, pool.device).reshape(-1)] = (values ^ -128).reshape(p, n_kv, -1)
     at = pages.to(torch.int64)
     pool[at] = line
     scales[at] = torch.stack([key_scales, value_scales], dim=2).to(torch.float32)
@@ -2071,20 +2085,29 @@ def q8_values(pool, scales, pages, head_dim, dtype=torch.float32):
     _q8_line("q8_values", pool, scales, n_kv, head_dim)
     if pages.dtype != torch.int32:
         raise KernelError("q8_values: pages must be int32")
-    _need_cuda(pool, scales, pages)
-    _on_current("q8_values", pool, scales, pages)
-    out = torch.zeros((pages.numel(), 2, n_kv, PAGE, head_dim), dtype=dtype, device=pool.device)
-    _call("attention_q8", "blm_q8_values", _ptr(pool), _ptr(scales), _ptr(pages), _ptr(out), _code(dtype), pages.numel(), n_kv, head_dim, n_pages,
-          _stream())
+    p_pool, p_pages = _launch_ptrs("q8_values", (pool,), (pages,))
+    out = torch.empty((pages.numel(), 2, n_kv, PAGE, head_dim), dtype=dtype, device=pool.device)
+    _call("attention_q8", "blm_q8_values", p_pool, p_pages, out.data_ptr(), _code(dtype), pages.numel(), n_kv, head_dim, n_pages, _stream())
     return out
 
 
 def _q8_step(what, step, block_table, tail, n_kv, head_dim, dtype):
-    for t in (step.cu_seqlens, step.slot_of_seq, step.start_pos, block_table):
-        if t.dtype != torch.int32:
-            raise KernelError(f"{what}: cu_seqlens, slot_of_seq, start_pos and the block table are int32")
-    if block_table.dim() != 2 or tail.dtype != dtype or tail.dim() != 5 or tuple(tail.shape) != (block_table.shape[0], 2, n_kv, PAGE, head_dim):
+    i32 = torch.int32
+    if step.cu_seqlens.dtype is not i32 or step.slot_of_seq.dtype is not i32 or step.start_pos.dtype is not i32 or block_table.dtype is not i32:
+        raise KernelError(f"{what}: cu_seqlens, slot_of_seq, start_pos and the block table are int32")
+    if step.cu_seqlens.numel() != step.n_seqs + 1 or step.slot_of_seq.numel() != step.n_seqs or step.start_pos.numel() != step.n_seqs:
+        raise KernelError(f"{what}: cu_seqlens [{step.n_seqs + 1}], slot_of_seq and start_pos [{step.n_seqs}] of the step's sequences")
+    if block_table.dim() != 2 or tail.dtype is not dtype or tail.shape != (block_table.shape[0], 2, n_kv, PAGE, head_dim):
         raise KernelError(f"{what}: block_table [slots, pages] and tail [slots, 2, {n_kv}, {PAGE}, {head_dim}] in the projection's dtype")
+
+
+def _step_ptrs(what, step):
+    """The addresses of a step's bounds, slots and positions: int32, wherever they begin."""
+    cu, slot, start = step.cu_seqlens, step.slot_of_seq, step.start_pos
+    device = cu.get_device()
+    if device < 0 or slot.get_device() != device or start.get_device() != device or not (cu.is_contiguous() and slot.is_contiguous() and start.is_contiguous()):
+        raise KernelError(f"{what}: a step's tensors are contiguous and lie on the CUDA device")
+    return cu.data_ptr(), slot.data_ptr(), start.data_ptr()
 
 
 def rope_append_q8(qkv, out, step, pool, scales, tail, block_table, inv_freq, rotary_dim, pairs, n_heads, n_kv, head_dim, table=None,
@@ -2103,7 +2126,7 @@ def rope_append_q8(qkv, out, step, pool, scales, tail, block_table, inv_freq, ro
     A step of one token a sequence may be run again with the same or another token before the sequence goes on; one of several
     tokens may not where it completes a block and leaves another unfinished.
     `pairs`, `table`, `turn_scale`: as for rope_append."""
-    if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv) * head_dim or out.shape != qkv.shape or out.dtype != qkv.dtype:
+    if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv) * head_dim or out.shape != qkv.shape or out.dtype is not qkv.dtype:
         raise KernelError("rope_append_q8: qkv and out [N, (heads + 2 kv heads) * head_dim] of one dtype")
     _q8_line("rope_append_q8", pool, scales, n_kv, head_dim)
     _q8_step("rope_append_q8", step, block_table, tail, n_kv, head_dim, qkv.dtype)
@@ -2111,15 +2134,14 @@ def rope_append_q8(qkv, out, step, pool, scales, tail, block_table, inv_freq, ro
         raise KernelError("rope_append_q8: inv_freq must be float64 [rotary_dim / 2]")
     if table is not None and (table.dtype != torch.float32 or tuple(table.shape[1:]) != (rotary_dim // 2, 2)):
         raise KernelError("rope_append_q8: table must be float32 [positions, rotary_dim / 2, 2]")
-    _need_cuda(qkv, out, pool, scales, tail, block_table, inv_freq, table, step.cu_seqlens, step.slot_of_seq, step.start_pos)
-    _on_current("rope_append_q8", qkv, out, pool, scales, tail, block_table)
-    _aligned("rope_append_q8", qkv, out, pool, tail, table)
     old = None
     if step.max_q_len > 1:
         old = torch.empty((step.n_seqs, 2, n_kv, PAGE, head_dim), dtype=qkv.dtype, device=qkv.device)
-    _call("attention_q8", "blm_rope_append_q8", _ptr(qkv), _ptr(out), _code(qkv.dtype), _ptr(step.cu_seqlens), _ptr(step.slot_of_seq),
-          _ptr(step.start_pos), _ptr(block_table), block_table.shape[1], _ptr(inv_freq), rotary_dim, int(pairs), _ptr(table),
-          table.shape[0] if table is not None else 0, turn_scale, _ptr(pool), _ptr(scales), _ptr(tail), _ptr(old), step.n_seqs,
+    p_qkv, p_out, p_pool, p_tail, p_table, p_old, p_block, p_freq = _launch_ptrs(
+        "rope_append_q8", (qkv, out, pool, tail, table, old), (block_table, inv_freq if rotary_dim else None))
+    p_cu, p_slot, p_start = _step_ptrs("rope_append_q8", step)
+    _call("attention_q8", "blm_rope_append_q8", p_qkv, p_out, _code(qkv.dtype), p_cu, p_slot, p_start, p_block, block_table.shape[1], p_freq,
+          rotary_dim, int(pairs), p_table, table.shape[0] if table is not None else 0, turn_scale, p_pool, p_tail, p_old, step.n_seqs,
           step.max_q_len, n_heads, n_kv, head_dim, pool.shape[0], _stream())
     return old
 
@@ -2130,7 +2152,10 @@ def attention_q8(rotated, step, pool, scales, tail, old, block_table, out, n_hea
     sees the keys 0 .. p (the last `window` of them when window > 0): those of earlier blocks of PAGE positions in 8 bits, those of its
     own block unrounded, from the step's rows and, before them, from `old` (steps of one token a sequence: from `tail`).  So the result
     depends on the tokens, not on how they were cut into steps.  Scores, softmax and sums are fp32; out [N, n_heads * head_dim] in
-    rotated's dtype.  Rows of no sequence are left as they are."""
+    rotated's dtype.  Rows of no sequence are left as they are.  bfloat16 steps of one token a sequence with heads of 64 or 128 lanes
+    stream the pages to the tensor cores (the probabilities, times the values' scale, are rounded to bfloat16) and may cut a sequence's
+    pages over several blocks: step.max_kv_len (the longest sequence after the step, or a bound) sizes that, step.workspace lends the
+    scratch."""
     n = rotated.shape[0]
     if rotated.dim() != 2 or rotated.shape[1] != (n_heads + 2 * n_kv) * head_dim or tuple(out.shape) != (n, n_heads * head_dim) or out.dtype != rotated.dtype:
         raise KernelError("attention_q8: rotated [N, (heads + 2 kv heads) * head_dim] and out [N, heads * head_dim] of one dtype")
@@ -2140,13 +2165,19 @@ def attention_q8(rotated, step, pool, scales, tail, old, block_table, out, n_hea
         raise KernelError(f"attention_q8: a window of {window} keys")
     if step.max_q_len > 1 and (old is None or old.dtype != rotated.dtype or tuple(old.shape) != (step.n_seqs, 2, n_kv, PAGE, head_dim)):
         raise KernelError("attention_q8: a step of several tokens a sequence needs what rope_append_q8 returned")
-    _need_cuda(rotated, pool, scales, tail, old, block_table, out, step.cu_seqlens, step.slot_of_seq, step.start_pos)
-    _on_current("attention_q8", rotated, pool, scales, tail, old, block_table, out)
-    _aligned("attention_q8", rotated, pool, tail, old, out)
     found = tail if step.max_q_len <= 1 else old
-    _call("attention_q8", "blm_attention_q8", _ptr(rotated), _ptr(pool), _ptr(scales), _ptr(found), 1 if step.max_q_len <= 1 else 0,
-          _code(rotated.dtype), _ptr(block_table), block_table.shape[1], _ptr(step.cu_seqlens), _ptr(step.slot_of_seq), _ptr(step.start_pos),
-          _ptr(out), n, step.n_seqs, n_heads, n_kv, head_dim, pool.shape[0], int(window or 0), scale, _stream())
+    p_rot, p_pool, p_found, p_out, p_block = _launch_ptrs("attention_q8", (rotated, pool, found, out), (block_table,))
+    p_cu, p_slot, p_start = _step_ptrs("attention_q8", step)
+    code, window = _code(rotated.dtype), int(window or 0)
+    splits = _ask("attention_q8", "blm_attention_q8_splits", code, step.n_seqs, step.max_q_len, step.max_kv_len, n_heads, n_kv, head_dim, window)
+    scratch = None
+    if splits > 1:
+        floats = n * n_heads * splits * (head_dim + 2)
+        scratch = (step.workspace.scratch("attention_q8", floats) if step.workspace is not None
+                   else torch.empty(floats, dtype=torch.float32, device=rotated.device))
+    _call("attention_q8", "blm_attention_q8", p_rot, p_pool, p_found, 1 if step.max_q_len <= 1 else 0, code, p_block, block_table.shape[1], p_cu,
+          p_slot, p_start, p_out, n, step.n_seqs, n_heads, n_kv, head_dim, pool.shape[0], window, scale, step.max_q_len, step.max_kv_len,
+          _ptr(scratch), splits, status_word(rotated.device).data_ptr(), _stream(), kernels=2 if splits > 1 else 1)
 
 
 # -- weights in 4 bits -----------------------------------------------------------------------------------------------------------
@@ -2282,7 +2313,9 @@ def product_q4(w, x, out=None, add_into=None, swiglu=False):
         raise KernelError("product_q4: the result is [N, M] (gated: [N, M / 2]) with unit stride along its rows")
     if not (x.is_cuda and y.is_cuda and w.packed.is_cuda):
         raise KernelError("burn-lm_b200 kernels run on a CUDA device only; got a CPU tensor")
-    _on_current("product_q4", x, y, w.packed)
+    now = x.get_device()
+    if y.get_device() != now or w.packed.get_device() != now or now != (_current_device() if _current_device is not None else torch.cuda.current_device()):
+        raise KernelError("product_q4: x, the weight and the result lie on the current device")
     if k % 8 or x.stride(0) % 8 or x.data_ptr() % 16:
         wide = torch.zeros((n, -(-k // 64) * 64), dtype=torch.bfloat16, device=x.device)
         wide[:, :k] = x

@@ -119,7 +119,7 @@ class Batch:
                 assert np.array_equal(new_tail[slot], was[slot], equal_nan=True)
         # pages that no sequence holds are untouched
         loose = sorted(set(range(self.pool.shape[0])) - set(self.table.flatten().tolist()))
-        assert (self.pool[loose] == -77).all() and torch.isnan(self.scales[loose]).all()
+        assert (self.pool[loose][:, :, :-16] == -77).all() and torch.isnan(self.scales[loose]).all()
 
     def attend(self, entries, step, out, old, window=0, padding=0, check=True):
         n = out.shape[0]
@@ -383,3 +383,58 @@ def test_the_definition_is_the_reference():
     """The oracle itself: a block of known numbers."""
     whole, scale = in_eight(np.array([[127.0, -63.5], [0.5, 1.5]], np.float32))
     assert scale == 1.0 and np.array_equal(whole, [[127, -64], [0, 2]])
+
+
+@pytest.mark.parametrize("heads,n_kv,dim", [(32, 8, 64), (8, 8, 64), (24, 8, 128), (16, 2, 64), (12, 1, 64), (9, 1, 128), (32, 2, 128), (7, 1, 64)])
+@pytest.mark.parametrize("lengths,window", [((1500,), 0), ((700, 3, 64), 0), ((1, 63, 128, 129, 640), 0), ((1500, 90), 200), ((1300,), 1100), ((70,) * 40, 0)])
+def test_single_tokens_of_long_and_short_sequences(heads, n_kv, dim, lengths, window):
+    """Sequences of unequal lengths in one step: shares of one sequence, none of another; groups of up to 16 query heads; over a
+    block's end."""
+    if len(lengths) > 8 and heads > 12:
+        heads, n_kv = 8, 4
+    b = Batch(len(lengths), heads, n_kv, dim, BF16, max(lengths) + 8, seed=heads + len(lengths))
+    b.append([(s, n) for s, n in enumerate(lengths)], check=False)
+    for i in range(2):
+        step, out, old = b.append([(s, 1) for s in range(len(lengths))], check=False)
+        if i == 1:
+            step.max_kv_len = 4 * max(lengths)           # a bound, as a captured step has
+        b.attend([(s, 1) for s in range(len(lengths))], step, out, old, window)
+    K().check_status(torch.device("cuda:0"))
+
+
+def test_one_key_towers():
+    """One key far above hundreds, in each block and at the borders of the warps' shares: single tokens and a portion."""
+    heads, n_kv, dim = 8, 2, 64
+    for where in (0, 15, 16, 63, 64, 200, 383, 384, 400, 401):
+        b = Batch(1, heads, n_kv, dim, BF16, 512, seed=where)
+        qkv = b.rows(401)
+        rows = qkv.view(401, -1, dim)
+        rows[:, heads: heads + n_kv] *= 0.25
+        query = b.rows(1)
+        if where < 401:
+            rows[where, heads: heads + n_kv] = query.view(1, -1, dim)[0, [0, 4]]
+        b.append([(0, 401)], qkv=qkv, rot=0, check=False)
+        step, out, old = b.append([(0, 1)], qkv=query, rot=0, check=False)
+        b.attend([(0, 1)], step, out, old)
+
+
+def test_a_page_that_is_none():
+    """A table that names a page outside the pool: its keys are not seen, by either kernel, and nothing is read or written there."""
+    k = K()
+    for dtype, dim in ((F32, 64), (BF16, 64), (BF16, 128)):
+        b = Batch(1, 8, 2, dim, dtype, 256, seed=2)
+        b.append([(0, 190)], check=False)
+        pool = b.pool.clone()
+        b.table[0, 1] = -1 if dim == 64 else b.pool.shape[0]
+        step, out, old = b.append([(0, 1)], check=False)
+        o = torch.empty((1, 8 * dim), dtype=dtype, device=DEV)
+        k.attention_q8(out, step, b.pool, b.scales, b.tail, None, b.table, o, 8, 2, dim, b.scale)
+        # the reference with those keys taken out: out of reach of a softmax
+        line = Line(1, 2, dim)
+        line.append(0, np.concatenate([b.line.rows[0][:64], b.line.rows[0][128:]]))
+        want, _, _ = line.attend(0, out.view(1, -1, dim)[:, :8].double().cpu().numpy(), 126, b.scale)
+        assert np.abs(o.view(1, 8, dim).double().cpu().numpy() - want).max() < 0.03
+        b.table[0, 2] = -5                               # the block that fills up next has no page: nothing is stored
+        for _ in range(2):
+            b.append([(0, 1)], check=False)
+        assert torch.equal(b.pool, pool)
