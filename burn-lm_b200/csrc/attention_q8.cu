@@ -12,7 +12,8 @@
 // copied to `old` (one entry a sequence of the step) before the tail takes the last block's, and attention reads the step's own
 // rows from the rotated projection and the rows before them from `old`.  Steps of one token a sequence read the tail itself.
 //
-// Layout of a kv head's part of a page: keys [64][D] bytes; then values so that the decode kernel's tensor-core fragments are 16-byte
+// Layout of a kv head's part of a page: keys [64][D] bytes, where D is a multiple of 32 with the 16-byte pieces of odd rows exchanged
+// pairwise (so that the decode kernel's reads of neighbouring rows meet in no bank of shared memory); then values so that the decode kernel's tensor-core fragments are 16-byte
 // pieces: for keys 16 w + 4 t + e and lanes d = g (D / 8) + n the byte at
 //     w (16 Dp) + (n / 4) 512 + (4 g + t) 16 + (n % 4) 4 + e,     Dp = D rounded up to a multiple of 32:
 // thread (g, t) of a warp finds four lanes of four keys in 16 bytes; then 16 bytes whose first eight are the two scales, so that one
@@ -34,6 +35,8 @@ __host__ __device__ constexpr int number_bytes(int hd) { return kPage * (hd + pa
 __host__ __device__ constexpr int line_bytes(int hd) { return number_bytes(hd) + 16; }             // ... and its scales
 __device__ __forceinline__ const float2* scales_of(const void* line, int hd) { return reinterpret_cast<const float2*>((const signed char*)line + number_bytes(hd)); }
 
+// where lanes d .. d + 15 (d a multiple of 16) of key k lie, from the start of the keys
+__device__ __forceinline__ int key_piece(int k, int d, int hd) { return k * hd + (hd % 32 == 0 ? d ^ ((k & 1) << 4) : d); }
 // where the word of the values of keys k .. k + 3 (k a multiple of 4) and lane d lies, from the start of the values
 __device__ __forceinline__ int value_word(int k, int d, int hd) {
     const int per = hd / 8, g = d / per, n = d - g * per;
@@ -216,7 +219,7 @@ __device__ void store_block(const AppendArgs& a, const T* rows, int ld, bool val
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (value) *reinterpret_cast<unsigned*>(line + kPage * hd + value_word(key, d + e, hd)) = q[0][e] | q[1][e] << 8 | q[2][e] << 16 | q[3][e] << 24;
-            else *reinterpret_cast<unsigned*>(line + (key + e) * hd + d) = q[e][0] | q[e][1] << 8 | q[e][2] << 16 | q[e][3] << 24;
+            else *reinterpret_cast<unsigned*>(line + key_piece(key + e, d & ~15, hd) + (d & 15)) = q[e][0] | q[e][1] << 8 | q[e][2] << 16 | q[e][3] << 24;
         }
     }
 }
@@ -332,7 +335,7 @@ __global__ void __launch_bounds__(256) values_kernel(const signed char* __restri
     if (is) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            k[e] = *reinterpret_cast<const unsigned*>(line + (key + e) * hd + d);
+            k[e] = *reinterpret_cast<const unsigned*>(line + key_piece(key + e, d & ~15, hd) + (d & 15));
             v[e] = *reinterpret_cast<const unsigned*>(line + kPage * hd + value_word(key, d + e, hd));
         }
     }
@@ -419,9 +422,8 @@ __global__ void __launch_bounds__(kGeneralWarps * 32) attend_general_kernel(cons
                     for (int e = 0; e < 8; ++e) sum = fmaf(q[d + e], x[e], sum);
                 }
             } else {
-                const signed char* kr = line + (key % kPage) * hd;
                 for (int d = 0; d < hd; d += 16) {
-                    const int4 w = *reinterpret_cast<const int4*>(kr + d);
+                    const int4 w = *reinterpret_cast<const int4*>(line + key_piece(key % kPage, d, hd));
                     const unsigned char* x = reinterpret_cast<const unsigned char*>(&w);
 #pragma unroll
                     for (int e = 0; e < 16; ++e) sum = fmaf(q[d + e], (float)((int)x[e] - 128), sum);
@@ -483,9 +485,11 @@ __global__ void __launch_bounds__(kGeneralWarps * 32) attend_general_kernel(cons
 // ---- single tokens -----------------------------------------------------------------------------------------------------------
 // One new token a sequence, bfloat16, heads of 64 or 128 lanes: a block owns (share of the sequence's pages, up to eight query heads
 // of a kv head, sequence).  Its producer warp streams the pages into a ring in shared memory, one bulk copy of 8 or 16 KB each (keys,
-// values and scales of the kv head), completion on mbarriers; eight consumer warps, WPP of them to a page, form scores and sums with
-// the query heads as rows of 16-row tensor-core tiles.  What bounds it, beside the memory, is the instructions that turn bytes into
+// values and scales of the kv head), completion on mbarriers; four consumer warps, WPP of them to a page, form scores and sums with
+// 16 keys (lanes) by the query heads a tensor-core tile.  What bounds it, beside the memory, is the instructions that turn bytes into
 // operands, so:
+//   * keys and lanes are the 16 rows of a product and the heads its 8 columns (with the heads as rows half of a product would be empty:
+//     20 to 30 % slower); probabilities change their place from one product's result to the other's operand by movmatrix;
 //   * a thread reads its bytes as 16-byte pieces that hold its fragments, and everything is in half precision: a byte behind 0x64 is
 //     1024 + 128 + q exactly, one permutation for two numbers;
 //   * of the keys the 1152 is not taken off: a score's sum starts at -1152 times the sum of its query, which is exact in what it takes
@@ -496,13 +500,13 @@ __global__ void __launch_bounds__(kGeneralWarps * 32) attend_general_kernel(cons
 //     product with the whole numbers needs no scale, and the sum of the probabilities gets p' / vs.  p' is rounded to half precision
 //     times 2^12 (11 bits from the largest down to 2^-26 of it).
 // Warps keep their own running maximum, sum and output and merge at the end; shares of a sequence meet in a second kernel.  The own
-// block's keys, unrounded, are read straight from the tail and the step's rows by the first four warps of the last share, in bfloat16,
+// block's keys, unrounded, are read straight from the tail and the step's rows by the four warps of the last share, in bfloat16,
 // while the first pages are on their way.  Waits are bounded; one that runs out leaves a code in the status word.
 struct TokenArgs {
     AttendArgs a;
     float* part_acc;             // [N, n_heads, n_splits, hd]
     float* part_ml;              // [N, n_heads, n_splits, 2]: maximum (base 2) and sum
-    int n_splits, head_tiles, heads_a_tile, pages_per_split, n_stages;
+    int n_splits, head_tiles, heads_a_tile, pages_per_split;
     int* status;
 };
 enum { Q8_TIMEOUT_PAGE = 51, Q8_TIMEOUT_FREE = 52 };
@@ -538,18 +542,24 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, unsigned b
                  "r"(smem_u32(bar))
                  : "memory");
 }
-// rows 8 .. 15 of A are zero
-__device__ __forceinline__ void mma_bf16(float (&c)[4], unsigned a0, unsigned a2, unsigned b0, unsigned b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1));
+template <bool HALF>
+__device__ __forceinline__ void mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    if (HALF)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_half(float (&c)[4], unsigned a0, unsigned a2, unsigned b0, unsigned b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1));
+// an 8 x 8 matrix of 16-bit numbers, a row's two a lane, transposed
+__device__ __forceinline__ unsigned transposed(unsigned v) {
+    unsigned r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+    return r;
 }
 // Bytes LO and LO + 1 of a word as two half-precision numbers, 1152 too large, and without that.
 template <int LO>
@@ -581,39 +591,45 @@ __host__ __device__ inline int active_splits(int n_pages, int n_splits, int page
 }
 
 constexpr float kPShift = 12.f;          // probabilities are kept times 2^12
-constexpr int kTokenWarps = 8;           // consumers of a block
 
-// What a warp knows of its rows: thread (g, t) has head g of the tile.
+// What a warp knows of its eight heads: thread (g, t) has heads 2 t and 2 t + 1, of the sums lanes g HD / 8 + n, n = 0 .. HD / 8 - 1:
+// o[n / 2][n % 2 * 2 + head].
 template <int HD>
 struct TokenState {
-    float o[HD / 8][4], m, l;
-    // a new maximum `top` of the thread's scores of row g (their own, or any of the row): moves the reference and gives what is to be
-    // added to a score in the exponent
-    __device__ __forceinline__ float refer(float top) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float now = fmaxf(m, top), ref = now == -INFINITY ? 0.f : now;
-        const float alpha = ex2(m - ref);
-        m = now;
-        if (__any_sync(0xffffffffu, alpha != 1.f)) {
-            l *= alpha;
+    float o[HD / 16][4], m[2], l[2];
+    // the thread's largest new scores of its two heads: moves the references and gives what is to be added to a score in the exponent
+    __device__ __forceinline__ void refer(float top0, float top1, float& shift0, float& shift1) {
 #pragma unroll
-            for (int n = 0; n < HD / 8; ++n) {
-                o[n][0] *= alpha;
-                o[n][1] *= alpha;
+        for (int x = 4; x < 32; x *= 2) {
+            top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, x));
+            top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, x));
+        }
+        const float now0 = fmaxf(m[0], top0), now1 = fmaxf(m[1], top1);
+        const float ref0 = now0 == -INFINITY ? 0.f : now0, ref1 = now1 == -INFINITY ? 0.f : now1;
+        if (__any_sync(0xffffffffu, now0 != m[0] || now1 != m[1])) {
+            const float a0 = ex2(m[0] - ref0), a1 = ex2(m[1] - ref1);
+            l[0] *= a0;
+            l[1] *= a1;
+#pragma unroll
+            for (int n = 0; n < HD / 16; ++n) {
+                o[n][0] *= a0; o[n][1] *= a1; o[n][2] *= a0; o[n][3] *= a1;
             }
         }
-        return kPShift - ref;
+        m[0] = now0;
+        m[1] = now1;
+        shift0 = kPShift - ref0;
+        shift1 = kPShift - ref1;
     }
 };
 
+constexpr int kTokenWarps = 4;           // consumers of a block
 template <int HD, int WPP>
 __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(const TokenArgs ta) {
     constexpr int WARPS = kTokenWarps, NG = WARPS / WPP, CH = 4 / WPP;   // groups of warps, 16-key chunks of a page that a warp has
+    constexpr int S = NG;                                                // pages of the ring; a stage always serves the same group
     constexpr int KS = HD / 16, PIECES = HD / 64;                        // PIECES: 16-byte pieces of a key row in a thread
     constexpr unsigned STAGE = line_bytes(HD);
     const AttendArgs& a = ta.a;
-    const int S = ta.n_stages;                                           // a multiple of NG: a stage always serves the same group
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* ring = smem_raw;                                      // [S][keys, values, scales]
     float* sm_acc = reinterpret_cast<float*>(ring);                      // [WARPS][8][HD], when the ring has been read
@@ -660,9 +676,14 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
                     continue;
                 }
                 ++i;
-                // (a page that the pool does not have: page 0's bytes; the consumers know as well)
+                unsigned char* stage = ring + (size_t)s * STAGE;
+                if (page < 0) {                          // none of the pool's: the consumers know it by a scale below zero
+                    *const_cast<float2*>(scales_of(stage, HD)) = make_float2(0.f, -1.f);
+                    mbar_arrive(full + s);
+                    continue;
+                }
                 mbar_expect_tx(full + s, STAGE);
-                bulk_copy(ring + (size_t)s * STAGE, a.pool + ((size_t)max(page, 0) * a.n_kv + kvh) * STAGE, STAGE, full + s);
+                bulk_copy(stage, a.pool + ((size_t)page * a.n_kv + kvh) * STAGE, STAGE, full + s);
             }
         }
         // every copy has landed before the ring is used otherwise or the block ends, whatever became of the consumers
@@ -682,14 +703,14 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
             }
         }
         TokenState<HD> st;
-        st.m = -INFINITY;
-        st.l = 0.f;
+        st.m[0] = st.m[1] = -INFINITY;
+        st.l[0] = st.l[1] = 0.f;
 #pragma unroll
-        for (int n = 0; n < HD / 8; ++n)
+        for (int n = 0; n < HD / 16; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) st.o[n][e] = 0.f;
 
-        if (split == active - 1 && warp < 4 && warp * 16 <= pos % kPage) {
+        for (int quarter = warp; split == active - 1 && quarter < 4 && quarter * 16 <= pos % kPage; quarter += WARPS) {
             // ---- the own block: 16 of its rows, unrounded ----
             const __nv_bfloat16* found = reinterpret_cast<const __nv_bfloat16*>(a.found) + ((size_t)slot * 2 * a.n_kv + kvh) * kPage * HD;
             auto row = [&](int k, int which) -> const __nv_bfloat16* {            // k of the own block, at most pos
@@ -697,55 +718,48 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
                 return found + ((size_t)which * a.n_kv * kPage + k) * HD;
             };
             const int own_lo = max(0, key_lo - mine * kPage), own_hi = pos % kPage;      // the keys seen
-            float sc[2][2];
+            const int k0 = quarter * 16 + 4 * (g >> 1) + (g & 1);                        // the thread's rows: k0 and k0 + 2
+            const bool seen0 = k0 <= own_hi && k0 >= own_lo, seen2 = k0 + 2 <= own_hi && k0 + 2 >= own_lo;
+            const uint4* r0 = reinterpret_cast<const uint4*>(row(min(k0, own_hi), 0) + t * (HD / 4));
+            const uint4* r2 = reinterpret_cast<const uint4*>(row(min(k0 + 2, own_hi), 0) + t * (HD / 4));
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                const int k = warp * 16 + 4 * (g >> 1) + 2 * i + (g & 1);
-                const bool seen = k <= own_hi && k >= own_lo;
-                const uint4* kr = reinterpret_cast<const uint4*>(row(min(k, own_hi), 0) + t * (HD / 4));
-#pragma unroll
-                for (int j = 0; j < KS / 2; ++j) {
-                    const uint4 v = seen ? kr[j] : make_uint4(0u, 0u, 0u, 0u);
-                    mma_bf16(c, qf[2 * j][0], qf[2 * j][1], v.x, v.y);
-                    mma_bf16(c, qf[2 * j + 1][0], qf[2 * j + 1][1], v.z, v.w);
-                }
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int key = warp * 16 + 4 * t + 2 * i + e;
-                    sc[i][e] = key <= own_hi && key >= own_lo ? c[e] * a.scale_log2e : -INFINITY;
-                }
+            for (int j = 0; j < KS / 2; ++j) {
+                const uint4 x = seen0 ? r0[j] : make_uint4(0u, 0u, 0u, 0u), y = seen2 ? r2[j] : make_uint4(0u, 0u, 0u, 0u);
+                mma<false>(c, x.x, y.x, x.y, y.y, qf[2 * j][0], qf[2 * j][1]);
+                mma<false>(c, x.z, y.z, x.w, y.w, qf[2 * j + 1][0], qf[2 * j + 1][1]);
             }
-            const float shift = st.refer(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])));
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int e = 0; e < 4; ++e) c[e] = (e < 2 ? seen0 : seen2) ? c[e] * a.scale_log2e : -INFINITY;
+            float shift0, shift1;
+            st.refer(fmaxf(c[0], c[2]), fmaxf(c[1], c[3]), shift0, shift1);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    sc[i][e] = ex2(sc[i][e] + shift);
-                    st.l += sc[i][e];
-                }
-            const unsigned p01 = pack_bf16(sc[0][0], sc[0][1]), p23 = pack_bf16(sc[1][0], sc[1][1]);
-            // lanes g HD / 8 .. + HD / 8 of the thread's four keys
+            for (int e = 0; e < 4; ++e) {
+                c[e] = ex2(c[e] + (e & 1 ? shift1 : shift0));
+                st.l[e & 1] += c[e];
+            }
+            const unsigned b0 = transposed(pack_bf16(c[0], c[1])), b1 = transposed(pack_bf16(c[2], c[3]));
+            // lanes g HD / 8 .. + HD / 8 of keys 4 t .. 4 t + 3
 #pragma unroll
             for (int j = 0; j < HD / 64; ++j) {
                 uint4 v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int key = warp * 16 + 4 * t + e;
+                    const int key = quarter * 16 + 4 * t + e;
                     const bool seen = key <= own_hi && key >= own_lo;
                     v[e] = seen ? reinterpret_cast<const uint4*>(row(min(key, own_hi), 1) + g * (HD / 8))[j] : make_uint4(0u, 0u, 0u, 0u);
                 }
 #pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    const unsigned w0 = n < 2 ? v[0].x : n < 4 ? v[0].y : n < 6 ? v[0].z : v[0].w, w1 = n < 2 ? v[1].x : n < 4 ? v[1].y : n < 6 ? v[1].z : v[1].w;
-                    const unsigned w2 = n < 2 ? v[2].x : n < 4 ? v[2].y : n < 6 ? v[2].z : v[2].w, w3 = n < 2 ? v[3].x : n < 4 ? v[3].y : n < 6 ? v[3].z : v[3].w;
-                    mma_bf16(st.o[8 * j + n], p01, p23, __byte_perm(w0, w1, n & 1 ? 0x7632 : 0x5410), __byte_perm(w2, w3, n & 1 ? 0x7632 : 0x5410));
+                for (int n = 0; n < 4; ++n) {
+                    const unsigned w0 = n == 0 ? v[0].x : n == 1 ? v[0].y : n == 2 ? v[0].z : v[0].w, w1 = n == 0 ? v[1].x : n == 1 ? v[1].y : n == 2 ? v[1].z : v[1].w;
+                    const unsigned w2 = n == 0 ? v[2].x : n == 1 ? v[2].y : n == 2 ? v[2].z : v[2].w, w3 = n == 0 ? v[3].x : n == 1 ? v[3].y : n == 2 ? v[3].z : v[3].w;
+                    mma<false>(st.o[4 * j + n], __byte_perm(w0, w1, 0x5410), __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x5410), __byte_perm(w2, w3, 0x7632), b0, b1);
                 }
             }
         }
 
         // the queries in half precision: times a power of two that brings the row's largest lane to 16 .. 32
-        float start, to_log2;
+        float start0, start1, to_log2_0, to_log2_1;         // of the thread's two heads
         {
             float q[KS][4], top = 0.f, sum = 0.f;
 #pragma unroll
@@ -772,18 +786,19 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
                 }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            start = -1152.f * sum;
-            to_log2 = a.scale_log2e / factor;
+            // (until here the lanes of a quad have head g)
+            start0 = -1152.f * __shfl_sync(0xffffffffu, sum, 8 * t);
+            start1 = -1152.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+            to_log2_0 = a.scale_log2e / __shfl_sync(0xffffffffu, factor, 8 * t);
+            to_log2_1 = a.scale_log2e / __shfl_sync(0xffffffffu, factor, 8 * t + 4);
         }
 
         // ---- the pages: this warp's group takes every NG-th, the warp CH chunks of 16 keys of each ----
         const int grp = warp / WPP, part = warp % WPP;
-        int s = grp - NG;
-        unsigned phase = 0;
+        const int s = grp;
+        unsigned phase = 1;
         for (int pg = pg_lo + grp; pg < pg_hi; pg += NG) {
-            s += NG;
-            if (s >= S) { s -= S; phase ^= 1; }
-            const bool none = page_of(a.block_table, a.table_stride, slot, pg, a.n_pages) < 0;
+            phase ^= 1;
             if (!mbar_wait(full + s, phase)) {
                 if (lane == 0) atomicCAS(ta.status, 0, Q8_TIMEOUT_PAGE);
                 break;
@@ -793,74 +808,80 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
             const float2 scale = *scales_of(keys, HD);
             // (a block whose values are all next to zero: any scale will do; a NaN stays one)
             const float vs = scale.y < 0x1p-100f ? 0x1p-100f : scale.y, lv = __log2f(vs);
-            const float factor = to_log2 * scale.x;
-            float sc[CH][2][2];
-            float top = -INFINITY;
+            const float f0 = to_log2_0 * scale.x, f1 = to_log2_1 * scale.x;
+            float sc[CH][4], top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-            for (int ch = 0; ch < CH; ++ch)
+            for (int ch = 0; ch < CH; ++ch) {
+                // the thread's rows of the chunk: keys k0 and k0 + 2
+                float (&c)[4] = sc[ch];
+                c[0] = c[2] = start0;
+                c[1] = c[3] = start1;
+                const int k0 = (part * CH + ch) * 16 + 4 * (g >> 1) + (g & 1);
+                const uint4* kr = reinterpret_cast<const uint4*>(keys + k0 * HD);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float c[4] = {start, start, 0.f, 0.f};
-                    const int k = (part * CH + ch) * 16 + 4 * (g >> 1) + 2 * i + (g & 1);
-                    const uint4* kr = reinterpret_cast<const uint4*>(keys + k * HD + t * (HD / 4));
-                    uint4 v[PIECES];
-                    // (with two pieces a thread, odd rows read theirs in the other order: no two threads of a phase meet in a bank)
+                for (int j = 0; j < PIECES; ++j) {
+                    const uint4 x = kr[(t * PIECES + j) ^ (g & 1)], y = kr[2 * HD / 16 + ((t * PIECES + j) ^ (g & 1))];
+                    const unsigned xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-                    for (int j = 0; j < PIECES; ++j) v[j] = kr[PIECES == 1 ? 0 : j ^ (g & 1)];
-                    if (PIECES == 2 && (g & 1)) { const uint4 x = v[0]; v[0] = v[PIECES - 1]; v[PIECES - 1] = x; }
-#pragma unroll
-                    for (int j = 0; j < PIECES; ++j) {
-                        const unsigned w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) mma_half(c, qf[4 * j + x][0], qf[4 * j + x][1], biased_two<0>(w[x]), biased_two<2>(w[x]));
-                    }
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        sc[ch][i][e] = fmaf(c[e], factor, lv);
-                        if (pg == pg_first && pg * kPage + (part * CH + ch) * 16 + 4 * t + 2 * i + e < key_lo) sc[ch][i][e] = -INFINITY;      // the window's edge
-                        top = fmaxf(top, sc[ch][i][e]);
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        mma<true>(c, biased_two<0>(xw[i]), biased_two<0>(yw[i]), biased_two<2>(xw[i]), biased_two<2>(yw[i]), qf[4 * j + i][0], qf[4 * j + i][1]);
                 }
-            if (!none) {
-                const float shift = st.refer(top);
-                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[e] = fmaf(c[e], e & 1 ? f1 : f0, lv);
+                top0 = fmaxf(top0, fmaxf(c[0], c[2]));
+                top1 = fmaxf(top1, fmaxf(c[1], c[3]));
+            }
+            if (pg * kPage < key_lo) {                   // the window's edge
+                top0 = top1 = -INFINITY;
+#pragma unroll
+                for (int ch = 0; ch < CH; ++ch)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (pg * kPage + (part * CH + ch) * 16 + 4 * (g >> 1) + (g & 1) + (e & 2) < key_lo) sc[ch][e] = -INFINITY;
+                        if (e & 1) top1 = fmaxf(top1, sc[ch][e]); else top0 = fmaxf(top0, sc[ch][e]);
+                    }
+            }
+            if (!(scale.y < 0.f)) {
+                float shift0, shift1, sum0 = 0.f, sum1 = 0.f;
+                st.refer(top0, top1, shift0, shift1);
                 const float to_sum = 1.f / vs;
                 const uint4* vr = reinterpret_cast<const uint4*>(values + part * CH * (16 * HD)) + lane;
 #pragma unroll
                 for (int ch = 0; ch < CH; ++ch) {
-                    float p[2][2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            p[i][e] = ex2(sc[ch][i][e] + shift);
-                            sum += p[i][e];
-                        }
-                    const unsigned p01 = pack_half(p[0][0], p[0][1]), p23 = pack_half(p[1][0], p[1][1]);
+                    const float p0 = ex2(sc[ch][0] + shift0), p1 = ex2(sc[ch][1] + shift1), p2 = ex2(sc[ch][2] + shift0), p3 = ex2(sc[ch][3] + shift1);
+                    sum0 += p0 + p2;
+                    sum1 += p1 + p3;
+                    const unsigned b0 = transposed(pack_half(p0, p1)), b1 = transposed(pack_half(p2, p3));
 #pragma unroll
                     for (int j = 0; j < HD / 32; ++j) {
                         const uint4 v = vr[(ch * (HD / 32) + j) * 32];
-                        const unsigned w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) mma_half(st.o[4 * j + x], p01, p23, two_of<0>(w[x]), two_of<2>(w[x]));
+                        mma<true>(st.o[2 * j], two_of<0>(v.x), two_of<0>(v.y), two_of<2>(v.x), two_of<2>(v.y), b0, b1);
+                        mma<true>(st.o[2 * j + 1], two_of<0>(v.z), two_of<0>(v.w), two_of<2>(v.z), two_of<2>(v.w), b0, b1);
                     }
                 }
-                st.l = fmaf(sum, to_sum, st.l);          // this lane's share
+                st.l[0] = fmaf(sum0, to_sum, st.l[0]);   // this thread's share
+                st.l[1] = fmaf(sum1, to_sum, st.l[1]);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty + s);
         }
-        st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
-        st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
-        if (t == 0) { sm_m[warp * 8 + g] = st.m; sm_l[warp * 8 + g] = st.l; }
+#pragma unroll
+        for (int x = 4; x < 32; x *= 2) {
+            st.l[0] += __shfl_xor_sync(0xffffffffu, st.l[0], x);
+            st.l[1] += __shfl_xor_sync(0xffffffffu, st.l[1], x);
+        }
+        if (g == 0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) { sm_m[warp * 8 + 2 * t + h] = st.m[h]; sm_l[warp * 8 + 2 * t + h] = st.l[h]; }
+        }
         // the ring is free when all consumers and the producer are here (named barrier: all threads of the block)
         asm volatile("bar.sync 1, %0;\n" ::"r"((WARPS + 1) * 32) : "memory");
-        // lanes 2 t HD / 8 + n and (2 t + 1) HD / 8 + n of row g
 #pragma unroll
-        for (int n = 0; n < HD / 8; n += 4) {
-            *reinterpret_cast<float4*>(sm_acc + (warp * 8 + g) * HD + 2 * t * (HD / 8) + n) = make_float4(st.o[n][0], st.o[n + 1][0], st.o[n + 2][0], st.o[n + 3][0]);
-            *reinterpret_cast<float4*>(sm_acc + (warp * 8 + g) * HD + (2 * t + 1) * (HD / 8) + n) = make_float4(st.o[n][1], st.o[n + 1][1], st.o[n + 2][1], st.o[n + 3][1]);
-        }
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = 0; n < HD / 16; n += 2)
+                *reinterpret_cast<float4*>(sm_acc + (warp * 8 + 2 * t + h) * HD + g * (HD / 8) + 2 * n) =
+                    make_float4(st.o[n][h], st.o[n][2 + h], st.o[n + 1][h], st.o[n + 1][2 + h]);
     }
     if (warp == WARPS) asm volatile("bar.sync 1, %0;\n" ::"r"((WARPS + 1) * 32) : "memory");
     __syncthreads();
@@ -937,7 +958,7 @@ __global__ void __launch_bounds__(128) merge_kernel(const TokenArgs ta) {
 }
 
 // The plan of a step of single tokens, the same for the caller that provides the scratch and for the launch.
-struct TokenPlan { int splits, pages_per_split, stages, wpp, head_tiles, heads_a_tile; };
+struct TokenPlan { int splits, pages_per_split, wpp, head_tiles, heads_a_tile; };
 static TokenPlan plan_tokens(int n_seqs, int n_heads, int n_kv, int hd, int max_kv_len, int window) {
     TokenPlan p;
     const int group = n_heads / n_kv, sms = blm_sm_count();
@@ -947,28 +968,30 @@ static TokenPlan plan_tokens(int n_seqs, int n_heads, int n_kv, int hd, int max_
     if (window > 0 && pages > window / kPage + 2) pages = window / kPage + 2;
     if (pages < 1) pages = 1;
     const int rows = n_seqs * n_kv * p.head_tiles;       // blocks of an unsplit step
-    // Walks of more than 8 pages are cut, as far as that fills the SMs about twice.
+    // Walks of more than 8 pages are cut, as far as that fills the SMs about twice (8 sequences of 2,000 tokens, heads of 128: 14.9 us in
+    // 4 shares, 18.6 in 8, 19.5 in one; one sequence of 32,000: 20.1 us in 37, 24.6 in 56).
     const int by_length = (pages + 7) / 8, to_fill = (2 * sms + rows - 1) / rows;
     p.splits = by_length < to_fill ? by_length : to_fill;
     if (p.splits > 64) p.splits = 64;
     if (p.splits < 1) p.splits = 1;
     const int blocks = rows * p.splits, each = (pages + p.splits - 1) / p.splits;
     p.pages_per_split = blocks > 2 * sms ? each : 1;
-    p.wpp = 2;
-    const int groups = kTokenWarps / p.wpp;
-    p.stages = (hd == 64 ? 8 : 4) / groups * groups;
+    // Four warps with a page each and a ring of four, three (heads of 128 lanes) or four blocks an SM; where three an SM are too few for
+    // all the blocks of heads of 128, two warps to a page and a ring of two pages, four an SM.  Measured, 64 sequences of 1,000 tokens
+    // with heads of 128: 30.4 us against 37.0; 8 of 8,000: 30.6 against 36.9.  Eight warps a block: 39.3 and 32.6 us.
+    p.wpp = hd == 128 && blocks > 3 * sms ? 2 : 1;
     return p;
 }
 
 template <int HD, int WPP>
 static int launch_tokens_as(const TokenArgs& ta, cudaStream_t stream) {
     const dim3 grid(ta.n_splits, ta.a.n_kv * ta.head_tiles, ta.a.n_seqs);
-    const size_t smem = (size_t)ta.n_stages * (line_bytes(HD) + 16) + (size_t)kTokenWarps * 8 * 2 * 4;
+    constexpr size_t smem = (size_t)kTokenWarps / WPP * (line_bytes(HD) + 16) + (size_t)kTokenWarps * 8 * 2 * 4;
     static bool opted_in[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !opted_in[dev]) {
-        if (cudaFuncSetAttribute(attend_token_kernel<HD, WPP>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024) != cudaSuccess)
+        if (cudaFuncSetAttribute(attend_token_kernel<HD, WPP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
             return blm_fail(BLM_CUDA_ERROR, "attention_q8: %s", cudaGetErrorString(cudaGetLastError()));
         if (dev >= 0 && dev < 64) opted_in[dev] = true;
     }
@@ -1052,8 +1075,9 @@ BLM_API int blm_attention_q8(const void* rotated, const void* pool, const void* 
         const TokenPlan p = plan_tokens(n_seqs, n_heads, n_kv, hd, max_kv_len, window);
         BLM_REQUIRE(p.splits == splits && (splits == 1 || scratch != nullptr), "attention_q8: scratch for %d shares, the step has %d", splits, p.splits);
         const TokenArgs ta{a, scratch, scratch ? scratch + (size_t)n_tokens * n_heads * splits * hd : nullptr, p.splits, p.head_tiles, p.heads_a_tile,
-                           p.pages_per_split, p.stages, status};
-        return hd == 64 ? launch_tokens_as<64, 2>(ta, stream) : launch_tokens_as<128, 2>(ta, stream);
+                           p.pages_per_split, status};
+        if (hd == 64) return launch_tokens_as<64, 1>(ta, stream);
+        return p.wpp == 1 ? launch_tokens_as<128, 1>(ta, stream) : launch_tokens_as<128, 2>(ta, stream);
     }
     const dim3 grid(n_heads * n_tokens);
     if (dtype == BLM_F32) blm_launch_dependent(attend_general_kernel<float>, grid, dim3(kGeneralWarps * 32), 0, stream, a);

@@ -2071,8 +2071,12 @@ def q8_write(pool, scales, pages, keys, key_scales, values, value_scales) -> Non
             or tuple(key_scales.shape) != (p, n_kv) or tuple(value_scales.shape) != (p, n_kv)):
         raise KernelError(f"q8_write: keys and values int8 [P, kv heads, {PAGE}, head_dim], scales [P, kv heads], a page for each")
     line = torch.full((p, n_kv, pool.shape[2]), -128, dtype=torch.int8, device=pool.device)      # a byte holds the number + 128
-    line[:, :, : PAGE * head_dim] = (keys ^ -128).reshape(p, n_kv, -1)
-    line[:, :, PAGE * head_dim:][:, :, _q8_value_places(head_dim, pool.device).reshape(-1)] = (values ^ -128).reshape(p, n_kv, -1)
+    k = (keys ^ -128).reshape(p, n_kv, PAGE // 2, 2, head_dim)
+    if head_dim % 32 == 0:                               # the 16-byte pieces of odd rows are exchanged pairwise
+        odd = k[:, :, :, 1].reshape(p, n_kv, PAGE // 2, head_dim // 32, 2, 16).flip(4)
+        k = torch.stack([k[:, :, :, 0], odd.reshape(p, n_kv, PAGE // 2, head_dim)], dim=3)
+    line[:, :, : PAGE * head_dim] = k.reshape(p, n_kv, PAGE * head_dim)
+    line[:, :, PAGE * head_dim:][:, :, _q8_value_places(head_dim, pool.device).reshape(-1)] = (values ^ -128).reshape(p, n_kv, PAGE * head_dim)
     at = pages.to(torch.int64)
     pool[at] = line
     scales[at] = torch.stack([key_scales, value_scales], dim=2).to(torch.float32)

@@ -76,6 +76,9 @@ def test_writing_refuses():
     eight, s = torch.zeros(2, 2, 64, 32, dtype=torch.int8), torch.zeros(2, 2)
     pages = torch.tensor([0, 2])
     K.q8_write(pool, scales, pages, eight, s, eight, s)
+    before = pool.clone()
+    K.q8_write(pool, scales, pages[:0], eight[:0], s[:0], eight[:0], s[:0])     # no block at all
+    assert torch.equal(pool, before)
     for bad in (dict(keys=eight.float()), dict(values=eight[:1]), dict(ks=s[:1]), dict(pages=pages[:1])):
         a = dict(pages=pages, keys=eight, ks=s, values=eight, vs=s)
         a.update(bad)
