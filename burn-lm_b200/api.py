@@ -24,17 +24,20 @@ class LanguageModel:
 
     def __init__(self, folder: Optional[str], dtype: str = "bfloat16", max_seq_len: int = 8192, max_batch: int = 8,
                  max_tokens: Optional[int] = None, device: str = "cuda:0", decode_ahead: bool = False,
-                 random_config: Optional[dict] = None, random_seed: int = 0):
+                 random_config: Optional[dict] = None, random_seed: int = 0, cache: str = "compute", weights: str = "stored"):
         """`folder`: a model folder; or None with `random_config` (a config.json dict) and `random_seed`: the model
         is then built with random weights drawn on the device (see model.random_model).
         `decode_ahead`: greedy generation enqueues the step after the one it waits for (fed on the device), so
         the GPU does not idle while the host looks at a step's tokens; off, every step brings its tokens from
-        the host.  The tokens are the same either way."""
+        the host.  The tokens are the same either way.
+        `cache` "int8": keys and values are kept in 8 bits, with a scale for every block of 64 positions and head (a sequence's unfinished
+        block unrounded); `weights` "int4": the layers' products hold their weights in 4 bits, with a scale for every 64 places."""
         self.folder, self.dtype, self.device = folder, dtype, device
         self.decode_ahead = decode_ahead
         if (folder is None) == (random_config is None):
             raise ValueError("a LanguageModel takes a folder, or a configuration to fill with random weights")
         self.random_config, self.random_seed = random_config, random_seed
+        self.cache, self.weights = cache, weights
         self.max_seq_len, self.max_batch, self.max_tokens = max_seq_len, max_batch, max_tokens
         self.engine: Optional[Engine] = None
         self.loop: Optional[GenerationLoop] = None
@@ -52,9 +55,9 @@ class LanguageModel:
         if self.engine is None:
             t0 = time.perf_counter()
             if self.folder is not None:
-                model = load_model(self.folder, self.dtype, self.device)
+                model = load_model(self.folder, self.dtype, self.device, self.cache, self.weights)
             else:
-                model = random_model(self.random_config, self.random_seed, self.dtype, self.device)
+                model = random_model(self.random_config, self.random_seed, self.dtype, self.device, cache=self.cache, weights=self.weights)
             seq = min(self.max_seq_len, model.plan.max_positions)
             tokens = self.max_tokens or -(-seq // PAGE) * PAGE * self.max_batch
             self.engine = Engine(model, max_tokens=tokens, max_seqs=max(self.max_batch, 1), max_seq_len=seq)
@@ -105,13 +108,15 @@ class LanguageModel:
 
 
 def load(folder: str, dtype: str = "bfloat16", max_seq_len: int = 8192, max_batch: int = 8,
-         max_tokens: Optional[int] = None, device: str = "cuda:0", decode_ahead: bool = False) -> LanguageModel:
+         max_tokens: Optional[int] = None, device: str = "cuda:0", decode_ahead: bool = False, cache: str = "compute",
+         weights: str = "stored") -> LanguageModel:
     """Load the model a folder's config.json names; see LanguageModel."""
-    return LanguageModel(folder, dtype, max_seq_len, max_batch, max_tokens, device, decode_ahead).load()
+    return LanguageModel(folder, dtype, max_seq_len, max_batch, max_tokens, device, decode_ahead, cache=cache, weights=weights).load()
 
 
 def load_random(config: dict, seed: int = 0, dtype: str = "bfloat16", max_seq_len: int = 8192, max_batch: int = 8,
-                max_tokens: Optional[int] = None, device: str = "cuda:0") -> LanguageModel:
+                max_tokens: Optional[int] = None, device: str = "cuda:0", cache: str = "compute", weights: str = "stored") -> LanguageModel:
     """A model of the configuration `config` (a config.json dict, e.g. config.preset("llama3_2_3b")) with random
     weights drawn on the device from `seed`."""
-    return LanguageModel(None, dtype, max_seq_len, max_batch, max_tokens, device, random_config=config, random_seed=seed).load()
+    return LanguageModel(None, dtype, max_seq_len, max_batch, max_tokens, device, random_config=config, random_seed=seed, cache=cache,
+                         weights=weights).load()

@@ -23,7 +23,7 @@ from typing import Optional
 
 import torch
 
-from ..kernels import PAGE
+from ..kernels import PAGE, q8_pool
 from .allocators import CacheError, CacheFull, ContextLengthExceeded, IdAllocator
 
 
@@ -43,12 +43,20 @@ class CacheView:
                                             # something of its own in the same state block puts its mixer behind it)
     window: Optional[int] = None
     keep_first: int = 0
+    scales: Optional[torch.Tensor] = None   # kv in 8 bits (the pool is then as kernels.q8_pool makes it): the view of its scales, and
+    tail: Optional[torch.Tensor] = None     # [max_seqs, 2, n_kv_heads, PAGE, head_dim]: the rows of every slot's unfinished block
 
 
 class _KVGroup:
     def __init__(self, need, runs, n_pages, max_seqs, max_pages_per_seq, dtype, device):
         self.need, self.runs = need, list(runs)
-        if need.kind == "ids":
+        self.lines = self.tails = None
+        if need.bits == 8:
+            # a run's pages and scales, and the rows of every slot's unfinished block beside them
+            self.lines = [q8_pool(n_pages, need.n_kv_heads, need.head_dim, device) for _ in runs]
+            self.pool = [pool for pool, _ in self.lines]
+            self.tails = torch.zeros((len(runs), max_seqs, 2, need.n_kv_heads, PAGE, need.head_dim), dtype=dtype, device=device)
+        elif need.kind == "ids":
             self.pool = torch.zeros((len(runs), n_pages, PAGE), dtype=torch.int32, device=device)
         elif need.kind == "rows":
             self.pool = torch.empty((len(runs), n_pages, PAGE, need.head_dim), dtype=dtype, device=device)
@@ -86,6 +94,8 @@ class _KVGroup:
             self.dropped[slot] = last
 
     def bytes(self):
+        if self.lines is not None:
+            return sum(pool.numel() for pool in self.pool) + self.tails.numel() * self.tails.element_size()
         return self.pool.numel() * self.pool.element_size()
 
 
@@ -123,6 +133,8 @@ class Cache:
         for name, need in (named or {}).items():
             by_need.setdefault(need, []).append(("named", name))
         for need, runs in by_need.items():
+            if need.bits not in (0, 8) or (need.bits and (need.kind != "kv" or need.keep_first or need.chunk or need.value_dim not in (None, need.head_dim))):
+                raise CacheError(f"a cache line in {need.bits} bits: 8 bits go with keys and values of one size, a window or none")
             if need.kind in ("kv", "ids", "rows"):
                 # (a windowed group has storage of its own; the window is applied in the kernels, and the
                 # group gives the pages before it back as the sequence grows)
@@ -154,8 +166,11 @@ class Cache:
     @staticmethod
     def _view_of(kind, g, i, writes):
         if kind == "kv":
-            return CacheView(g.need.kind, writes, pool=g.pool[i], block_table=g.block_table, window=g.need.window,
+            view = CacheView(g.need.kind, writes, pool=g.pool[i], block_table=g.block_table, window=g.need.window,
                              keep_first=g.need.keep_first)
+            if g.lines is not None:
+                view.scales, view.tail = g.lines[i][1], g.tails[i]
+            return view
         if kind == "state":
             return CacheView("state", writes, state=g.state[i])
         return CacheView("none", writes)
@@ -171,6 +186,7 @@ class Cache:
         for v in views:
             if v.kind in ("kv", "ids", "rows"):
                 out.pool, out.block_table, out.window, out.keep_first = v.pool, v.block_table, v.window, v.keep_first
+                out.scales, out.tail = v.scales, v.tail
             elif v.kind == "state":
                 out.state = v.state
         return out

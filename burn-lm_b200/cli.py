@@ -61,6 +61,10 @@ def add_request_flags(p):
     p.add_argument("--seed", type=int, default=0,
                    help="The seed to use when generating random samples. If it is 0 then a random seed is used.")
     p.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"], help="Compute dtype.")
+    p.add_argument("--cache", default="compute", choices=["compute", "int8"],
+                   help="What keys and values are kept in: the compute dtype, or 8 bits with a scale for every block of 64 positions and head.")
+    p.add_argument("--weights", default="stored", choices=["stored", "int4"],
+                   help="What the layers' weights are held in: as stored, or 4 bits with a scale for every 64 places.")
     p.add_argument("--include-stop", action="store_true", help="Print the stop token that ended the answer as well.")
 
 
@@ -110,7 +114,8 @@ def cmd_random(args):
 
 def _load(args):
     print(f"loading model '{args.model}'...", file=sys.stderr)
-    lm = api.load(args.model, dtype=args.dtype, max_seq_len=args.max_seq_len, max_batch=1)
+    fewer = {name: value for name, value, usual in (("cache", args.cache, "compute"), ("weights", args.weights, "stored")) if value != usual}
+    lm = api.load(args.model, dtype=args.dtype, max_seq_len=args.max_seq_len, max_batch=1, **fewer)
     print("model loaded!", file=sys.stderr)
     return lm
 

@@ -88,8 +88,8 @@ class Engine:
 
     @classmethod
     def from_folder(cls, folder, dtype="bfloat16", max_tokens=4096, max_seqs=None, max_seq_len=None, device="cuda",
-                    max_step_tokens=None):
-        return cls(load_model(folder, dtype, device), max_tokens, max_seqs, max_seq_len, max_step_tokens)
+                    max_step_tokens=None, cache="compute", weights="stored"):
+        return cls(load_model(folder, dtype, device, cache, weights), max_tokens, max_seqs, max_seq_len, max_step_tokens)
 
     # -- sequences -----------------------------------------------------------------------------------
     def acquire(self) -> int:

@@ -74,8 +74,10 @@ def main(argv=None) -> int:
     ap.add_argument("--max-tokens", type=int, required=True,
                     help="most tokens live requests hold at any time; the cache is sized by it, with room for every "
                          "request's last, partly filled page")
+    ap.add_argument("--cache", default="compute", choices=["compute", "int8"], help="what keys and values are kept in")
+    ap.add_argument("--weights", default="stored", choices=["stored", "int4"], help="what the layers' weights are held in")
     args = ap.parse_args(argv)
-    engine = Engine.from_folder(args.model, dtype=args.dtype, max_tokens=cache_tokens(args.max_tokens))
+    engine = Engine.from_folder(args.model, dtype=args.dtype, max_tokens=cache_tokens(args.max_tokens), cache=args.cache, weights=args.weights)
     rp = Replayer(engine, args.out)
     for line in sys.stdin:
         line = line.strip()

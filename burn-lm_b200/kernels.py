@@ -2204,6 +2204,12 @@ class Q4Weight:
     def bytes(self) -> int:
         return self.packed.numel() + 2 * self.scales.numel()
 
+    def first_rows(self, rows: int) -> "Q4Weight":
+        """The weight's first `rows` rows (a view; whole tiles of 16)."""
+        if rows % 16 or not 0 < rows <= self.out_features:
+            raise KernelError(f"a weight in 4 bits gives its first rows by tiles of 16; {rows} of {self.out_features} asked for")
+        return Q4Weight(self.packed[: rows // 16], self.scales[:rows], rows, self.in_features, self.group)
+
 
 def _five_bits(x):
     """float32 rounded to five significant bits (to nearest, ties to even)."""

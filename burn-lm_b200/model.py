@@ -64,6 +64,21 @@ class Layer:
         return mixers[0].cache_need()
 
 
+CACHES, WEIGHTS = ("compute", "int8"), ("stored", "int4")
+
+
+def make_runtime(dtype, device, cache="compute", weights="stored") -> Runtime:
+    """The runtime of a model: its compute dtype, what its cache keeps keys and values in and what its products' weights are held in."""
+    if cache not in CACHES:
+        raise ValueError(f"the cache is one of {CACHES}, got {cache!r}")
+    if weights not in WEIGHTS:
+        raise ValueError(f"the weights are one of {WEIGHTS}, got {weights!r}")
+    runtime = Runtime(parse_dtype(dtype), torch.device(device), cache, weights)
+    if weights == "int4" and runtime.exact:
+        raise ValueError("weights in 4 bits go with bfloat16 compute; the 32-bit path keeps every bit of a weight")
+    return runtime
+
+
 class Model:
     def __init__(self, plan: ModelPlan, runtime: Runtime, config=None):
         self.plan, self.runtime, self.config = plan, runtime, config
@@ -74,6 +89,25 @@ class Model:
         self.final_norm = _build(plan.final_norm, "norm", runtime)
         self.head = _build(plan.head, "head", runtime)
         self.bound = False
+        if runtime.cache == "int8":
+            self._check_eight_bits()
+        if runtime.weights == "int4" and not any(getattr(p, "four_bit", ()) for p in self.parts()):
+            raise ValueError("weights in 4 bits: none of this model's parts holds products that take them")
+
+    def _check_eight_bits(self) -> None:
+        """Every run that keeps keys and values does so in 8 bits, and no run reads another's line (whose unfinished block it would need
+        as it was before the step)."""
+        some = False
+        for run, e in enumerate(self.plan.schedule):
+            needs = self.layers[e.layer].cache_need()
+            for need in needs if isinstance(needs, tuple) else (needs,):
+                if need.kind == "rows" or (need.kind == "kv" and need.bits != 8):
+                    raise ValueError(f"a cache in 8 bits: the mixer of layer {e.layer} keeps its cache in the compute dtype only")
+                some = some or need.bits == 8
+            if e.cache_of is not None and some:
+                raise ValueError(f"a cache in 8 bits: run {run} of the schedule reads the cache line of run {e.cache_of}, which lines in 8 bits do not offer")
+        if not some:
+            raise ValueError("a cache in 8 bits: this model keeps no keys and values")
 
     # -- weights ---------------------------------------------------------------------------------
     def parts(self):
@@ -102,6 +136,13 @@ class Model:
         for layer in self.layers:
             if hasattr(layer.block, "bound"):
                 layer.block.bound()                # a block may join its parts' weights
+        if self.runtime.weights == "int4":
+            for p in self.parts():
+                for name in getattr(p, "four_bit", ()):
+                    getattr(p, name).to_4bit()
+            for layer in self.layers:
+                if getattr(layer.block, "joint", None) is not None:
+                    layer.block.joint.to_4bit()
         # a run that reads another run's cache line must agree with its writer on how the entries lie there
         for run, e in enumerate(self.plan.schedule):
             if e.cache_of is not None:
@@ -135,6 +176,8 @@ class Model:
         names = set()
         for p in self.parts() + [layer.block for layer in self.layers]:
             names.update(getattr(p, "kernel_modules", ("elementwise",)))
+        if self.runtime.weights == "int4":
+            names.add("gemm_q4")
         return sorted(names)
 
     # -- forward ---------------------------------------------------------------------------------
@@ -208,11 +251,13 @@ def tensor_specs_of(config: dict):
     return Model(plan, Runtime(torch.bfloat16, torch.device("cpu"))).tensor_specs()
 
 
-def load_model(folder: str, dtype="bfloat16", device="cuda") -> Model:
-    """Build the model a folder's config.json names and bind its safetensors weights."""
+def load_model(folder: str, dtype="bfloat16", device="cuda", cache="compute", weights="stored") -> Model:
+    """Build the model a folder's config.json names and bind its safetensors weights.  `cache` "int8": keys and values in 8 bits with a
+    scale for every block of 64 positions and head; `weights` "int4": the weights of the layers' products rounded to 4 bits with a
+    scale for every 64 places (embeddings, norms and the output projection stay as stored)."""
     config = read_config_json(folder)
     _, typed, plan = plan_of(config)
-    runtime = Runtime(parse_dtype(dtype), torch.device(device))
+    runtime = make_runtime(dtype, device, cache, weights)
     model = Model(plan, runtime, typed)
     loaded = load_tensors(folder, model.tensor_specs(), runtime.dtype, runtime.device, plan.ignorable_tensors,
                           plan.duplicate_tensors)
@@ -220,7 +265,7 @@ def load_model(folder: str, dtype="bfloat16", device="cuda") -> Model:
     return model
 
 
-def random_model(config: dict, seed: int = 0, dtype="bfloat16", device="cuda", stored_dtype="bfloat16") -> Model:
+def random_model(config: dict, seed: int = 0, dtype="bfloat16", device="cuda", stored_dtype="bfloat16", cache="compute", weights="stored") -> Model:
     """The model `config` names with random weights drawn on the device, without a folder in between: for
     shapes whose files would take minutes to write and read back.  The numbers are the ones
     `write_random_model(..., device=<the same device>)` stores (every tensor from its own generator, seeded
@@ -228,7 +273,7 @@ def random_model(config: dict, seed: int = 0, dtype="bfloat16", device="cuda", s
     from .weights.loader import _target_dtype
     from .weights.random_init import _DTYPES, random_tensor
     _, typed, plan = plan_of(config)
-    runtime = Runtime(parse_dtype(dtype), torch.device(device))
+    runtime = make_runtime(dtype, device, cache, weights)
     model = Model(plan, runtime, typed)
     loaded = {}
     for spec in model.tensor_specs():

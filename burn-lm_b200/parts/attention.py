@@ -2,7 +2,7 @@
 
 q = x Wq, k = x Wk, v = x Wv without bias, feature c of q belonging to head c // head_dim
 (crates/burn-lm-llama/src/nn/attention/mha.rs:121-140); q and k are rotated, k and v appended to
-the cache (:91-95); query head h reads kv head h // (heads / kv heads) (:174-185); scores are
+the cache (:91-95), which may keep complete blocks of positions in 8 bits (Runtime.cache); query head h reads kv head h // (heads / kv heads) (:174-185); scores are
 q.k / sqrt(head_dim), keys after the query's position are hidden, softmax, times v (:157-166);
 heads are merged and projected by Wo (:168-170, :118).  The three projections run as one product
 with a fused [q; k; v] weight built when the weights are bound.
@@ -69,6 +69,9 @@ class Attention(Part):
             # attention kernels of this package compute q.k * scale and the mask only
             raise ValueError(f"position encoding {spec.position.kind!r} asks for a bias on the attention scores, which "
                              f"the attention kernels do not have; it needs a mixer of its own")
+        self.eight = runtime.cache == "int8"
+        if self.eight:
+            self.kernel_modules = ("elementwise", "attention_q8")
         self.scale = spec.softmax_scale if spec.softmax_scale is not None else 1.0 / math.sqrt(spec.head_dim)
 
     def tensor_specs(self):
@@ -90,14 +93,14 @@ class Attention(Part):
         s = self.spec
         _, rot, interleaved = self.position.rotation() if hasattr(self.position, "rotation") else (None, 0, False)
         self.pairs = K.PAIRS_INTERLEAVED if interleaved else K.PAIRS_HALVES
-        if q.dtype == torch.bfloat16 and rot == s.head_dim and not interleaved:
+        if q.dtype == torch.bfloat16 and rot == s.head_dim and not interleaved and not self.eight:
             order = torch.tensor(K.tiled_pair_order(s.head_dim), device=q.device)
             q = q.view(s.n_heads, s.head_dim, -1)[:, order].reshape(q.shape)
             k = k.view(s.n_kv_heads, s.head_dim, -1)[:, order].reshape(k.shape)
             self.pairs = K.PAIRS_TILED
         fused = torch.cat([q, k, v], dim=0).contiguous()
         self.qkv = Linear(fused)
-        self.q_only = Linear(fused[: self.spec.n_heads * self.spec.head_dim])
+        self.q_rows = self.spec.n_heads * self.spec.head_dim
         self.o = Linear(loaded[t["o"]])
         self.position.bind(loaded)
 
@@ -112,7 +115,7 @@ class Attention(Part):
 
     def cache_need(self) -> CacheNeed:
         s = self.spec
-        return CacheNeed("kv", n_kv_heads=s.n_kv_heads, head_dim=s.head_dim, window=s.window)
+        return CacheNeed("kv", n_kv_heads=s.n_kv_heads, head_dim=s.head_dim, window=s.window, bits=8 if self.eight else 0)
 
     def _splits(self, step) -> int:
         if step.max_q_len != 1:
@@ -127,13 +130,29 @@ class Attention(Part):
 
     takes_pending_norm = True
     adds_to_stream = True
+    four_bit = ("qkv", "o")
+
+    def _over_eight_bits(self, x, step, cache, stream):
+        """The same over a cache line in 8 bits: product, rotation and append, attention, output product."""
+        s, rt = self.spec, self.runtime
+        inv_freq, rot, _ = self.position.rotation()
+        table = self.position.table() if hasattr(self.position, "table") else None
+        qkv = self.qkv(x, out_dtype=rt.dtype)
+        old = K.rope_append_q8(qkv, qkv, step, cache.pool, cache.scales, cache.tail, cache.block_table, inv_freq, rot, self.pairs, s.n_heads,
+                               s.n_kv_heads, s.head_dim, table=table, turn_scale=getattr(self.position, "turn_scale", 1.0))
+        out = torch.empty((step.n_tokens, s.n_heads * s.head_dim), dtype=rt.dtype, device=qkv.device)
+        K.attention_q8(qkv, step, cache.pool, cache.scales, cache.tail, old, cache.block_table, out, s.n_heads, s.n_kv_heads, s.head_dim,
+                       self.scale, window=s.window or 0)
+        return self.o.into_stream(out, stream, rt.dtype, handoff=getattr(step, "handoff", None))
 
     def forward(self, x, step, cache, stream=None):
+        if self.eight:
+            return self._over_eight_bits(x, step, cache, stream)
         s, rt = self.spec, self.runtime
         inv_freq, rot, interleaved = self.position.rotation()
         table = self.position.table() if hasattr(self.position, "table") else None
         n = step.n_tokens
-        product = self.qkv if cache.writes else self.q_only     # a run that reads another run's cache line needs q only
+        product = self.qkv if cache.writes else self.qkv.first_rows(self.q_rows)     # a run that reads another run's cache line needs q only
         qkv = None
         ahead = False
         # the page of every new token and the sequences' rows of the block table: looked up once per step for all

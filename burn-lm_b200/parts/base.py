@@ -35,6 +35,8 @@ import torch
 class Runtime:
     dtype: torch.dtype           # compute dtype of activations and of the cache: bfloat16 or float32
     device: torch.device
+    cache: str = "compute"       # what keys and values are kept in: "compute" (the compute dtype) or "int8" (blocks in 8 bits, kernels.q8_pool)
+    weights: str = "stored"      # what the weights of large products are held in: "stored" or "int4" (kernels.Q4Weight)
 
     @property
     def exact(self) -> bool:
@@ -49,7 +51,7 @@ class CacheNeed:
     kind "kv":    keys and values per position: n_kv_heads x head_dim each (values of `value_dim` lanes when
                   that is set and differs; 0: the values are the keys, nothing is kept beside them); `window` None keeps all positions, a number keeps that many of the
                   latest, and beside them the first `keep_first` positions of the sequence; `chunk`: a position looks back to the
-                  start of its own chunk of that many positions, counted from the sequence's start.
+                  start of its own chunk of that many positions, counted from the sequence's start; `bits` 8: in 8 bits (kernels.q8_pool).
     kind "rows":  one row of `head_dim` lanes per position in the compute dtype, shared by all heads (a latent that keys
                   and values are made from), paged like keys and values; `window` as above.
     kind "ids":   one int32 per position (a token id, say), paged like keys and values; `window` as above.
@@ -65,6 +67,7 @@ class CacheNeed:
     value_dim: Optional[int] = None
     keep_first: int = 0
     chunk: Optional[int] = None
+    bits: int = 0                # kind "kv": 8: complete blocks of PAGE positions in 8 bits, the unfinished one in the compute dtype; 0: all in that
 
     def first_needed(self, length: int) -> int:
         """The first position that tokens at positions >= length look back to (what the sequence keeps from its start aside)."""
@@ -106,6 +109,7 @@ class Part:
     # cope with the padding of captured prompt steps: rows whose token_seq is -1 belong to no sequence and
     # must not reach a cache or a state; sequences of no tokens may follow the real ones.
     graph_safe = False
+    four_bit: tuple = ()         # names of the Linear attributes that a model with weights in 4 bits rounds after binding
 
     def __init__(self, spec, tensors: dict, runtime: Runtime):
         self.spec = spec

@@ -51,6 +51,7 @@ class SwiGLU(Part):
 
     takes_pending_norm = True
     adds_to_stream = True
+    four_bit = ("gate_up", "down")
 
     def forward(self, x, step, stream=None):
         rt = self.runtime
@@ -86,6 +87,7 @@ class BiasedMLP(Part):
     graph_safe = True
     roles = ("up", "up_bias", "down", "down_bias", "act")
     kernel_modules = ("stream_ops",)
+    four_bit = ("up", "down")
 
     def __init__(self, spec, tensors, runtime):
         super().__init__(spec, tensors, runtime)
@@ -127,6 +129,8 @@ class MLP(Part):
     kernel_modules = ("elementwise", "stream_ops")
     takes_pending_norm = True
     adds_to_stream = True
+
+    four_bit = ("up", "down")
 
     ACTIVATIONS = {"relu2": K.ACT_RELU2}
 

@@ -9,6 +9,10 @@ through the library product (cuBLAS via torch.mm), as the reference's engine use
 `Linear` (crates/burn-lm-llama/src/nn/attention/mha.rs:124-126).  float32 weights go through this package's
 own fp32 kernel, which has no reduced-precision mode: that is the 32-bit path, and also what a
 layer stored in 32-bit inside a bfloat16 model gets.
+
+A bfloat16 weight may be rounded to 4 bits after it is bound (`to_4bit`): every product then runs this
+package's kernels for such weights (kernels.product_q4), with the gated activation or the sum into the
+residual stream behind it; a norm in front of it, the next norm's input and the rotation have kernels of their own.
 """
 from __future__ import annotations
 
@@ -107,11 +111,46 @@ class Linear:
         if weight.dim() != 2:
             raise ValueError("a linear weight is [out, in]")
         self.weight = weight
+        self.q4 = None           # kernels.Q4Weight once to_4bit() has been called; `weight` is None then
         self.gate_tile = gate_tile
         self.out_features, self.in_features = weight.shape
+        self._first = {}
+
+    def to_4bit(self, group: int = 64) -> None:
+        """Round the weight to 4 bits with a scale for every `group` places along K, and let go of the stored one."""
+        if self.weight.dtype != torch.bfloat16:
+            raise ValueError(f"weights in 4 bits are rounded from bfloat16 ones; this one is {self.weight.dtype}")
+        self.q4 = K.quantize_q4(self.weight, group)
+        self.weight = None
+        self._first = {}
+
+    def first_rows(self, rows: int) -> "Linear":
+        """The product with the first `rows` outputs alone (a view of the same weight)."""
+        part = self._first.get(rows)
+        if part is None:
+            part = Linear.__new__(Linear)
+            part.weight, part.gate_tile, part._first = None, self.gate_tile, {}
+            part.out_features, part.in_features = rows, self.in_features
+            part.q4 = None if self.q4 is None else self.q4.first_rows(rows)
+            if self.q4 is None:
+                part.weight = self.weight[:rows]
+            self._first[rows] = part
+        return part
+
+    def _four_bit_rows(self, x) -> torch.Tensor:
+        """x (a tensor or a pending norm) as the bfloat16 rows that products with 4-bit weights take."""
+        if isinstance(x, NormedStream):
+            x = x.materialize()
+        if x.dtype != torch.bfloat16:
+            xc = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+            K.convert(x, xc)
+            x = xc
+        return x
 
     def _skinny(self, n_tokens: int, m: int, x=None) -> bool:
         w = self.weight
+        if w is None:
+            return False
         plain = isinstance(x, torch.Tensor) and x.dtype == torch.bfloat16
         return (w.dtype == torch.bfloat16 and w.is_cuda and n_tokens <= SKINNY_TOKENS
                 and K.gemv_supported(n_tokens, m, self.in_features, plain_tokens=plain))
@@ -119,7 +158,7 @@ class Linear:
     def _sk(self, n_tokens: int) -> bool:
         """Whether the step runs kernels.gemm_sk (asked after _skinny has said no)."""
         w = self.weight
-        return (w.dtype == torch.bfloat16 and w.is_cuda and w.is_contiguous() and n_tokens <= min(SK_TOKENS, K.SK_TOKENS)
+        return (w is not None and w.dtype == torch.bfloat16 and w.is_cuda and w.is_contiguous() and n_tokens <= min(SK_TOKENS, K.SK_TOKENS)
                 and K.gemm_sk_supported(n_tokens, self.out_features, self.in_features))
 
     @staticmethod
@@ -157,6 +196,9 @@ class Linear:
 
     def __call__(self, x, out_dtype: torch.dtype | None = None) -> torch.Tensor:
         n = self._tokens(x)
+        if self.q4 is not None:
+            out_dtype = out_dtype or (torch.bfloat16 if isinstance(x, NormedStream) else x.dtype)
+            return K.product_q4(self.q4, self._four_bit_rows(x), out=torch.empty((n, self.out_features), dtype=out_dtype, device=self.q4.device))
         if self._skinny(n, self.out_features, x):
             out_dtype = out_dtype or torch.bfloat16
             if out_dtype in (torch.bfloat16, torch.float32):
@@ -178,6 +220,9 @@ class Linear:
         norm, the kernel also leaves that norm's input there.  `bias` (float32) joins the stream with the product; a product that
         is handed back comes without it."""
         n = self._tokens(x)
+        if self.q4 is not None and stream is not None and bias is None and tuple(stream.shape) == (n, self.out_features):
+            K.product_q4(self.q4, self._four_bit_rows(x), add_into=stream)
+            return None
         if stream is not None and self._skinny(n, self.out_features, x):
             hand_over = None
             norm = handoff.wanted if handoff is not None else None
@@ -202,7 +247,7 @@ class Linear:
             if hand_over is not None:
                 handoff.leave(stream, norm.gamma, handed)
             return None
-        if (OWN_PRODUCTS and stream is not None and bias is None and self.weight.dtype == torch.bfloat16 and n >= OWN_PRODUCTS_TOKENS
+        if (OWN_PRODUCTS and stream is not None and bias is None and self.q4 is None and self.weight.dtype == torch.bfloat16 and n >= OWN_PRODUCTS_TOKENS
                 and K.gemm_tc_supported(n, self.out_features, self.in_features)):
             if isinstance(x, NormedStream):
                 x = x.materialize()
@@ -231,7 +276,13 @@ class Linear:
         """silu(x Wgate^T) * (x Wup^T) for a fused [gate; up] weight; into `out` (it may be a column range) when given."""
         n = self._tokens(x)
         inner = self.out_features // 2
-        act = out if out is not None else torch.empty((n, inner), dtype=out_dtype, device=self.weight.device)
+        act = out if out is not None else torch.empty((n, inner), dtype=out_dtype, device=(self.weight if self.q4 is None else self.q4).device)
+        if self.q4 is not None:
+            if self.gate_tile == K.GATE_TILE:
+                K.product_q4(self.q4, self._four_bit_rows(x), out=act, swiglu=True)
+            else:
+                K.swiglu(self(x, out_dtype), act, tile=self.gate_tile)
+            return act
         aligned = act.data_ptr() % 16 == 0 and act.stride(0) % 8 == 0
         if out_dtype == torch.bfloat16 and self.gate_tile == K.GATE_TILE and self._skinny(n, inner, x):
             K.gemv(self.weight, n, out=act, swiglu=True, **self._source(x))
@@ -254,7 +305,7 @@ class Linear:
         """act(x W^T), the activation (kernels.ACT_*) taken in fp32 on the product's sums; the skinny and the tcgen05 product
         square a relu in their own epilogue."""
         n = self._tokens(x)
-        if act == K.ACT_RELU2 and out_dtype == torch.bfloat16 and self.weight.dtype == torch.bfloat16:
+        if act == K.ACT_RELU2 and out_dtype == torch.bfloat16 and self.q4 is None and self.weight.dtype == torch.bfloat16:
             out = torch.empty((n, self.out_features), dtype=out_dtype, device=self.weight.device)
             if self._skinny(n, self.out_features, x):
                 K.gemv(self.weight, n, out=out, relu2=True, **self._source(x))
