@@ -259,7 +259,7 @@ _protos = {
         "blm_gemm_sk_squares_row": [],
     },
     "gemm_q4": {
-        "blm_gemm_q4": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p],
+        "blm_gemm_q4": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     },
     "sampling": {
         "blm_argmax": [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -1119,7 +1119,8 @@ _WAITS = {
     37: "prompt attention: the producer waited in vain for a free stage",
     41: "gemm_sk: the tensor-core thread waited in vain for a stage", 42: "gemm_sk: the producer waited in vain for a free stage",
     43: "gemm_sk: the epilogue waited in vain for the accumulator",
-    51: "attention over 8 bits: a consumer waited in vain for a page", 52: "attention over 8 bits: the producer waited in vain for a free stage"}
+    51: "attention over 8 bits: a consumer waited in vain for a page", 52: "attention over 8 bits: the producer waited in vain for a free stage",
+    53: "product with 4-bit weights: a wait ran out"}
 
 
 def check_status(device) -> None:
@@ -2331,5 +2332,6 @@ def product_q4(w, x, out=None, add_into=None, swiglu=False):
         wide[:, :k] = x
         x, k = wide, wide.shape[1]
     _call("gemm_q4", "blm_gemm_q4", _ptr(w.packed), _ptr(w.scales), w.scales.shape[1], w.group, _ptr(x), x.stride(0), _ptr(y), y.stride(0),
-          1 if y.dtype == torch.float32 else 0, Q4_ADD if add_into is not None else (Q4_GATED if swiglu else Q4_STORE), n, m, k, _stream())
+          1 if y.dtype == torch.float32 else 0, Q4_ADD if add_into is not None else (Q4_GATED if swiglu else Q4_STORE), n, m, k,
+          status_word(x.device).data_ptr(), _stream())
     return y
