@@ -2192,7 +2192,8 @@ _Q4_STRETCH = 256             # places of K that a warp of the product's kernels
 
 class Q4Weight:
     """A weight [out_features, in_features] in 4 bits, as pack_q4 and quantize_q4 make it: whole numbers of -8 .. 7 in the order in which
-    the kernels read them, and bfloat16 scales [rows filled up to 16, groups filled up to 256 places]."""
+    the kernels read them, and bfloat16 scales [rows filled up to 16, one for every 32 places (groups of 32) or 64 (a group of 128 has its
+    own twice), filled up to 256 places]."""
 
     def __init__(self, packed, scales, out_features, in_features, group):
         self.packed, self.scales = packed, scales
@@ -2243,7 +2244,9 @@ def pack_q4(values, scales, group) -> Q4Weight:
         raise KernelError("pack_q4: scales are finite and have five significant bits at most")
     tiles, k_tiles = -(-m // 16), -(-k // 64)
     stretches = -(-k_tiles * 64 // _Q4_STRETCH)
-    packed_scales = torch.zeros((tiles * 16, stretches * (_Q4_STRETCH // group)), dtype=torch.bfloat16, device=values.device)
+    packed_scales = torch.zeros((tiles * 16, stretches * (_Q4_STRETCH // min(group, 64))), dtype=torch.bfloat16, device=values.device)
+    if group == 128:
+        s = s.repeat_interleave(2, dim=1)[:, : packed_scales.shape[1]]
     packed_scales[:m, : s.shape[1]] = s
     row, place = _q4_order(values.device)
     packed = torch.empty((tiles, k_tiles, 512), dtype=torch.uint8, device=values.device)
@@ -2294,7 +2297,7 @@ def q4_values(w) -> torch.Tensor:
         n = torch.stack([p & 15, p >> 4], dim=-1).reshape(p.shape[0], k_tiles, 32, 4, 8)
         tile = torch.empty((p.shape[0], k_tiles, 16, 64), dtype=torch.bfloat16, device=w.device)
         tile[:, :, row, place] = n.to(torch.bfloat16) - 8
-        s = w.scales[t0 * 16: (t0 + p.shape[0]) * 16].repeat_interleave(w.group, dim=1)[:, : k_tiles * 64]
+        s = w.scales[t0 * 16: (t0 + p.shape[0]) * 16].repeat_interleave(min(w.group, 64), dim=1)[:, : k_tiles * 64]
         out[t0 * 16: (t0 + p.shape[0]) * 16] = tile.permute(0, 2, 1, 3).reshape(-1, k_tiles * 64) * s
     return out[: w.out_features, : w.in_features].contiguous()
 
