@@ -3,12 +3,12 @@
 // A scale has five significant bits, so scale * v is a bfloat16 number exactly: whichever kernel forms the product, the weights are
 // the same numbers, and the only roundings are those of float32 sums (and of the result to its type).
 //
-// Weights are packed once, by tiles of 16 rows and 64 places of K, 512 bytes each: 16 bytes for every lane (g, t) of a warp, one word
-// for each of four steps of 16 places (mma.sync.m16n8k16's K).  Lane (g, t)'s places of step s are 32 (s / 2) + 8 t + 4 (s % 2) + j,
-// j = 0 .. 3, of rows g and g + 8; the nibbles of a word are, from the lowest, (g, 0) (g + 8, 0) (g, 2) (g + 8, 2) (g, 1) (g + 8, 1)
-// (g, 3) (g + 8, 3): a shift and a mask by 0x000f000f leave two neighbours of one row in the two halves of a register.  A nibble
-// holds v + 8.  Scales are bfloat16 [rows][one for every 32 places where groups have 32, else for every 64 (a group of 128 has its own
-// twice)], filled up to whole stretches of 256 places.
+// Weights are packed once, by tiles of 16 rows and stretches of 256 places of K (four tiles of 64), 512 bytes a tile: 16 bytes for every
+// lane (g, t) of a warp, one word for each of four steps of 16 places (mma.sync.m16n8k16's K).  Lane (g, t)'s places of step s are
+// 32 (s / 2) + 8 t + 4 (s % 2) + j, j = 0 .. 3, of rows g and g + 8; the nibbles of a word are, from the lowest, (g, 0) (g + 8, 0) (g, 2)
+// (g + 8, 2) (g, 1) (g + 8, 1) (g, 3) (g + 8, 3): a shift and a mask by 0x000f000f leave two neighbours of one row in the two halves of
+// a register.  A nibble holds v + 8.  Behind a stretch's four tiles stand its scales, bfloat16 [16 rows][4], one for every 64 places (a
+// group of 128 has its own twice), or [16 rows][8] where groups have 32: one copy of 2,176 or 2,304 bytes brings all that a warp needs.
 #include "tcgen05.cuh"
 
 BLM_API const char* blm_gemm_q4_last_error() { return g_blm_error; }
@@ -20,14 +20,13 @@ constexpr int kBatch = 4;            // tiles that a warp loads together: 256 pl
 enum { END_STORE = 0, END_ADD = 1, END_GATED = 2 };
 
 struct Args {
-    const uint4* w;                  // [row tiles][k tiles][32]
-    const __nv_bfloat16* scales;     // [row tiles * 16][groups]
+    const unsigned char* w;          // [row tiles][stretches][unit]
     const __nv_bfloat16* x;          // [N, K], rows ldx apart
     long long ldx;
     void* y;                         // [N, M] (END_GATED: [N, M / 2]), rows ldy apart; END_ADD: float32, added to
     long long ldy;
     int y_f32, end;
-    int N, M, K, k_tiles, row_scales, per_tile;      // scales of a row, and of a tile: 1 or 2
+    int N, M, K, k_tiles, stretches, unit, per_tile; // bytes of a stretch of a tile of rows; scales of a tile of 64 places: 1 or 2
 };
 
 __device__ __forceinline__ void mma16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
@@ -36,131 +35,303 @@ __device__ __forceinline__ void mma16(float (&c)[4], unsigned a0, unsigned a1, u
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16_onto(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1, const float (&c)[4]) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
 // Two whole numbers of a word: 0x43 in front of a nibble is the bfloat16 number 128 + nibble, and the nibble is v + 8.
 __device__ __forceinline__ unsigned pair(unsigned word, int p) {
     const unsigned biased = ((word >> (4 * p)) & 0x000f000fu) | 0x43004300u;
     const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&biased), __float2bfloat162_rn(136.f));
     return *reinterpret_cast<const unsigned*>(&v);
 }
-__device__ __forceinline__ uint4 load_once(const uint4* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+__device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+// the same place in the shared memory of a block of the cluster
+__device__ __forceinline__ float shared_of(unsigned mine, int rank) {
+    unsigned at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(mine), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(at) : "memory");
     return v;
 }
 __device__ __forceinline__ float bf16_of(unsigned two, int which) { return __uint_as_float(which ? two & 0xffff0000u : two << 16); }
 
-// Few tokens: a block has R tiles of 16 rows and up to 8 NT tokens; its warps take stretches of 256 places of K in turn and meet in
-// shared memory.  Bound by the weights' bytes: every lane loads R x 64 bytes of weights before it waits for anything.
-constexpr int kWarps = 8;
-template <int R, int NT>
-__global__ void __launch_bounds__(kWarps * 32) skinny_kernel(const Args a) {
-    __shared__ float sums[kWarps][R * 16][8 * NT + 1];
+// ---- few tokens ------------------------------------------------------------------------------------------------------------
+// Up to 16 tokens a block (a block for each 16 of up to 32).  A cluster's blocks cut K into chunks of 2,048 places, a block's eight warps a
+// chunk into stretches of 256, so that a warp meets the same tokens for every row: their fragments stay in its registers, and it does
+// nothing but stream its places of one tile of 16 rows after the other, AHEAD tiles ahead.  What bounds it beside the weights' bytes is
+// the instructions that make operands of them, so they are used as they are: sixteen bits that hold a whole number n below 256 are the
+// bfloat16 number n 2^-133 (below 2^-126, and still with that step in the next binade), so a mask by 0x000f000f or 0x00f000f0 and one
+// shift of a word by eight bits give all of its weights, of rows g as n = v + 8, of rows g + 8 as 16 (v + 8).  The tokens are multiplied by
+// a power of two that brings the largest of a warp's stretch to 2^120 (exactly: bfloat16 has the exponents for it), so that products and
+// sums are of ordinary size.  The 8 is not taken off the weights: a part's sum starts at -8 (-128) times the sum of its tokens' places,
+// formed by the tensor cores, once.  A part's scale multiplies its sum.  The warps' sums meet in shared memory, the cluster's blocks in
+// distributed shared memory, in a fixed order.
+constexpr int kWarps = 8, kChunk = kWarps * kBatch;      // k tiles of a block
+enum { Q4_TIMEOUT_WEIGHTS = 54 };
+template <int NT> struct Few {
+    static constexpr int kAhead = NT == 1 ? 3 : 4, kBlocks = NT == 1 ? 2 : 1;      // tiles of rows on their way a warp; blocks of an SM
+    static constexpr int kUnit = kBatch * kTileBytes + 256;                        // room for a stretch of a tile of rows
+    static constexpr int kSlots = NT == 1 ? 12 : 16;                                 // tiles of rows between two meetings
+    static constexpr int kSums = 16 * 8 * NT;                                      // of a tile: [16 rows][8 NT tokens]
+    static constexpr int kSmem = kWarps * kAhead * kUnit + kSlots * (kWarps + 1) * kSums * 4 + kWarps * kAhead * 8;
+};
+
+struct FewArgs {
+    Args a;
+    int chunks, clusters;        // blocks of a cluster, clusters
+    int* status;
+};
+
+template <int NT, bool TWO>
+__global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(const FewArgs fa) {
+    using F = Few<NT>;
+    constexpr int AHEAD = F::kAhead, PARTS = TWO ? 2 : 1;                          // parts of a tile with a scale of their own
+    const Args& a = fa.a;
+    extern __shared__ __align__(128) unsigned char smem_few[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int tile0 = blockIdx.x * R, n = a.N, tiles = (a.M + 15) / 16;
+    unsigned char* ring = smem_few + warp * AHEAD * F::kUnit;                      // this warp's units
+    float* partial = reinterpret_cast<float*>(smem_few + kWarps * AHEAD * F::kUnit);       // [slots][warps][16][8 NT], then [slots][16][8 NT]
+    float* sums = partial + F::kSlots * kWarps * F::kSums;
+    unsigned long long* full = reinterpret_cast<unsigned long long*>(sums + F::kSlots * F::kSums) + warp * AHEAD;
+    const int rank = blockIdx.x % fa.chunks, cluster = blockIdx.x / fa.chunks, tok0 = blockIdx.y * 8 * NT, n = min(8 * NT, a.N - tok0);
+    const int stretch = rank * kWarps + warp, kt = stretch * kBatch, tiles = (a.M + 15) / 16;
+    const int t_lo = (int)((long long)tiles * cluster / fa.clusters), t_hi = (int)((long long)tiles * (cluster + 1) / fa.clusters);
+    const bool here = stretch < a.stretches;
+    const int total_units = here ? t_hi - t_lo : 0;
     pdl_launch_dependents();
-    float total[R][NT][4];
+    // the weights, AHEAD units ahead: one lane copies
+    const unsigned char* w_at = a.w + ((size_t)t_lo * a.stretches + (here ? stretch : 0)) * a.unit;
+    const size_t w_step = (size_t)a.stretches * a.unit;
+    auto fetch = [&](int slot) {
+        tc5::mbar_expect_tx(full + slot, a.unit);
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(ring + slot * F::kUnit)),
+                     "l"(w_at), "r"(a.unit), "r"(smem_u32(full + slot))
+                     : "memory");
+        w_at += w_step;
+    };
+    if (lane == 0) {
+        for (int j = 0; j < AHEAD; ++j) tc5::mbar_init(full + j, 1);
+        tc5::mbar_init_fence();
+        for (int j = 0; j < AHEAD && j < total_units; ++j) fetch(j);
+    }
+    __syncwarp();
+    pdl_wait();                                          // the tokens are the work of the kernel before
+    uint4 x[kBatch][NT][2];
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int j = 0; j < kBatch; ++j)
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) total[r][i][e] = 0.f;
-    bool waited = false;
-    for (int kt = warp * kBatch; kt < a.k_tiles; kt += kWarps * kBatch) {
-        uint4 w[R][kBatch];
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int j = 0; j < kBatch; ++j)
-                w[r][j] = tile0 + r < tiles && kt + j < a.k_tiles ? load_once(a.w + ((size_t)(tile0 + r) * a.k_tiles + kt + j) * 32 + lane)
-                                                                  : make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-        // the stretch's scales of rows g and g + 8: of each tile's first and second 32 places
-        unsigned sc[R][2][kBatch];
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const __nv_bfloat16* s = a.scales + (size_t)(min(tile0 + r, tiles - 1) * 16 + g + 8 * h) * a.row_scales + kt * a.per_tile;
-                if (a.per_tile == 2) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(s);
-                    sc[r][h][0] = v.x; sc[r][h][1] = v.y; sc[r][h][2] = v.z; sc[r][h][3] = v.w;
-                } else {
-                    const uint2 v = *reinterpret_cast<const uint2*>(s);
-                    sc[r][h][0] = __byte_perm(v.x, 0, 0x1010); sc[r][h][1] = __byte_perm(v.x, 0, 0x3232);
-                    sc[r][h][2] = __byte_perm(v.y, 0, 0x1010); sc[r][h][3] = __byte_perm(v.y, 0, 0x3232);
-                }
+                const int k = (kt + j) * 64 + 32 * h + 8 * t, tok = 8 * i + g;
+                x[j][i][h] = tok < n && k < a.K ? *reinterpret_cast<const uint4*>(a.x + (size_t)(tok0 + tok) * a.ldx + k) : make_uint4(0u, 0u, 0u, 0u);
             }
-        if (!waited) { pdl_wait(); waited = true; }      // the tokens are the work of the kernel before
-        uint4 x[kBatch][NT][2];
+    // times a power of two: the largest of this stretch to 2^120 (zeros, infinities and NaN: as they are)
+    float back[NT][2];                                   // of tokens 2 t and 2 t + 1: what takes that and the weights' 2^-133 off again, over 2^66
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        unsigned top = 0;                                // of two magnitudes' bits at once
 #pragma unroll
         for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint4 v = x[j][i][h];
+                top = __vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), __vmaxu2(__vmaxu2(v.y & 0x7fff7fffu, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu));
+            }
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = (int)(max(top & 0xffffu, top >> 16) >> 7);                  // the largest exponent, 127 too large
+        const int by = e == 0 || e == 255 ? 0 : min(127, 247 - e);                // (-7 at least)
+        const unsigned factor = (unsigned)(127 + by) << 7, both = factor << 16 | factor;
+        auto times = [&](unsigned v) {
+            const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&both));
+            return *reinterpret_cast<const unsigned*>(&r);
+        };
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint4& v = x[j][i][h];
+                v = make_uint4(times(v.x), times(v.y), times(v.z), times(v.w));
+            }
+        const float mine = __uint_as_float((unsigned)(127 + 67 - by) << 23);      // 2^(133 - 66 - by), of token g
+        back[i][0] = __shfl_sync(0xffffffffu, mine, 8 * t);
+        back[i][1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
+    }
+    // where a part's sum starts: -8 times the sum of its places for row g, -128 times for row g + 8
+    float start[kBatch][PARTS][NT][4];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float (&d)[4] = start[j][TWO ? h : 0][i];
+                if (TWO || h == 0) d[0] = d[1] = d[2] = d[3] = 0.f;
+                constexpr unsigned k8 = 0x80088008u, k128 = 0x80808080u;
+                mma16(d, k8, k128, k8, k128, x[j][i][h].x, x[j][i][h].y);
+                mma16(d, k8, k128, k8, k128, x[j][i][h].z, x[j][i][h].w);
+            }
+
+    const int m_out = a.end == END_GATED ? a.M / 2 : a.M, rows = a.end == END_GATED ? 8 : 16;
+    int unit = 0, slot = 0;                              // the next of this warp's, and where it lies
+    unsigned phase = 0;
+    bool ok = true;
+    for (int b0 = t_lo; b0 < t_hi; b0 += F::kSlots) {
+        const int count = min(F::kSlots, t_hi - b0);
+        float* to = partial + warp * F::kSums + g * 8 * NT + 2 * t;
+#pragma unroll 1
+        for (int r = 0; r < count; ++r, to += kWarps * F::kSums) {
+            float total[NT][4];
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
+                for (int e = 0; e < 4; ++e) total[i][e] = 0.f;
+            if (here && ok) {
+                if (!tc5::mbar_wait(full + slot, phase)) {
+                    if (lane == 0) atomicCAS(fa.status, 0, Q4_TIMEOUT_WEIGHTS);
+                    ok = false;
+                }
+                const unsigned char* at_unit = ring + slot * F::kUnit;
+                uint4 w[kBatch];
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) w[j] = *reinterpret_cast<const uint4*>(at_unit + j * kTileBytes + lane * 16);
+                unsigned sc[2][2 * PARTS];               // rows g and g + 8: the stretch's 4 or 8 scales
+#pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int k = (kt + j) * 64 + 32 * h + 8 * t, tok = 8 * i + g;
-                    x[j][i][h] = tok < n && k < a.K ? *reinterpret_cast<const uint4*>(a.x + (size_t)tok * a.ldx + k) : make_uint4(0u, 0u, 0u, 0u);
-                }
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    float part[NT][4];
-#pragma unroll
-                    for (int i = 0; i < NT; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) part[i][e] = 0.f;
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const unsigned word = h ? (s ? w[r][j].w : w[r][j].z) : (s ? w[r][j].y : w[r][j].x);
-                        const unsigned a0 = pair(word, 0), a1 = pair(word, 1), a2 = pair(word, 2), a3 = pair(word, 3);
-#pragma unroll
-                        for (int i = 0; i < NT; ++i) mma16(part[i], a0, a1, a2, a3, s ? x[j][i][h].z : x[j][i][h].x, s ? x[j][i][h].w : x[j][i][h].y);
-                    }
-                    const float s0 = bf16_of(sc[r][0][j], h), s1 = bf16_of(sc[r][1][j], h);
-#pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        total[r][i][0] = fmaf(s0, part[i][0], total[r][i][0]);
-                        total[r][i][1] = fmaf(s0, part[i][1], total[r][i][1]);
-                        total[r][i][2] = fmaf(s1, part[i][2], total[r][i][2]);
-                        total[r][i][3] = fmaf(s1, part[i][3], total[r][i][3]);
+                    const unsigned char* s = at_unit + kBatch * kTileBytes + (g + 8 * h) * (TWO ? 16 : 8);
+                    if (TWO) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(s);
+                        sc[h][0] = v.x; sc[h][1] = v.y; sc[h][2 * PARTS - 2] = v.z; sc[h][2 * PARTS - 1] = v.w;
+                    } else {
+                        const uint2 v = *reinterpret_cast<const uint2*>(s);
+                        sc[h][0] = v.x; sc[h][1] = v.y;
                     }
                 }
-    }
-    if (!waited) pdl_wait();
+                __syncwarp();                            // the unit is in registers
+                ++unit;
+                if (lane == 0 && unit + AHEAD <= total_units && ok) fetch(slot);
+                if (++slot == AHEAD) { slot = 0; phase ^= 1; }
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+                for (int j = 0; j < kBatch; ++j)
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+                    for (int p = 0; p < PARTS; ++p) {
+                        float part[NT][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sums[warp][r * 16 + g + 8 * (e >> 1)][8 * i + 2 * t + (e & 1)] = total[r][i][e];
-    __syncthreads();
-    const int rows = a.end == END_GATED ? R * 8 : R * 16, m_out = a.end == END_GATED ? a.M / 2 : a.M;
-    for (int i = threadIdx.x; i < rows * n; i += kWarps * 32) {
-        const int row = i % rows, tok = i / rows, out = tile0 * (a.end == END_GATED ? 8 : 16) + row;
-        if (out >= m_out) continue;
-        const int at = a.end == END_GATED ? (row >> 3) * 16 + (row & 7) : row;
-        float y = 0.f, up = 0.f;
+                        for (int q = 0; q < 4 / PARTS; ++q) {
+                            const int s = p * 2 + q;
+                            const unsigned lo = s == 0 ? w[j].x : s == 1 ? w[j].y : s == 2 ? w[j].z : w[j].w, hi = lo >> 8;
+                            const unsigned a0 = lo & 0x000f000fu, a1 = lo & 0x00f000f0u, a2 = hi & 0x000f000fu, a3 = hi & 0x00f000f0u;
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) y += sums[k][at][tok];
-        if (a.end == END_GATED) {
+                            for (int i = 0; i < NT; ++i) {
+                                const uint4& v = x[j][i][s >> 1];
+                                mma16_onto(part[i], a0, a1, a2, a3, s & 1 ? v.z : v.x, s & 1 ? v.w : v.y, q == 0 ? start[j][p][i] : part[i]);
+                            }
+                        }
+                        const int at = j * PARTS + p;    // of the stretch's scales
+                        const float m0 = bf16_of(sc[0][at >> 1], at & 1), m8 = bf16_of(sc[1][at >> 1], at & 1);
 #pragma unroll
-            for (int k = 0; k < kWarps; ++k) up += sums[k][at + 8][tok];
-            y = y / (1.0f + __expf(-y)) * up;
+                        for (int i = 0; i < NT; ++i) {
+                            total[i][0] = fmaf(m0, part[i][0], total[i][0]);
+                            total[i][1] = fmaf(m0, part[i][1], total[i][1]);
+                            total[i][2] = fmaf(m8, part[i][2], total[i][2]);
+                            total[i][3] = fmaf(m8, part[i][3], total[i][3]);
+                        }
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                *reinterpret_cast<float2*>(to + 8 * i) = make_float2(total[i][0] * 0x1p66f * back[i][0], total[i][1] * 0x1p66f * back[i][1]);
+                *reinterpret_cast<float2*>(to + 8 * 8 * NT + 8 * i) = make_float2(total[i][2] * 0x1p62f * back[i][0], total[i][3] * 0x1p62f * back[i][1]);
+            }
         }
-        const size_t to = (size_t)tok * a.ldy + out;
-        if (a.end == END_ADD) reinterpret_cast<float*>(a.y)[to] += y;
-        else if (a.y_f32) reinterpret_cast<float*>(a.y)[to] = y;
-        else reinterpret_cast<__nv_bfloat16*>(a.y)[to] = __float2bfloat16_rn(y);
+        __syncthreads();
+        for (int i = threadIdx.x; i < count * F::kSums; i += kWarps * 32) {
+            const float* from = partial + i / F::kSums * kWarps * F::kSums + i % F::kSums;
+            float y = 0.f;
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) y += from[k * F::kSums];
+            sums[i] = y;
+        }
+        if (fa.chunks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+        else __syncthreads();
+        // out: the cluster's blocks take tiles in turn
+        const unsigned base = smem_u32(sums);
+        const int mine = (count - rank + fa.chunks - 1) / fa.chunks;
+        for (int i = threadIdx.x; i < mine * rows * n; i += kWarps * 32) {
+            const int row = i % rows, tok = i / rows % n, slot = i / (rows * n) * fa.chunks + rank, out = (b0 + slot) * rows + row;
+            if (out >= m_out) continue;
+            const unsigned at = base + (unsigned)((slot * 16 + row) * 8 * NT + tok) * 4;
+            float y = 0.f, up = 0.f;
+            for (int r = 0; r < fa.chunks; ++r) {
+                y += shared_of(at, r);
+                if (a.end == END_GATED) up += shared_of(at + 8 * 8 * NT * 4, r);
+            }
+            if (a.end == END_GATED) y = y / (1.0f + __expf(-y)) * up;
+            const size_t to = (size_t)(tok0 + tok) * a.ldy + out;
+            if (a.end == END_ADD) reinterpret_cast<float*>(a.y)[to] += y;
+            else if (a.y_f32) reinterpret_cast<float*>(a.y)[to] = y;
+            else reinterpret_cast<__nv_bfloat16*>(a.y)[to] = __float2bfloat16_rn(y);
+        }
+        // nobody writes sums again while another block reads them, nor leaves
+        if (fa.chunks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+        else if (b0 + F::kSlots < t_hi) __syncthreads();
     }
+    // (a wait that ran out: what is still on its way lands before the block ends)
+    if (!ok && lane == 0)
+        for (int j = 0; j < AHEAD && unit + j < total_units; ++j) tc5::mbar_wait(full + (slot + j) % AHEAD, slot + j < AHEAD ? phase : phase ^ 1);
 }
 
-template <int R, int NT>
-static void launch_skinny(const Args& a, cudaStream_t stream) {
-    const dim3 grid(((a.M + 15) / 16 + R - 1) / R);
-    blm_launch_dependent(skinny_kernel<R, NT>, grid, dim3(kWarps * 32), 0, stream, a);
+// The places of a cluster of eight blocks: longer rows run the other kernel whatever the tokens.
+constexpr int kFewTokens = 32, kFewTiles = 8 * kChunk;
+
+template <int NT, bool TWO>
+static int launch_few(const Args& a, int* status, cudaStream_t stream) {
+    using F = Few<NT>;
+    FewArgs fa{a, (a.stretches + kWarps - 1) / kWarps, 0, status};
+    const int tiles = (a.M + 15) / 16, tok_blocks = (a.N + 8 * NT - 1) / (8 * NT);
+    static bool opted_in[64] = {};
+    static int resident[64][9] = {};                     // clusters of so many blocks that the device holds at once
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return blm_fail(BLM_CUDA_ERROR, "gemm_q4: device %d", dev);
+    if (!opted_in[dev]) {
+        if (cudaFuncSetAttribute(few_kernel<NT, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem) != cudaSuccess)
+            return blm_fail(BLM_CUDA_ERROR, "gemm_q4: %s", cudaGetErrorString(cudaGetLastError()));
+        opted_in[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = F::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = fa.chunks;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = fa.chunks > 1 ? 2 : 1;
+    if (resident[dev][fa.chunks] == 0) {
+        // (a cluster lies in one group of SMs, which a number of blocks need not divide)
+        int fit = blm_sm_count() * F::kBlocks;
+        cfg.gridDim = dim3(fa.chunks);
+        if (fa.chunks > 1 && (cudaOccupancyMaxActiveClusters(&fit, few_kernel<NT, TWO>, &cfg) != cudaSuccess || fit < 1)) {
+            cudaGetLastError();
+            fit = blm_sm_count() * F::kBlocks / (2 * fa.chunks);
+        }
+        resident[dev][fa.chunks] = fit < 1 ? 1 : fit;
+    }
+    fa.clusters = resident[dev][fa.chunks] / tok_blocks;
+    if (fa.clusters > tiles) fa.clusters = tiles;
+    if (fa.clusters < 1) fa.clusters = 1;
+    cfg.gridDim = dim3(fa.chunks * fa.clusters, tok_blocks);
+    cudaLaunchKernelEx(&cfg, few_kernel<NT, TWO>, fa);
+    return blm_check_launch("gemm_q4");
 }
 
 // ---- many tokens -----------------------------------------------------------------------------------------------------------
@@ -177,7 +348,7 @@ __host__ __device__ constexpr int rho_of(int g) { return (g & 1) << 2 | g >> 1; 
 
 struct WideArgs {
     Args a;
-    int share;                   // k tiles of a block of the cluster, a multiple of 4 where there are several
+    int share;                   // k tiles of a block of the cluster, whole stretches
     int vec;                     // rows of y and their beginnings allow four results at once
     int* status;
 };
@@ -199,7 +370,7 @@ __device__ __forceinline__ void copy_async(unsigned dst, const void* src, int by
     else if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(dst), "l"(src) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ float4 shared_of(unsigned mine, int rank) {                    // the same place in the shared memory of a block of the cluster
+__device__ __forceinline__ float4 four_of(unsigned mine, int rank) {
     unsigned at;
     float4 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(mine), "r"(rank));
@@ -210,6 +381,7 @@ __device__ __forceinline__ float4 shared_of(unsigned mine, int rank) {          
 template <int N>
 __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kernel(const WideArgs wa, const __grid_constant__ CUtensorMap xmap) {
     using namespace tc5;
+    using tc5::smem_u32;
     using W = Wide<N>;
     constexpr int S = W::kStages, AHEAD = W::kAhead;
     const Args& a = wa.a;
@@ -282,13 +454,14 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
         const bool here = row0 / 16 + rows16 < tiles, two = a.per_tile == 2;      // (rows beyond the last tile are not written: any numbers do)
         unsigned char* mine = packed + (warp - 2) * AHEAD * W::kUnit;
         const unsigned at = smem_u32(mine);
-        const uint4* w_at = a.w + ((size_t)tile * a.k_tiles + kt0 + x) * 32 + lane;
-        const __nv_bfloat16* s_at = a.scales + (size_t)(tile * 16 + (lane & 15)) * a.row_scales + kt0 * a.per_tile;      // lanes 0 .. 15: a row each
+        const unsigned char* w_at = a.w + ((size_t)tile * a.stretches + kt0 / kBatch) * a.unit;
         auto fetch = [&](int p, int slot_of) {
             if (here && 2 * p + x < n_k) {
                 const unsigned to = at + slot_of * W::kUnit;
-                copy_async(to + lane * 16, w_at + (size_t)p * 64, 16);
-                if (lane < 16) copy_async(to + kTileBytes + lane * 8, s_at + p * 2 * a.per_tile, 4 * a.per_tile);
+                const unsigned char* from = w_at + (size_t)(p >> 1) * a.unit;      // the pair's stretch
+                copy_async(to + lane * 16, from + (2 * (p & 1) + x) * kTileBytes + lane * 16, 16);
+                if (lane < 16)                           // the pair's scales, lanes 0 .. 15 a row each
+                    copy_async(to + kTileBytes + lane * 8, from + kBatch * kTileBytes + (lane * 2 + (p & 1)) * 4 * a.per_tile, 4 * a.per_tile);
             }
             asm volatile("cp.async.commit_group;\n" ::: "memory");
         };
@@ -377,10 +550,10 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
             const unsigned place = base + (unsigned)(c * 128 + row) * 4;
             float y[4] = {0.f, 0.f, 0.f, 0.f}, up[4] = {0.f, 0.f, 0.f, 0.f};
             for (int r = 0; r < ranks; ++r) {
-                const float4 v = shared_of(place, r);
+                const float4 v = four_of(place, r);
                 y[0] += v.x; y[1] += v.y; y[2] += v.z; y[3] += v.w;
                 if (gated) {
-                    const float4 u = shared_of(place + 32, r);
+                    const float4 u = four_of(place + 32, r);
                     up[0] += u.x; up[1] += u.y; up[2] += u.z; up[3] += u.w;
                 }
             }
@@ -461,22 +634,22 @@ static int launch_wide(const Args& a, int* status, cudaStream_t stream) {
 }
 }  // namespace q4
 
-BLM_API int blm_gemm_q4(const void* w, const void* scales, int row_scales, int group, const void* x, long long ldx, void* y, long long ldy, int y_f32,
-                        int end, int n, int m, int k, int* status, cudaStream_t stream) {
+BLM_API int blm_gemm_q4(const void* w, int stretches, int group, const void* x, long long ldx, void* y, long long ldy, int y_f32, int end, int n, int m,
+                        int k, int* status, cudaStream_t stream) {
     using namespace q4;
     if (n == 0 || m == 0) return BLM_OK;
     BLM_REQUIRE(group == 32 || group == 64 || group == 128, "gemm_q4: groups of %d places (32, 64 or 128)", group);
     BLM_REQUIRE(k > 0 && k % 8 == 0 && ldx % 8 == 0 && ((size_t)x & 15) == 0, "gemm_q4: rows of tokens in pieces of 16 bytes");
+    BLM_REQUIRE(((size_t)w & 15) == 0, "gemm_q4: weights begin at a multiple of 16 bytes");
     BLM_REQUIRE(end != END_GATED || m % 16 == 0, "gemm_q4: gated rows come in tiles of 16, got %d", m);
-    const int k_tiles = (k + 63) / 64;
-    const int per_tile = group == 32 ? 2 : 1;
-    BLM_REQUIRE(row_scales == (k_tiles + kBatch - 1) / kBatch * kBatch * per_tile, "gemm_q4: %d scales a row for %d places", row_scales, k);
-    const Args a{(const uint4*)w, (const __nv_bfloat16*)scales, (const __nv_bfloat16*)x, ldx, y, ldy, y_f32, end, n, m, k, k_tiles, row_scales, per_tile};
-    if (n > 16) {
+    const int k_tiles = (k + 63) / 64, per_tile = group == 32 ? 2 : 1;
+    BLM_REQUIRE(stretches == (k_tiles + kBatch - 1) / kBatch, "gemm_q4: %d stretches a row for %d places", stretches, k);
+    const Args a{(const unsigned char*)w, (const __nv_bfloat16*)x, ldx, y, ldy, y_f32, end, n, m, k, k_tiles, stretches, kBatch * kTileBytes + 128 * per_tile, per_tile};
+    if (n > kFewTokens || k_tiles > kFewTiles) {
         BLM_REQUIRE((m + 127) / 128 <= 65535 && (n + 255) / 256 <= 65535, "gemm_q4: %d tokens, %d rows", n, m);
         return n <= 32 ? launch_wide<32>(a, status, stream) : n <= 64 ? launch_wide<64>(a, status, stream)
                : n <= 128 ? launch_wide<128>(a, status, stream) : launch_wide<256>(a, status, stream);
     }
-    if (n <= 8) launch_skinny<2, 1>(a, stream); else launch_skinny<2, 2>(a, stream);
-    return blm_check_launch("gemm_q4");
+    if (n <= 8) return per_tile == 2 ? launch_few<1, true>(a, status, stream) : launch_few<1, false>(a, status, stream);
+    return per_tile == 2 ? launch_few<2, true>(a, status, stream) : launch_few<2, false>(a, status, stream);
 }

@@ -259,7 +259,7 @@ _protos = {
         "blm_gemm_sk_squares_row": [],
     },
     "gemm_q4": {
-        "blm_gemm_q4": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
+        "blm_gemm_q4": [c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
     },
     "sampling": {
         "blm_argmax": [c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -1120,7 +1120,7 @@ _WAITS = {
     41: "gemm_sk: the tensor-core thread waited in vain for a stage", 42: "gemm_sk: the producer waited in vain for a free stage",
     43: "gemm_sk: the epilogue waited in vain for the accumulator",
     51: "attention over 8 bits: a consumer waited in vain for a page", 52: "attention over 8 bits: the producer waited in vain for a free stage",
-    53: "product with 4-bit weights: a wait ran out"}
+    53: "product with 4-bit weights, many tokens: a wait ran out", 54: "product with 4-bit weights, few tokens: a warp waited in vain for its weights"}
 
 
 def check_status(device) -> None:
@@ -2191,12 +2191,11 @@ _Q4_STRETCH = 256             # places of K that a warp of the product's kernels
 
 
 class Q4Weight:
-    """A weight [out_features, in_features] in 4 bits, as pack_q4 and quantize_q4 make it: whole numbers of -8 .. 7 in the order in which
-    the kernels read them, and bfloat16 scales [rows filled up to 16, one for every 32 places (groups of 32) or 64 (a group of 128 has its
-    own twice), filled up to 256 places]."""
+    """A weight [out_features, in_features] in 4 bits, as pack_q4 and quantize_q4 make it: `packed` uint8 [tiles of 16 rows, stretches of 256
+    places, bytes], a stretch's whole numbers of -8 .. 7 in the order in which the kernels read them and behind them its bfloat16 scales."""
 
-    def __init__(self, packed, scales, out_features, in_features, group):
-        self.packed, self.scales = packed, scales
+    def __init__(self, packed, out_features, in_features, group):
+        self.packed = packed
         self.out_features, self.in_features, self.group = out_features, in_features, group
 
     @property
@@ -2204,13 +2203,13 @@ class Q4Weight:
         return self.packed.device
 
     def bytes(self) -> int:
-        return self.packed.numel() + 2 * self.scales.numel()
+        return self.packed.numel()
 
     def first_rows(self, rows: int) -> "Q4Weight":
         """The weight's first `rows` rows (a view; whole tiles of 16)."""
         if rows % 16 or not 0 < rows <= self.out_features:
             raise KernelError(f"a weight in 4 bits gives its first rows by tiles of 16; {rows} of {self.out_features} asked for")
-        return Q4Weight(self.packed[: rows // 16], self.scales[:rows], rows, self.in_features, self.group)
+        return Q4Weight(self.packed[: rows // 16], rows, self.in_features, self.group)
 
 
 def _five_bits(x):
@@ -2242,22 +2241,22 @@ def pack_q4(values, scales, group) -> Q4Weight:
     s = scales.to(torch.float32)
     if not torch.equal(_five_bits(s), s) or not torch.isfinite(s).all():
         raise KernelError("pack_q4: scales are finite and have five significant bits at most")
-    tiles, k_tiles = -(-m // 16), -(-k // 64)
-    stretches = -(-k_tiles * 64 // _Q4_STRETCH)
-    packed_scales = torch.zeros((tiles * 16, stretches * (_Q4_STRETCH // min(group, 64))), dtype=torch.bfloat16, device=values.device)
-    if group == 128:
-        s = s.repeat_interleave(2, dim=1)[:, : packed_scales.shape[1]]
-    packed_scales[:m, : s.shape[1]] = s
+    tiles, stretches, per = -(-m // 16), -(-k // _Q4_STRETCH), _Q4_STRETCH // min(group, 64)
+    wide = torch.zeros((tiles * 16, stretches * per), dtype=torch.bfloat16, device=values.device)
+    if group == 128:                                     # a scale for every 64 places
+        s = s.repeat_interleave(2, dim=1)[:, : wide.shape[1]]
+    wide[:m, : s.shape[1]] = s
     row, place = _q4_order(values.device)
-    packed = torch.empty((tiles, k_tiles, 512), dtype=torch.uint8, device=values.device)
+    packed = torch.empty((tiles, stretches, 2048 + 32 * per), dtype=torch.uint8, device=values.device)
+    packed[:, :, 2048:] = wide.view(tiles, 16, stretches, per).permute(0, 2, 1, 3).contiguous().view(torch.uint8).view(tiles, stretches, -1)
     for t0 in range(0, tiles, 256):                      # some tiles at a time: an embedding's table would fill the memory
         t1 = min(tiles, t0 + 256)
-        u = torch.full(((t1 - t0) * 16, k_tiles * 64), 8, dtype=torch.uint8, device=values.device)
+        u = torch.full(((t1 - t0) * 16, stretches * _Q4_STRETCH), 8, dtype=torch.uint8, device=values.device)
         part = values[t0 * 16: min(m, t1 * 16)]
         u[: part.shape[0], :k] = (part + 8).to(torch.uint8)
-        u = u.view(t1 - t0, 16, k_tiles, 64).permute(0, 2, 1, 3)[:, :, row, place]          # [tiles, k tiles, 32, 4, 8]
-        packed[t0:t1] = (u[..., 0::2] | (u[..., 1::2] << 4)).reshape(t1 - t0, k_tiles, 512)
-    return Q4Weight(packed, packed_scales, m, k, group)
+        u = u.view(t1 - t0, 16, stretches * 4, 64).permute(0, 2, 1, 3)[:, :, row, place]          # [tiles, k tiles, 32, 4, 8]
+        packed[t0:t1, :, :2048] = (u[..., 0::2] | (u[..., 1::2] << 4)).reshape(t1 - t0, stretches, 2048)
+    return Q4Weight(packed, m, k, group)
 
 
 def quantize_q4(w, group=64) -> Q4Weight:
@@ -2289,16 +2288,18 @@ def quantize_q4(w, group=64) -> Q4Weight:
 
 def q4_values(w) -> torch.Tensor:
     """The bfloat16 weight [out_features, in_features] that a weight in 4 bits stands for, exactly.  Plain tensor operations, on any device."""
-    tiles, k_tiles = w.packed.shape[:2]
+    tiles, stretches = w.packed.shape[:2]
     row, place = _q4_order(w.device)
-    out = torch.empty((tiles * 16, k_tiles * 64), dtype=torch.bfloat16, device=w.device)
+    out = torch.empty((tiles * 16, stretches * _Q4_STRETCH), dtype=torch.bfloat16, device=w.device)
     for t0 in range(0, tiles, 256):
-        p = w.packed[t0: t0 + 256].view(-1, k_tiles, 32, 4, 4)
-        n = torch.stack([p & 15, p >> 4], dim=-1).reshape(p.shape[0], k_tiles, 32, 4, 8)
-        tile = torch.empty((p.shape[0], k_tiles, 16, 64), dtype=torch.bfloat16, device=w.device)
-        tile[:, :, row, place] = n.to(torch.bfloat16) - 8
-        s = w.scales[t0 * 16: (t0 + p.shape[0]) * 16].repeat_interleave(min(w.group, 64), dim=1)[:, : k_tiles * 64]
-        out[t0 * 16: (t0 + p.shape[0]) * 16] = tile.permute(0, 2, 1, 3).reshape(-1, k_tiles * 64) * s
+        unit = w.packed[t0: t0 + 256]
+        n = unit.shape[0]
+        p = unit[:, :, :2048].reshape(n, stretches * 4, 32, 4, 4)
+        u = torch.stack([p & 15, p >> 4], dim=-1).reshape(n, stretches * 4, 32, 4, 8)
+        tile = torch.empty((n, stretches * 4, 16, 64), dtype=torch.bfloat16, device=w.device)
+        tile[:, :, row, place] = u.to(torch.bfloat16) - 8
+        s = unit[:, :, 2048:].contiguous().view(torch.bfloat16).view(n, stretches, 16, -1).permute(0, 2, 1, 3).reshape(n * 16, -1)
+        out[t0 * 16: (t0 + n) * 16] = tile.permute(0, 2, 1, 3).reshape(n * 16, -1) * s.repeat_interleave(min(w.group, 64), dim=1)
     return out[: w.out_features, : w.in_features].contiguous()
 
 
@@ -2334,7 +2335,7 @@ def product_q4(w, x, out=None, add_into=None, swiglu=False):
         wide = torch.zeros((n, -(-k // 64) * 64), dtype=torch.bfloat16, device=x.device)
         wide[:, :k] = x
         x, k = wide, wide.shape[1]
-    _call("gemm_q4", "blm_gemm_q4", _ptr(w.packed), _ptr(w.scales), w.scales.shape[1], w.group, _ptr(x), x.stride(0), _ptr(y), y.stride(0),
+    _call("gemm_q4", "blm_gemm_q4", _ptr(w.packed), w.packed.shape[1], w.group, _ptr(x), x.stride(0), _ptr(y), y.stride(0),
           1 if y.dtype == torch.float32 else 0, Q4_ADD if add_into is not None else (Q4_GATED if swiglu else Q4_STORE), n, m, k,
           status_word(x.device).data_ptr(), _stream())
     return y
