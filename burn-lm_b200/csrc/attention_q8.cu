@@ -22,7 +22,7 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 BLM_API const char* blm_attention_q8_last_error() { return g_blm_error; }
 
@@ -510,40 +510,19 @@ struct TokenArgs {
     int* status;
 };
 enum { Q8_TIMEOUT_PAGE = 51, Q8_TIMEOUT_FREE = 52 };
-constexpr unsigned kSpinLimit = 1u << 22;
+using tc5::mbar_arrive;
+using tc5::mbar_expect_tx;
+using tc5::mbar_init;
+using tc5::mbar_wait;
+using tc5::smem_u32;
 
-__device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void mbar_init(unsigned long long* bar, unsigned count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(count));
-}
-__device__ __forceinline__ void mbar_expect_tx(unsigned long long* bar, unsigned bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(unsigned long long* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ bool mbar_wait(unsigned long long* bar, unsigned parity) {
-    const unsigned addr = smem_u32(bar);
-    for (unsigned spin = 0; spin < kSpinLimit; ++spin) {
-        unsigned done;
-        asm volatile(
-            "{\n.reg .pred p;\n"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-            "selp.u32 %0, 1, 0, p;\n}\n"
-            : "=r"(done)
-            : "r"(addr), "r"(parity)
-            : "memory");
-        if (done) return true;
-    }
-    return false;
-}
 __device__ __forceinline__ void bulk_copy(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
                  "r"(smem_u32(bar))
                  : "memory");
 }
 template <bool HALF>
-__device__ __forceinline__ void mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+__device__ __forceinline__ void mma_sync(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
     if (HALF)
         asm volatile(
             "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -726,8 +705,8 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
 #pragma unroll
             for (int j = 0; j < KS / 2; ++j) {
                 const uint4 x = seen0 ? r0[j] : make_uint4(0u, 0u, 0u, 0u), y = seen2 ? r2[j] : make_uint4(0u, 0u, 0u, 0u);
-                mma<false>(c, x.x, y.x, x.y, y.y, qf[2 * j][0], qf[2 * j][1]);
-                mma<false>(c, x.z, y.z, x.w, y.w, qf[2 * j + 1][0], qf[2 * j + 1][1]);
+                mma_sync<false>(c, x.x, y.x, x.y, y.y, qf[2 * j][0], qf[2 * j][1]);
+                mma_sync<false>(c, x.z, y.z, x.w, y.w, qf[2 * j + 1][0], qf[2 * j + 1][1]);
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) c[e] = (e < 2 ? seen0 : seen2) ? c[e] * a.scale_log2e : -INFINITY;
@@ -753,7 +732,7 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
                 for (int n = 0; n < 4; ++n) {
                     const unsigned w0 = n == 0 ? v[0].x : n == 1 ? v[0].y : n == 2 ? v[0].z : v[0].w, w1 = n == 0 ? v[1].x : n == 1 ? v[1].y : n == 2 ? v[1].z : v[1].w;
                     const unsigned w2 = n == 0 ? v[2].x : n == 1 ? v[2].y : n == 2 ? v[2].z : v[2].w, w3 = n == 0 ? v[3].x : n == 1 ? v[3].y : n == 2 ? v[3].z : v[3].w;
-                    mma<false>(st.o[4 * j + n], __byte_perm(w0, w1, 0x5410), __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x5410), __byte_perm(w2, w3, 0x7632), b0, b1);
+                    mma_sync<false>(st.o[4 * j + n], __byte_perm(w0, w1, 0x5410), __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x5410), __byte_perm(w2, w3, 0x7632), b0, b1);
                 }
             }
         }
@@ -824,7 +803,7 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
                     const unsigned xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        mma<true>(c, biased_two<0>(xw[i]), biased_two<0>(yw[i]), biased_two<2>(xw[i]), biased_two<2>(yw[i]), qf[4 * j + i][0], qf[4 * j + i][1]);
+                        mma_sync<true>(c, biased_two<0>(xw[i]), biased_two<0>(yw[i]), biased_two<2>(xw[i]), biased_two<2>(yw[i]), qf[4 * j + i][0], qf[4 * j + i][1]);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) c[e] = fmaf(c[e], e & 1 ? f1 : f0, lv);
@@ -855,8 +834,8 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
 #pragma unroll
                     for (int j = 0; j < HD / 32; ++j) {
                         const uint4 v = vr[(ch * (HD / 32) + j) * 32];
-                        mma<true>(st.o[2 * j], two_of<0>(v.x), two_of<0>(v.y), two_of<2>(v.x), two_of<2>(v.y), b0, b1);
-                        mma<true>(st.o[2 * j + 1], two_of<0>(v.z), two_of<0>(v.w), two_of<2>(v.z), two_of<2>(v.w), b0, b1);
+                        mma_sync<true>(st.o[2 * j], two_of<0>(v.x), two_of<0>(v.y), two_of<2>(v.x), two_of<2>(v.y), b0, b1);
+                        mma_sync<true>(st.o[2 * j + 1], two_of<0>(v.z), two_of<0>(v.w), two_of<2>(v.z), two_of<2>(v.w), b0, b1);
                     }
                 }
                 st.l[0] = fmaf(sum0, to_sum, st.l[0]);   // this thread's share
@@ -1004,6 +983,428 @@ static bool tokens_take(int dtype, int hd, int max_q_len, int n_seqs, int n_kv, 
     return dtype == BLM_BF16 && (hd == 64 || hd == 128) && max_q_len == 1 && n_seqs <= 65535 && (n_heads / n_kv + 7) / 8 * n_kv <= 65535;
 }
 
+// ---- several tokens ------------------------------------------------------------------------------------------------------
+// bfloat16 portions with heads of 64 or 128 lanes, on tcgen05.  A block owns the queries of one 64-position block of a sequence for up to
+// four heads of a kv head, in one or two tiles of 128 rows (two heads by 64 positions), and walks the sequence's blocks: those before its
+// own in 8 bits, unmasked but for a window's edge, then its own, unrounded and causal.  So every border of a page is a border of the mask.
+//   warp 13 copies pages (one bulk copy each: keys, values, scales) into a ring of three;
+//   warps 8 .. 11 turn a page into operands, once for both tiles: keys [64][D] and values transposed, [D][64], bfloat16 with the 128-byte
+//     swizzle, into rings of three each; a byte q + 128 in sixteen bits is the bfloat16 number (q + 128) 2^-133, and one subtraction makes
+//     it q 2^-133: two instructions for two numbers.  The values' rows stand in an order that keeps their eight-byte writes to two a bank;
+//   warp 12 (one thread) issues S = Q K^T and O += P V of both tiles.  Q lies in tensor memory (as a second operand in shared memory its
+//     reads, 32 KB a page and tile, would cost more than the products);
+//   warps 0 .. 7 are the softmax, a row a thread: Q times a power of two that brings the row's largest lane to 2^60 (the keys' 2^-133 has to
+//     meet ordinary numbers), scores times the keys' scale, a reference maximum that moves when a score exceeds it by 2^8, probabilities
+//     times the values' scale times 2^60, rounded to bfloat16, over the scores' columns.
+// A tile's scores of the next page are issued behind its product of this one, by the same thread, so one set of columns does; while one
+// tile waits for its products the other's softmax has the exponential unit, which bounds the whole together with the products.
+constexpr int kPromptThreads = 14 * 32, kPromptStages = 3;
+enum { Q8_TIMEOUT_PROMPT = 55 };
+struct PromptArgs {
+    AttendArgs a;
+    int head_groups, heads_a_group;      // of a kv head's queries: at most four heads each
+    int* status;
+};
+template <int HD> struct Prompt {
+    static constexpr int kTile = 64 * HD * 2;                                // bytes of a page's keys (or values) as operands
+    static constexpr int kRaw = (line_bytes(HD) + 127) / 128 * 128;
+    static constexpr int kSmem = kPromptStages * (2 * kTile + kRaw) + 4 * 8 + 24 * 8 + 16 + 1024;
+};
+// two bytes of a word as two bfloat16 numbers, (byte - 128) 2^-133
+template <int LO>
+__device__ __forceinline__ unsigned tiny_two(unsigned word) {
+    const unsigned p = __byte_perm(word, 0u, LO == 0 ? 0x4140 : 0x4342), less = 0x00800080u;
+    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&p), *reinterpret_cast<const __nv_bfloat162*>(&less));
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+
+// the halves of two bfloat16 numbers that are infinities or NaN, as masks
+__device__ __forceinline__ unsigned odd_two(unsigned v) {
+    return ((v & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((v & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const PromptArgs pa) {
+    using P = Prompt<HD>;
+    constexpr int KS = kPromptStages;
+    const AttendArgs& a = pa.a;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    unsigned char* keys = smem;                                              // [KS][HD / 64][64 keys][128 bytes]
+    unsigned char* values = keys + KS * P::kTile;                            // [KS][HD lanes][128 bytes: 64 keys]
+    unsigned char* raw = values + KS * P::kTile;                             // [KS][page]
+    float2* scales = reinterpret_cast<float2*>(raw + KS * P::kRaw);          // [4] of the pages in the works
+    unsigned long long* raw_full = reinterpret_cast<unsigned long long*>(scales + 4);
+    unsigned long long* raw_free = raw_full + KS;
+    unsigned long long* k_full = raw_free + KS;
+    unsigned long long* k_free = k_full + KS;
+    unsigned long long* v_full = k_free + KS;
+    unsigned long long* v_free = v_full + KS;
+    unsigned long long* s_full = v_free + KS;                                // [2] a tile's scores are formed
+    unsigned long long* p_full = s_full + 2;                                 // [2] its probabilities are written
+    unsigned long long* q_full = p_full + 2;
+    unsigned long long* o_done = q_full + 1;
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(o_done + 1);
+    unsigned* odd_values = tmem_slot + 1;                                    // [2] bits: keys of the own block whose values hold an infinity or a NaN
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int kvh = blockIdx.x / pa.head_groups, hg = blockIdx.x % pa.head_groups, seq = blockIdx.z;
+    pdl_wait();
+    const int tok0 = a.cu_seqlens[seq], n = a.cu_seqlens[seq + 1] - tok0, start = a.start_pos[seq], slot = a.slot_of_seq[seq], end = start + n;
+    // the sequence's last blocks, which walk furthest, begin first
+    const int mine = (end - 1) / kPage - (int)blockIdx.y;
+    if (n <= 0 || mine < start / kPage) return;          // (the whole block)
+    const int p0 = mine * kPage, group = a.n_heads / a.n_kv, head0 = kvh * group + hg * pa.heads_a_group;
+    const int G = min(pa.heads_a_group, group - hg * pa.heads_a_group), tiles = (G + 1) / 2;
+    auto first_key = [&](int pos) { return a.window > 0 ? max(0, pos + 1 - a.window) : 0; };
+    const int pg_lo = first_key(max(start, p0)) / kPage, steps = mine - pg_lo + 1;          // the last step is the own block
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < KS; ++s) {
+            mbar_init(raw_full + s, 1);
+            mbar_init(raw_free + s, 4);
+            mbar_init(k_full + s, 4);
+            mbar_init(k_free + s, 1);
+            mbar_init(v_full + s, 4);
+            mbar_init(v_free + s, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full + i, 1);
+            mbar_init(p_full + i, 4);
+        }
+        mbar_init(q_full, 4 * tiles);
+        mbar_init(o_done, 1);
+        odd_values[0] = odd_values[1] = 0u;
+        tc5::mbar_init_fence();
+    }
+    if (warp == 12) tc5::tmem_alloc(tmem_slot, 512);
+    tc5::fence_before();
+    __syncthreads();
+    tc5::fence_after();
+    pdl_launch_dependents();                              // (not before this block has its tensor memory: the next kernel may take some too)
+    // a tile's columns: 64 of scores (and probabilities), HD of sums, HD / 2 of queries
+    const unsigned tmem = *tmem_slot;
+    constexpr unsigned kTileCols = 256, kOCol = 64, kQCol = 64 + HD;
+    const int width = a.n_heads + 2 * a.n_kv;
+    const __nv_bfloat16* rows = reinterpret_cast<const __nv_bfloat16*>(a.rotated);
+    auto gave_up = [&] { atomicCAS(pa.status, 0, Q8_TIMEOUT_PROMPT); };
+
+    if (warp == 13) {
+        // ---- pages ----
+        int i = 0;
+        bool failed = false;
+        for (int base = pg_lo; base < mine; base += 32) {
+            const int count = min(32, mine - base);
+            const int my_page = lane < count ? page_of(a.block_table, a.table_stride, slot, base + lane, a.n_pages) : -1;
+            for (int j = 0; j < count; ++j) {
+                const int page = __shfl_sync(0xffffffffu, my_page, j);
+                if (lane != 0 || failed) continue;
+                const int s = i % KS;
+                if (i >= KS && !mbar_wait(raw_free + s, (i / KS - 1) & 1)) { gave_up(); failed = true; continue; }
+                ++i;
+                unsigned char* stage = raw + s * P::kRaw;
+                if (page < 0) {                          // none of the pool's: known by a scale below zero
+                    *const_cast<float2*>(scales_of(stage, HD)) = make_float2(0.f, -1.f);
+                    mbar_arrive(raw_full + s);
+                    continue;
+                }
+                mbar_expect_tx(raw_full + s, line_bytes(HD));
+                bulk_copy(stage, a.pool + ((size_t)page * a.n_kv + kvh) * line_bytes(HD), line_bytes(HD), raw_full + s);
+            }
+        }
+        if (lane == 0)
+            for (int k = max(0, i - KS); k < i; ++k) mbar_wait(raw_full + k % KS, (k / KS) & 1);     // nothing is on its way when the block ends
+    } else if (warp == 12) {
+        // ---- products ----
+        if (lane == 0) {
+            constexpr unsigned kScores = tc5::instruction(64), kSums = tc5::instruction(HD);
+            const unsigned long long k_desc = tc5::operand(keys, 2, 1024), v_desc = tc5::operand(values, 2, 1024);
+            auto scores = [&](int i, int j) {
+                const unsigned long long kd = k_desc + (unsigned)((j % KS) * (P::kTile >> 4));
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k)
+                    tc5::mma_ts(tmem + i * kTileCols, tmem + i * kTileCols + kQCol + 8 * k, kd + (unsigned)((k >> 2) * (8192 >> 4) + 2 * (k & 3)), kScores, k > 0);
+                tc5::commit(s_full + i);
+                if (i == tiles - 1) tc5::commit(k_free + j % KS);
+            };
+            bool ok = mbar_wait(q_full, 0) && mbar_wait(k_full, 0);
+            if (ok) {
+                tc5::fence_after();
+                for (int i = 0; i < tiles; ++i) scores(i, 0);
+            }
+            for (int j = 0; j < steps && ok; ++j) {
+                const int s = j % KS;
+                for (int i = 0; i < tiles && ok; ++i) {
+                    ok = mbar_wait(p_full + i, j & 1) && (i > 0 || mbar_wait(v_full + s, (j / KS) & 1));
+                    if (!ok) break;
+                    tc5::fence_after();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        tc5::mma_ts(tmem + i * kTileCols + kOCol, tmem + i * kTileCols + 8 * k, v_desc + (unsigned)(s * (P::kTile >> 4) + 2 * k), kSums, j > 0 || k > 0);
+                    if (i == tiles - 1) tc5::commit(v_free + s);
+                    if (j + 1 == steps) continue;
+                    ok = i > 0 || mbar_wait(k_full + (j + 1) % KS, ((j + 1) / KS) & 1);
+                    if (!ok) break;
+                    tc5::fence_after();
+                    scores(i, j + 1);
+                }
+            }
+            if (!ok) gave_up();
+            tc5::commit(o_done);                         // when all products so far are over
+        }
+    } else if (warp >= 8) {
+        // ---- operands ----
+        const int me = threadIdx.x - 256, cw = warp - 8;
+        bool ok = true;
+        for (int j = 0; j < steps && ok; ++j) {
+            const int s = j % KS, parity = (j / KS - 1) & 1;
+            const bool own = j == steps - 1;
+            unsigned char* kt = keys + s * P::kTile;
+            unsigned char* vt = values + s * P::kTile;
+            const unsigned char* page = raw + s * P::kRaw;
+            // row r of the own block: from the step, from what the step found, or none
+            auto own_row = [&](int r, int which) -> const __nv_bfloat16* {
+                const int pos = p0 + r;
+                if (pos >= end) return nullptr;
+                if (pos >= start) return rows + ((size_t)(tok0 + pos - start) * width + a.n_heads + which * a.n_kv + kvh) * HD;
+                return reinterpret_cast<const __nv_bfloat16*>(a.found) + ((((size_t)seq * 2 + which) * a.n_kv + kvh) * kPage + r) * HD;
+            };
+            if (!own && !mbar_wait(raw_full + s, (j / KS) & 1)) { ok = false; break; }
+            const float2 scale = own ? make_float2(1.f, 1.f) : *scales_of(page, HD);
+            const bool none = scale.y < 0.f;
+            if (j >= KS && !mbar_wait(k_free + s, parity)) { ok = false; break; }
+            if (own || none) {
+                for (int i = me; i < 64 * (HD / 8); i += 128) {
+                    const int r = i / (HD / 8), c = i % (HD / 8);
+                    const __nv_bfloat16* from = own ? own_row(r, 0) : nullptr;
+                    const uint4 v = from ? reinterpret_cast<const uint4*>(from)[c] : make_uint4(0u, 0u, 0u, 0u);
+                    *reinterpret_cast<uint4*>(kt + (c >> 3) * 8192 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+                }
+            } else {
+                // sixteen lanes of a key a thread: four pieces of a 64-lane half by eight keys a warp
+#pragma unroll
+                for (int i = 0; i < 64 * (HD / 16) / 128; ++i) {
+                    const int at = i * 4 + cw, half = HD == 128 ? at & 1 : 0, r = (HD == 128 ? at >> 1 : at) * 8 + (lane >> 2), piece = half * 4 + (lane & 3);
+                    const uint4 v = *reinterpret_cast<const uint4*>(page + key_piece(r, piece * 16, HD));
+                    unsigned char* to = kt + half * 8192 + r * 128;
+                    const int c = (lane & 3) * 2;
+                    *reinterpret_cast<uint4*>(to + ((c ^ (r & 7)) << 4)) = make_uint4(tiny_two<0>(v.x), tiny_two<2>(v.x), tiny_two<0>(v.y), tiny_two<2>(v.y));
+                    *reinterpret_cast<uint4*>(to + (((c + 1) ^ (r & 7)) << 4)) = make_uint4(tiny_two<0>(v.z), tiny_two<2>(v.z), tiny_two<0>(v.w), tiny_two<2>(v.w));
+                }
+            }
+            if (me == 0) scales[j & 3] = scale;
+            tc5::fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(k_full + s);
+            if (j >= KS && !mbar_wait(v_free + s, parity)) { ok = false; break; }
+            // the value of lane d stands in row d % (HD / 8) * 8 + d / (HD / 8)
+            if (own || none) {
+                for (int i = me; i < 16 * (HD / 8); i += 128) {
+                    const int k = i / (HD / 8) * 4, d = i % (HD / 8) * 8;
+                    uint4 v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const __nv_bfloat16* from = own ? own_row(k + e, 1) : nullptr;
+                        v[e] = from ? *reinterpret_cast<const uint4*>(from + d) : make_uint4(0u, 0u, 0u, 0u);
+                        // (a probability of zero does not silence an infinity or a NaN: those are put in at the end, by the rows that see them)
+                        if (odd_two(v[e].x) | odd_two(v[e].y) | odd_two(v[e].z) | odd_two(v[e].w)) {
+                            v[e] = make_uint4(v[e].x & ~odd_two(v[e].x), v[e].y & ~odd_two(v[e].y), v[e].z & ~odd_two(v[e].z), v[e].w & ~odd_two(v[e].w));
+                            atomicOr(odd_values + ((k + e) >> 5), 1u << ((k + e) & 31));
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        const unsigned w0 = x < 2 ? v[0].x : x < 4 ? v[0].y : x < 6 ? v[0].z : v[0].w, w1 = x < 2 ? v[1].x : x < 4 ? v[1].y : x < 6 ? v[1].z : v[1].w;
+                        const unsigned w2 = x < 2 ? v[2].x : x < 4 ? v[2].y : x < 6 ? v[2].z : v[2].w, w3 = x < 2 ? v[3].x : x < 4 ? v[3].y : x < 6 ? v[3].z : v[3].w;
+                        const int row = (d + x) % (HD / 8) * 8 + (d + x) / (HD / 8);
+                        *reinterpret_cast<uint2*>(vt + row * 128 + (((k >> 3) ^ (row & 7)) << 4) + (k & 4) * 2) =
+                            make_uint2(__byte_perm(w0, w1, x & 1 ? 0x7632 : 0x5410), __byte_perm(w2, w3, x & 1 ? 0x7632 : 0x5410));
+                    }
+                }
+            } else {
+                const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+                for (int i = 0; i < HD / 32; ++i) {      // warp cw has keys 16 cw .. 16 cw + 15
+                    const uint4 v = *reinterpret_cast<const uint4*>(page + kPage * HD + cw * (16 * HD) + i * 512 + lane * 16);
+                    const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int row = (4 * i + x) * 8 + g, c = 2 * cw + (t >> 1);
+                        *reinterpret_cast<uint2*>(vt + row * 128 + ((c ^ g) << 4) + (t & 1) * 8) = make_uint2(tiny_two<0>(w[x]), tiny_two<2>(w[x]));
+                    }
+                }
+            }
+            tc5::fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(v_full + s);
+                if (!own) mbar_arrive(raw_free + s);
+            }
+        }
+        if (!ok && lane == 0) gave_up();
+    } else if (warp < 4 * tiles) {
+        // ---- softmax: a row a thread ----
+        const int tile = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, pos = p0 + (r & 63), h = 2 * tile + (r >> 6);
+        const bool live = h < G && pos >= start && pos < end;
+        const unsigned at = tmem + tile * kTileCols + ((unsigned)(quarter * 32) << 16);
+        const size_t tok = (size_t)(tok0 + pos - start);
+        float to_log2;                                   // of a score of unrounded keys; of the others 2^133 times that
+        {
+            unsigned q[HD / 2];
+            const uint4* from = reinterpret_cast<const uint4*>(rows + (tok * width + head0 + h) * HD);
+            unsigned top = 0;                            // of two magnitudes' bits at once
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) {
+                const uint4 v = live ? from[i] : make_uint4(0u, 0u, 0u, 0u);
+                q[4 * i] = v.x; q[4 * i + 1] = v.y; q[4 * i + 2] = v.z; q[4 * i + 3] = v.w;
+                top = __vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), __vmaxu2(__vmaxu2(v.y & 0x7fff7fffu, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu));
+            }
+            const int e = (int)(max(top & 0xffffu, top >> 16) >> 7), by = e == 0 || e == 255 ? 60 : max(-59, min(127, 187 - e));
+            const unsigned factor = (unsigned)(127 + by) << 7, both = factor << 16 | factor;
+#pragma unroll
+            for (int i = 0; i < HD / 2; ++i) {
+                const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&q[i]), *reinterpret_cast<const __nv_bfloat162*>(&both));
+                q[i] = *reinterpret_cast<const unsigned*>(&v);
+            }
+#pragma unroll
+            for (int c = 0; c < HD / 2; c += 16) {
+                unsigned part[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) part[i] = q[c + i];
+                tc5::tmem_st16(at + kQCol + c, part);
+            }
+            tc5::wait_st();
+            to_log2 = a.scale_log2e * __uint_as_float((unsigned)(127 + 67 - by) << 23);    // times 2^66, or 2^-67
+            tc5::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+        const int lo = first_key(pos), warp_lo = first_key(p0 + (quarter & 1) * 32 + 31);          // the latest first key of the warp's rows
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int j = 0; j < steps; ++j) {
+            if (!mbar_wait(s_full + tile, j & 1)) { ok = false; break; }
+            tc5::fence_after();
+            const bool own = j == steps - 1;
+            const int key0 = (pg_lo + j) * kPage;
+            const float2 scale = scales[j & 3];
+            const float f = own ? to_log2 * 0x1p-67f : to_log2 * (0x1p66f * scale.x), by = own ? 0x1p-73f : (key0 + 63 < lo ? 0.f : scale.y * 0x1p60f);      // (a page that the row sees nothing of: whatever its scale)
+            float x[64];
+#pragma unroll
+            for (int c = 0; c < 64; c += 16) tc5::tmem_ld16(at + c, x + c);
+            tc5::wait_ld(x);
+            if (own || key0 < warp_lo || scale.y < 0.f) {
+#pragma unroll
+                for (int i = 0; i < 64; ++i)
+                    if ((own && key0 + i > pos) || key0 + i < lo || scale.y < 0.f) x[i] = -INFINITY;      // (f is not below zero)
+            }
+            float top[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+            for (int i = 4; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], x[i]);
+            const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
+            // (nothing seen: the product is minus infinity, or none where f is zero or none: neither moves the reference)
+            const bool move = mx > m + 8.f;
+            if (__any_sync(0xffffffffu, move)) {
+                const float alpha = move ? ex2(m - mx) : 1.f;
+                if (move) {
+                    m = mx;
+                    l *= alpha;
+                }
+                if (j > 0) {
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 16) {
+                        float o[16];
+                        tc5::tmem_ld16(at + kOCol + c, o);
+                        tc5::wait_ld(o);
+                        unsigned w[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(o[i] * alpha);
+                        tc5::tmem_st16(at + kOCol + c, w);
+                    }
+                }
+            }
+            const float less = m == -INFINITY ? 0.f : -m;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 32; c += 16) {
+                unsigned w[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    // (a hidden key's minus infinity times an f of zero would be none)
+                    const float a0 = x[2 * (c + i)], a1 = x[2 * (c + i) + 1];
+                    const float e0 = ex2(a0 == -INFINITY ? a0 : fmaf(a0, f, less)), e1 = ex2(a1 == -INFINITY ? a1 : fmaf(a1, f, less));
+                    sum[i & 3] += e0 + e1;
+                    w[i] = pack_bf16(e0 * by, e1 * by);
+                }
+                tc5::tmem_st16(at + c, w);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tc5::wait_st();
+            tc5::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + tile);
+        }
+        if (ok) ok = mbar_wait(o_done, 0);
+        if (!ok && lane == 0) gave_up();
+        tc5::fence_after();
+        if (ok) {
+            const float by = 1.f / l;
+            // the odd values among the keys that the row sees in its block
+            unsigned long long seen_odd = (unsigned long long)odd_values[1] << 32 | odd_values[0];
+            if (seen_odd != 0) {
+                seen_odd &= ~0ull >> (63 - (r & 63));
+                if (lo > p0) seen_odd &= ~0ull << (lo - p0);
+            }
+            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (tok * a.n_heads + head0 + h) * HD;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {           // columns n 8 + g: lanes g HD / 8 + n
+                float o[32];
+                tc5::tmem_ld16(at + kOCol + c, o);
+                tc5::tmem_ld16(at + kOCol + c + 16, o + 16);
+                tc5::wait_ld(o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] *= 0x1p73f * by;
+                if (live && seen_odd != 0)
+                    for (int k = 0; k < 64; ++k)
+                        if (seen_odd >> k & 1)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const int p = p0 + k;
+                                const __nv_bfloat16* from = p >= start ? rows + ((size_t)(tok0 + p - start) * width + a.n_heads + a.n_kv + kvh) * HD
+                                                                       : reinterpret_cast<const __nv_bfloat16*>(a.found) + ((((size_t)seq * 2 + 1) * a.n_kv + kvh) * kPage + k) * HD;
+                                const float v = __bfloat162float(from[(i & 7) * (HD / 8) + c / 8 + (i >> 3)]);
+                                if (!(fabsf(v) < INFINITY)) o[i] += v;
+                            }
+                if (live)
+#pragma unroll
+                    for (int g = 0; g < 8; ++g)
+                        *reinterpret_cast<uint2*>(out + g * (HD / 8) + c / 8) =
+                            make_uint2(pack_bf16(o[g], o[8 + g]), pack_bf16(o[16 + g], o[24 + g]));
+                __syncwarp();
+            }
+        }
+    }
+    tc5::fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc5::fence_after();
+        tc5::tmem_free(tmem, 512);
+    }
+}
+
+template <int HD>
+static int launch_prompt(const PromptArgs& pa, int max_q_len, cudaStream_t stream) {
+    const dim3 grid(pa.a.n_kv * pa.head_groups, (max_q_len + kPage - 2) / kPage + 1, pa.a.n_seqs);
+    static bool opted_in[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !opted_in[dev]) {
+        if (cudaFuncSetAttribute(attend_prompt_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Prompt<HD>::kSmem) != cudaSuccess)
+            return blm_fail(BLM_CUDA_ERROR, "attention_q8: %s", cudaGetErrorString(cudaGetLastError()));
+        if (dev >= 0 && dev < 64) opted_in[dev] = true;
+    }
+    blm_launch_dependent(attend_prompt_kernel<HD>, grid, dim3(kPromptThreads), Prompt<HD>::kSmem, stream, pa);
+    return blm_check_launch("attention_q8");
+}
+
 template <typename T, bool VEC>
 static int launch_append(const AppendArgs& a, int n_seqs, int max_q_len, cudaStream_t stream) {
     const size_t smem = (size_t)kPage * (a.hd + 16 / sizeof(T)) * sizeof(T) + kAppendThreads / 32 * sizeof(float);
@@ -1078,6 +1479,11 @@ BLM_API int blm_attention_q8(const void* rotated, const void* pool, const void* 
                            p.pages_per_split, status};
         if (hd == 64) return launch_tokens_as<64, 1>(ta, stream);
         return p.wpp == 1 ? launch_tokens_as<128, 1>(ta, stream) : launch_tokens_as<128, 2>(ta, stream);
+    }
+    if (dtype == BLM_BF16 && (hd == 64 || hd == 128) && max_q_len > 1 && n_seqs <= 65535 && max_q_len <= 4000000) {
+        const int group = n_heads / n_kv, groups = (group + 3) / 4;
+        const PromptArgs pa{a, groups, (group + groups - 1) / groups, status};
+        return hd == 64 ? launch_prompt<64>(pa, max_q_len, stream) : launch_prompt<128>(pa, max_q_len, stream);
     }
     const dim3 grid(n_heads * n_tokens);
     if (dtype == BLM_F32) blm_launch_dependent(attend_general_kernel<float>, grid, dim3(kGeneralWarps * 32), 0, stream, a);

@@ -395,7 +395,6 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = blockIdx.x, ranks = gridDim.x, row0 = blockIdx.y * 128, tok0 = blockIdx.z * N;
     const int kt0 = rank * wa.share, n_k = max(0, min(a.k_tiles - kt0, wa.share));          // this block's tiles of K
-    pdl_launch_dependents();
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(full + s, 1 + W::kWidenWarps);     // the tokens and every warp's weights
@@ -408,6 +407,7 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
     fence_before();
     __syncthreads();
     fence_after();
+    pdl_launch_dependents();                              // (not before this block has its tensor memory: the next kernel may take some too)
     const unsigned tmem = *slot;
     const int pairs = (n_k + 1) / 2;
 
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
             float v[16];
             if (n_k > 0) {
                 tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)c, v);
-                wait_ld();
+                wait_ld(v);
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) to[(c + e) * 128] = n_k > 0 ? v[e] : 0.f;

@@ -111,6 +111,13 @@ __device__ __forceinline__ void tmem_ld16(unsigned taddr, float* v) {
         : "r"(taddr));
 }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+// nothing that uses the registers is moved in front of the wait
+template <int N>
+__device__ __forceinline__ void wait_ld(float (&v)[N]) {
+    wait_ld();
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
+}
 __device__ __forceinline__ void tmem_st16(unsigned taddr, const unsigned (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(taddr),

@@ -1120,7 +1120,8 @@ _WAITS = {
     41: "gemm_sk: the tensor-core thread waited in vain for a stage", 42: "gemm_sk: the producer waited in vain for a free stage",
     43: "gemm_sk: the epilogue waited in vain for the accumulator",
     51: "attention over 8 bits: a consumer waited in vain for a page", 52: "attention over 8 bits: the producer waited in vain for a free stage",
-    53: "product with 4-bit weights, many tokens: a wait ran out", 54: "product with 4-bit weights, few tokens: a warp waited in vain for its weights"}
+    53: "product with 4-bit weights, many tokens: a wait ran out", 54: "product with 4-bit weights, few tokens: a warp waited in vain for its weights",
+    55: "attention over 8 bits, several tokens: a wait ran out"}
 
 
 def check_status(device) -> None:

@@ -438,3 +438,61 @@ def test_a_page_that_is_none():
         for _ in range(2):
             b.append([(0, 1)], check=False)
         assert torch.equal(b.pool, pool)
+
+
+@pytest.mark.parametrize("heads,n_kv,dim", [(8, 8, 64), (4, 2, 64), (6, 2, 128), (8, 2, 128), (5, 1, 64), (8, 1, 128), (12, 1, 64)])
+@pytest.mark.parametrize("window", [0, 100, 64, 1])
+def test_portions_of_any_group(heads, n_kv, dim, window):
+    """Portions of unequal lengths, from anywhere in a block, with one to twelve query heads a kv head."""
+    b = Batch(3, heads, n_kv, dim, BF16, 640, seed=heads + dim + window)
+    b.go([(0, 300), (1, 65), (2, 2)], window=window)
+    b.go([(0, 17), (1, 130), (2, 1)], window=window, padding=3)
+    b.go([(0, 3), (2, 61)], window=window)
+    b.go([(0, 64), (1, 2), (2, 200)], window=window)
+    K().check_status(torch.device("cuda:0"))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_later_tokens_that_are_no_numbers(dim, bad):
+    """A NaN or an infinity in a later key or value of the same block does not reach the queries before it; the rows that see it show it."""
+    k = K()
+    for which in (0, 1):                                 # in a key, in a value
+        b = Batch(1, 4, 1, dim, BF16, 256, seed=6)
+        qkv = b.rows(130)
+        clean = qkv.clone()
+        qkv.view(130, 6, dim)[100, 4 + which, 5] = bad
+        outs = []
+        for rows in (clean, qkv):
+            b = Batch(1, 4, 1, dim, BF16, 256, seed=6)
+            step, out, old = b.append([(0, 130)], qkv=rows.clone(), rot=0, check=False)
+            outs.append(b.attend([(0, 130)], step, out, old, check=False).view(130, 4, dim))
+        assert torch.equal(outs[0][:100], outs[1][:100]) and torch.isfinite(outs[1][:100]).all()
+        if which == 0:
+            assert not torch.isfinite(outs[1][100:]).any() or bad == float("inf")
+        else:
+            assert not torch.isfinite(outs[1][100:128, :, 5]).any()
+            others = [i for i in range(dim) if i != 5]
+            assert torch.equal(outs[1][100:128][:, :, others], outs[0][100:128][:, :, others])
+        assert not torch.isfinite(outs[1][128:]).all()   # the block with it reads as none of them numbers
+
+
+def test_a_page_of_nan_outside_a_window():
+    """A window's edge lies in a page whose scales are NaN: the rows that see none of it are untouched by it."""
+    b = Batch(1, 4, 1, 64, BF16, 512, seed=7)
+    b.append([(0, 64)], check=False)
+    page = int(b.table[0, 0])
+    step, out, old = b.append([(0, 130)], check=False)
+    good = b.attend([(0, 130)], step, out, old, window=40)
+    b.scales[page] = float("nan")
+    bad = b.attend([(0, 130)], step, out, old, window=40, check=False)
+    # positions 64 + t see keys from 64 + t - 39 on: those of the first page while t < 39
+    assert not torch.isfinite(bad[:39]).any() and torch.equal(bad[39:], good[39:])
+
+
+def test_long_portions():
+    b = Batch(2, 8, 2, 128, BF16, 3000, seed=13)
+    b.append([(0, 1800), (1, 70)], check=False)
+    step, out, old = b.append([(0, 90), (1, 300)], check=False)
+    b.attend([(0, 90), (1, 300)], step, out, old)
+    K().check_status(torch.device("cuda:0"))
