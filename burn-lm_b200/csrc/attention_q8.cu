@@ -1286,15 +1286,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             const bool own = j == steps - 1;
             const int key0 = (pg_lo + j) * kPage;
             const float2 scale = scales[j & 3];
-            const float f = own ? to_log2 * 0x1p-67f : to_log2 * (0x1p66f * scale.x), by = own ? 0x1p-73f : (key0 + 63 < lo ? 0.f : scale.y * 0x1p60f);      // (a page that the row sees nothing of: whatever its scale)
+            // probabilities leave times 2^shift, the values' scale times 2^60 (the own block's: 2^-73), and their sum is divided by it again
+            // (a block whose values are all next to zero: any scale will do; of a page that the row sees nothing of, whatever its scale)
+            const float f = own ? to_log2 * 0x1p-67f : to_log2 * (0x1p66f * scale.x);
+            const float vs = own ? 1.f : (key0 + 63 < lo || scale.y < 0x1p-100f ? 0x1p-100f : scale.y);
+            const float shift = own ? -73.f : __log2f(vs) + 60.f, to_sum = own ? 0x1p73f : 0x1p-60f / vs;
             float x[64];
 #pragma unroll
             for (int c = 0; c < 64; c += 16) tc5::tmem_ld16(at + c, x + c);
             tc5::wait_ld(x);
-            if (own || key0 < warp_lo || scale.y < 0.f) {
+            const bool masked = own || key0 < warp_lo || scale.y < 0.f;
+            auto hidden = [&](int i) { return (own && key0 + i > pos) || key0 + i < lo || scale.y < 0.f; };
+            if (masked) {
 #pragma unroll
                 for (int i = 0; i < 64; ++i)
-                    if ((own && key0 + i > pos) || key0 + i < lo || scale.y < 0.f) x[i] = -INFINITY;      // (f is not below zero)
+                    if (hidden(i)) x[i] = -INFINITY;     // (f is not below zero)
             }
             float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
@@ -1321,22 +1327,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                     }
                 }
             }
-            const float less = m == -INFINITY ? 0.f : -m;
+            const float less = shift - (m == -INFINITY ? 0.f : m);
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 64; ++i) {           // (a hidden key's minus infinity times an f of zero would be none)
+                    x[i] = x[i] == -INFINITY ? 0.f : ex2(fmaf(x[i], f, less));
+                    sum[i & 3] += x[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 64; ++i) {
+                    x[i] = ex2(fmaf(x[i], f, less));
+                    sum[i & 3] += x[i];
+                }
+            }
 #pragma unroll
             for (int c = 0; c < 32; c += 16) {
                 unsigned w[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    // (a hidden key's minus infinity times an f of zero would be none)
-                    const float a0 = x[2 * (c + i)], a1 = x[2 * (c + i) + 1];
-                    const float e0 = ex2(a0 == -INFINITY ? a0 : fmaf(a0, f, less)), e1 = ex2(a1 == -INFINITY ? a1 : fmaf(a1, f, less));
-                    sum[i & 3] += e0 + e1;
-                    w[i] = pack_bf16(e0 * by, e1 * by);
-                }
+                for (int i = 0; i < 16; ++i) w[i] = pack_bf16(x[2 * (c + i)], x[2 * (c + i) + 1]);
                 tc5::tmem_st16(at + c, w);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), to_sum, l);
             tc5::wait_st();
             tc5::fence_before();
             __syncwarp();
