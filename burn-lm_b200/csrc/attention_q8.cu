@@ -1008,7 +1008,8 @@ struct PromptArgs {
 template <int HD> struct Prompt {
     static constexpr int kTile = 64 * HD * 2;                                // bytes of a page's keys (or values) as operands
     static constexpr int kRaw = (line_bytes(HD) + 127) / 128 * 128;
-    static constexpr int kSmem = kPromptStages * (2 * kTile + kRaw) + 4 * 8 + 24 * 8 + 16 + 1024;
+    static constexpr int kRows = 256 * HD * 2;                               // queries on their way in, sums on their way out
+    static constexpr int kSmem = kPromptStages * (2 * kTile + kRaw) + kRows + 4 * 8 + 24 * 8 + 16 + 1024;
 };
 // two bytes of a word as two bfloat16 numbers, (byte - 128) 2^-133
 template <int LO>
@@ -1033,7 +1034,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     unsigned char* keys = smem;                                              // [KS][HD / 64][64 keys][128 bytes]
     unsigned char* values = keys + KS * P::kTile;                            // [KS][HD lanes][128 bytes: 64 keys]
     unsigned char* raw = values + KS * P::kTile;                             // [KS][page]
-    float2* scales = reinterpret_cast<float2*>(raw + KS * P::kRaw);          // [4] of the pages in the works
+    unsigned char* staged = raw + KS * P::kRaw;                              // [8 warps][32 rows][HD], the 16-byte pieces of row r at c ^ (r & 7)
+    float2* scales = reinterpret_cast<float2*>(staged + P::kRows);           // [4] of the pages in the works
     unsigned long long* raw_full = reinterpret_cast<unsigned long long*>(scales + 4);
     unsigned long long* raw_free = raw_full + KS;
     unsigned long long* k_full = raw_free + KS;
@@ -1172,11 +1174,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             const bool none = scale.y < 0.f;
             if (j >= KS && !mbar_wait(k_free + s, parity)) { ok = false; break; }
             if (own || none) {
-                for (int i = me; i < 64 * (HD / 8); i += 128) {
-                    const int r = i / (HD / 8), c = i % (HD / 8);
+                constexpr int kEach = HD / 16;           // (all loads before the first use: one latency, not eight)
+                uint4 v[kEach];
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int r = (me + i * 128) / (HD / 8), c = me % (HD / 8);
                     const __nv_bfloat16* from = own ? own_row(r, 0) : nullptr;
-                    const uint4 v = from ? reinterpret_cast<const uint4*>(from)[c] : make_uint4(0u, 0u, 0u, 0u);
-                    *reinterpret_cast<uint4*>(kt + (c >> 3) * 8192 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+                    v[i] = from ? reinterpret_cast<const uint4*>(from)[c] : make_uint4(0u, 0u, 0u, 0u);
+                }
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int r = (me + i * 128) / (HD / 8), c = me % (HD / 8);
+                    *reinterpret_cast<uint4*>(kt + (c >> 3) * 8192 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[i];
                 }
             } else {
                 // sixteen lanes of a key a thread: four pieces of a 64-lane half by eight keys a warp
@@ -1197,26 +1206,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             if (j >= KS && !mbar_wait(v_free + s, parity)) { ok = false; break; }
             // the value of lane d stands in row d % (HD / 8) * 8 + d / (HD / 8)
             if (own || none) {
-                for (int i = me; i < 16 * (HD / 8); i += 128) {
-                    const int k = i / (HD / 8) * 4, d = i % (HD / 8) * 8;
-                    uint4 v[4];
+                constexpr int kEach = HD / 64;
+                uint4 v[kEach][4];
+#pragma unroll
+                for (int i = 0; i < kEach; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const __nv_bfloat16* from = own ? own_row(k + e, 1) : nullptr;
-                        v[e] = from ? *reinterpret_cast<const uint4*>(from + d) : make_uint4(0u, 0u, 0u, 0u);
+                        const __nv_bfloat16* from = own ? own_row((me + i * 128) / (HD / 8) * 4 + e, 1) : nullptr;
+                        v[i][e] = from ? reinterpret_cast<const uint4*>(from)[me % (HD / 8)] : make_uint4(0u, 0u, 0u, 0u);
+                    }
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int k = (me + i * 128) / (HD / 8) * 4, d = me % (HD / 8) * 8;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
                         // (a probability of zero does not silence an infinity or a NaN: those are put in at the end, by the rows that see them)
-                        if (odd_two(v[e].x) | odd_two(v[e].y) | odd_two(v[e].z) | odd_two(v[e].w)) {
-                            v[e] = make_uint4(v[e].x & ~odd_two(v[e].x), v[e].y & ~odd_two(v[e].y), v[e].z & ~odd_two(v[e].z), v[e].w & ~odd_two(v[e].w));
+                        uint4& u = v[i][e];
+                        const uint4 odd = make_uint4(odd_two(u.x), odd_two(u.y), odd_two(u.z), odd_two(u.w));
+                        if (odd.x | odd.y | odd.z | odd.w) {
+                            u = make_uint4(u.x & ~odd.x, u.y & ~odd.y, u.z & ~odd.z, u.w & ~odd.w);
                             atomicOr(odd_values + ((k + e) >> 5), 1u << ((k + e) & 31));
                         }
                     }
 #pragma unroll
                     for (int x = 0; x < 8; ++x) {
-                        const unsigned w0 = x < 2 ? v[0].x : x < 4 ? v[0].y : x < 6 ? v[0].z : v[0].w, w1 = x < 2 ? v[1].x : x < 4 ? v[1].y : x < 6 ? v[1].z : v[1].w;
-                        const unsigned w2 = x < 2 ? v[2].x : x < 4 ? v[2].y : x < 6 ? v[2].z : v[2].w, w3 = x < 2 ? v[3].x : x < 4 ? v[3].y : x < 6 ? v[3].z : v[3].w;
+                        auto word = [&](const uint4& u) { return x < 2 ? u.x : x < 4 ? u.y : x < 6 ? u.z : u.w; };
                         const int row = (d + x) % (HD / 8) * 8 + (d + x) / (HD / 8);
                         *reinterpret_cast<uint2*>(vt + row * 128 + (((k >> 3) ^ (row & 7)) << 4) + (k & 4) * 2) =
-                            make_uint2(__byte_perm(w0, w1, x & 1 ? 0x7632 : 0x5410), __byte_perm(w2, w3, x & 1 ? 0x7632 : 0x5410));
+                            make_uint2(__byte_perm(word(v[i][0]), word(v[i][1]), x & 1 ? 0x7632 : 0x5410), __byte_perm(word(v[i][2]), word(v[i][3]), x & 1 ? 0x7632 : 0x5410));
                     }
                 }
             } else {
@@ -1245,15 +1262,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         const int tile = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane, pos = p0 + (r & 63), h = 2 * tile + (r >> 6);
         const bool live = h < G && pos >= start && pos < end;
         const unsigned at = tmem + tile * kTileCols + ((unsigned)(quarter * 32) << 16);
-        const size_t tok = (size_t)(tok0 + pos - start);
+        uint4* my_rows = reinterpret_cast<uint4*>(staged) + warp * (32 * HD / 8);
+        constexpr int kRowsAtOnce = 256 / HD;            // of the warp's 32, whole ones, between the threads and memory
+        const int my_row = lane / (HD / 8), my_piece = lane % (HD / 8);
         float to_log2;                                   // of a score of unrounded keys; of the others 2^133 times that
         {
             unsigned q[HD / 2];
-            const uint4* from = reinterpret_cast<const uint4*>(rows + (tok * width + head0 + h) * HD);
+            // (a row a thread from memory itself would be 32 places a load: 3 us before the first product, and 4.5 for the sums' way out)
+            uint4 v[HD / 8];
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) {
+                const int row = i * kRowsAtOnce + my_row, p = p0 + (quarter & 1) * 32 + row;
+                const bool there = h < G && p >= start && p < end;
+                v[i] = there ? reinterpret_cast<const uint4*>(rows + ((size_t)(tok0 + p - start) * width + head0 + h) * HD)[my_piece] : make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) {
+                const int row = i * kRowsAtOnce + my_row;
+                my_rows[row * (HD / 8) + (my_piece ^ (row & 7))] = v[i];
+            }
+            __syncwarp();
             unsigned top = 0;                            // of two magnitudes' bits at once
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i) {
-                const uint4 v = live ? from[i] : make_uint4(0u, 0u, 0u, 0u);
+                const uint4 v = my_rows[lane * (HD / 8) + (i ^ (lane & 7))];
                 q[4 * i] = v.x; q[4 * i + 1] = v.y; q[4 * i + 2] = v.z; q[4 * i + 3] = v.w;
                 top = __vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), __vmaxu2(__vmaxu2(v.y & 0x7fff7fffu, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu));
             }
@@ -1288,7 +1320,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             const float2 scale = scales[j & 3];
             // probabilities leave times 2^shift, the values' scale times 2^60 (the own block's: 2^-73), and their sum is divided by it again
             // (a block whose values are all next to zero: any scale will do; of a page that the row sees nothing of, whatever its scale)
-            const float f = own ? to_log2 * 0x1p-67f : to_log2 * (0x1p66f * scale.x);
+            float f = own ? to_log2 * 0x1p-67f : to_log2 * (0x1p66f * scale.x);
+            // keys of zeros: their scores stay zeros, and a hidden key's minus infinity; of a page that the row sees nothing of, whatever its scale
+            if (f == 0.f || key0 + 63 < lo) f = 0x1p-126f;
             const float vs = own ? 1.f : (key0 + 63 < lo || scale.y < 0x1p-100f ? 0x1p-100f : scale.y);
             const float shift = own ? -73.f : __log2f(vs) + 60.f, to_sum = own ? 0x1p73f : 0x1p-60f / vs;
             float x[64];
@@ -1296,11 +1330,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             for (int c = 0; c < 64; c += 16) tc5::tmem_ld16(at + c, x + c);
             tc5::wait_ld(x);
             const bool masked = own || key0 < warp_lo || scale.y < 0.f;
-            auto hidden = [&](int i) { return (own && key0 + i > pos) || key0 + i < lo || scale.y < 0.f; };
             if (masked) {
+                const int from = scale.y < 0.f ? 64 : lo - key0, to = own ? pos - key0 : 63;
 #pragma unroll
                 for (int i = 0; i < 64; ++i)
-                    if (hidden(i)) x[i] = -INFINITY;     // (f is not below zero)
+                    if (i < from || i > to) x[i] = -INFINITY;
             }
             float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
@@ -1329,18 +1363,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             }
             const float less = shift - (m == -INFINITY ? 0.f : m);
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
-            if (masked) {
 #pragma unroll
-                for (int i = 0; i < 64; ++i) {           // (a hidden key's minus infinity times an f of zero would be none)
-                    x[i] = x[i] == -INFINITY ? 0.f : ex2(fmaf(x[i], f, less));
-                    sum[i & 3] += x[i];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 64; ++i) {
-                    x[i] = ex2(fmaf(x[i], f, less));
-                    sum[i & 3] += x[i];
-                }
+            for (int i = 0; i < 64; ++i) {
+                x[i] = ex2(fmaf(x[i], f, less));
+                sum[i & 3] += x[i];
             }
 #pragma unroll
             for (int c = 0; c < 32; c += 16) {
@@ -1366,32 +1392,38 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                 seen_odd &= ~0ull >> (63 - (r & 63));
                 if (lo > p0) seen_odd &= ~0ull << (lo - p0);
             }
-            __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + (tok * a.n_heads + head0 + h) * HD;
-#pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {           // columns n 8 + g: lanes g HD / 8 + n
-                float o[32];
-                tc5::tmem_ld16(at + kOCol + c, o);
-                tc5::tmem_ld16(at + kOCol + c + 16, o + 16);
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c) {          // columns n 8 + g: lanes g HD / 8 + n
+                float o[64];
+#pragma unroll
+                for (int i = 0; i < 64; i += 16) tc5::tmem_ld16(at + kOCol + c * 64 + i, o + i);
                 tc5::wait_ld(o);
+                const float times = 0x1p73f * by;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] *= 0x1p73f * by;
-                if (live && seen_odd != 0)
-                    for (int k = 0; k < 64; ++k)
-                        if (seen_odd >> k & 1)
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                const int p = p0 + k;
-                                const __nv_bfloat16* from = p >= start ? rows + ((size_t)(tok0 + p - start) * width + a.n_heads + a.n_kv + kvh) * HD
-                                                                       : reinterpret_cast<const __nv_bfloat16*>(a.found) + ((((size_t)seq * 2 + 1) * a.n_kv + kvh) * kPage + k) * HD;
-                                const float v = __bfloat162float(from[(i & 7) * (HD / 8) + c / 8 + (i >> 3)]);
-                                if (!(fabsf(v) < INFINITY)) o[i] += v;
-                            }
-                if (live)
-#pragma unroll
-                    for (int g = 0; g < 8; ++g)
-                        *reinterpret_cast<uint2*>(out + g * (HD / 8) + c / 8) =
-                            make_uint2(pack_bf16(o[g], o[8 + g]), pack_bf16(o[16 + g], o[24 + g]));
-                __syncwarp();
+                for (int g = 0; g < 8; ++g)
+                    my_rows[lane * (HD / 8) + ((g * (HD / 64) + c) ^ (lane & 7))] =
+                        make_uint4(pack_bf16(o[g] * times, o[8 + g] * times), pack_bf16(o[16 + g] * times, o[24 + g] * times),
+                                   pack_bf16(o[32 + g] * times, o[40 + g] * times), pack_bf16(o[48 + g] * times, o[56 + g] * times));
+            }
+            if (live && seen_odd != 0)
+                for (int k = 0; k < 64; ++k)
+                    if (seen_odd >> k & 1) {
+                        const int p = p0 + k;
+                        const __nv_bfloat16* from = p >= start ? rows + ((size_t)(tok0 + p - start) * width + a.n_heads + a.n_kv + kvh) * HD
+                                                               : reinterpret_cast<const __nv_bfloat16*>(a.found) + ((((size_t)seq * 2 + 1) * a.n_kv + kvh) * kPage + k) * HD;
+                        for (int d = 0; d < HD; ++d) {
+                            const float v = __bfloat162float(from[d]);
+                            __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(my_rows + lane * (HD / 8) + ((d >> 3) ^ (lane & 7))) + (d & 7);
+                            if (!(fabsf(v) < INFINITY)) *o = __float2bfloat16(__bfloat162float(*o) + v);
+                        }
+                    }
+            __syncwarp();
+#pragma unroll 4
+            for (int i = 0; i < HD / 8; ++i) {
+                const int row = i * kRowsAtOnce + my_row, p = p0 + (quarter & 1) * 32 + row;
+                if (h < G && p >= start && p < end)
+                    reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + ((size_t)(tok0 + p - start) * a.n_heads + head0 + h) * HD)[my_piece] =
+                        my_rows[row * (HD / 8) + (my_piece ^ (row & 7))];
             }
         }
     }
