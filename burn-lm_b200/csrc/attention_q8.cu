@@ -482,6 +482,257 @@ __global__ void __launch_bounds__(kGeneralWarps * 32) attend_general_kernel(cons
     }
 }
 
+// The general kernel of portions: any type and head size, on the 32-bit units.  A block owns 32 rows, HB query heads of a kv head by
+// 32 / HB positions inside one 64-position block of a sequence, and walks the sequence's pages with numbers widened once into shared
+// memory for all of them: scores a thread 4 rows by 4 keys, sums a thread 8 rows by 4 NL lanes of half of the keys, so that a read of
+// shared memory feeds 4 or 8 multiply-adds.  The next page's bytes are on their way into registers meanwhile.
+constexpr int kTileThreads = 128, kTileRows = 32;
+__host__ __device__ constexpr size_t tile_smem(int hd) {
+    return ((size_t)hd * kTileRows + (size_t)hd * (kPage + 4) + (size_t)kPage * (hd + 4) + kPage * (kTileRows + 4) + 2 * kTileRows) * 4;
+}
+template <typename T, int NL>
+__global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendArgs a, int hb) {
+    extern __shared__ __align__(16) float tile_shared[];
+    __shared__ unsigned odd_keys[2];                     // bits: keys of the own block whose values hold an infinity or a NaN
+    constexpr int kKeyRow = kPage + 4, kPRow = kTileRows + 4;
+    const int hd = a.hd, v_row = hd + 4;
+    float* q = tile_shared;                              // [hd][32 rows]
+    float* keys = q + (size_t)hd * kTileRows;            // [hd][64 keys + 4]
+    float* values = keys + (size_t)hd * kKeyRow;         // [64 keys][hd + 4]
+    float* probs = values + (size_t)kPage * v_row;       // [64 keys][32 rows + 4]
+    float* alphas = probs + kPage * kPRow;               // [32]: what the rows' sums so far are multiplied by
+    float* totals = alphas + kTileRows;                  // [32]
+    const int tid = threadIdx.x, group = a.n_heads / a.n_kv, per_kv = group / hb, tb = kTileRows / hb;
+    const int kvh = blockIdx.x / per_kv, head0 = kvh * group + blockIdx.x % per_kv * hb, seq = blockIdx.z;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int tok0 = a.cu_seqlens[seq], n = a.cu_seqlens[seq + 1] - tok0, start = a.start_pos[seq], slot = a.slot_of_seq[seq], end = start + n;
+    const int tile = (end - 1) / tb - (int)blockIdx.y;   // (the tiles that walk furthest begin first)
+    if (n <= 0 || tile < start / tb) return;
+    const int t0 = tile * tb, mine = t0 / kPage, p0 = mine * kPage, width = a.n_heads + 2 * a.n_kv;
+    auto first_key = [&](int pos) { return a.window > 0 ? max(0, pos + 1 - a.window) : 0; };
+    const int pg_lo = first_key(max(start, t0)) / kPage;
+    const T* rows = reinterpret_cast<const T*>(a.rotated);
+    const T* found = reinterpret_cast<const T*>(a.found) + ((size_t)(a.found_by_slot ? slot : seq) * 2 * a.n_kv + kvh) * kPage * hd;
+    auto own_row = [&](int pos, int which) -> const T* { // of a position of the own block before the sequence's end
+        return pos >= start ? rows + ((size_t)(tok0 + pos - start) * width + a.n_heads + which * a.n_kv + kvh) * hd
+                            : found + ((size_t)which * a.n_kv * kPage + pos % kPage) * hd;
+    };
+    if (tid < 2) odd_keys[tid] = 0u;
+    for (int i = tid; i < kTileRows * (hd / 8); i += kTileThreads) {
+        const int r = i % kTileRows, d = i / kTileRows * 8, pos = t0 + r % tb;
+        float x[8] = {};
+        if (pos >= start && pos < end) load_n<8>(rows + ((size_t)(tok0 + pos - start) * width + head0 + r / tb) * hd + d, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[(d + e) * kTileRows + r] = x[e] * a.scale_log2e;
+    }
+    // scores: rows 4 rg .. 4 rg + 3 by keys 4 kg .. 4 kg + 3; sums: rows 8 pr .. 8 pr + 7, lanes 4 lg + 64 i, of half of the keys
+    const int rg = tid >> 4, kg = tid & 15, half = tid >> 6, pr = (tid >> 4) & 3, lg = tid & 15;
+    float m[4], l[4], acc[8][4 * NL];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) { m[r] = -INFINITY; l[r] = 0.f; }
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int i = 0; i < 4 * NL; ++i) acc[r][i] = 0.f;
+    const int pieces = 4 * hd, chunks = 4 * padded(hd), per = hd / 8;            // of sixteen bytes: of a page's keys, of its values
+    uint4 next_k[2 * NL], next_v[2 * NL];
+    float2 next_scale = make_float2(0.f, 0.f);
+    bool next_there = false;
+    auto fetch = [&](int b) {
+        const int page = page_of(a.block_table, a.table_stride, slot, b, a.n_pages);
+        next_there = page >= 0;
+        if (!next_there) return;
+        const signed char* line = a.pool + ((size_t)page * a.n_kv + kvh) * line_bytes(hd);
+        next_scale = *scales_of(line, hd);
+#pragma unroll
+        for (int i = 0; i < 2 * NL; ++i) {
+            const int c = tid + i * kTileThreads;
+            if (c < pieces) next_k[i] = *reinterpret_cast<const uint4*>(line + key_piece(c % kPage, c / kPage * 16, hd));
+            if (c < chunks) next_v[i] = *reinterpret_cast<const uint4*>(line + kPage * hd + c * 16);
+        }
+    };
+    auto wide = [](unsigned word, int e) { return (float)((int)(word >> (8 * e) & 0xffu) - 128); };
+    if (pg_lo < mine) fetch(pg_lo);
+    for (int b = pg_lo; b <= mine; ++b) {
+        const bool own = b == mine;
+        const float2 scale = own ? make_float2(1.f, 1.f) : next_scale;
+        if (!own) {
+            if (!next_there) {                           // (the same for the whole block)
+                if (b + 1 < mine) fetch(b + 1);
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * NL; ++i) {
+                const int c = tid + i * kTileThreads;
+                if (c < pieces) {
+                    float* to = keys + (c / kPage * 16) * kKeyRow + c % kPage;
+                    const unsigned w[4] = {next_k[i].x, next_k[i].y, next_k[i].z, next_k[i].w};
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) to[e * kKeyRow] = wide(w[e >> 2], e & 3);
+                }
+                if (c < chunks) {                        // four lanes of four keys
+                    const int rem = c % padded(hd), lane = rem & 31, lanes0 = rem / 32 * 4, key = c / padded(hd) * 16 + (lane & 3) * 4;
+                    float* to = values + key * v_row + (lane >> 2) * per + lanes0;
+                    const unsigned w[4] = {next_v[i].x, next_v[i].y, next_v[i].z, next_v[i].w};
+                    if (per % 4 == 0) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            *reinterpret_cast<float4*>(to + e * v_row) = make_float4(wide(w[0], e), wide(w[1], e), wide(w[2], e), wide(w[3], e));
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            if (lanes0 + x < per)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) to[e * v_row + x] = wide(w[x], e);
+                    }
+                }
+            }
+            if (b + 1 < mine) fetch(b + 1);
+        } else {
+            for (int c = tid; c < kPage * per; c += kTileThreads) {
+                const int key = c % kPage, d = c / kPage * 8, pos = p0 + key;
+                float k[8] = {}, v[8] = {};
+                if (pos < end) {
+                    load_n<8>(own_row(pos, 0) + d, k);
+                    load_n<8>(own_row(pos, 1) + d, v);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    keys[(d + e) * kKeyRow + key] = k[e];
+                    // (a probability of zero does not silence an infinity or a NaN: those are put in at the end, by the rows that see them)
+                    if (!(fabsf(v[e]) < INFINITY)) {
+                        v[e] = 0.f;
+                        atomicOr(odd_keys + (key >> 5), 1u << (key & 31));
+                    }
+                }
+                *reinterpret_cast<float4*>(values + key * v_row + d) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4*>(values + key * v_row + d + 4) = make_float4(v[4], v[5], v[6], v[7]);
+            }
+        }
+        __syncthreads();
+        float s[4][4] = {};
+#pragma unroll 8
+        for (int d = 0; d < hd; ++d) {
+            const float4 x = *reinterpret_cast<const float4*>(q + d * kTileRows + 4 * rg), y = *reinterpret_cast<const float4*>(keys + d * kKeyRow + 4 * kg);
+            const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[r][k] = fmaf(xs[r], ys[k], s[r][k]);
+        }
+        float p[4][4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int pos = t0 + (4 * rg + r) % tb, lo = first_key(pos);
+            float top = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int key = b * kPage + 4 * kg + k;
+                s[r][k] = key <= pos && key >= lo ? s[r][k] * scale.x : -INFINITY;
+                top = fmaxf(top, s[r][k]);
+            }
+#pragma unroll
+            for (int w = 1; w < 16; w *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            const float now = fmaxf(m[r], top), ref = now == -INFINITY ? 0.f : now, alpha = exp2f(m[r] - ref);
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool seen = b * kPage + 4 * kg + k <= pos && b * kPage + 4 * kg + k >= lo;
+                const float e = exp2f(s[r][k] - ref);
+                p[r][k] = seen ? e * scale.y : 0.f;      // (of what is not seen, whatever the scale)
+                sum += seen ? e : 0.f;
+            }
+            l[r] = l[r] * alpha + sum;                   // of the thread's keys; the sixteen threads of a row meet at the end
+            m[r] = now;
+            if (kg == 0) alphas[4 * rg + r] = alpha;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<float4*>(probs + (4 * kg + k) * kPRow + 4 * rg) = make_float4(p[0][k], p[1][k], p[2][k], p[3][k]);
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const float alpha = alphas[8 * pr + r];
+#pragma unroll
+            for (int i = 0; i < 4 * NL; ++i) acc[r][i] *= alpha;
+        }
+#pragma unroll 4
+        for (int k = half * 32; k < half * 32 + 32; ++k) {
+            const float4 p0 = *reinterpret_cast<const float4*>(probs + k * kPRow + 8 * pr), p1 = *reinterpret_cast<const float4*>(probs + k * kPRow + 8 * pr + 4);
+            const float ps[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+#pragma unroll
+            for (int i = 0; i < NL; ++i)
+                if (4 * lg + 64 * i < hd) {
+                    const float4 v = *reinterpret_cast<const float4*>(values + k * v_row + 4 * lg + 64 * i);
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        acc[r][4 * i] = fmaf(ps[r], v.x, acc[r][4 * i]);
+                        acc[r][4 * i + 1] = fmaf(ps[r], v.y, acc[r][4 * i + 1]);
+                        acc[r][4 * i + 2] = fmaf(ps[r], v.z, acc[r][4 * i + 2]);
+                        acc[r][4 * i + 3] = fmaf(ps[r], v.w, acc[r][4 * i + 3]);
+                    }
+                }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int w = 1; w < 16; w *= 2) l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
+        if (kg == 0) totals[4 * rg + r] = l[r];
+    }
+    if (half == 1)                                       // the second half of the keys, over the values
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+            if (4 * lg + 64 * i < hd)
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    *reinterpret_cast<float4*>(values + (8 * pr + r) * v_row + 4 * lg + 64 * i) =
+                        make_float4(acc[r][4 * i], acc[r][4 * i + 1], acc[r][4 * i + 2], acc[r][4 * i + 3]);
+    __syncthreads();
+    if (half == 1) return;
+    const unsigned long long odd = (unsigned long long)odd_keys[1] << 32 | odd_keys[0];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        const int row = 8 * pr + r, pos = t0 + row % tb;
+        if (pos < start || pos >= end) continue;
+        const float by = 1.f / totals[row];
+        const int from = first_key(pos);
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+            if (4 * lg + 64 * i < hd) {
+                const int d = 4 * lg + 64 * i;
+                const float4 other = *reinterpret_cast<const float4*>(values + row * v_row + d);
+                float o[4] = {(acc[r][4 * i] + other.x) * by, (acc[r][4 * i + 1] + other.y) * by, (acc[r][4 * i + 2] + other.z) * by, (acc[r][4 * i + 3] + other.w) * by};
+                if (odd != 0)
+                    for (int k = p0; k <= pos; ++k)
+                        if ((odd >> (k - p0) & 1) && k >= from)
+                            for (int e = 0; e < 4; ++e) {
+                                const float v = to_f32(own_row(k, 1)[d + e]);
+                                if (!(fabsf(v) < INFINITY)) o[e] += v;
+                            }
+                T* out = reinterpret_cast<T*>(a.out) + ((size_t)(tok0 + pos - start) * a.n_heads + head0 + row / tb) * hd + d;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) out[e] = from_f32<T>(o[e]);
+            }
+    }
+}
+
+template <typename T, int NL>
+static int launch_tile(const AttendArgs& a, int max_q_len, cudaStream_t stream) {
+    const int group = a.n_heads / a.n_kv, hb = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1, tb = kTileRows / hb;
+    const dim3 grid(a.n_kv * (group / hb), (max_q_len + tb - 2) / tb + 1, a.n_seqs);
+    const size_t smem = tile_smem(a.hd);
+    if (cudaFuncSetAttribute(attend_tile_kernel<T, NL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+        return blm_fail(BLM_CUDA_ERROR, "attention_q8: %s", cudaGetErrorString(cudaGetLastError()));
+    blm_launch_dependent(attend_tile_kernel<T, NL>, grid, dim3(kTileThreads), smem, stream, a, hb);
+    return blm_check_launch("attention_q8");
+}
+template <typename T>
+static int launch_tile(const AttendArgs& a, int max_q_len, cudaStream_t stream) {
+    return a.hd <= 64 ? launch_tile<T, 1>(a, max_q_len, stream) : a.hd <= 128 ? launch_tile<T, 2>(a, max_q_len, stream) : launch_tile<T, 4>(a, max_q_len, stream);
+}
+
 // ---- single tokens -----------------------------------------------------------------------------------------------------------
 // One new token a sequence, bfloat16, heads of 64 or 128 lanes: a block owns (share of the sequence's pages, up to eight query heads
 // of a kv head, sequence).  Its producer warp streams the pages into a ring in shared memory, one bulk copy of 8 or 16 KB each (keys,
@@ -1529,6 +1780,10 @@ BLM_API int blm_attention_q8(const void* rotated, const void* pool, const void* 
         const int group = n_heads / n_kv, groups = (group + 3) / 4;
         const PromptArgs pa{a, groups, (group + groups - 1) / groups, status};
         return hd == 64 ? launch_prompt<64>(pa, max_q_len, stream) : launch_prompt<128>(pa, max_q_len, stream);
+    }
+    if (max_q_len > 1 && n_seqs <= 65535 && max_q_len <= 500000) {
+        if (dtype == BLM_F32) return launch_tile<float>(a, max_q_len, stream);
+        if (dtype == BLM_BF16) return launch_tile<__nv_bfloat16>(a, max_q_len, stream);
     }
     const dim3 grid(n_heads * n_tokens);
     if (dtype == BLM_F32) blm_launch_dependent(attend_general_kernel<float>, grid, dim3(kGeneralWarps * 32), 0, stream, a);
