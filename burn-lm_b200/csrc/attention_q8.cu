@@ -22,6 +22,7 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include "cluster.cuh"
 #include "tcgen05.cuh"
 
 BLM_API const char* blm_attention_q8_last_error() { return g_blm_error; }
@@ -491,7 +492,7 @@ __host__ __device__ constexpr size_t tile_smem(int hd) {
     return ((size_t)hd * kTileRows + (size_t)hd * (kPage + 4) + (size_t)kPage * (hd + 4) + kPage * (kTileRows + 4) + 2 * kTileRows) * 4;
 }
 template <typename T, int NL>
-__global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendArgs a, int hb) {
+__global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendArgs a, int hb, int ranks) {
     extern __shared__ __align__(16) float tile_shared[];
     __shared__ unsigned odd_keys[2];                     // bits: keys of the own block whose values hold an infinity or a NaN
     constexpr int kKeyRow = kPage + 4, kPRow = kTileRows + 4;
@@ -500,15 +501,15 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
     float* keys = q + (size_t)hd * kTileRows;            // [hd][64 keys + 4]
     float* values = keys + (size_t)hd * kKeyRow;         // [64 keys][hd + 4]
     float* probs = values + (size_t)kPage * v_row;       // [64 keys][32 rows + 4]
-    float* alphas = probs + kPage * kPRow;               // [32]: what the rows' sums so far are multiplied by
+    float* alphas = probs + kPage * kPRow;               // [32]: what the rows' sums so far are multiplied by; at the end their maxima
     float* totals = alphas + kTileRows;                  // [32]
     const int tid = threadIdx.x, group = a.n_heads / a.n_kv, per_kv = group / hb, tb = kTileRows / hb;
-    const int kvh = blockIdx.x / per_kv, head0 = kvh * group + blockIdx.x % per_kv * hb, seq = blockIdx.z;
+    const int rank = blockIdx.x % ranks, heads = blockIdx.x / ranks, kvh = heads / per_kv, head0 = kvh * group + heads % per_kv * hb, seq = blockIdx.z;
     pdl_wait();
     pdl_launch_dependents();
     const int tok0 = a.cu_seqlens[seq], n = a.cu_seqlens[seq + 1] - tok0, start = a.start_pos[seq], slot = a.slot_of_seq[seq], end = start + n;
     const int tile = (end - 1) / tb - (int)blockIdx.y;   // (the tiles that walk furthest begin first)
-    if (n <= 0 || tile < start / tb) return;
+    if (n <= 0 || tile < start / tb) return;             // (the whole cluster)
     const int t0 = tile * tb, mine = t0 / kPage, p0 = mine * kPage, width = a.n_heads + 2 * a.n_kv;
     auto first_key = [&](int pos) { return a.window > 0 ? max(0, pos + 1 - a.window) : 0; };
     const int pg_lo = first_key(max(start, t0)) / kPage;
@@ -553,13 +554,13 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
         }
     };
     auto wide = [](unsigned word, int e) { return (float)((int)(word >> (8 * e) & 0xffu) - 128); };
-    if (pg_lo < mine) fetch(pg_lo);
-    for (int b = pg_lo; b <= mine; ++b) {
+    if (pg_lo + rank < mine) fetch(pg_lo + rank);
+    for (int b = pg_lo + rank; b <= mine; b += ranks) {
         const bool own = b == mine;
         const float2 scale = own ? make_float2(1.f, 1.f) : next_scale;
         if (!own) {
             if (!next_there) {                           // (the same for the whole block)
-                if (b + 1 < mine) fetch(b + 1);
+                if (b + ranks < mine) fetch(b + ranks);
                 continue;
             }
 #pragma unroll
@@ -588,7 +589,7 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
                     }
                 }
             }
-            if (b + 1 < mine) fetch(b + 1);
+            if (b + ranks < mine) fetch(b + ranks);
         } else {
             for (int c = tid; c < kPage * per; c += kTileThreads) {
                 const int key = c % kPage, d = c / kPage * 8, pos = p0 + key;
@@ -679,58 +680,82 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
     for (int r = 0; r < 4; ++r) {
 #pragma unroll
         for (int w = 1; w < 16; w *= 2) l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
-        if (kg == 0) totals[4 * rg + r] = l[r];
+        if (kg == 0) {
+            totals[4 * rg + r] = l[r];
+            alphas[4 * rg + r] = m[r];
+        }
     }
-    if (half == 1)                                       // the second half of the keys, over the values
+    // the two halves of the keys meet over the values, then the cluster's blocks, a share of the rows each
 #pragma unroll
-        for (int i = 0; i < NL; ++i)
-            if (4 * lg + 64 * i < hd)
+    for (int h = 0; h < 2; ++h) {
+        if (half == h)
 #pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    *reinterpret_cast<float4*>(values + (8 * pr + r) * v_row + 4 * lg + 64 * i) =
-                        make_float4(acc[r][4 * i], acc[r][4 * i + 1], acc[r][4 * i + 2], acc[r][4 * i + 3]);
-    __syncthreads();
-    if (half == 1) return;
-    const unsigned long long odd = (unsigned long long)odd_keys[1] << 32 | odd_keys[0];
+            for (int i = 0; i < NL; ++i)
+                if (4 * lg + 64 * i < hd)
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-        const int row = 8 * pr + r, pos = t0 + row % tb;
+                    for (int r = 0; r < 8; ++r) {
+                        float4* to = reinterpret_cast<float4*>(values + (8 * pr + r) * v_row + 4 * lg + 64 * i);
+                        const float4 first = h == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *to;
+                        *to = make_float4(first.x + acc[r][4 * i], first.y + acc[r][4 * i + 1], first.z + acc[r][4 * i + 2], first.w + acc[r][4 * i + 3]);
+                    }
+        __syncthreads();
+    }
+    if (ranks > 1) cluster_sync();
+    const unsigned odd_at = tc5::smem_u32(odd_keys), m_at = tc5::smem_u32(alphas), l_at = tc5::smem_u32(totals), o_at = tc5::smem_u32(values);
+    const int last = (mine - pg_lo) % ranks, share = kTileRows / ranks;          // (whose step was the own block)
+    unsigned long long odd = 0;
+    for (int w = 0; w < 2; ++w) odd |= (unsigned long long)(ranks > 1 ? __float_as_uint(cluster_float(odd_at + 4 * w, last)) : odd_keys[w]) << (32 * w);
+    for (int i = tid; i < share * (hd / 4); i += kTileThreads) {
+        const int row = rank * share + i / (hd / 4), d = i % (hd / 4) * 4, pos = t0 + row % tb;
         if (pos < start || pos >= end) continue;
-        const float by = 1.f / totals[row];
+        float top = -INFINITY, total = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+        if (ranks == 1) top = alphas[row];
+        else for (int k = 0; k < ranks; ++k) top = fmaxf(top, cluster_float(m_at + 4 * row, k));
+        for (int k = 0; k < ranks; ++k) {
+            const float mk = ranks == 1 ? top : cluster_float(m_at + 4 * row, k), lk = ranks == 1 ? totals[row] : cluster_float(l_at + 4 * row, k);
+            const float4 v = ranks == 1 ? *reinterpret_cast<const float4*>(values + row * v_row + d) : cluster_float4(o_at + (row * v_row + d) * 4, k);
+            // (a share that the row saw nothing of has nothing; one whose scores were no numbers has none, which its sum tells)
+            const float by = mk == top ? 1.f : exp2f(mk - (top == -INFINITY ? 0.f : top));
+            total = fmaf(lk, by, total);
+            o[0] = fmaf(v.x, by, o[0]); o[1] = fmaf(v.y, by, o[1]); o[2] = fmaf(v.z, by, o[2]); o[3] = fmaf(v.w, by, o[3]);
+        }
+        const float by = 1.f / total;
         const int from = first_key(pos);
+        T* out = reinterpret_cast<T*>(a.out) + ((size_t)(tok0 + pos - start) * a.n_heads + head0 + row / tb) * hd + d;
 #pragma unroll
-        for (int i = 0; i < NL; ++i)
-            if (4 * lg + 64 * i < hd) {
-                const int d = 4 * lg + 64 * i;
-                const float4 other = *reinterpret_cast<const float4*>(values + row * v_row + d);
-                float o[4] = {(acc[r][4 * i] + other.x) * by, (acc[r][4 * i + 1] + other.y) * by, (acc[r][4 * i + 2] + other.z) * by, (acc[r][4 * i + 3] + other.w) * by};
-                if (odd != 0)
-                    for (int k = p0; k <= pos; ++k)
-                        if ((odd >> (k - p0) & 1) && k >= from)
-                            for (int e = 0; e < 4; ++e) {
-                                const float v = to_f32(own_row(k, 1)[d + e]);
-                                if (!(fabsf(v) < INFINITY)) o[e] += v;
-                            }
-                T* out = reinterpret_cast<T*>(a.out) + ((size_t)(tok0 + pos - start) * a.n_heads + head0 + row / tb) * hd + d;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) out[e] = from_f32<T>(o[e]);
-            }
+        for (int e = 0; e < 4; ++e) {
+            float x = o[e] * by;
+            if (odd != 0)
+                for (int k = max(p0, from); k <= pos; ++k)
+                    if (odd >> (k - p0) & 1) {
+                        const float v = to_f32(own_row(k, 1)[d + e]);
+                        if (!(fabsf(v) < INFINITY)) x += v;
+                    }
+            out[e] = from_f32<T>(x);
+        }
     }
+    if (ranks > 1) cluster_sync();                       // what others read stays until they have
 }
 
 template <typename T, int NL>
-static int launch_tile(const AttendArgs& a, int max_q_len, cudaStream_t stream) {
+static int launch_tile(const AttendArgs& a, int n_tokens, int max_q_len, int max_kv_len, cudaStream_t stream) {
     const int group = a.n_heads / a.n_kv, hb = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1, tb = kTileRows / hb;
-    const dim3 grid(a.n_kv * (group / hb), (max_q_len + tb - 2) / tb + 1, a.n_seqs);
+    // a walk of several pages is shared by the blocks of a cluster, as far as that gives an SM no more than four
+    const int tiles = a.n_kv * (group / hb) * ((n_tokens + tb - 1) / tb + a.n_seqs - 1);
+    int pages = (max_kv_len + kPage - 1) / kPage, ranks = 1;
+    if (a.window > 0 && pages > a.window / kPage + 2) pages = a.window / kPage + 2;
+    while (ranks < 8 && (long long)tiles * ranks * 2 <= 4ll * blm_sm_count() && pages >= 2 * ranks) ranks *= 2;
+    const dim3 grid(a.n_kv * (group / hb) * ranks, (max_q_len + tb - 2) / tb + 1, a.n_seqs);
     const size_t smem = tile_smem(a.hd);
     if (cudaFuncSetAttribute(attend_tile_kernel<T, NL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return blm_fail(BLM_CUDA_ERROR, "attention_q8: %s", cudaGetErrorString(cudaGetLastError()));
-    blm_launch_dependent(attend_tile_kernel<T, NL>, grid, dim3(kTileThreads), smem, stream, a, hb);
+    blm_launch_cluster(attend_tile_kernel<T, NL>, ranks, grid, dim3(kTileThreads), smem, stream, a, hb, ranks);
     return blm_check_launch("attention_q8");
 }
 template <typename T>
-static int launch_tile(const AttendArgs& a, int max_q_len, cudaStream_t stream) {
-    return a.hd <= 64 ? launch_tile<T, 1>(a, max_q_len, stream) : a.hd <= 128 ? launch_tile<T, 2>(a, max_q_len, stream) : launch_tile<T, 4>(a, max_q_len, stream);
+static int launch_tile(const AttendArgs& a, int n_tokens, int max_q_len, int max_kv_len, cudaStream_t stream) {
+    return a.hd <= 64 ? launch_tile<T, 1>(a, n_tokens, max_q_len, max_kv_len, stream) : a.hd <= 128 ? launch_tile<T, 2>(a, n_tokens, max_q_len, max_kv_len, stream)
+                                                                                      : launch_tile<T, 4>(a, n_tokens, max_q_len, max_kv_len, stream);
 }
 
 // ---- single tokens -----------------------------------------------------------------------------------------------------------
@@ -1782,8 +1807,8 @@ BLM_API int blm_attention_q8(const void* rotated, const void* pool, const void* 
         return hd == 64 ? launch_prompt<64>(pa, max_q_len, stream) : launch_prompt<128>(pa, max_q_len, stream);
     }
     if (max_q_len > 1 && n_seqs <= 65535 && max_q_len <= 500000) {
-        if (dtype == BLM_F32) return launch_tile<float>(a, max_q_len, stream);
-        if (dtype == BLM_BF16) return launch_tile<__nv_bfloat16>(a, max_q_len, stream);
+        if (dtype == BLM_F32) return launch_tile<float>(a, n_tokens, max_q_len, max_kv_len, stream);
+        if (dtype == BLM_BF16) return launch_tile<__nv_bfloat16>(a, n_tokens, max_q_len, max_kv_len, stream);
     }
     const dim3 grid(n_heads * n_tokens);
     if (dtype == BLM_F32) blm_launch_dependent(attend_general_kernel<float>, grid, dim3(kGeneralWarps * 32), 0, stream, a);

@@ -9,6 +9,7 @@
 // (g + 8, 2) (g, 1) (g + 8, 1) (g, 3) (g + 8, 3): a shift and a mask by 0x000f000f leave two neighbours of one row in the two halves of
 // a register.  A nibble holds v + 8.  Behind a stretch's four tiles stand its scales, bfloat16 [16 rows][4], one for every 64 places (a
 // group of 128 has its own twice), or [16 rows][8] where groups have 32: one copy of 2,176 or 2,304 bytes brings all that a warp needs.
+#include "cluster.cuh"
 #include "tcgen05.cuh"
 
 BLM_API const char* blm_gemm_q4_last_error() { return g_blm_error; }
@@ -48,14 +49,6 @@ __device__ __forceinline__ unsigned pair(unsigned word, int p) {
     return *reinterpret_cast<const unsigned*>(&v);
 }
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
-// the same place in the shared memory of a block of the cluster
-__device__ __forceinline__ float shared_of(unsigned mine, int rank) {
-    unsigned at;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(mine), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(at) : "memory");
-    return v;
-}
 __device__ __forceinline__ float bf16_of(unsigned two, int which) { return __uint_as_float(which ? two & 0xffff0000u : two << 16); }
 
 // ---- few tokens ------------------------------------------------------------------------------------------------------------
@@ -256,7 +249,7 @@ __global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(cons
             for (int k = 0; k < kWarps; ++k) y += from[k * F::kSums];
             sums[i] = y;
         }
-        if (fa.chunks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+        if (fa.chunks > 1) cluster_sync();
         else __syncthreads();
         // out: the cluster's blocks take tiles in turn
         const unsigned base = smem_u32(sums);
@@ -267,8 +260,8 @@ __global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(cons
             const unsigned at = base + (unsigned)((slot * 16 + row) * 8 * NT + tok) * 4;
             float y = 0.f, up = 0.f;
             for (int r = 0; r < fa.chunks; ++r) {
-                y += shared_of(at, r);
-                if (a.end == END_GATED) up += shared_of(at + 8 * 8 * NT * 4, r);
+                y += cluster_float(at, r);
+                if (a.end == END_GATED) up += cluster_float(at + 8 * 8 * NT * 4, r);
             }
             if (a.end == END_GATED) y = y / (1.0f + __expf(-y)) * up;
             const size_t to = (size_t)(tok0 + tok) * a.ldy + out;
@@ -277,7 +270,7 @@ __global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(cons
             else reinterpret_cast<__nv_bfloat16*>(a.y)[to] = __float2bfloat16_rn(y);
         }
         // nobody writes sums again while another block reads them, nor leaves
-        if (fa.chunks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+        if (fa.chunks > 1) cluster_sync();
         else if (b0 + F::kSlots < t_hi) __syncthreads();
     }
     // (a wait that ran out: what is still on its way lands before the block ends)
@@ -369,13 +362,6 @@ __device__ __forceinline__ void copy_async(unsigned dst, const void* src, int by
     if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
     else if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(dst), "l"(src) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ float4 four_of(unsigned mine, int rank) {
-    unsigned at;
-    float4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(mine), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-    return v;
 }
 
 template <int N>
@@ -533,7 +519,7 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
         }
     }
     fence_before();
-    if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    if (ranks > 1) cluster_sync();
     else __syncthreads();
 
     // ---- and out: four rows of a token a thread; the tokens shared by the cluster's blocks ----
@@ -550,10 +536,10 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
             const unsigned place = base + (unsigned)(c * 128 + row) * 4;
             float y[4] = {0.f, 0.f, 0.f, 0.f}, up[4] = {0.f, 0.f, 0.f, 0.f};
             for (int r = 0; r < ranks; ++r) {
-                const float4 v = four_of(place, r);
+                const float4 v = cluster_float4(place, r);
                 y[0] += v.x; y[1] += v.y; y[2] += v.z; y[3] += v.w;
                 if (gated) {
-                    const float4 u = four_of(place + 32, r);
+                    const float4 u = cluster_float4(place + 32, r);
                     up[0] += u.x; up[1] += u.y; up[2] += u.z; up[3] += u.w;
                 }
             }
@@ -586,7 +572,7 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
         }
     }
     __syncwarp();
-    if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    if (ranks > 1) cluster_sync();
     if (warp == 1) {
         fence_after();
         tmem_free(tmem, N);
@@ -615,21 +601,7 @@ static int launch_wide(const Args& a, int* status, cudaStream_t stream) {
             return blm_fail(BLM_CUDA_ERROR, "gemm_q4: %s", cudaGetErrorString(cudaGetLastError()));
         if (dev >= 0 && dev < 64) opted_in[dev] = true;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ranks, row_blocks, tok_blocks);
-    cfg.blockDim = dim3(W::kThreads);
-    cfg.dynamicSmemBytes = W::kSmem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = ranks;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = ranks > 1 ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, wide_kernel<N>, wa, map);
+    blm_launch_cluster(wide_kernel<N>, ranks, dim3(ranks, row_blocks, tok_blocks), dim3(W::kThreads), W::kSmem, stream, wa, map);
     return blm_check_launch("gemm_q4");
 }
 }  // namespace q4
