@@ -42,10 +42,11 @@ __device__ __forceinline__ void mma16_onto(float (&d)[4], unsigned a0, unsigned 
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-// Two whole numbers of a word: 0x43 in front of a nibble is the bfloat16 number 128 + nibble, and the nibble is v + 8.
-__device__ __forceinline__ unsigned pair(unsigned word, int p) {
-    const unsigned biased = ((word >> (4 * p)) & 0x000f000fu) | 0x43004300u;
-    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&biased), __float2bfloat162_rn(136.f));
+// Two whole numbers of a word times their scale, exactly: 0x43 in front of a nibble is the bfloat16 number 128 + nibble, and the nibble
+// is v + 8.  (One multiply-add that takes off 136 times the scale would do it in less, but that has ten bits.)
+__device__ __forceinline__ unsigned scaled_two(unsigned word, unsigned scale) {
+    const unsigned biased = (word & 0x000f000fu) | 0x43004300u;
+    const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&biased), __float2bfloat162_rn(136.f)), *reinterpret_cast<const __nv_bfloat162*>(&scale));
     return *reinterpret_cast<const unsigned*>(&v);
 }
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -329,15 +330,15 @@ static int launch_few(const Args& a, int* status, cudaStream_t stream) {
 
 // ---- many tokens -----------------------------------------------------------------------------------------------------------
 // The tcgen05 product with the weight's rows as the 128 rows of the accumulator and N tokens (32 to 256) as its columns.  A stage holds
-// 128 places of K: one thread fetches the tokens (TMA, 128-byte swizzle, zeros beyond the last token and place), one issues the products,
-// and sixteen warps turn a tile of 16 rows x 64 places each into bfloat16 in shared memory: a lane fetches its 16 bytes of packed weights
-// with cp.async, kAhead stages ahead, and writes four pieces of eight places where the tensor core's swizzle wants them (a number is the
-// whole number times its scale, exactly; three and a half instructions for two).  With 64 places a stage the threads' waits for one
-// another, not the arithmetic, were what took the time (0.36 us a tile of 128 x 64 weights whatever the tokens).  Where a weight has too few rows to fill the SMs, K is cut
-// over the blocks of a cluster.  The sums go from tensor memory to shared memory as they are, a row a lane; then each token's results
-// are read, four rows a thread (from all the cluster's blocks, in their order), finished, and written as whole lines.  Waits are bounded.
+// 64 places of K: one thread fetches the tokens (TMA, 128-byte swizzle, zeros beyond the last token and place), one issues the products,
+// and the other warps turn weights into bfloat16 in tensor memory, a row a lane, each group of four warps every kGroups-th tile of K: a
+// lane loads its row's four 16-byte pieces (which hold row g + 8 too) two tiles ahead, straight into registers, and a number is the
+// whole number times its scale, exactly, in four instructions for two.  (Weights in shared memory instead, written and then read by the
+// products beside 256 tokens, took 100 KB of its traffic a tile, 780 cycles for 512 of the tensor core's.)  Where a weight has too few
+// rows to fill the SMs, K is cut over the blocks of a cluster.  The sums go from tensor memory to shared memory as they are, a row a
+// lane; then each token's results are read, four rows a thread (from all the cluster's blocks, in their order), finished, and written
+// as whole lines.  Waits are bounded.
 enum { Q4_TIMEOUT_PRODUCT = 53 };
-__host__ __device__ constexpr int rho_of(int g) { return (g & 1) << 2 | g >> 1; }         // and back: (r & 3) << 1 | r >> 2
 
 struct WideArgs {
     Args a;
@@ -348,33 +349,26 @@ struct WideArgs {
 
 template <int N> struct Wide {
     static constexpr int kBlocks = N <= 64 ? 2 : 1;          // of an SM
-    static constexpr int kStages = N == 128 ? 3 : 2, kAhead = N == 64 ? 1 : 3;
-    static constexpr int kWidenWarps = 16, kThreads = (2 + kWidenWarps) * 32;
-    static constexpr int kABytes = 128 * 128, kBBytes = N * 128;                           // of a tile of 64 places of K
-    static constexpr int kStage = 2 * (kABytes + kBBytes);                                 // two: weights, weights, tokens, tokens
-    static constexpr int kUnit = kTileBytes + 128;           // a warp's tile, and the scales of its pair: [16 rows][8 bytes]
+    static constexpr int kStages = N == 256 ? 6 : N == 128 ? 8 : N == 64 ? 6 : 7;
+    static constexpr int kGroups = N <= 64 ? 2 : 4, kThreads = (2 + 4 * kGroups) * 32;
+    static constexpr int kCols = N <= 64 ? 256 : 512;        // of tensor memory: N of sums, 32 a stage of weights
+    static constexpr int kStage = N * 128;                   // bytes of the tokens of a tile of 64 places
     static constexpr int kSums = N * 128 * 4;
     static constexpr int kRing = kStages * kStage > kSums ? kStages * kStage : kSums;
-    static constexpr int kSmem = kRing + kWidenWarps * kAhead * kUnit + 1024 + 256;
+    static constexpr int kSmem = kRing + 1024 + 256;
+    static_assert(N + 32 * kStages <= kCols && kBlocks * kCols <= 512, "tensor memory");
 };
-
-__device__ __forceinline__ void copy_async(unsigned dst, const void* src, int bytes) {
-    if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
-    else if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(dst), "l"(src) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
-}
 
 template <int N>
 __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kernel(const WideArgs wa, const __grid_constant__ CUtensorMap xmap) {
     using namespace tc5;
     using tc5::smem_u32;
     using W = Wide<N>;
-    constexpr int S = W::kStages, AHEAD = W::kAhead;
+    constexpr int S = W::kStages, KG = W::kGroups;
     const Args& a = wa.a;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    unsigned char* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);     // [S][weights 128 x 128 bytes, tokens N x 128 bytes]
-    unsigned char* packed = ring + W::kRing;                                               // [warps][AHEAD][unit]
-    unsigned long long* full = reinterpret_cast<unsigned long long*>(packed + W::kWidenWarps * AHEAD * W::kUnit);
+    unsigned char* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);     // [S][N tokens x 128 bytes]
+    unsigned long long* full = reinterpret_cast<unsigned long long*>(ring + W::kRing);
     unsigned long long* empty = full + S;
     unsigned long long* done = empty + S;
     unsigned* slot = reinterpret_cast<unsigned*>(done + 1);
@@ -383,34 +377,31 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
     const int kt0 = rank * wa.share, n_k = max(0, min(a.k_tiles - kt0, wa.share));          // this block's tiles of K
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
-            mbar_init(full + s, 1 + W::kWidenWarps);     // the tokens and every warp's weights
+            mbar_init(full + s, 1 + 4);                  // the tokens and four warps' weights
             mbar_init(empty + s, 1);
         }
         mbar_init(done, 1);
         mbar_init_fence();
     }
-    if (warp == 1) tmem_alloc(slot, N);
+    if (warp == 1) tmem_alloc(slot, W::kCols);
     fence_before();
     __syncthreads();
     fence_after();
     pdl_launch_dependents();                              // (not before this block has its tensor memory: the next kernel may take some too)
     const unsigned tmem = *slot;
-    const int pairs = (n_k + 1) / 2;
 
     if (warp == 0) {
         if (lane == 0) {
             pdl_wait();                                  // the tokens are the work of the kernel before
             int i = 0;
-            for (; i < pairs; ++i) {
+            for (; i < n_k; ++i) {
                 const int s = i % S;
                 if (i >= S && !mbar_wait(empty + s, (i / S - 1) & 1)) { atomicCAS(wa.status, 0, Q4_TIMEOUT_PRODUCT); break; }
-                const int n = min(2, n_k - 2 * i);       // (an odd last tile has no second)
-                mbar_expect_tx(full + s, n * W::kBBytes);
-                for (int x = 0; x < n; ++x)
-                    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(
-                                     smem_u32(ring + s * W::kStage + 2 * W::kABytes + x * W::kBBytes)),
-                                 "l"(&xmap), "r"((kt0 + 2 * i + x) * 64), "r"(tok0), "r"(smem_u32(full + s))
-                                 : "memory");
+                mbar_expect_tx(full + s, W::kStage);
+                asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(
+                                 smem_u32(ring + s * W::kStage)),
+                             "l"(&xmap), "r"((kt0 + i) * 64), "r"(tok0), "r"(smem_u32(full + s))
+                             : "memory");
             }
             for (int k = max(0, i - S); k < i; ++k) mbar_wait(full + k % S, (k / S) & 1);   // nothing is on its way when the block ends
         }
@@ -419,82 +410,71 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
             constexpr unsigned id = instruction(N);
             int s = 0;
             unsigned phase = 0;
-            for (int i = 0; i < pairs; ++i) {
+            for (int i = 0; i < n_k; ++i) {
                 if (!mbar_wait(full + s, phase)) { atomicCAS(wa.status, 0, Q4_TIMEOUT_PRODUCT); break; }
                 fence_after();
-                const unsigned long long ad = operand(ring + s * W::kStage, 2, 1024), bd = operand(ring + s * W::kStage + 2 * W::kABytes, 2, 1024);
+                const unsigned long long bd = operand(ring + s * W::kStage, 2, 1024);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mma(tmem, ad + 2 * k, bd + 2 * k, id, i > 0 || k > 0);
-                if (2 * i + 1 < n_k)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) mma(tmem, ad + (W::kABytes >> 4) + 2 * k, bd + (W::kBBytes >> 4) + 2 * k, id, true);
+                for (int k = 0; k < 4; ++k) mma_ts(tmem, tmem + N + s * 32 + 8 * k, bd + 2 * k, id, i > 0 || k > 0);
                 commit(empty + s);
                 if (++s == S) { s = 0; phase ^= 1; }
             }
             commit(done);                                // when all products so far are over
         }
     } else {
-        // ---- weights: this warp's tile of 16 rows, the first or the second of every pair of K tiles ----
-        const int rows16 = (warp - 2) & 7, x = (warp - 2) >> 3;
-        const int tiles = (a.M + 15) / 16, tile = min(row0 / 16 + rows16, tiles - 1), g = lane >> 2, t = lane & 3;
-        const bool here = row0 / 16 + rows16 < tiles, two = a.per_tile == 2;      // (rows beyond the last tile are not written: any numbers do)
-        unsigned char* mine = packed + (warp - 2) * AHEAD * W::kUnit;
-        const unsigned at = smem_u32(mine);
-        const unsigned char* w_at = a.w + ((size_t)tile * a.stretches + kt0 / kBatch) * a.unit;
-        auto fetch = [&](int p, int slot_of) {
-            if (here && 2 * p + x < n_k) {
-                const unsigned to = at + slot_of * W::kUnit;
-                const unsigned char* from = w_at + (size_t)(p >> 1) * a.unit;      // the pair's stretch
-                copy_async(to + lane * 16, from + (2 * (p & 1) + x) * kTileBytes + lane * 16, 16);
-                if (lane < 16)                           // the pair's scales, lanes 0 .. 15 a row each
-                    copy_async(to + kTileBytes + lane * 8, from + kBatch * kTileBytes + (lane * 2 + (p & 1)) * 4 * a.per_tile, 4 * a.per_tile);
-            }
-            asm volatile("cp.async.commit_group;\n" ::: "memory");
-        };
+        // ---- weights: the quarter of the rows that the warp's lanes of tensor memory are, a row a lane ----
+        const int quarter = warp & 3, first = (warp - 2) / 4, row = row0 + quarter * 32 + lane, tiles = (a.M + 15) / 16;
+        const int tile = min(row >> 4, tiles - 1), g = lane & 7;                            // (rows beyond the last tile are not written: any numbers do)
+        const unsigned high = lane >> 1 & 4;             // of a byte's two nibbles the second is row g + 8's: a shift of 0 or 4
+        const unsigned char* pieces = a.w + ((size_t)tile * a.stretches + kt0 / kBatch) * a.unit;
+        const unsigned char* scales = pieces + kBatch * kTileBytes + (lane & 15) * 8 * a.per_tile;
+        struct Tile { uint4 w[4]; unsigned scale; };     // (of 64 places; the scales of its halves)
+        Tile ahead[2];
+        auto fetch = [&](Tile& to, int kt) {
+            if (kt >= n_k) return;
+            const size_t at = (size_t)(kt / kBatch) * a.unit;
+            const uint4* from = reinterpret_cast<const uint4*>(pieces + at + kt % kBatch * kTileBytes) + 4 * g;
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) fetch(j, j);
-        auto times = [](unsigned v, unsigned m) {
-            const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&m));
-            return *reinterpret_cast<const unsigned*>(&r);
+            for (int t = 0; t < 4; ++t) to.w[t] = __ldg(from + t);
+            if (a.per_tile == 2) to.scale = __ldg(reinterpret_cast<const unsigned*>(scales + at) + kt % kBatch);
+            else to.scale = __ldg(reinterpret_cast<const unsigned short*>(scales + at) + kt % kBatch) * 0x10001u;
         };
-        // Row g of the tile becomes row rho(g) of the accumulator, so that the eight lanes of a phase (two g) meet in no bank: the swizzle
-        // puts piece t of rows 0 .. 3 (mod 8) into one half of a row's 128 bytes and of rows 4 .. 7 into the other.
-        const unsigned rho = rho_of(g), first_at = x * W::kABytes + ((t ^ rho) << 4) + (rows16 * 16 + rho) * 128;
-        // the scale of the tile's first (second) 32 places, twice, from the pair's 4 or 8 bytes
-        const unsigned sel_first = x == 1 && !two ? 0x3232u : 0x1010u, sel_second = x == 1 || two ? 0x3232u : 0x1010u;
-        int s = 0, held = 0;                             // the next stage; the slot of the next tile
-        unsigned parity = 1;                             // of the phase before the first: a new barrier counts as past it
-        for (int p = 0; p < pairs; ++p) {
-            asm volatile("cp.async.wait_group %0;\n" ::"n"(AHEAD - 1) : "memory");
-            __syncwarp();                                // the scales are other lanes' copies
-            const unsigned char* unit = mine + held * W::kUnit;
-            const uint4 now = *reinterpret_cast<const uint4*>(unit + lane * 16);
-            const unsigned s0 = *reinterpret_cast<const unsigned*>(unit + kTileBytes + g * 8 + (two ? 4 * x : 0));
-            const unsigned s8 = *reinterpret_cast<const unsigned*>(unit + kTileBytes + (g + 8) * 8 + (two ? 4 * x : 0));
-            __syncwarp();
-            fetch(p + AHEAD, held);
-            held = held + 1 == AHEAD ? 0 : held + 1;
-            if (!mbar_wait(empty + s, parity)) {
+        auto one = [&](Tile& now, int kt) {
+            unsigned w[2][16];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const unsigned scale = __byte_perm(now.scale, 0, h == 0 ? 0x1010 : 0x3232);
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const unsigned word = (h == 0 ? (e == 0 ? now.w[t].x : now.w[t].y) : (e == 0 ? now.w[t].z : now.w[t].w)) >> high;
+                        w[h][4 * t + 2 * e] = scaled_two(word, scale);
+                        w[h][4 * t + 2 * e + 1] = scaled_two(word >> 8, scale);
+                    }
+            }
+            fetch(now, kt + 2 * KG);
+            const int s = kt % S;
+            if (kt >= S && !mbar_wait(empty + s, (kt / S - 1) & 1)) {
                 if (lane == 0) atomicCAS(wa.status, 0, Q4_TIMEOUT_PRODUCT);
-                break;
+                return false;
             }
-            if (2 * p + x < n_k) {
-                unsigned char* stage = ring + s * W::kStage;
-                auto half = [&](unsigned lo, unsigned hi, unsigned sel, unsigned at) {
-                    const unsigned m0 = __byte_perm(s0, 0, sel), m8 = __byte_perm(s8, 0, sel);
-                    *reinterpret_cast<uint4*>(stage + at) = make_uint4(times(pair(lo, 0), m0), times(pair(lo, 2), m0), times(pair(hi, 0), m0), times(pair(hi, 2), m0));
-                    *reinterpret_cast<uint4*>(stage + at + 8 * 128) =
-                        make_uint4(times(pair(lo, 1), m8), times(pair(lo, 3), m8), times(pair(hi, 1), m8), times(pair(hi, 3), m8));
-                };
-                half(now.x, now.y, sel_first, first_at);
-                half(now.z, now.w, sel_second, first_at ^ 64u);
-                fence_async_smem();
-                __syncwarp();
-            }
+            fence_after();
+            const unsigned to = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)(N + s * 32);
+            tmem_st16(to, w[0]);
+            tmem_st16(to + 16, w[1]);
+            wait_st();
+            fence_before();
+            __syncwarp();
             if (lane == 0) mbar_arrive(full + s);
-            if (++s == S) { s = 0; parity ^= 1; }
+            return true;
+        };
+        fetch(ahead[0], first);
+        fetch(ahead[1], first + KG);
+        for (int kt = first; kt < n_k; kt += 2 * KG) {
+            if (!one(ahead[0], kt)) break;
+            if (kt + KG < n_k && !one(ahead[1], kt + KG)) break;
         }
-        asm volatile("cp.async.wait_group 0;\n" ::: "memory");
     }
     __syncwarp();
 
@@ -505,10 +485,10 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
         over = mbar_wait(done, 0);
         if (!over && lane == 0) atomicCAS(wa.status, 0, Q4_TIMEOUT_PRODUCT);
         fence_after();
-        // (warps 2 .. 17: quarters 2 3 0 1 2 3 0 1 .., four warps to each)
-        const int quarter = warp & 3, row = quarter * 32 + lane;
-        float* to = sums + (row & ~7) + ((row & 3) << 1 | (row & 7) >> 2);       // the weight's row behind this row of the accumulator
-        for (int c = (warp - 2) / 4 * 16; c < N; c += 64) {
+        // (warps 2 and up: quarters 2 3 0 1 2 3 0 1 .., kGroups warps to each)
+        const int quarter = warp & 3;
+        float* to = sums + quarter * 32 + lane;
+        for (int c = (warp - 2) / 4 * 16; c < N; c += KG * 16) {
             float v[16];
             if (n_k > 0) {
                 tmem_ld16(tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)c, v);
@@ -529,7 +509,7 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
         const int each = N / ranks, n_here = min(each, a.N - tok0 - rank * each), per = gated ? 16 : 32;
         const int m_out = gated ? a.M / 2 : a.M, m0 = gated ? row0 / 2 : row0;
         const unsigned base = smem_u32(sums + rank * each * 128);
-        for (int i = threadIdx.x - 64; i < n_here * per; i += W::kWidenWarps * 32) {
+        for (int i = threadIdx.x - 64; i < n_here * per; i += KG * 128) {
             const int c = i / per, q = i % per, out = m0 + q * 4;
             if (out >= m_out) continue;
             const int row = gated ? q / 2 * 16 + q % 2 * 4 : q * 4;
@@ -575,7 +555,7 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
     if (ranks > 1) cluster_sync();
     if (warp == 1) {
         fence_after();
-        tmem_free(tmem, N);
+        tmem_free(tmem, W::kCols);
     }
 }
 
