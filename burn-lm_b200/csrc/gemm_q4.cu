@@ -42,11 +42,12 @@ __device__ __forceinline__ void mma16_onto(float (&d)[4], unsigned a0, unsigned 
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-// Two whole numbers of a word times their scale, exactly: 0x43 in front of a nibble is the bfloat16 number 128 + nibble, and the nibble
-// is v + 8.  (One multiply-add that takes off 136 times the scale would do it in less, but that has ten bits.)
-__device__ __forceinline__ unsigned scaled_two(unsigned word, unsigned scale) {
-    const unsigned biased = (word & 0x000f000fu) | 0x43004300u;
-    const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&biased), __float2bfloat162_rn(136.f)), *reinterpret_cast<const __nv_bfloat162*>(&scale));
+// Two whole numbers of a word times their scale, exactly, where a rotation to the right by `by` brings the nibbles to bits 3 .. 6 of the
+// halves: behind the bits of 16 they are the bfloat16 numbers 16 + v + 8, and 24 times the scale, which is taken off their product,
+// has seven bits.  (At bits 0 .. 3 it would be 136 times, ten bits, and take a subtraction and a product.)
+__device__ __forceinline__ unsigned scaled_two(unsigned word, int by, __nv_bfloat162 scale, __nv_bfloat162 less) {
+    const unsigned biased = (__funnelshift_r(word, word, by) & 0x00780078u) | 0x41804180u;
+    const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&biased), scale, less);
     return *reinterpret_cast<const unsigned*>(&v);
 }
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -332,8 +333,8 @@ static int launch_few(const Args& a, int* status, cudaStream_t stream) {
 // The tcgen05 product with the weight's rows as the 128 rows of the accumulator and N tokens (32 to 256) as its columns.  A stage holds
 // 64 places of K: one thread fetches the tokens (TMA, 128-byte swizzle, zeros beyond the last token and place), one issues the products,
 // and the other warps turn weights into bfloat16 in tensor memory, a row a lane, each group of four warps every kGroups-th tile of K: a
-// lane loads its row's four 16-byte pieces (which hold row g + 8 too) two tiles ahead, straight into registers, and a number is the
-// whole number times its scale, exactly, in four instructions for two.  (Weights in shared memory instead, written and then read by the
+// lane copies 16 bytes of each of the warp's two tiles of rows kAhead tiles ahead (cp.async), reads its row's four pieces (which hold
+// row g + 8 too), and a number is the whole number times its scale, exactly, in three instructions for two.  (Weights in shared memory instead, written and then read by the
 // products beside 256 tokens, took 100 KB of its traffic a tile, 780 cycles for 512 of the tensor core's.)  Where a weight has too few
 // rows to fill the SMs, K is cut over the blocks of a cluster.  The sums go from tensor memory to shared memory as they are, a row a
 // lane; then each token's results are read, four rows a thread (from all the cluster's blocks, in their order), finished, and written
@@ -349,15 +350,20 @@ struct WideArgs {
 
 template <int N> struct Wide {
     static constexpr int kBlocks = N <= 64 ? 2 : 1;          // of an SM
-    static constexpr int kStages = N == 256 ? 6 : N == 128 ? 8 : N == 64 ? 6 : 7;
+    static constexpr int kStages = N == 256 ? 5 : N == 128 ? 8 : N == 64 ? 6 : 7;
     static constexpr int kGroups = N <= 64 ? 2 : 4, kThreads = (2 + 4 * kGroups) * 32;
     static constexpr int kCols = N <= 64 ? 256 : 512;        // of tensor memory: N of sums, 32 a stage of weights
     static constexpr int kStage = N * 128;                   // bytes of the tokens of a tile of 64 places
     static constexpr int kSums = N * 128 * 4;
     static constexpr int kRing = kStages * kStage > kSums ? kStages * kStage : kSums;
-    static constexpr int kSmem = kRing + 1024 + 256;
+    static constexpr int kAhead = N == 256 ? 3 : N == 128 ? 4 : 6;               // packed tiles of a warp on their way
+    static constexpr int kUnit = 2 * kTileBytes + 128;       // two tiles of 16 rows, a scale (two, where groups have 32) a row
+    static constexpr int kSmem = kRing + 4 * kGroups * kAhead * kUnit + 1024 + 256;
     static_assert(N + 32 * kStages <= kCols && kBlocks * kCols <= 512, "tensor memory");
 };
+
+__device__ __forceinline__ void copy_async16(unsigned to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void copy_async4(unsigned to, const void* from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(to), "l"(from) : "memory"); }
 
 template <int N>
 __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kernel(const WideArgs wa, const __grid_constant__ CUtensorMap xmap) {
@@ -368,7 +374,8 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
     const Args& a = wa.a;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);     // [S][N tokens x 128 bytes]
-    unsigned long long* full = reinterpret_cast<unsigned long long*>(ring + W::kRing);
+    unsigned char* packed = ring + W::kRing;                                               // [warps][kAhead][unit]
+    unsigned long long* full = reinterpret_cast<unsigned long long*>(packed + 4 * KG * W::kAhead * W::kUnit);
     unsigned long long* empty = full + S;
     unsigned long long* done = empty + S;
     unsigned* slot = reinterpret_cast<unsigned*>(done + 1);
@@ -424,40 +431,55 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
     } else {
         // ---- weights: the quarter of the rows that the warp's lanes of tensor memory are, a row a lane ----
         const int quarter = warp & 3, first = (warp - 2) / 4, row = row0 + quarter * 32 + lane, tiles = (a.M + 15) / 16;
-        const int tile = min(row >> 4, tiles - 1), g = lane & 7;                            // (rows beyond the last tile are not written: any numbers do)
-        const unsigned high = lane >> 1 & 4;             // of a byte's two nibbles the second is row g + 8's: a shift of 0 or 4
-        const unsigned char* pieces = a.w + ((size_t)tile * a.stretches + kt0 / kBatch) * a.unit;
-        const unsigned char* scales = pieces + kBatch * kTileBytes + (lane & 15) * 8 * a.per_tile;
-        struct Tile { uint4 w[4]; unsigned scale; };     // (of 64 places; the scales of its halves)
-        Tile ahead[2];
-        auto fetch = [&](Tile& to, int kt) {
-            if (kt >= n_k) return;
-            const size_t at = (size_t)(kt / kBatch) * a.unit;
-            const uint4* from = reinterpret_cast<const uint4*>(pieces + at + kt % kBatch * kTileBytes) + 4 * g;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) to.w[t] = __ldg(from + t);
-            if (a.per_tile == 2) to.scale = __ldg(reinterpret_cast<const unsigned*>(scales + at) + kt % kBatch);
-            else to.scale = __ldg(reinterpret_cast<const unsigned short*>(scales + at) + kt % kBatch) * 0x10001u;
+        const int g = lane & 7;                          // (rows beyond the last tile are not written: any numbers do)
+        const int by0 = lane & 8 ? 1 : 29, by2 = lane & 8 ? 9 : 5;                          // (of a byte's two nibbles the second is row g + 8's)
+        const int tile_lo = min((row - lane) >> 4, tiles - 1), tile_hi = min(((row - lane) >> 4) + 1, tiles - 1);      // the warp's two
+        const size_t lo = ((size_t)tile_lo * a.stretches + kt0 / kBatch) * a.unit, hi = ((size_t)tile_hi * a.stretches + kt0 / kBatch) * a.unit;
+        const unsigned char* mine = packed + (warp - 2) * W::kAhead * W::kUnit;
+        // a lane brings piece (g, t) of both tiles and its row's scale; pieces stand at t ^ (g / 2), so that eight rows' meet in no bank
+        const unsigned put = smem_u32(mine) + ((lane & ~3) + ((lane & 3) ^ (lane >> 3))) * 16;
+        auto fetch = [&](int kt, int at) {
+            if (kt < n_k) {
+                const unsigned char* from = a.w + (size_t)(kt / kBatch) * a.unit + kt % kBatch * kTileBytes + lane * 16;
+                copy_async16(put + at * W::kUnit, from + lo);
+                copy_async16(put + at * W::kUnit + kTileBytes, from + hi);
+                copy_async4(smem_u32(mine) + at * W::kUnit + 2 * kTileBytes + lane * 4,
+                            a.w + (lane < 16 ? lo : hi) + (size_t)(kt / kBatch) * a.unit + kBatch * kTileBytes +
+                                ((lane & 15) * 2 * a.per_tile + (a.per_tile == 2 ? kt % kBatch : kt % kBatch / 2)) * 4);
+            }
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
         };
-        auto one = [&](Tile& now, int kt) {
+        for (int i = 0; i < W::kAhead; ++i) fetch(first + i * KG, i);
+        for (int kt = first, held = 0; kt < n_k; kt += KG) {
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(W::kAhead - 1) : "memory");
+            __syncwarp();                                // the pieces are other lanes' copies
+            const unsigned char* unit = mine + held * W::kUnit;
+            uint4 now[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) now[t] = *reinterpret_cast<const uint4*>(unit + (lane >> 4) * kTileBytes + (4 * g + (t ^ (g >> 1))) * 16);
+            unsigned scales = *reinterpret_cast<const unsigned*>(unit + 2 * kTileBytes + lane * 4);
+            if (a.per_tile == 1) scales = __byte_perm(scales, 0, kt & 1 ? 0x3232 : 0x1010);
+            __syncwarp();
+            fetch(kt + W::kAhead * KG, held);
+            held = held + 1 == W::kAhead ? 0 : held + 1;
             unsigned w[2][16];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const unsigned scale = __byte_perm(now.scale, 0, h == 0 ? 0x1010 : 0x3232);
+                const unsigned both = __byte_perm(scales, 0, h == 0 ? 0x1010 : 0x3232);
+                const __nv_bfloat162 scale = *reinterpret_cast<const __nv_bfloat162*>(&both), less = __hmul2(scale, __float2bfloat162_rn(-24.f));
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const unsigned word = (h == 0 ? (e == 0 ? now.w[t].x : now.w[t].y) : (e == 0 ? now.w[t].z : now.w[t].w)) >> high;
-                        w[h][4 * t + 2 * e] = scaled_two(word, scale);
-                        w[h][4 * t + 2 * e + 1] = scaled_two(word >> 8, scale);
+                        const unsigned word = h == 0 ? (e == 0 ? now[t].x : now[t].y) : (e == 0 ? now[t].z : now[t].w);
+                        w[h][4 * t + 2 * e] = scaled_two(word, by0, scale, less);
+                        w[h][4 * t + 2 * e + 1] = scaled_two(word, by2, scale, less);
                     }
             }
-            fetch(now, kt + 2 * KG);
             const int s = kt % S;
             if (kt >= S && !mbar_wait(empty + s, (kt / S - 1) & 1)) {
                 if (lane == 0) atomicCAS(wa.status, 0, Q4_TIMEOUT_PRODUCT);
-                return false;
+                break;
             }
             fence_after();
             const unsigned to = tmem + ((unsigned)(quarter * 32) << 16) + (unsigned)(N + s * 32);
@@ -467,14 +489,8 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(full + s);
-            return true;
-        };
-        fetch(ahead[0], first);
-        fetch(ahead[1], first + KG);
-        for (int kt = first; kt < n_k; kt += 2 * KG) {
-            if (!one(ahead[0], kt)) break;
-            if (kt + KG < n_k && !one(ahead[1], kt + KG)) break;
         }
+        asm volatile("cp.async.wait_group 0;\n" ::: "memory");
     }
     __syncwarp();
 
