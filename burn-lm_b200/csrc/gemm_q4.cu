@@ -54,7 +54,7 @@ __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)_
 __device__ __forceinline__ float bf16_of(unsigned two, int which) { return __uint_as_float(which ? two & 0xffff0000u : two << 16); }
 
 // ---- few tokens ------------------------------------------------------------------------------------------------------------
-// Up to 16 tokens a block (a block for each 16 of up to 32).  A cluster's blocks cut K into chunks of 2,048 places, a block's eight warps a
+// Up to 16 tokens.  A cluster's blocks cut K into chunks of 2,048 places, a block's eight warps a
 // chunk into stretches of 256, so that a warp meets the same tokens for every row: their fragments stay in its registers, and it does
 // nothing but stream its places of one tile of 16 rows after the other, AHEAD tiles ahead.  What bounds it beside the weights' bytes is
 // the instructions that make operands of them, so they are used as they are: sixteen bits that hold a whole number n below 256 are the
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(cons
     float* partial = reinterpret_cast<float*>(smem_few + kWarps * AHEAD * F::kUnit);       // [slots][warps][16][8 NT], then [slots][16][8 NT]
     float* sums = partial + F::kSlots * kWarps * F::kSums;
     unsigned long long* full = reinterpret_cast<unsigned long long*>(sums + F::kSlots * F::kSums) + warp * AHEAD;
-    const int rank = blockIdx.x % fa.chunks, cluster = blockIdx.x / fa.chunks, tok0 = blockIdx.y * 8 * NT, n = min(8 * NT, a.N - tok0);
+    const int rank = blockIdx.x % fa.chunks, cluster = blockIdx.x / fa.chunks, n = a.N;
     const int stretch = rank * kWarps + warp, kt = stretch * kBatch, tiles = (a.M + 15) / 16;
     const int t_lo = (int)((long long)tiles * cluster / fa.clusters), t_hi = (int)((long long)tiles * (cluster + 1) / fa.clusters);
     const bool here = stretch < a.stretches;
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(cons
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int k = (kt + j) * 64 + 32 * h + 8 * t, tok = 8 * i + g;
-                x[j][i][h] = tok < n && k < a.K ? *reinterpret_cast<const uint4*>(a.x + (size_t)(tok0 + tok) * a.ldx + k) : make_uint4(0u, 0u, 0u, 0u);
+                x[j][i][h] = tok < n && k < a.K ? *reinterpret_cast<const uint4*>(a.x + (size_t)tok * a.ldx + k) : make_uint4(0u, 0u, 0u, 0u);
             }
     // times a power of two: the largest of this stretch to 2^120 (zeros, infinities and NaN: as they are)
     float back[NT][2];                                   // of tokens 2 t and 2 t + 1: what takes that and the weights' 2^-133 off again, over 2^66
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(cons
                 if (a.end == END_GATED) up += cluster_float(at + 8 * 8 * NT * 4, r);
             }
             if (a.end == END_GATED) y = y / (1.0f + __expf(-y)) * up;
-            const size_t to = (size_t)(tok0 + tok) * a.ldy + out;
+            const size_t to = (size_t)tok * a.ldy + out;
             if (a.end == END_ADD) reinterpret_cast<float*>(a.y)[to] += y;
             else if (a.y_f32) reinterpret_cast<float*>(a.y)[to] = y;
             else reinterpret_cast<__nv_bfloat16*>(a.y)[to] = __float2bfloat16_rn(y);
@@ -280,14 +280,17 @@ __global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(cons
         for (int j = 0; j < AHEAD && unit + j < total_units; ++j) tc5::mbar_wait(full + (slot + j) % AHEAD, slot + j < AHEAD ? phase : phase ^ 1);
 }
 
-// The places of a cluster of eight blocks: longer rows run the other kernel whatever the tokens.
-constexpr int kFewTokens = 32, kFewTiles = 8 * kChunk;
+// Which kernel: up to 8 tokens the one for few, as far as a cluster of eight blocks reaches (16,384 places); up to 16 half as far.
+// Measured, a step of 1, 8 (and of 9 .. 16) tokens against the other kernel: 2,048 x 2,048 3.1, 3.3 (3.9) us against 4.4, 4.6 (4.8);
+// 28,672 x 4,096 16.5, 18.6 (30) against 36; 2,048 x 8,192 5.8, 7.0 (8.6) against 8.6, 8.8 (9.0); 4,096 x 14,336 11.5, 12.8 (23)
+// against 16.6, 17.0 (17.2).  With 17 to 32 tokens it took 15 against 14, 55 against 36, 11 against 9, and 42 against 17.
+static bool few_take(int n, int k_tiles) { return n <= 8 ? k_tiles <= 8 * kChunk : n <= 16 && k_tiles <= 4 * kChunk; }
 
 template <int NT, bool TWO>
 static int launch_few(const Args& a, int* status, cudaStream_t stream) {
     using F = Few<NT>;
     FewArgs fa{a, (a.stretches + kWarps - 1) / kWarps, 0, status};
-    const int tiles = (a.M + 15) / 16, tok_blocks = (a.N + 8 * NT - 1) / (8 * NT);
+    const int tiles = (a.M + 15) / 16;
     static bool opted_in[64] = {};
     static int resident[64][9] = {};                     // clusters of so many blocks that the device holds at once
     int dev = 0;
@@ -321,10 +324,10 @@ static int launch_few(const Args& a, int* status, cudaStream_t stream) {
         }
         resident[dev][fa.chunks] = fit < 1 ? 1 : fit;
     }
-    fa.clusters = resident[dev][fa.chunks] / tok_blocks;
+    fa.clusters = resident[dev][fa.chunks];
     if (fa.clusters > tiles) fa.clusters = tiles;
     if (fa.clusters < 1) fa.clusters = 1;
-    cfg.gridDim = dim3(fa.chunks * fa.clusters, tok_blocks);
+    cfg.gridDim = dim3(fa.chunks * fa.clusters);
     cudaLaunchKernelEx(&cfg, few_kernel<NT, TWO>, fa);
     return blm_check_launch("gemm_q4");
 }
@@ -620,7 +623,7 @@ BLM_API int blm_gemm_q4(const void* w, int stretches, int group, const void* x, 
     const int k_tiles = (k + 63) / 64, per_tile = group == 32 ? 2 : 1;
     BLM_REQUIRE(stretches == (k_tiles + kBatch - 1) / kBatch, "gemm_q4: %d stretches a row for %d places", stretches, k);
     const Args a{(const unsigned char*)w, (const __nv_bfloat16*)x, ldx, y, ldy, y_f32, end, n, m, k, k_tiles, stretches, kBatch * kTileBytes + 128 * per_tile, per_tile};
-    if (n > kFewTokens || k_tiles > kFewTiles) {
+    if (!few_take(n, k_tiles)) {
         BLM_REQUIRE((m + 127) / 128 <= 65535 && (n + 255) / 256 <= 65535, "gemm_q4: %d tokens, %d rows", n, m);
         return n <= 32 ? launch_wide<32>(a, status, stream) : n <= 64 ? launch_wide<64>(a, status, stream)
                : n <= 128 ? launch_wide<128>(a, status, stream) : launch_wide<256>(a, status, stream);
