@@ -344,18 +344,24 @@ static int launch_few(const Args& a, int* status, cudaStream_t stream) {
 // as whole lines.  Waits are bounded.
 enum { Q4_TIMEOUT_PRODUCT = 53 };
 
+// A grid that fills the SMs some times and leaves a few blocks is two launches: WAVES, whole times, then the REST with K cut over clusters.
+// The rest may run beside the last of the others: what both read is ready once WAVES has waited for the kernel before it, so that is when it
+// lets the rest begin, and the rest waits for WAVES at its end only (so that what follows waits for both).
+enum { ALONE = 0, WAVES = 1, REST = 2 };
 struct WideArgs {
     Args a;
     int share;                   // k tiles of a block of the cluster, whole stretches
     int vec;                     // rows of y and their beginnings allow four results at once
+    int ranks;                   // blocks of a cluster
+    int first, tok_blocks, part; // this launch's first block of rows and tokens (tokens first), blocks of tokens; ALONE, WAVES or REST
     int* status;
 };
 
 template <int N> struct Wide {
-    static constexpr int kBlocks = N <= 64 ? 2 : 1;          // of an SM
-    static constexpr int kStages = N == 256 ? 5 : N == 128 ? 8 : N == 64 ? 6 : 7;
-    static constexpr int kGroups = N <= 64 ? 2 : 4, kThreads = (2 + 4 * kGroups) * 32;
-    static constexpr int kCols = N <= 64 ? 256 : 512;        // of tensor memory: N of sums, 32 a stage of weights
+    static constexpr int kBlocks = N <= 128 ? 2 : 1;         // of an SM
+    static constexpr int kStages = N == 256 ? 5 : N == 128 ? 4 : N == 64 ? 6 : 7;
+    static constexpr int kGroups = N <= 128 ? 2 : 4, kThreads = (2 + 4 * kGroups) * 32;
+    static constexpr int kCols = N <= 128 ? 256 : 512;       // of tensor memory: N of sums, 32 a stage of weights
     static constexpr int kStage = N * 128;                   // bytes of the tokens of a tile of 64 places
     static constexpr int kSums = N * 128 * 4;
     static constexpr int kRing = kStages * kStage > kSums ? kStages * kStage : kSums;
@@ -383,7 +389,7 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
     unsigned long long* done = empty + S;
     unsigned* slot = reinterpret_cast<unsigned*>(done + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = blockIdx.x, ranks = gridDim.x, row0 = blockIdx.y * 128, tok0 = blockIdx.z * N;
+    const int ranks = wa.ranks, rank = blockIdx.x % ranks, block = wa.first + blockIdx.x / ranks, row0 = block / wa.tok_blocks * 128, tok0 = block % wa.tok_blocks * N;
     const int kt0 = rank * wa.share, n_k = max(0, min(a.k_tiles - kt0, wa.share));          // this block's tiles of K
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
@@ -397,12 +403,13 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
     fence_before();
     __syncthreads();
     fence_after();
-    pdl_launch_dependents();                              // (not before this block has its tensor memory: the next kernel may take some too)
+    if (wa.part != WAVES) pdl_launch_dependents();        // (not before this block has its tensor memory: the next kernel may take some too)
     const unsigned tmem = *slot;
 
     if (warp == 0) {
         if (lane == 0) {
-            pdl_wait();                                  // the tokens are the work of the kernel before
+            if (wa.part != REST) pdl_wait();             // the tokens are the work of the kernel before
+            if (wa.part == WAVES) pdl_launch_dependents();
             int i = 0;
             for (; i < n_k; ++i) {
                 const int s = i % S;
@@ -523,7 +530,7 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
 
     // ---- and out: four rows of a token a thread; the tokens shared by the cluster's blocks ----
     if (warp >= 2 && over) {
-        pdl_wait();                                      // (what is added to, or what the kernel before still reads)
+        if (wa.part != REST) pdl_wait();                 // (what is added to, or what the kernel before still reads)
         const bool gated = a.end == END_GATED;
         const int each = N / ranks, n_here = min(each, a.N - tok0 - rank * each), at_once = gated ? 4 : 5;        // (log2 of a token's threads)
         const int m_out = gated ? a.M / 2 : a.M, m0 = gated ? row0 / 2 : row0;
@@ -578,6 +585,7 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
             }
     }
     __syncwarp();
+    if (wa.part == REST) pdl_wait();
     if (ranks > 1) cluster_sync();
     if (warp == 1) {
         fence_after();
@@ -593,12 +601,6 @@ static int launch_wide(const Args& a, int* status, cudaStream_t stream) {
     const int box[2] = {64, N};
     if (!tc5::make_map<2>(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.x, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
         return blm_fail(BLM_CUDA_ERROR, "gemm_q4: no tensor map for %d tokens of %d places, rows %lld apart", a.N, a.K, a.ldx);
-    // blocks of a cluster: as many as it takes to have blocks for four of five SMs, each with a stretch of 256 places at least
-    const int row_blocks = (a.M + 127) / 128, tok_blocks = (a.N + N - 1) / N;
-    int ranks = 1;
-    while (ranks < 8 && (long long)row_blocks * tok_blocks * ranks * 5 < (long long)blm_sm_count() * W::kBlocks * 4 && a.k_tiles >= ranks * 2 * kBatch) ranks *= 2;
-    const int share = (a.k_tiles + ranks - 1) / ranks, unit = a.end == END_ADD || a.y_f32 ? 16 : 8;
-    const WideArgs wa{a, ranks == 1 ? share : (share + 3) / 4 * 4, a.ldy % 4 == 0 && (size_t)a.y % unit == 0, status};
     static bool opted_in[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -607,7 +609,25 @@ static int launch_wide(const Args& a, int* status, cudaStream_t stream) {
             return blm_fail(BLM_CUDA_ERROR, "gemm_q4: %s", cudaGetErrorString(cudaGetLastError()));
         if (dev >= 0 && dev < 64) opted_in[dev] = true;
     }
-    blm_launch_cluster(wide_kernel<N>, ranks, dim3(ranks, row_blocks, tok_blocks), dim3(W::kThreads), W::kSmem, stream, wa, map);
+    const int row_blocks = (a.M + 127) / 128, tok_blocks = (a.N + N - 1) / N, at_once = blm_sm_count() * W::kBlocks;
+    const int unit = a.end == END_ADD || a.y_f32 ? 16 : 8, vec = a.ldy % 4 == 0 && (size_t)a.y % unit == 0;
+    auto launch = [&](int first, int blocks, int part) {
+        // blocks of a cluster: the number with the shortest time, that of so many turns of a share of K each and, about as long as 16
+        // tiles of K, a block's beginning and end; no share below a stretch of 256 places
+        int ranks = 1;
+        auto tiles = [&](int r) { return (long long)((blocks * r + at_once - 1) / at_once) * ((a.k_tiles + r - 1) / r + 16); };
+        for (int r = 2; r <= 8 && a.k_tiles >= r * kBatch; r *= 2)
+            if (tiles(r) < tiles(ranks)) ranks = r;
+        const int share = (a.k_tiles + ranks - 1) / ranks;
+        const WideArgs wa{a, ranks == 1 ? share : (share + 3) / 4 * 4, vec, ranks, first, tok_blocks, part, status};
+        blm_launch_cluster(wide_kernel<N>, ranks, dim3(ranks * blocks), dim3(W::kThreads), W::kSmem, stream, wa, map);
+    };
+    // (512 tokens by 28,672 x 4,096 are 448 blocks for 148 SMs: 104 us in four times, the last of 4 blocks)
+    const int blocks = row_blocks * tok_blocks, rest = blocks % at_once;
+    if (blocks > at_once && rest > 0 && 2 * rest <= at_once && a.k_tiles >= 2 * kBatch) {
+        launch(0, blocks - rest, WAVES);
+        launch(blocks - rest, rest, REST);
+    } else launch(0, blocks, ALONE);
     return blm_check_launch("gemm_q4");
 }
 }  // namespace q4
@@ -624,7 +644,7 @@ BLM_API int blm_gemm_q4(const void* w, int stretches, int group, const void* x, 
     BLM_REQUIRE(stretches == (k_tiles + kBatch - 1) / kBatch, "gemm_q4: %d stretches a row for %d places", stretches, k);
     const Args a{(const unsigned char*)w, (const __nv_bfloat16*)x, ldx, y, ldy, y_f32, end, n, m, k, k_tiles, stretches, kBatch * kTileBytes + 128 * per_tile, per_tile};
     if (!few_take(n, k_tiles)) {
-        BLM_REQUIRE((m + 127) / 128 <= 65535 && (n + 255) / 256 <= 65535, "gemm_q4: %d tokens, %d rows", n, m);
+        BLM_REQUIRE((long long)((m + 127) / 128) * ((n + 255) / 256) < 1 << 28, "gemm_q4: %d tokens, %d rows", n, m);
         return n <= 32 ? launch_wide<32>(a, status, stream) : n <= 64 ? launch_wide<64>(a, status, stream)
                : n <= 128 ? launch_wide<128>(a, status, stream) : launch_wide<256>(a, status, stream);
     }
