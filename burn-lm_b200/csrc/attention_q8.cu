@@ -839,6 +839,19 @@ __device__ __forceinline__ float ex2(float x) {          // 2^x (x = -inf gives 
     return y;
 }
 
+// three numbers' largest, and two sums or products with a sum at once
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;\n" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+__device__ __forceinline__ void fma_two(float& x, float& y, float by, float plus) {
+    asm("{\n.reg .b64 v, b, p;\nmov.b64 v, {%0, %1};\nmov.b64 b, {%2, %2};\nmov.b64 p, {%3, %3};\nfma.rn.f32x2 v, v, b, p;\nmov.b64 {%0, %1}, v;\n}\n" : "+f"(x), "+f"(y) : "f"(by), "f"(plus));
+}
+__device__ __forceinline__ void add_two(float& x, float& y, float a, float b) {
+    asm("{\n.reg .b64 v, w;\nmov.b64 v, {%0, %1};\nmov.b64 w, {%2, %3};\nadd.rn.f32x2 v, v, w;\nmov.b64 {%0, %1}, v;\n}\n" : "+f"(x), "+f"(y) : "f"(a), "f"(b));
+}
+
 // How many of the n_splits shares of a sequence work: one per `pages_per_split` pages of 8-bit blocks.
 __host__ __device__ inline int active_splits(int n_pages, int n_splits, int pages_per_split) {
     const int want = (n_pages + pages_per_split - 1) / pages_per_split;
@@ -1324,7 +1337,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     unsigned long long* o_done = q_full + 1;
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(o_done + 1);
     unsigned* odd_values = tmem_slot + 1;                                    // [2] bits: keys of the own block whose values hold an infinity or a NaN
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int kvh = blockIdx.x / pa.head_groups, hg = blockIdx.x % pa.head_groups, seq = blockIdx.z;
     pdl_wait();
     const int tok0 = a.cu_seqlens[seq], n = a.cu_seqlens[seq + 1] - tok0, start = a.start_pos[seq], slot = a.slot_of_seq[seq], end = start + n;
@@ -1359,7 +1372,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     tc5::fence_after();
     pdl_launch_dependents();                              // (not before this block has its tensor memory: the next kernel may take some too)
     // a tile's columns: 64 of scores (and probabilities), HD of sums, HD / 2 of queries
-    const unsigned tmem = *tmem_slot;
+    const unsigned tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);                 // (one number for a warp: what the products are issued with)
     constexpr unsigned kTileCols = 256, kOCol = 64, kQCol = 64 + HD;
     const int width = a.n_heads + 2 * a.n_kv;
     const __nv_bfloat16* rows = reinterpret_cast<const __nv_bfloat16*>(a.rotated);
@@ -1392,16 +1405,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             for (int k = max(0, i - KS); k < i; ++k) mbar_wait(raw_full + k % KS, (k / KS) & 1);     // nothing is on its way when the block ends
     } else if (warp == 12) {
         // ---- products ----
-        if (lane == 0) {
+        {
             constexpr unsigned kScores = tc5::instruction(64), kSums = tc5::instruction(HD);
             const unsigned long long k_desc = tc5::operand(keys, 2, 1024), v_desc = tc5::operand(values, 2, 1024);
             auto scores = [&](int i, int j) {
+                if (tc5::elect()) {
                 const unsigned long long kd = k_desc + (unsigned)((j % KS) * (P::kTile >> 4));
 #pragma unroll
                 for (int k = 0; k < HD / 16; ++k)
                     tc5::mma_ts(tmem + i * kTileCols, tmem + i * kTileCols + kQCol + 8 * k, kd + (unsigned)((k >> 2) * (8192 >> 4) + 2 * (k & 3)), kScores, k > 0);
                 tc5::commit(s_full + i);
                 if (i == tiles - 1) tc5::commit(k_free + j % KS);
+                }
             };
             bool ok = mbar_wait(q_full, 0) && mbar_wait(k_full, 0);
             if (ok) {
@@ -1414,10 +1429,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                     ok = mbar_wait(p_full + i, j & 1) && (i > 0 || mbar_wait(v_full + s, (j / KS) & 1));
                     if (!ok) break;
                     tc5::fence_after();
+                    if (tc5::elect()) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         tc5::mma_ts(tmem + i * kTileCols + kOCol, tmem + i * kTileCols + 8 * k, v_desc + (unsigned)(s * (P::kTile >> 4) + 2 * k), kSums, j > 0 || k > 0);
                     if (i == tiles - 1) tc5::commit(v_free + s);
+                    }
+                    __syncwarp();
                     if (j + 1 == steps) continue;
                     ok = i > 0 || mbar_wait(k_full + (j + 1) % KS, ((j + 1) / KS) & 1);
                     if (!ok) break;
@@ -1425,8 +1443,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                     scores(i, j + 1);
                 }
             }
-            if (!ok) gave_up();
-            tc5::commit(o_done);                         // when all products so far are over
+            if (!ok && lane == 0) gave_up();
+            if (tc5::elect()) tc5::commit(o_done);                         // when all products so far are over
         }
     } else if (warp >= 8) {
         // ---- operands ----
@@ -1448,6 +1466,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             if (!own && !mbar_wait(raw_full + s, (j / KS) & 1)) { ok = false; break; }
             const float2 scale = own ? make_float2(1.f, 1.f) : *scales_of(page, HD);
             const bool none = scale.y < 0.f;
+            // a thread's pieces, all before the first use (each read waiting for the write before it would be the most of a page's time):
+            // of the keys sixteen lanes, four pieces of a 64-lane half by eight keys a warp; of the values four lanes of four keys
+            constexpr int kPieces = HD / 32;
+            auto key_at = [&](int i, int& half, int& r) {
+                const int at = i * 4 + cw;
+                half = HD == 128 ? at & 1 : 0;
+                r = (HD == 128 ? at >> 1 : at) * 8 + (lane >> 2);
+            };
+            uint4 kv[kPieces], vv[kPieces];
+            if (!own && !none) {
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    int half, r;
+                    key_at(i, half, r);
+                    kv[i] = *reinterpret_cast<const uint4*>(page + key_piece(r, (half * 4 + (lane & 3)) * 16, HD));
+                    vv[i] = *reinterpret_cast<const uint4*>(page + kPage * HD + cw * (16 * HD) + i * 512 + lane * 16);      // keys 16 cw .. 16 cw + 15
+                }
+            }
+            if (!own) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(raw_free + s);
+            }
             if (j >= KS && !mbar_wait(k_free + s, parity)) { ok = false; break; }
             if (own || none) {
                 constexpr int kEach = HD / 16;           // (all loads before the first use: one latency, not eight)
@@ -1464,11 +1504,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                     *reinterpret_cast<uint4*>(kt + (c >> 3) * 8192 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[i];
                 }
             } else {
-                // sixteen lanes of a key a thread: four pieces of a 64-lane half by eight keys a warp
 #pragma unroll
-                for (int i = 0; i < 64 * (HD / 16) / 128; ++i) {
-                    const int at = i * 4 + cw, half = HD == 128 ? at & 1 : 0, r = (HD == 128 ? at >> 1 : at) * 8 + (lane >> 2), piece = half * 4 + (lane & 3);
-                    const uint4 v = *reinterpret_cast<const uint4*>(page + key_piece(r, piece * 16, HD));
+                for (int i = 0; i < kPieces; ++i) {
+                    int half, r;
+                    key_at(i, half, r);
+                    const uint4 v = kv[i];
                     unsigned char* to = kt + half * 8192 + r * 128;
                     const int c = (lane & 3) * 2;
                     *reinterpret_cast<uint4*>(to + ((c ^ (r & 7)) << 4)) = make_uint4(tiny_two<0>(v.x), tiny_two<2>(v.x), tiny_two<0>(v.y), tiny_two<2>(v.y));
@@ -1515,8 +1555,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             } else {
                 const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-                for (int i = 0; i < HD / 32; ++i) {      // warp cw has keys 16 cw .. 16 cw + 15
-                    const uint4 v = *reinterpret_cast<const uint4*>(page + kPage * HD + cw * (16 * HD) + i * 512 + lane * 16);
+                for (int i = 0; i < kPieces; ++i) {
+                    const uint4 v = vv[i];
                     const unsigned w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
@@ -1527,10 +1567,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             }
             tc5::fence_async_smem();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(v_full + s);
-                if (!own) mbar_arrive(raw_free + s);
-            }
+            if (lane == 0) mbar_arrive(v_full + s);
         }
         if (!ok && lane == 0) gave_up();
     } else if (warp < 4 * tiles) {
@@ -1614,7 +1651,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             }
             float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-            for (int i = 4; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], x[i]);
+            for (int i = 4; i < 60; i += 8)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) top[k] = max3(top[k], x[i + k], x[i + k + 4]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], x[60 + k]);
             const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
             // (nothing seen: the product is minus infinity, or none where f is zero or none: neither moves the reference)
             const bool move = mx > m + 8.f;
@@ -1640,9 +1681,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             const float less = shift - (m == -INFINITY ? 0.f : m);
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 64; ++i) {
-                x[i] = ex2(fmaf(x[i], f, less));
-                sum[i & 3] += x[i];
+            for (int i = 0; i < 64; i += 2) {
+                fma_two(x[i], x[i + 1], f, less);
+                x[i] = ex2(x[i]);
+                x[i + 1] = ex2(x[i + 1]);
+                add_two(sum[i & 2], sum[(i & 2) + 1], x[i], x[i + 1]);
             }
 #pragma unroll
             for (int c = 0; c < 32; c += 16) {

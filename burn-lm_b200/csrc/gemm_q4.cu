@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
     unsigned long long* empty = full + S;
     unsigned long long* done = empty + S;
     unsigned* slot = reinterpret_cast<unsigned*>(done + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int ranks = wa.ranks, rank = blockIdx.x % ranks, block = wa.first + blockIdx.x / ranks, row0 = block / wa.tok_blocks * 128, tok0 = block % wa.tok_blocks * N;
     const int kt0 = rank * wa.share, n_k = max(0, min(a.k_tiles - kt0, wa.share));          // this block's tiles of K
     if (threadIdx.x == 0) {
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
     __syncthreads();
     fence_after();
     if (wa.part != WAVES) pdl_launch_dependents();        // (not before this block has its tensor memory: the next kernel may take some too)
-    const unsigned tmem = *slot;
+    const unsigned tmem = __shfl_sync(0xffffffffu, *slot, 0);
 
     if (warp == 0) {
         if (lane == 0) {
@@ -423,21 +423,27 @@ __global__ void __launch_bounds__(Wide<N>::kThreads, Wide<N>::kBlocks) wide_kern
             for (int k = max(0, i - S); k < i; ++k) mbar_wait(full + k % S, (k / S) & 1);   // nothing is on its way when the block ends
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr unsigned id = instruction(N);
-            int s = 0;
-            unsigned phase = 0;
-            for (int i = 0; i < n_k; ++i) {
-                if (!mbar_wait(full + s, phase)) { atomicCAS(wa.status, 0, Q4_TIMEOUT_PRODUCT); break; }
-                fence_after();
+        // (the whole warp, so that what a product is issued with is known to be one number for all its lanes: behind `lane == 0` the
+        // issue of a product took 65 cycles and a wait 400)
+        constexpr unsigned id = instruction(N);
+        int s = 0;
+        unsigned phase = 0;
+        for (int i = 0; i < n_k; ++i) {
+            if (!mbar_wait(full + s, phase)) {
+                if (lane == 0) atomicCAS(wa.status, 0, Q4_TIMEOUT_PRODUCT);
+                break;
+            }
+            fence_after();
+            if (elect()) {
                 const unsigned long long bd = operand(ring + s * W::kStage, 2, 1024);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) mma_ts(tmem, tmem + N + s * 32 + 8 * k, bd + 2 * k, id, i > 0 || k > 0);
                 commit(empty + s);
-                if (++s == S) { s = 0; phase ^= 1; }
             }
-            commit(done);                                // when all products so far are over
+            __syncwarp();
+            if (++s == S) { s = 0; phase ^= 1; }
         }
+        if (elect()) commit(done);                       // when all products so far are over
     } else {
         // ---- weights: the quarter of the rows that the warp's lanes of tensor memory are, a row a lane ----
         const int quarter = warp & 3, first = (warp - 2) / 4, row = row0 + quarter * 32 + lane, tiles = (a.M + 15) / 16;
