@@ -54,7 +54,7 @@ __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)_
 __device__ __forceinline__ float bf16_of(unsigned two, int which) { return __uint_as_float(which ? two & 0xffff0000u : two << 16); }
 
 // ---- few tokens ------------------------------------------------------------------------------------------------------------
-// Up to 16 tokens.  A cluster's blocks cut K into chunks of 2,048 places, a block's eight warps a
+// Up to 8 tokens.  A cluster's blocks cut K into chunks of 2,048 places, a block's eight warps a
 // chunk into stretches of 256, so that a warp meets the same tokens for every row: their fragments stay in its registers, and it does
 // nothing but stream its places of one tile of 16 rows after the other, AHEAD tiles ahead.  What bounds it beside the weights' bytes is
 // the instructions that make operands of them, so they are used as they are: sixteen bits that hold a whole number n below 256 are the
@@ -66,11 +66,11 @@ __device__ __forceinline__ float bf16_of(unsigned two, int which) { return __uin
 // distributed shared memory, in a fixed order.
 constexpr int kWarps = 8, kChunk = kWarps * kBatch;      // k tiles of a block
 enum { Q4_TIMEOUT_WEIGHTS = 54 };
-template <int NT> struct Few {
-    static constexpr int kAhead = NT == 1 ? 3 : 4, kBlocks = NT == 1 ? 2 : 1;      // tiles of rows on their way a warp; blocks of an SM
+struct Few {
+    static constexpr int kAhead = 3, kBlocks = 2;                                  // tiles of rows on their way a warp; blocks of an SM
     static constexpr int kUnit = kBatch * kTileBytes + 256;                        // room for a stretch of a tile of rows
-    static constexpr int kSlots = NT == 1 ? 12 : 16;                                 // tiles of rows between two meetings
-    static constexpr int kSums = 16 * 8 * NT;                                      // of a tile: [16 rows][8 NT tokens]
+    static constexpr int kSlots = 12;                                              // tiles of rows between two meetings
+    static constexpr int kSums = 16 * 8;                                           // of a tile: [16 rows][8 tokens]
     static constexpr int kSmem = kWarps * kAhead * kUnit + kSlots * (kWarps + 1) * kSums * 4 + kWarps * kAhead * 8;
 };
 
@@ -80,15 +80,15 @@ struct FewArgs {
     int* status;
 };
 
-template <int NT, bool TWO>
-__global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(const FewArgs fa) {
-    using F = Few<NT>;
+template <bool TWO>
+__global__ void __launch_bounds__(kWarps * 32, Few::kBlocks) few_kernel(const FewArgs fa) {
+    using F = Few;
     constexpr int AHEAD = F::kAhead, PARTS = TWO ? 2 : 1;                          // parts of a tile with a scale of their own
     const Args& a = fa.a;
     extern __shared__ __align__(128) unsigned char smem_few[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     unsigned char* ring = smem_few + warp * AHEAD * F::kUnit;                      // this warp's units
-    float* partial = reinterpret_cast<float*>(smem_few + kWarps * AHEAD * F::kUnit);       // [slots][warps][16][8 NT], then [slots][16][8 NT]
+    float* partial = reinterpret_cast<float*>(smem_few + kWarps * AHEAD * F::kUnit);       // [slots][warps][16][8], then [slots][16][8]
     float* sums = partial + F::kSlots * kWarps * F::kSums;
     unsigned long long* full = reinterpret_cast<unsigned long long*>(sums + F::kSlots * F::kSums) + warp * AHEAD;
     const int rank = blockIdx.x % fa.chunks, cluster = blockIdx.x / fa.chunks, n = a.N;
@@ -114,26 +114,22 @@ __global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(cons
     }
     __syncwarp();
     pdl_wait();                                          // the tokens are the work of the kernel before
-    uint4 x[kBatch][NT][2];
+    uint4 x[kBatch][2];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int k = (kt + j) * 64 + 32 * h + 8 * t, tok = 8 * i + g;
-                x[j][i][h] = tok < n && k < a.K ? *reinterpret_cast<const uint4*>(a.x + (size_t)tok * a.ldx + k) : make_uint4(0u, 0u, 0u, 0u);
-            }
+        for (int h = 0; h < 2; ++h) {
+            const int k = (kt + j) * 64 + 32 * h + 8 * t;
+            x[j][h] = g < n && k < a.K ? *reinterpret_cast<const uint4*>(a.x + (size_t)g * a.ldx + k) : make_uint4(0u, 0u, 0u, 0u);
+        }
     // times a power of two: the largest of this stretch to 2^120 (zeros, infinities and NaN: as they are)
-    float back[NT][2];                                   // of tokens 2 t and 2 t + 1: what takes that and the weights' 2^-133 off again, over 2^66
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
+    float back[2];                                   // of tokens 2 t and 2 t + 1: what takes that and the weights' 2^-133 off again, over 2^66
+    {
         unsigned top = 0;                                // of two magnitudes' bits at once
 #pragma unroll
         for (int j = 0; j < kBatch; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint4 v = x[j][i][h];
+                const uint4 v = x[j][h];
                 top = __vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), __vmaxu2(__vmaxu2(v.y & 0x7fff7fffu, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu));
             }
         top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -149,27 +145,25 @@ __global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(cons
         for (int j = 0; j < kBatch; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                uint4& v = x[j][i][h];
+                uint4& v = x[j][h];
                 v = make_uint4(times(v.x), times(v.y), times(v.z), times(v.w));
             }
         const float mine = __uint_as_float((unsigned)(127 + 67 - by) << 23);      // 2^(133 - 66 - by), of token g
-        back[i][0] = __shfl_sync(0xffffffffu, mine, 8 * t);
-        back[i][1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
+        back[0] = __shfl_sync(0xffffffffu, mine, 8 * t);
+        back[1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
     }
     // where a part's sum starts: -8 times the sum of its places for row g, -128 times for row g + 8
-    float start[kBatch][PARTS][NT][4];
+    float start[kBatch][PARTS][4];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float (&d)[4] = start[j][TWO ? h : 0][i];
-                if (TWO || h == 0) d[0] = d[1] = d[2] = d[3] = 0.f;
-                constexpr unsigned k8 = 0x80088008u, k128 = 0x80808080u;
-                mma16(d, k8, k128, k8, k128, x[j][i][h].x, x[j][i][h].y);
-                mma16(d, k8, k128, k8, k128, x[j][i][h].z, x[j][i][h].w);
-            }
+        for (int h = 0; h < 2; ++h) {
+            float (&d)[4] = start[j][TWO ? h : 0];
+            if (TWO || h == 0) d[0] = d[1] = d[2] = d[3] = 0.f;
+            constexpr unsigned k8 = 0x80088008u, k128 = 0x80808080u;
+            mma16(d, k8, k128, k8, k128, x[j][h].x, x[j][h].y);
+            mma16(d, k8, k128, k8, k128, x[j][h].z, x[j][h].w);
+        }
 
     const int m_out = a.end == END_GATED ? a.M / 2 : a.M, rows = a.end == END_GATED ? 8 : 16;
     int unit = 0, slot = 0;                              // the next of this warp's, and where it lies
@@ -177,14 +171,10 @@ __global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(cons
     bool ok = true;
     for (int b0 = t_lo; b0 < t_hi; b0 += F::kSlots) {
         const int count = min(F::kSlots, t_hi - b0);
-        float* to = partial + warp * F::kSums + g * 8 * NT + 2 * t;
+        float* to = partial + warp * F::kSums + g * 8 + 2 * t;
 #pragma unroll 1
         for (int r = 0; r < count; ++r, to += kWarps * F::kSums) {
-            float total[NT][4];
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) total[i][e] = 0.f;
+            float total[4] = {0.f, 0.f, 0.f, 0.f};
             if (here && ok) {
                 if (!tc5::mbar_wait(full + slot, phase)) {
                     if (lane == 0) atomicCAS(fa.status, 0, Q4_TIMEOUT_WEIGHTS);
@@ -214,34 +204,25 @@ __global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(cons
                 for (int j = 0; j < kBatch; ++j)
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p) {
-                        float part[NT][4];
+                        float part[4];
 #pragma unroll
                         for (int q = 0; q < 4 / PARTS; ++q) {
                             const int s = p * 2 + q;
                             const unsigned lo = s == 0 ? w[j].x : s == 1 ? w[j].y : s == 2 ? w[j].z : w[j].w, hi = lo >> 8;
                             const unsigned a0 = lo & 0x000f000fu, a1 = lo & 0x00f000f0u, a2 = hi & 0x000f000fu, a3 = hi & 0x00f000f0u;
-#pragma unroll
-                            for (int i = 0; i < NT; ++i) {
-                                const uint4& v = x[j][i][s >> 1];
-                                mma16_onto(part[i], a0, a1, a2, a3, s & 1 ? v.z : v.x, s & 1 ? v.w : v.y, q == 0 ? start[j][p][i] : part[i]);
-                            }
+                            const uint4& v = x[j][s >> 1];
+                            mma16_onto(part, a0, a1, a2, a3, s & 1 ? v.z : v.x, s & 1 ? v.w : v.y, q == 0 ? start[j][p] : part);
                         }
                         const int at = j * PARTS + p;    // of the stretch's scales
                         const float m0 = bf16_of(sc[0][at >> 1], at & 1), m8 = bf16_of(sc[1][at >> 1], at & 1);
-#pragma unroll
-                        for (int i = 0; i < NT; ++i) {
-                            total[i][0] = fmaf(m0, part[i][0], total[i][0]);
-                            total[i][1] = fmaf(m0, part[i][1], total[i][1]);
-                            total[i][2] = fmaf(m8, part[i][2], total[i][2]);
-                            total[i][3] = fmaf(m8, part[i][3], total[i][3]);
-                        }
+                        total[0] = fmaf(m0, part[0], total[0]);
+                        total[1] = fmaf(m0, part[1], total[1]);
+                        total[2] = fmaf(m8, part[2], total[2]);
+                        total[3] = fmaf(m8, part[3], total[3]);
                     }
             }
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                *reinterpret_cast<float2*>(to + 8 * i) = make_float2(total[i][0] * 0x1p66f * back[i][0], total[i][1] * 0x1p66f * back[i][1]);
-                *reinterpret_cast<float2*>(to + 8 * 8 * NT + 8 * i) = make_float2(total[i][2] * 0x1p62f * back[i][0], total[i][3] * 0x1p62f * back[i][1]);
-            }
+            *reinterpret_cast<float2*>(to) = make_float2(total[0] * 0x1p66f * back[0], total[1] * 0x1p66f * back[1]);
+            *reinterpret_cast<float2*>(to + 8 * 8) = make_float2(total[2] * 0x1p62f * back[0], total[3] * 0x1p62f * back[1]);
         }
         __syncthreads();
         for (int i = threadIdx.x; i < count * F::kSums; i += kWarps * 32) {
@@ -259,11 +240,11 @@ __global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(cons
         for (int i = threadIdx.x; i < mine * rows * n; i += kWarps * 32) {
             const int row = i % rows, tok = i / rows % n, slot = i / (rows * n) * fa.chunks + rank, out = (b0 + slot) * rows + row;
             if (out >= m_out) continue;
-            const unsigned at = base + (unsigned)((slot * 16 + row) * 8 * NT + tok) * 4;
+            const unsigned at = base + (unsigned)((slot * 16 + row) * 8 + tok) * 4;
             float y = 0.f, up = 0.f;
             for (int r = 0; r < fa.chunks; ++r) {
                 y += cluster_float(at, r);
-                if (a.end == END_GATED) up += cluster_float(at + 8 * 8 * NT * 4, r);
+                if (a.end == END_GATED) up += cluster_float(at + 8 * 8 * 4, r);
             }
             if (a.end == END_GATED) y = y / (1.0f + __expf(-y)) * up;
             const size_t to = (size_t)tok * a.ldy + out;
@@ -280,15 +261,15 @@ __global__ void __launch_bounds__(kWarps * 32, Few<NT>::kBlocks) few_kernel(cons
         for (int j = 0; j < AHEAD && unit + j < total_units; ++j) tc5::mbar_wait(full + (slot + j) % AHEAD, slot + j < AHEAD ? phase : phase ^ 1);
 }
 
-// Which kernel: up to 8 tokens the one for few, as far as a cluster of eight blocks reaches (16,384 places); up to 16 half as far.
-// Measured, a step of 1, 8 (and of 9 .. 16) tokens against the other kernel: 2,048 x 2,048 3.1, 3.3 (3.9) us against 4.4, 4.6 (4.8);
-// 28,672 x 4,096 16.5, 18.6 (30) against 36; 2,048 x 8,192 5.8, 7.0 (8.6) against 8.6, 8.8 (9.0); 4,096 x 14,336 11.5, 12.8 (23)
-// against 16.6, 17.0 (17.2).  With 17 to 32 tokens it took 15 against 14, 55 against 36, 11 against 9, and 42 against 17.
-static bool few_take(int n, int k_tiles) { return n <= 8 ? k_tiles <= 8 * kChunk : n <= 16 && k_tiles <= 4 * kChunk; }
+// Which kernel: up to 8 tokens the one for few, as far as a cluster of eight blocks reaches (16,384 places).  Measured, 1 and 8 tokens
+// against the other kernel: 2,048 x 2,048 3.1 and 3.3 us against 4.0 and 4.2; 6,144 x 4,096 6.7 and 7.6 against 8.2 and 8.5; 28,672 x 4,096
+// 16.5 and 18.5 against 28 and 27; 4,096 x 14,336 11.5 and 12.8 against 14.7 and 15.0.  (With two products a piece of weights for 16
+// tokens: 3.9, 10.6, 30 and 23 against 4.4, 8.7, 27 and 15.3.)
+static bool few_take(int n, int k_tiles) { return n <= 8 && k_tiles <= 8 * kChunk; }
 
-template <int NT, bool TWO>
+template <bool TWO>
 static int launch_few(const Args& a, int* status, cudaStream_t stream) {
-    using F = Few<NT>;
+    using F = Few;
     FewArgs fa{a, (a.stretches + kWarps - 1) / kWarps, 0, status};
     const int tiles = (a.M + 15) / 16;
     static bool opted_in[64] = {};
@@ -297,7 +278,7 @@ static int launch_few(const Args& a, int* status, cudaStream_t stream) {
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return blm_fail(BLM_CUDA_ERROR, "gemm_q4: device %d", dev);
     if (!opted_in[dev]) {
-        if (cudaFuncSetAttribute(few_kernel<NT, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem) != cudaSuccess)
+        if (cudaFuncSetAttribute(few_kernel<TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem) != cudaSuccess)
             return blm_fail(BLM_CUDA_ERROR, "gemm_q4: %s", cudaGetErrorString(cudaGetLastError()));
         opted_in[dev] = true;
     }
@@ -318,7 +299,7 @@ static int launch_few(const Args& a, int* status, cudaStream_t stream) {
         // (a cluster lies in one group of SMs, which a number of blocks need not divide)
         int fit = blm_sm_count() * F::kBlocks;
         cfg.gridDim = dim3(fa.chunks);
-        if (fa.chunks > 1 && (cudaOccupancyMaxActiveClusters(&fit, few_kernel<NT, TWO>, &cfg) != cudaSuccess || fit < 1)) {
+        if (fa.chunks > 1 && (cudaOccupancyMaxActiveClusters(&fit, few_kernel<TWO>, &cfg) != cudaSuccess || fit < 1)) {
             cudaGetLastError();
             fit = blm_sm_count() * F::kBlocks / (2 * fa.chunks);
         }
@@ -328,7 +309,7 @@ static int launch_few(const Args& a, int* status, cudaStream_t stream) {
     if (fa.clusters > tiles) fa.clusters = tiles;
     if (fa.clusters < 1) fa.clusters = 1;
     cfg.gridDim = dim3(fa.chunks * fa.clusters);
-    cudaLaunchKernelEx(&cfg, few_kernel<NT, TWO>, fa);
+    cudaLaunchKernelEx(&cfg, few_kernel<TWO>, fa);
     return blm_check_launch("gemm_q4");
 }
 
@@ -358,7 +339,7 @@ struct WideArgs {
 };
 
 template <int N> struct Wide {
-    static constexpr int kBlocks = N <= 128 ? 2 : 1;         // of an SM
+    static constexpr int kBlocks = N <= 128 ? 2 : 1;         // of an SM (128 tokens by 28,672 x 4,096: 36 us with two, 52 with one of 18 warps)
     static constexpr int kStages = N == 256 ? 5 : N == 128 ? 4 : N == 64 ? 6 : 7;
     static constexpr int kGroups = N <= 128 ? 2 : 4, kThreads = (2 + 4 * kGroups) * 32;
     static constexpr int kCols = N <= 128 ? 256 : 512;       // of tensor memory: N of sums, 32 a stage of weights
@@ -654,6 +635,5 @@ BLM_API int blm_gemm_q4(const void* w, int stretches, int group, const void* x, 
         return n <= 32 ? launch_wide<32>(a, status, stream) : n <= 64 ? launch_wide<64>(a, status, stream)
                : n <= 128 ? launch_wide<128>(a, status, stream) : launch_wide<256>(a, status, stream);
     }
-    if (n <= 8) return per_tile == 2 ? launch_few<1, true>(a, status, stream) : launch_few<1, false>(a, status, stream);
-    return per_tile == 2 ? launch_few<2, true>(a, status, stream) : launch_few<2, false>(a, status, stream);
+    return per_tile == 2 ? launch_few<true>(a, status, stream) : launch_few<false>(a, status, stream);
 }
