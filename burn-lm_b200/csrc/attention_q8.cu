@@ -1292,6 +1292,7 @@ enum { Q8_TIMEOUT_PROMPT = 55 };
 struct PromptArgs {
     AttendArgs a;
     int head_groups, heads_a_group;      // of a kv head's queries: at most four heads each
+    int ranks;                           // blocks of a cluster, which share a walk
     int* status;
 };
 template <int HD> struct Prompt {
@@ -1338,16 +1339,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(o_done + 1);
     unsigned* odd_values = tmem_slot + 1;                                    // [2] bits: keys of the own block whose values hold an infinity or a NaN
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int kvh = blockIdx.x / pa.head_groups, hg = blockIdx.x % pa.head_groups, seq = blockIdx.z;
+    const int ranks = pa.ranks, rank = blockIdx.x % ranks, kv_group = blockIdx.x / ranks;
+    const int kvh = kv_group / pa.head_groups, hg = kv_group % pa.head_groups, seq = blockIdx.z;
     pdl_wait();
     const int tok0 = a.cu_seqlens[seq], n = a.cu_seqlens[seq + 1] - tok0, start = a.start_pos[seq], slot = a.slot_of_seq[seq], end = start + n;
     // the sequence's last blocks, which walk furthest, begin first
     const int mine = (end - 1) / kPage - (int)blockIdx.y;
-    if (n <= 0 || mine < start / kPage) return;          // (the whole block)
+    if (n <= 0 || mine < start / kPage) return;          // (the whole cluster)
     const int p0 = mine * kPage, group = a.n_heads / a.n_kv, head0 = kvh * group + hg * pa.heads_a_group;
     const int G = min(pa.heads_a_group, group - hg * pa.heads_a_group), tiles = (G + 1) / 2;
     auto first_key = [&](int pos) { return a.window > 0 ? max(0, pos + 1 - a.window) : 0; };
-    const int pg_lo = first_key(max(start, p0)) / kPage, steps = mine - pg_lo + 1;          // the last step is the own block
+    // this block's share of the walk (some may have none); the last step of the last is the own block
+    const int pg_first = first_key(max(start, p0)) / kPage, share = (mine - pg_first + ranks) / ranks;
+    const int pg_lo = pg_first + rank * share, steps = max(0, min(share, mine + 1 - pg_lo)), own_rank = (mine - pg_first) / share;
+    const int own_step = rank == own_rank ? steps - 1 : steps;
     if (threadIdx.x == 0) {
         for (int s = 0; s < KS; ++s) {
             mbar_init(raw_full + s, 1);
@@ -1376,14 +1381,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     constexpr unsigned kTileCols = 256, kOCol = 64, kQCol = 64 + HD;
     const int width = a.n_heads + 2 * a.n_kv;
     const __nv_bfloat16* rows = reinterpret_cast<const __nv_bfloat16*>(a.rotated);
+    // where the cluster's blocks leave their sums, over the rings: [256 rows][HD] with row r's 16-byte pieces at c ^ (r & 7), then maxima and sums
+    static_assert(256 * (HD + 2) * 4 <= KS * (2 * P::kTile + P::kRaw), "room for the sums");
+    auto met_at = [&](int row, int c) { return reinterpret_cast<float4*>(smem + row * (HD * 4) + ((c ^ (row & 7)) << 4)); };
+    float* met_m = reinterpret_cast<float*>(smem + 256 * HD * 4);
+    float* met_l = met_m + 256;
     auto gave_up = [&] { atomicCAS(pa.status, 0, Q8_TIMEOUT_PROMPT); };
 
     if (warp == 13) {
         // ---- pages ----
         int i = 0;
         bool failed = false;
-        for (int base = pg_lo; base < mine; base += 32) {
-            const int count = min(32, mine - base);
+        for (int base = pg_lo; base < pg_lo + own_step; base += 32) {
+            const int count = min(32, pg_lo + own_step - base);
             const int my_page = lane < count ? page_of(a.block_table, a.table_stride, slot, base + lane, a.n_pages) : -1;
             for (int j = 0; j < count; ++j) {
                 const int page = __shfl_sync(0xffffffffu, my_page, j);
@@ -1418,8 +1428,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                 if (i == tiles - 1) tc5::commit(k_free + j % KS);
                 }
             };
-            bool ok = mbar_wait(q_full, 0) && mbar_wait(k_full, 0);
-            if (ok) {
+            bool ok = mbar_wait(q_full, 0) && (steps == 0 || mbar_wait(k_full, 0));
+            if (ok && steps > 0) {
                 tc5::fence_after();
                 for (int i = 0; i < tiles; ++i) scores(i, 0);
             }
@@ -1452,7 +1462,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         bool ok = true;
         for (int j = 0; j < steps && ok; ++j) {
             const int s = j % KS, parity = (j / KS - 1) & 1;
-            const bool own = j == steps - 1;
+            const bool own = j == own_step;
             unsigned char* kt = keys + s * P::kTile;
             unsigned char* vt = values + s * P::kTile;
             const unsigned char* page = raw + s * P::kRaw;
@@ -1628,7 +1638,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         for (int j = 0; j < steps; ++j) {
             if (!mbar_wait(s_full + tile, j & 1)) { ok = false; break; }
             tc5::fence_after();
-            const bool own = j == steps - 1;
+            const bool own = j == own_step;
             const int key0 = (pg_lo + j) * kPage;
             const float2 scale = scales[j & 3];
             // probabilities leave times 2^shift, the values' scale times 2^60 (the own block's: 2^-73), and their sum is divided by it again
@@ -1703,7 +1713,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         if (ok) ok = mbar_wait(o_done, 0);
         if (!ok && lane == 0) gave_up();
         tc5::fence_after();
-        if (ok) {
+        if (ok && ranks > 1) {                           // the sums as they are, for the cluster
+            met_m[r + tile * 128] = m;
+            met_l[r + tile * 128] = l;
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c) {          // columns n 8 + g: lanes g HD / 8 + n
+                float o[64];
+#pragma unroll
+                for (int i = 0; i < 64; i += 16) {
+                    if (steps > 0) tc5::tmem_ld16(at + kOCol + c * 64 + i, o + i);
+                    else
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) o[i + k] = 0.f;
+                }
+                tc5::wait_ld(o);
+#pragma unroll
+                for (int g = 0; g < 8; ++g)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        *met_at(tile * 128 + r, g * (HD / 32) + c * 2 + x) = make_float4(o[32 * x + g], o[32 * x + 8 + g], o[32 * x + 16 + g], o[32 * x + 24 + g]);
+            }
+        } else if (ok) {
             const float by = 1.f / l;
             // the odd values among the keys that the row sees in its block
             unsigned long long seen_odd = (unsigned long long)odd_values[1] << 32 | odd_values[0];
@@ -1746,26 +1776,109 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             }
         }
     }
+    __syncwarp();
     tc5::fence_before();
-    __syncthreads();
+    if (ranks > 1) {
+        // ---- the cluster's shares meet: some of the rows each, four lanes a thread ----
+        cluster_sync();
+        const int some = tiles * 128 / ranks;
+        unsigned long long odd = 0;
+        for (int w = 0; w < 2; ++w) odd |= (unsigned long long)__float_as_uint(cluster_float(smem_u32(odd_values + w), own_rank)) << (32 * w);
+        // the shares' weights, a thread each: a row's are neighbours
+        float* weights = reinterpret_cast<float*>(staged);                       // [rows][ranks]
+        if (threadIdx.x < some * ranks) {
+            const int row = rank * some + threadIdx.x / ranks, k = threadIdx.x % ranks;
+            const float mk = cluster_float(smem_u32(met_m + row), k), lk = cluster_float(smem_u32(met_l + row), k);
+            float top = mk;
+            for (int w = 1; w < ranks; w *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            const float by = mk == top ? 1.f : ex2(mk - top);
+            float l = lk * by;
+            for (int w = 1; w < ranks; w *= 2) l += __shfl_xor_sync(0xffffffffu, l, w);
+            weights[threadIdx.x] = by * (0x1p73f / l);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < some * (HD / 4); i += kPromptThreads) {
+            const int mine = i / (HD / 4), row = rank * some + mine, c = i % (HD / 4), pos = p0 + (row & 63), h = row >> 6;
+            if (h >= G || pos < start || pos >= end) continue;
+            float o[4] = {0.f, 0.f, 0.f, 0.f};
+            float4 v[8];                                 // (all reads before the first use)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < ranks) v[k] = cluster_float4(smem_u32(met_at(row, c)), k);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < ranks) {
+                    const float by = weights[mine * ranks + k];
+                    o[0] = fmaf(v[k].x, by, o[0]); o[1] = fmaf(v[k].y, by, o[1]); o[2] = fmaf(v[k].z, by, o[2]); o[3] = fmaf(v[k].w, by, o[3]);
+                }
+            const int lo = first_key(pos);
+            __nv_bfloat16 y[4];
+            for (int e = 0; e < 4; ++e) {
+                float x = o[e];
+                if (odd != 0)
+                    for (int k = max(lo, p0); k <= pos; ++k)
+                        if (odd >> (k - p0) & 1) {
+                            const __nv_bfloat16* from = k >= start ? rows + ((size_t)(tok0 + k - start) * width + a.n_heads + a.n_kv + kvh) * HD
+                                                                   : reinterpret_cast<const __nv_bfloat16*>(a.found) + ((((size_t)seq * 2 + 1) * a.n_kv + kvh) * kPage + k - p0) * HD;
+                            const float v = __bfloat162float(from[c * 4 + e]);
+                            if (!(fabsf(v) < INFINITY)) x += v;
+                        }
+                y[e] = __float2bfloat16(x);
+            }
+            *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + ((size_t)(tok0 + pos - start) * a.n_heads + head0 + h) * HD + c * 4) = *reinterpret_cast<const uint2*>(y);
+        }
+        cluster_sync();                                  // what others read stays until they have
+    } else {
+        __syncthreads();
+    }
     if (warp == 12) {
         tc5::fence_after();
         tc5::tmem_free(tmem, 512);
     }
 }
 
+// `touched` 64-position blocks of all sequences, the longest walk of so many `pages`.
 template <int HD>
-static int launch_prompt(const PromptArgs& pa, int max_q_len, cudaStream_t stream) {
-    const dim3 grid(pa.a.n_kv * pa.head_groups, (max_q_len + kPage - 2) / kPage + 1, pa.a.n_seqs);
-    static bool opted_in[64] = {};
+static int launch_prompt(PromptArgs pa, int max_q_len, long long touched, int pages, cudaStream_t stream) {
+    static int resident[64][4] = {};                     // clusters of 1, 2, 4 and 8 blocks that the device holds at once
     int dev = 0;
     cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !opted_in[dev]) {
+    if (dev < 0 || dev >= 64) return blm_fail(BLM_CUDA_ERROR, "attention_q8: device %d", dev);
+    if (resident[dev][0] == 0) {
         if (cudaFuncSetAttribute(attend_prompt_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Prompt<HD>::kSmem) != cudaSuccess)
             return blm_fail(BLM_CUDA_ERROR, "attention_q8: %s", cudaGetErrorString(cudaGetLastError()));
-        if (dev >= 0 && dev < 64) opted_in[dev] = true;
+        for (int i = 3; i >= 0; --i) {                   // (a cluster lies in one group of SMs, which a number of blocks need not divide)
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(1 << i);
+            cfg.blockDim = dim3(kPromptThreads);
+            cfg.dynamicSmemBytes = Prompt<HD>::kSmem;
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = 1 << i;
+            attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
+            int fit = 0;
+            if (i > 0 && cudaOccupancyMaxActiveClusters(&fit, attend_prompt_kernel<HD>, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                fit = 0;
+            }
+            resident[dev][i] = i > 0 ? fit : blm_sm_count();
+        }
     }
-    blm_launch_dependent(attend_prompt_kernel<HD>, grid, dim3(kPromptThreads), Prompt<HD>::kSmem, stream, pa);
+    // A walk is shared by as many blocks as make the step shortest: its turns, each a share of the longest walk's pages and, about as long
+    // as six pages, a block's beginning and end, and five more where the shares have to meet.  Heads of 128, 32 to 8 kv heads, in 1, 2, 4
+    // and 8 blocks: 64 tokens alone 8.9, 14.1, 13.5, 14.8 us; 64 behind 1,000 25.8, 20.6, 16.3, 26.6; 64 behind 8,192 145, 82, 48, 32;
+    // 256 behind 8,192 149, 85, 50, 94.
+    const long long walks = (long long)pa.a.n_kv * pa.head_groups * touched;
+    long long best = (walks + resident[dev][0] - 1) / resident[dev][0] * (pages + 6);
+    for (int i = 1; i < 4; ++i) {
+        if (resident[dev][i] < 1) continue;
+        const long long length = (walks + resident[dev][i] - 1) / resident[dev][i] * ((pages + (1 << i) - 1 >> i) + 11);
+        if (length < best) { best = length; pa.ranks = 1 << i; }
+    }
+    const dim3 grid(pa.a.n_kv * pa.head_groups * pa.ranks, (max_q_len + kPage - 2) / kPage + 1, pa.a.n_seqs);
+    blm_launch_cluster(attend_prompt_kernel<HD>, pa.ranks, grid, dim3(kPromptThreads), Prompt<HD>::kSmem, stream, pa);
     return blm_check_launch("attention_q8");
 }
 
@@ -1846,8 +1959,13 @@ BLM_API int blm_attention_q8(const void* rotated, const void* pool, const void* 
     }
     if (dtype == BLM_BF16 && (hd == 64 || hd == 128) && max_q_len > 1 && n_seqs <= 65535 && max_q_len <= 4000000) {
         const int group = n_heads / n_kv, groups = (group + 3) / 4;
-        const PromptArgs pa{a, groups, (group + groups - 1) / groups, status};
-        return hd == 64 ? launch_prompt<64>(pa, max_q_len, stream) : launch_prompt<128>(pa, max_q_len, stream);
+        int pages = (max_kv_len + kPage - 1) / kPage;
+        if (window > 0 && pages > window / kPage + 2) pages = window / kPage + 2;
+        // 64-position blocks that the step touches: one sequence's are known, of several their mean
+        const int from = max_kv_len > max_q_len ? max_kv_len - max_q_len : 0;
+        const long long touched = n_seqs == 1 ? (from + n_tokens - 1) / kPage - from / kPage + 1 : (n_tokens + 63ll * n_seqs + 63) / kPage;
+        const PromptArgs pa{a, groups, (group + groups - 1) / groups, 1, status};
+        return hd == 64 ? launch_prompt<64>(pa, max_q_len, touched, pages, stream) : launch_prompt<128>(pa, max_q_len, touched, pages, stream);
     }
     if (max_q_len > 1 && n_seqs <= 65535 && max_q_len <= 500000) {
         if (dtype == BLM_F32) return launch_tile<float>(a, n_tokens, max_q_len, max_kv_len, stream);
