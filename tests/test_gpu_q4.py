@@ -145,3 +145,38 @@ def test_quantized_on_the_device():
     out = torch.empty((5, 520), dtype=F32, device=DEV)
     k_.product_q4(here, x, out=out)
     check(out, x, k_.q4_values(here).double(), 1000)
+
+
+@pytest.mark.parametrize("n,over", [(40, 5), (100, 1), (200, 3), (300, 70)])
+def test_a_grid_with_a_few_blocks_over(n, over):
+    """Some blocks more than the SMs hold at once, whose last run as a launch of their own: alone, before a product that reads the result,
+    and captured with it; each end."""
+    k_ = K()
+    blocks = torch.cuda.get_device_properties(0).multi_processor_count * (2 if n <= 128 else 1)
+    m, k = -(-(blocks + over) // -(-n // 256)) * 128 - 24, 520
+    w, dense = weight(m, k, 64)
+    after, after_dense = weight(64, 512, 32)
+    x = tokens(n, k, n)
+    out, last = torch.empty((n, m), dtype=BF16, device=DEV), torch.empty((n, 64), dtype=F32, device=DEV)
+    def both():
+        k_.product_q4(w, x, out=out)
+        k_.product_q4(after, out[:, m - 512:], out=last)
+    for run in range(3):
+        if run == 1:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                both()
+        x.copy_(tokens(n, k, n + run))
+        out.fill_(float("nan"))
+        both() if run == 0 else g.replay()
+        check(out, x, dense, k)
+        check(last, out[:, m - 512:], after_dense, 512)
+    stream = torch.randn((n, m), device=DEV)
+    y = stream.clone()
+    k_.product_q4(w, x, add_into=y)
+    check(y, x, dense, k, extra=stream)
+    gated = torch.empty((n, (m - m % 16) // 2), dtype=BF16, device=DEV)
+    rows = w.first_rows(m - m % 16)
+    k_.product_q4(rows, x, out=gated, swiglu=True)
+    check(gated, x, dense[: m - m % 16], k, gated=True)
+    k_.check_status(torch.device("cuda:0"))

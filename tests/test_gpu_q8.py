@@ -496,3 +496,89 @@ def test_long_portions():
     step, out, old = b.append([(0, 90), (1, 300)], check=False)
     b.attend([(0, 90), (1, 300)], step, out, old)
     K().check_status(torch.device("cuda:0"))
+
+
+@pytest.mark.parametrize("heads,n_kv,dim,dtype", [(8, 2, 64, BF16), (8, 2, 128, BF16), (6, 2, 128, BF16), (12, 1, 64, BF16), (4, 2, 80, BF16), (8, 2, 64, F32),
+                                                  (3, 1, 128, F32), (2, 1, 256, F32), (6, 3, 16, F32)])
+@pytest.mark.parametrize("window", [0, 700, 70])
+def test_portions_behind_long_contexts(heads, n_kv, dim, dtype, window):
+    """Few new tokens on many pages, whose walk several blocks share: some of them with no page at all, sequences of unequal lengths."""
+    b = Batch(3, heads, n_kv, dim, dtype, 1800, seed=heads + dim + window)
+    b.append([(0, 1500), (1, 330), (2, 60)], check=False)
+    b.go([(0, 70), (1, 2), (2, 9)], window=window, padding=2)
+    b.go([(0, 2)], window=window)
+    b.go([(1, 40), (0, 1), (2, 3)], window=window)
+    K().check_status(torch.device("cuda:0"))
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, BF16), (80, BF16), (64, F32)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_later_values_that_are_no_numbers_behind_a_long_context(dim, dtype, bad):
+    """As above, where the rows that see such a value and those that do not meet from several blocks."""
+    outs = []
+    for with_it in (False, True):
+        b = Batch(1, 4, 1, dim, dtype, 1300, seed=6)
+        b.append([(0, 1200)], rot=0, check=False)
+        qkv = b.rows(70)
+        if with_it:
+            qkv.view(70, 6, dim)[10, 5, 5] = bad         # position 1,210, of the block of 1,152 .. 1,215
+        step, out, old = b.append([(0, 70)], qkv=qkv, rot=0, check=False)
+        outs.append(b.attend([(0, 70)], step, out, old, check=False).view(70, 4, dim))
+    others = [i for i in range(dim) if i != 5]
+    assert torch.equal(outs[0][:10], outs[1][:10]) and torch.isfinite(outs[1][:10]).all()
+    assert torch.equal(outs[0][10:16][:, :, others], outs[1][10:16][:, :, others])
+    assert torch.isnan(outs[1][10:16, :, 5]).all() if bad != bad else (outs[1][10:16, :, 5] == bad).all()
+    assert not torch.isfinite(outs[1][16:]).all(dim=2).any()          # the block with it reads as none of them numbers
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, BF16), (48, BF16), (64, F32)])
+@pytest.mark.parametrize("gone", [(0,), (3, 4), (9,), tuple(range(10))])
+def test_pages_that_are_none_in_a_portions_walk(dim, dtype, gone):
+    """Pages outside the pool, at a walk's beginning, inside and at its end, or all of them: their keys are not seen."""
+    b = Batch(1, 8, 2, dim, dtype, 800, seed=2)
+    b.append([(0, 640)], rot=0, check=False)
+    for page in gone:
+        b.table[0, page] = -1 if page % 2 else b.pool.shape[0]
+    step, out, old = b.append([(0, 64)], rot=0, check=False)
+    o = b.attend([(0, 64)], step, out, old, check=False)
+    line = Line(1, 2, dim)
+    kept = [i for i in range(704) if i // PAGE not in gone]
+    line.append(0, np.asarray(b.line.rows[0])[kept])
+    b.line = line
+    step.start_pos = torch.tensor([640 - PAGE * len(gone)], dtype=torch.int32)
+    b.check_attention([(0, 64)], step, out, o, 0)
+
+
+def test_a_portion_captured_and_two_graphs_at_once():
+    """A portion's append and attention in two graphs that are replayed in turns, behind a long context."""
+    k = K()
+    b = Batch(2, 8, 2, 128, BF16, 1400, seed=21)
+    b.append([(0, 1100), (1, 900)], check=False)
+    step = make_step([40, 40], b.length, [0, 1])
+    freq = b.freq(128)
+    graphs = []
+    for i in range(2):
+        qkv = b.rows(80)
+        out, o = torch.empty_like(qkv), torch.empty((80, 8 * 128), dtype=BF16, device=DEV)
+        tail = b.tail.clone()
+        def both():
+            b.tail.copy_(tail)
+            old = k.rope_append_q8(qkv, out, step, b.pool, b.scales, b.tail, b.table, freq, 128, 0, 8, 2, 128)
+            k.attention_q8(out, step, b.pool, b.scales, b.tail, old, b.table, o, 8, 2, 128, b.scale)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            both()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        plain = o.clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            both()
+        graphs.append((g, qkv, out, o, plain))
+    for i in (0, 1, 0, 1, 1):
+        g, qkv, out, o, plain = graphs[i]
+        o.fill_(float("nan"))
+        g.replay()
+        assert torch.equal(o, plain)
+    k.check_status(torch.device("cuda:0"))
