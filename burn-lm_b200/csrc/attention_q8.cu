@@ -50,6 +50,11 @@ __device__ __forceinline__ int page_of(const int* block_table, int table_stride,
     return page < n_pages ? page : -1;
 }
 
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+
 // sixteen bytes of T, as floats
 template <typename T> struct Vec { static constexpr int n = 16 / sizeof(T); };
 __device__ __forceinline__ void load_vec(const float* p, float* o) {
@@ -483,27 +488,50 @@ __global__ void __launch_bounds__(kGeneralWarps * 32) attend_general_kernel(cons
     }
 }
 
-// The general kernel of portions: any type and head size, on the 32-bit units.  A block owns 32 rows, HB query heads of a kv head by
-// 32 / HB positions inside one 64-position block of a sequence, and walks the sequence's pages with numbers widened once into shared
-// memory for all of them: scores a thread 4 rows by 4 keys, sums a thread 8 rows by 4 NL lanes of half of the keys, so that a read of
-// shared memory feeds 4 or 8 multiply-adds.  The next page's bytes are on their way into registers meanwhile.
+// The general kernel of portions: any type and head size, on mma.sync.  A block owns 32 rows, HB query heads of a kv head by 32 / HB
+// positions inside one 64-position block of a sequence, and walks the sequence's pages, whose numbers are widened once into shared memory
+// for all of them; a cluster's blocks take the pages in turn.  Four warps have 16 rows by 32 keys of a page each, with a maximum, sums and
+// a result of their own, which meet at the end.  The whole numbers of a page are exact in bfloat16; a float32 operand is the sum of three
+// bfloat16 numbers (8 bits each of its 24), so three products with a page's numbers are exact, and six of the nine with the own block's
+// float32 rows leave out 2^-25 of a product.  The tensor cores cut their 32-bit sums off, so a page's result is formed from zero and added
+// to the others as a float.  (On the 32-bit units, 4 by 4 results a thread: 63 us against 32 for 137 tokens behind 700 in float32;
+// what bounded it was reads of shared memory.)  The next page's bytes are on their way into registers meanwhile.
 constexpr int kTileThreads = 128, kTileRows = 32;
-__host__ __device__ constexpr size_t tile_smem(int hd) {
-    return ((size_t)hd * kTileRows + (size_t)hd * (kPage + 4) + (size_t)kPage * (hd + 4) + kPage * (kTileRows + 4) + 2 * kTileRows) * 4;
+template <typename T> struct Tile {
+    static constexpr int kPieces = sizeof(T) == 4 ? 3 : 1, kSlots = kPieces < 2 ? 2 : kPieces;       // of a query; room for the pieces of keys or values
+    static constexpr size_t smem(int hd) { return (size_t)(kPieces * kTileRows + kSlots * kPage) * (hd + 8) * 2; }
+};
+__device__ __forceinline__ void ldmatrix4(unsigned (&r)[4], unsigned at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
+__device__ __forceinline__ void ldmatrix4_turned(unsigned (&r)[4], unsigned at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x and y as bfloat16 numbers side by side, and what is left of them
+__device__ __forceinline__ unsigned take_two(float& x, float& y) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    x -= __low2float(v);
+    y -= __high2float(v);
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+
 template <typename T, int NL>
 __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendArgs a, int hb, int ranks) {
-    extern __shared__ __align__(16) float tile_shared[];
+    constexpr int PIECES = Tile<T>::kPieces;
+    extern __shared__ __align__(16) unsigned char tile_shared[];
     __shared__ unsigned odd_keys[2];                     // bits: keys of the own block whose values hold an infinity or a NaN
-    constexpr int kKeyRow = kPage + 4, kPRow = kTileRows + 4;
-    const int hd = a.hd, v_row = hd + 4;
-    float* q = tile_shared;                              // [hd][32 rows]
-    float* keys = q + (size_t)hd * kTileRows;            // [hd][64 keys + 4]
-    float* values = keys + (size_t)hd * kKeyRow;         // [64 keys][hd + 4]
-    float* probs = values + (size_t)kPage * v_row;       // [64 keys][32 rows + 4]
-    float* alphas = probs + kPage * kPRow;               // [32]: what the rows' sums so far are multiplied by; at the end their maxima
-    float* totals = alphas + kTileRows;                  // [32]
-    const int tid = threadIdx.x, group = a.n_heads / a.n_kv, per_kv = group / hb, tb = kTileRows / hb;
+    __shared__ float met_m[2][kTileRows], met_l[2][kTileRows], weights[2 * kTileRows];
+    const int hd = a.hd, row_of = hd + 8;                // numbers between rows: eight rows' 16-byte pieces meet in no bank
+    __nv_bfloat16* q = reinterpret_cast<__nv_bfloat16*>(tile_shared);            // [PIECES][32 rows][hd + 8]
+    __nv_bfloat16* page = q + (size_t)PIECES * kTileRows * row_of;               // [slots][64 keys][hd + 8]
+    float* met = reinterpret_cast<float*>(tile_shared);                          // [2 halves][32 rows][hd + 4], at the end
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = a.n_heads / a.n_kv, per_kv = group / hb, tb = kTileRows / hb;
     const int rank = blockIdx.x % ranks, heads = blockIdx.x / ranks, kvh = heads / per_kv, head0 = kvh * group + heads % per_kv * hb, seq = blockIdx.z;
     pdl_wait();
     pdl_launch_dependents();
@@ -519,32 +547,41 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
         return pos >= start ? rows + ((size_t)(tok0 + pos - start) * width + a.n_heads + which * a.n_kv + kvh) * hd
                             : found + ((size_t)which * a.n_kv * kPage + pos % kPage) * hd;
     };
+    // eight numbers as pieces, `apart` numbers between the pieces
+    auto put = [&](__nv_bfloat16* to, size_t apart, float (&x)[8]) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+            *reinterpret_cast<uint4*>(to + i * apart) = make_uint4(take_two(x[0], x[1]), take_two(x[2], x[3]), take_two(x[4], x[5]), take_two(x[6], x[7]));
+    };
     if (tid < 2) odd_keys[tid] = 0u;
     for (int i = tid; i < kTileRows * (hd / 8); i += kTileThreads) {
         const int r = i % kTileRows, d = i / kTileRows * 8, pos = t0 + r % tb;
         float x[8] = {};
         if (pos >= start && pos < end) load_n<8>(rows + ((size_t)(tok0 + pos - start) * width + head0 + r / tb) * hd + d, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q[(d + e) * kTileRows + r] = x[e] * a.scale_log2e;
+        for (int e = 0; e < 8; ++e) x[e] *= PIECES > 1 ? a.scale_log2e : 1.f;    // (a bfloat16 query stays as it is: its scores are multiplied)
+        put(q + (size_t)r * row_of + d, (size_t)kTileRows * row_of, x);
     }
-    // scores: rows 4 rg .. 4 rg + 3 by keys 4 kg .. 4 kg + 3; sums: rows 8 pr .. 8 pr + 7, lanes 4 lg + 64 i, of half of the keys
-    const int rg = tid >> 4, kg = tid & 15, half = tid >> 6, pr = (tid >> 4) & 3, lg = tid & 15;
-    float m[4], l[4], acc[8][4 * NL];
+    // this warp's 16 rows and 32 keys of a page; a thread has rows g and g + 8 and columns 2 t, 2 t + 1 of every eight
+    const int m0 = (warp & 1) * 16, half = warp >> 1, g = lane >> 2, t = lane & 3;
+    const int pos_of[2] = {t0 + (m0 + g) % tb, t0 + (m0 + g + 8) % tb}, lo_of[2] = {first_key(pos_of[0]), first_key(pos_of[1])};
+    // where a lane's row of the 8 x 8 matrices begins: of 16 rows by 16 numbers of q; of 16 keys by 16 numbers; turned, of 16 keys by 16 lanes
+    const unsigned q_at = tc5::smem_u32(q + (size_t)(m0 + (lane & 15)) * row_of + (lane >> 4) * 8);
+    const unsigned k_at = tc5::smem_u32(page + (size_t)(half * 32 + (lane & 7) + (lane >> 4) * 8) * row_of + (lane >> 3 & 1) * 8);
+    const unsigned v_at = tc5::smem_u32(page + (size_t)(half * 32 + (lane & 15)) * row_of + (lane >> 4) * 8);
+    const unsigned q_piece = kTileRows * row_of * 2, page_piece = kPage * row_of * 2;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[8 * NL][4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) { m[r] = -INFINITY; l[r] = 0.f; }
-#pragma unroll
-    for (int r = 0; r < 8; ++r)
-#pragma unroll
-        for (int i = 0; i < 4 * NL; ++i) acc[r][i] = 0.f;
+    for (int i = 0; i < 8 * NL; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
     const int pieces = 4 * hd, chunks = 4 * padded(hd), per = hd / 8;            // of sixteen bytes: of a page's keys, of its values
     uint4 next_k[2 * NL], next_v[2 * NL];
     float2 next_scale = make_float2(0.f, 0.f);
     bool next_there = false;
     auto fetch = [&](int b) {
-        const int page = page_of(a.block_table, a.table_stride, slot, b, a.n_pages);
-        next_there = page >= 0;
+        const int number = page_of(a.block_table, a.table_stride, slot, b, a.n_pages);
+        next_there = number >= 0;
         if (!next_there) return;
-        const signed char* line = a.pool + ((size_t)page * a.n_kv + kvh) * line_bytes(hd);
+        const signed char* line = a.pool + ((size_t)number * a.n_kv + kvh) * line_bytes(hd);
         next_scale = *scales_of(line, hd);
 #pragma unroll
         for (int i = 0; i < 2 * NL; ++i) {
@@ -553,185 +590,211 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
             if (c < chunks) next_v[i] = *reinterpret_cast<const uint4*>(line + kPage * hd + c * 16);
         }
     };
-    auto wide = [](unsigned word, int e) { return (float)((int)(word >> (8 * e) & 0xffu) - 128); };
+    // a byte behind 0x4b0000 is 2^23 + 128 + a whole number
+    auto wide = [](unsigned word, int e) { return __uint_as_float(__byte_perm(word, 0x4b000000u, 0x7440 | e)) - 8388736.f; };
     if (pg_lo + rank < mine) fetch(pg_lo + rank);
     for (int b = pg_lo + rank; b <= mine; b += ranks) {
         const bool own = b == mine;
-        const float2 scale = own ? make_float2(1.f, 1.f) : next_scale;
+        float2 scale = own ? make_float2(1.f, 1.f) : next_scale;
+        if (PIECES == 1) scale.x *= a.scale_log2e;
+        __syncthreads();                                 // (the page before has been read)
         if (!own) {
             if (!next_there) {                           // (the same for the whole block)
                 if (b + ranks < mine) fetch(b + ranks);
                 continue;
             }
+            __nv_bfloat16* values = page + (size_t)kPage * row_of;
 #pragma unroll
             for (int i = 0; i < 2 * NL; ++i) {
                 const int c = tid + i * kTileThreads;
                 if (c < pieces) {
-                    float* to = keys + (c / kPage * 16) * kKeyRow + c % kPage;
-                    const unsigned w[4] = {next_k[i].x, next_k[i].y, next_k[i].z, next_k[i].w};
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) to[e * kKeyRow] = wide(w[e >> 2], e & 3);
+                    uint4* to = reinterpret_cast<uint4*>(page + (size_t)(c % kPage) * row_of + c / kPage * 16);
+                    auto four = [&](unsigned w) { return make_uint2(pack_bf16(wide(w, 0), wide(w, 1)), pack_bf16(wide(w, 2), wide(w, 3))); };
+                    const uint2 x = four(next_k[i].x), y = four(next_k[i].y), z = four(next_k[i].z), w = four(next_k[i].w);
+                    to[0] = make_uint4(x.x, x.y, y.x, y.y);
+                    to[1] = make_uint4(z.x, z.y, w.x, w.y);
                 }
                 if (c < chunks) {                        // four lanes of four keys
-                    const int rem = c % padded(hd), lane = rem & 31, lanes0 = rem / 32 * 4, key = c / padded(hd) * 16 + (lane & 3) * 4;
-                    float* to = values + key * v_row + (lane >> 2) * per + lanes0;
+                    const int rem = c % padded(hd), piece = rem & 31, lanes0 = rem / 32 * 4, key = c / padded(hd) * 16 + (piece & 3) * 4;
+                    __nv_bfloat16* to = values + (size_t)key * row_of + (piece >> 2) * per + lanes0;
                     const unsigned w[4] = {next_v[i].x, next_v[i].y, next_v[i].z, next_v[i].w};
                     if (per % 4 == 0) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            *reinterpret_cast<float4*>(to + e * v_row) = make_float4(wide(w[0], e), wide(w[1], e), wide(w[2], e), wide(w[3], e));
+                            *reinterpret_cast<uint2*>(to + (size_t)e * row_of) = make_uint2(pack_bf16(wide(w[0], e), wide(w[1], e)), pack_bf16(wide(w[2], e), wide(w[3], e)));
                     } else {
 #pragma unroll
                         for (int x = 0; x < 4; ++x)
                             if (lanes0 + x < per)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) to[e * v_row + x] = wide(w[x], e);
+                                for (int e = 0; e < 4; ++e) to[(size_t)e * row_of + x] = __float2bfloat16(wide(w[x], e));
                     }
                 }
             }
             if (b + ranks < mine) fetch(b + ranks);
         } else {
             for (int c = tid; c < kPage * per; c += kTileThreads) {
-                const int key = c % kPage, d = c / kPage * 8, pos = p0 + key;
-                float k[8] = {}, v[8] = {};
-                if (pos < end) {
-                    load_n<8>(own_row(pos, 0) + d, k);
-                    load_n<8>(own_row(pos, 1) + d, v);
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    keys[(d + e) * kKeyRow + key] = k[e];
-                    // (a probability of zero does not silence an infinity or a NaN: those are put in at the end, by the rows that see them)
-                    if (!(fabsf(v[e]) < INFINITY)) {
-                        v[e] = 0.f;
-                        atomicOr(odd_keys + (key >> 5), 1u << (key & 31));
-                    }
-                }
-                *reinterpret_cast<float4*>(values + key * v_row + d) = make_float4(v[0], v[1], v[2], v[3]);
-                *reinterpret_cast<float4*>(values + key * v_row + d + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                const int key = c % kPage, d = c / kPage * 8;
+                float x[8] = {};
+                if (p0 + key < end) load_n<8>(own_row(p0 + key, 0) + d, x);
+                put(page + (size_t)key * row_of + d, (size_t)kPage * row_of, x);
             }
         }
         __syncthreads();
-        float s[4][4] = {};
-#pragma unroll 8
-        for (int d = 0; d < hd; ++d) {
-            const float4 x = *reinterpret_cast<const float4*>(q + d * kTileRows + 4 * rg), y = *reinterpret_cast<const float4*>(keys + d * kKeyRow + 4 * kg);
-            const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        float s[4][4] = {};                              // 16 rows by four times eight keys
+#pragma unroll 4
+        for (int k = 0; k < hd / 16; ++k) {
+            unsigned x[PIECES][4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int i = 0; i < PIECES; ++i) ldmatrix4(x[i], q_at + i * q_piece + k * 32);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s[r][k] = fmaf(xs[r], ys[k], s[r][k]);
+            for (int j = 0; j < PIECES; ++j) {           // (a page's keys have one piece)
+                if (j > 0 && !own) break;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    unsigned y[4];
+                    ldmatrix4(y, k_at + j * page_piece + c * 16 * row_of * 2 + k * 32);
+#pragma unroll
+                    for (int i = 0; i < PIECES - j; ++i) {
+                        mma_bf16(s[2 * c], x[i], y[0], y[1]);
+                        mma_bf16(s[2 * c + 1], x[i], y[2], y[3]);
+                    }
+                }
+            }
         }
-        float p[4][4];
+        float alpha[2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int pos = t0 + (4 * rg + r) % tb, lo = first_key(pos);
+        for (int r = 0; r < 2; ++r) {
             float top = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int key = b * kPage + 4 * kg + k;
-                s[r][k] = key <= pos && key >= lo ? s[r][k] * scale.x : -INFINITY;
-                top = fmaxf(top, s[r][k]);
+            for (int i = 0; i < 8; ++i) {
+                const int key = b * kPage + half * 32 + i / 2 * 8 + 2 * t + (i & 1);
+                float& x = s[i / 2][2 * r + (i & 1)];
+                x = key <= pos_of[r] && key >= lo_of[r] ? x * scale.x : -INFINITY;
+                top = fmaxf(top, x);
             }
-#pragma unroll
-            for (int w = 1; w < 16; w *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-            const float now = fmaxf(m[r], top), ref = now == -INFINITY ? 0.f : now, alpha = exp2f(m[r] - ref);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float now = fmaxf(m[r], top), ref = now == -INFINITY ? 0.f : now;
+            alpha[r] = exp2f(m[r] - ref);
+            m[r] = now;
             float sum = 0.f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const bool seen = b * kPage + 4 * kg + k <= pos && b * kPage + 4 * kg + k >= lo;
-                const float e = exp2f(s[r][k] - ref);
-                p[r][k] = seen ? e * scale.y : 0.f;      // (of what is not seen, whatever the scale)
+            for (int i = 0; i < 8; ++i) {
+                const int key = b * kPage + half * 32 + i / 2 * 8 + 2 * t + (i & 1);
+                float& x = s[i / 2][2 * r + (i & 1)];
+                const float e = exp2f(x - ref);
+                const bool seen = key <= pos_of[r] && key >= lo_of[r];
+                x = seen ? e * scale.y : 0.f;            // (of what is not seen, whatever the scale)
                 sum += seen ? e : 0.f;
             }
-            l[r] = l[r] * alpha + sum;                   // of the thread's keys; the sixteen threads of a row meet at the end
-            m[r] = now;
-            if (kg == 0) alphas[4 * rg + r] = alpha;
+            l[r] = l[r] * alpha[r] + sum;                // of the thread's keys; the four threads of a row meet at the end
         }
+        unsigned p[2][PIECES][4];                        // 16 rows by twice sixteen keys
 #pragma unroll
-        for (int k = 0; k < 4; ++k) *reinterpret_cast<float4*>(probs + (4 * kg + k) * kPRow + 4 * rg) = make_float4(p[0][k], p[1][k], p[2][k], p[3][k]);
-        __syncthreads();
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const float alpha = alphas[8 * pr + r];
+            for (int i = 0; i < PIECES; ++i)
 #pragma unroll
-            for (int i = 0; i < 4 * NL; ++i) acc[r][i] *= alpha;
+                for (int e = 0; e < 4; ++e) p[c][i][e] = take_two(s[2 * c + e / 2][2 * (e & 1)], s[2 * c + e / 2][2 * (e & 1) + 1]);
+        if (own) {                                       // the values take the keys' place
+            __syncthreads();
+            for (int c = tid; c < kPage * per; c += kTileThreads) {
+                const int key = c % kPage, d = c / kPage * 8;
+                float x[8] = {};
+                if (p0 + key < end) load_n<8>(own_row(p0 + key, 1) + d, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    // (a probability of zero does not silence an infinity or a NaN: those are put in at the end, by the rows that see them)
+                    if (!(fabsf(x[e]) < INFINITY)) {
+                        x[e] = 0.f;
+                        atomicOr(odd_keys + (key >> 5), 1u << (key & 31));
+                    }
+                put(page + (size_t)key * row_of + d, (size_t)kPage * row_of, x);
+            }
+            __syncthreads();
         }
-#pragma unroll 4
-        for (int k = half * 32; k < half * 32 + 32; ++k) {
-            const float4 p0 = *reinterpret_cast<const float4*>(probs + k * kPRow + 8 * pr), p1 = *reinterpret_cast<const float4*>(probs + k * kPRow + 8 * pr + 4);
-            const float ps[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+        const unsigned values_at = v_at + (own ? 0u : page_piece);
 #pragma unroll
-            for (int i = 0; i < NL; ++i)
-                if (4 * lg + 64 * i < hd) {
-                    const float4 v = *reinterpret_cast<const float4*>(values + k * v_row + 4 * lg + 64 * i);
+        for (int d = 0; d < 4 * NL; ++d) {               // sixteen lanes at a time
+            if (d * 16 >= hd) break;
+            float part[2][4] = {};
 #pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        acc[r][4 * i] = fmaf(ps[r], v.x, acc[r][4 * i]);
-                        acc[r][4 * i + 1] = fmaf(ps[r], v.y, acc[r][4 * i + 1]);
-                        acc[r][4 * i + 2] = fmaf(ps[r], v.z, acc[r][4 * i + 2]);
-                        acc[r][4 * i + 3] = fmaf(ps[r], v.w, acc[r][4 * i + 3]);
+            for (int j = 0; j < PIECES; ++j) {
+                if (j > 0 && !own) break;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    unsigned y[4];
+                    ldmatrix4_turned(y, values_at + j * page_piece + c * 16 * row_of * 2 + d * 32);
+#pragma unroll
+                    for (int i = 0; i < PIECES - j; ++i) {
+                        mma_bf16(part[0], p[c][i], y[0], y[1]);
+                        mma_bf16(part[1], p[c][i], y[2], y[3]);
                     }
                 }
-        }
-        __syncthreads();
-    }
+            }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int w = 1; w < 16; w *= 2) l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
-        if (kg == 0) {
-            totals[4 * rg + r] = l[r];
-            alphas[4 * rg + r] = m[r];
+                for (int e = 0; e < 4; ++e) acc[2 * d + x][e] = fmaf(acc[2 * d + x][e], alpha[e >> 1], part[x][e]);
         }
     }
-    // the two halves of the keys meet over the values, then the cluster's blocks, a share of the rows each
+    __syncthreads();
+    // ---- the warps' halves and the cluster's blocks meet, a share of the rows each ----
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        if (half == h)
-#pragma unroll
-            for (int i = 0; i < NL; ++i)
-                if (4 * lg + 64 * i < hd)
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        float4* to = reinterpret_cast<float4*>(values + (8 * pr + r) * v_row + 4 * lg + 64 * i);
-                        const float4 first = h == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *to;
-                        *to = make_float4(first.x + acc[r][4 * i], first.y + acc[r][4 * i + 1], first.z + acc[r][4 * i + 2], first.w + acc[r][4 * i + 3]);
-                    }
-        __syncthreads();
+    for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        if (t == 0) {
+            met_m[half][m0 + g + 8 * r] = m[r];
+            met_l[half][m0 + g + 8 * r] = l[r];
+        }
     }
+    auto met_at = [&](int h, int row, int d) { return met + ((size_t)h * kTileRows + row) * (hd + 4) + d; };
+#pragma unroll
+    for (int i = 0; i < 8 * NL; ++i)
+        if (i * 8 < hd)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) *reinterpret_cast<float2*>(met_at(half, m0 + g + 8 * r, i * 8 + 2 * t)) = make_float2(acc[i][2 * r], acc[i][2 * r + 1]);
     if (ranks > 1) cluster_sync();
-    const unsigned odd_at = tc5::smem_u32(odd_keys), m_at = tc5::smem_u32(alphas), l_at = tc5::smem_u32(totals), o_at = tc5::smem_u32(values);
-    const int last = (mine - pg_lo) % ranks, share = kTileRows / ranks;          // (whose step was the own block)
+    else __syncthreads();
+    const int parts = 2 * ranks, share = kTileRows / ranks, last = (mine - pg_lo) % ranks;       // (whose step was the own block)
     unsigned long long odd = 0;
-    for (int w = 0; w < 2; ++w) odd |= (unsigned long long)(ranks > 1 ? __float_as_uint(cluster_float(odd_at + 4 * w, last)) : odd_keys[w]) << (32 * w);
+    for (int w = 0; w < 2; ++w) odd |= (unsigned long long)(ranks > 1 ? __float_as_uint(cluster_float(tc5::smem_u32(odd_keys + w), last)) : odd_keys[w]) << (32 * w);
+    if (tid < share * parts) {                           // the parts' weights, a thread each: a row's are neighbours
+        const int row = rank * share + tid / parts, k = tid % parts;
+        const float mk = cluster_float(tc5::smem_u32(&met_m[k & 1][row]), k >> 1), lk = cluster_float(tc5::smem_u32(&met_l[k & 1][row]), k >> 1);
+        float top = mk;
+        for (int w = 1; w < parts; w *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+        // (a part that the row saw nothing of has nothing; one whose scores were no numbers has none, which its sum tells)
+        const float by = mk == top ? 1.f : exp2f(mk - (top == -INFINITY ? 0.f : top));
+        float total = lk * by;
+        for (int w = 1; w < parts; w *= 2) total += __shfl_xor_sync(0xffffffffu, total, w);
+        weights[tid] = by / total;
+    }
+    __syncthreads();
     for (int i = tid; i < share * (hd / 4); i += kTileThreads) {
-        const int row = rank * share + i / (hd / 4), d = i % (hd / 4) * 4, pos = t0 + row % tb;
+        const int here = i / (hd / 4), row = rank * share + here, d = i % (hd / 4) * 4, pos = t0 + row % tb;
         if (pos < start || pos >= end) continue;
-        float top = -INFINITY, total = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-        if (ranks == 1) top = alphas[row];
-        else for (int k = 0; k < ranks; ++k) top = fmaxf(top, cluster_float(m_at + 4 * row, k));
-        for (int k = 0; k < ranks; ++k) {
-            const float mk = ranks == 1 ? top : cluster_float(m_at + 4 * row, k), lk = ranks == 1 ? totals[row] : cluster_float(l_at + 4 * row, k);
-            const float4 v = ranks == 1 ? *reinterpret_cast<const float4*>(values + row * v_row + d) : cluster_float4(o_at + (row * v_row + d) * 4, k);
-            // (a share that the row saw nothing of has nothing; one whose scores were no numbers has none, which its sum tells)
-            const float by = mk == top ? 1.f : exp2f(mk - (top == -INFINITY ? 0.f : top));
-            total = fmaf(lk, by, total);
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int k = 0; k < parts; ++k) {
+            const float* at = met_at(k & 1, row, d);
+            const float4 v = ranks == 1 ? *reinterpret_cast<const float4*>(at) : cluster_float4(tc5::smem_u32(at), k >> 1);
+            const float by = weights[here * parts + k];
             o[0] = fmaf(v.x, by, o[0]); o[1] = fmaf(v.y, by, o[1]); o[2] = fmaf(v.z, by, o[2]); o[3] = fmaf(v.w, by, o[3]);
         }
-        const float by = 1.f / total;
         const int from = first_key(pos);
         T* out = reinterpret_cast<T*>(a.out) + ((size_t)(tok0 + pos - start) * a.n_heads + head0 + row / tb) * hd + d;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float x = o[e] * by;
             if (odd != 0)
                 for (int k = max(p0, from); k <= pos; ++k)
                     if (odd >> (k - p0) & 1) {
                         const float v = to_f32(own_row(k, 1)[d + e]);
-                        if (!(fabsf(v) < INFINITY)) x += v;
+                        if (!(fabsf(v) < INFINITY)) o[e] += v;
                     }
-            out[e] = from_f32<T>(x);
+            out[e] = from_f32<T>(o[e]);
         }
     }
     if (ranks > 1) cluster_sync();                       // what others read stays until they have
@@ -746,7 +809,7 @@ static int launch_tile(const AttendArgs& a, int n_tokens, int max_q_len, int max
     if (a.window > 0 && pages > a.window / kPage + 2) pages = a.window / kPage + 2;
     while (ranks < 8 && (long long)tiles * ranks * 2 <= 4ll * blm_sm_count() && pages >= 2 * ranks) ranks *= 2;
     const dim3 grid(a.n_kv * (group / hb) * ranks, (max_q_len + tb - 2) / tb + 1, a.n_seqs);
-    const size_t smem = tile_smem(a.hd);
+    const size_t smem = Tile<T>::smem(a.hd);
     if (cudaFuncSetAttribute(attend_tile_kernel<T, NL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return blm_fail(BLM_CUDA_ERROR, "attention_q8: %s", cudaGetErrorString(cudaGetLastError()));
     blm_launch_cluster(attend_tile_kernel<T, NL>, ranks, grid, dim3(kTileThreads), smem, stream, a, hb, ranks);
@@ -827,10 +890,6 @@ __device__ __forceinline__ unsigned two_of(unsigned word) {
 }
 __device__ __forceinline__ unsigned pack_half(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const unsigned*>(&v);
-}
-__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const unsigned*>(&v);
 }
 __device__ __forceinline__ float ex2(float x) {          // 2^x (x = -inf gives 0)
