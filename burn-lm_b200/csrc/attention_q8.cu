@@ -372,123 +372,7 @@ struct AttendArgs {
     float scale_log2e;
 };
 
-// The general kernel: any type, head size and number of heads.  A block is (token, head); its warps take pages in turn, a lane a key
-// for the scores and D / 32 lanes for the sums, each warp with its own running maximum and sum; they meet in shared memory.
-constexpr int kGeneralWarps = 8;
-template <typename T>
-__global__ void __launch_bounds__(kGeneralWarps * 32) attend_general_kernel(const AttendArgs a) {
-    __shared__ __align__(16) float q[256];
-    __shared__ float sm_acc[kGeneralWarps][256], sm_m[kGeneralWarps], sm_l[kGeneralWarps];
-    pdl_wait();
-    const int head = blockIdx.x % a.n_heads, tok = blockIdx.x / a.n_heads, hd = a.hd, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // the sequence of this row: the last one that begins at or before it
-    int lo_s = 0, hi_s = a.n_seqs;
-    if (tok >= a.cu_seqlens[hi_s]) return;               // a row of no sequence
-    while (hi_s - lo_s > 1) {
-        const int mid = (lo_s + hi_s) / 2;
-        if (a.cu_seqlens[mid] <= tok) lo_s = mid; else hi_s = mid;
-    }
-    const int seq = lo_s, tok0 = a.cu_seqlens[seq], start = a.start_pos[seq], pos = start + tok - tok0, slot = a.slot_of_seq[seq];
-    const int kvh = head / (a.n_heads / a.n_kv), width = a.n_heads + 2 * a.n_kv;
-    const int key_lo = a.window > 0 ? max(0, pos + 1 - a.window) : 0, mine = pos / kPage;
-    const T* rows = reinterpret_cast<const T*>(a.rotated);
-    for (int d = tid; d < hd; d += blockDim.x) q[d] = to_f32(rows[((size_t)tok * width + head) * hd + d]) * a.scale_log2e;
-    __syncthreads();
-    float m_run = -INFINITY, l_run = 0.f, acc[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-    const T* found = reinterpret_cast<const T*>(a.found) + ((size_t)(a.found_by_slot ? slot : seq) * 2 * a.n_kv + kvh) * kPage * hd;
-    for (int c = key_lo / 32 + warp; c <= pos / 32; c += kGeneralWarps) {        // 32 keys a step
-        const int b = c / 2, key = c * 32 + lane;
-        const bool own = b == mine, seen = key <= pos && key >= key_lo;
-        // where a row of the own block lies
-        auto own_row = [&](int k, int which) -> const T* {
-            if (k >= start) return rows + ((size_t)(tok0 + k - start) * width + a.n_heads + which * a.n_kv + kvh) * hd;
-            return found + ((size_t)which * a.n_kv * kPage + k % kPage) * hd;
-        };
-        const signed char* line = nullptr;
-        float ks = 0.f, vs = 0.f;
-        if (!own) {
-            const int page = page_of(a.block_table, a.table_stride, slot, b, a.n_pages);
-            if (page < 0) continue;
-            line = a.pool + ((size_t)page * a.n_kv + kvh) * line_bytes(hd);
-            const float2 scale = *scales_of(line, hd);
-            ks = scale.x;
-            vs = scale.y;
-        }
-        float s = -INFINITY;
-        if (seen) {
-            float sum = 0.f;
-            if (own) {
-                const T* kr = own_row(key, 0);
-                for (int d = 0; d < hd; d += 8) {
-                    float x[8];
-                    load_n<8>(kr + d, x);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) sum = fmaf(q[d + e], x[e], sum);
-                }
-            } else {
-                for (int d = 0; d < hd; d += 16) {
-                    const int4 w = *reinterpret_cast<const int4*>(line + key_piece(key % kPage, d, hd));
-                    const unsigned char* x = reinterpret_cast<const unsigned char*>(&w);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) sum = fmaf(q[d + e], (float)((int)x[e] - 128), sum);
-                }
-                sum *= ks;
-            }
-            s = sum;
-        }
-        const float m_new = fmaxf(m_run, warp_max(s));
-        if (m_new == -INFINITY) continue;
-        const float alpha = m_run == -INFINITY ? 0.f : exp2f(m_run - m_new), p = seen ? exp2f(s - m_new) : 0.f;
-        m_run = m_new;
-        l_run = l_run * alpha + warp_sum(p);
-        const float pv = own ? p : p * vs;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] *= alpha;
-        // keys that are not seen are not read: what lies there may be anything
-        const int k_first = max(c * 32, key_lo), k_last = min(c * 32 + 31, pos);
-        if (own) {
-            for (int k = k_first; k <= k_last; ++k) {
-                const float w = __shfl_sync(0xffffffffu, pv, k & 31);
-                const T* vr = own_row(k, 1);
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (lane + 32 * i < hd) acc[i] = fmaf(w, to_f32(vr[lane + 32 * i]), acc[i]);
-            }
-        } else {
-            for (int k = (c * 32) % kPage; k < (c * 32) % kPage + 32; k += 4) {
-                float w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = __shfl_sync(0xffffffffu, pv, (k & 31) + e);
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (lane + 32 * i < hd) {
-                        const uchar4 v = *reinterpret_cast<const uchar4*>(line + kPage * hd + value_word(k, lane + 32 * i, hd));
-                        acc[i] = fmaf(w[0], (float)((int)v.x - 128), acc[i]);
-                        acc[i] = fmaf(w[1], (float)((int)v.y - 128), acc[i]);
-                        acc[i] = fmaf(w[2], (float)((int)v.z - 128), acc[i]);
-                        acc[i] = fmaf(w[3], (float)((int)v.w - 128), acc[i]);
-                    }
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (lane + 32 * i < hd) sm_acc[warp][lane + 32 * i] = acc[i];
-    if (lane == 0) { sm_m[warp] = m_run; sm_l[warp] = l_run; }
-    __syncthreads();
-    float m = -INFINITY, l = 0.f;
-    for (int w = 0; w < kGeneralWarps; ++w) m = fmaxf(m, sm_m[w]);
-    for (int w = 0; w < kGeneralWarps; ++w) l += sm_m[w] == -INFINITY ? 0.f : sm_l[w] * exp2f(sm_m[w] - m);
-    for (int d = tid; d < hd; d += blockDim.x) {
-        float o = 0.f;
-        for (int w = 0; w < kGeneralWarps; ++w) o += sm_m[w] == -INFINITY ? 0.f : sm_acc[w][d] * exp2f(sm_m[w] - m);
-        reinterpret_cast<T*>(a.out)[((size_t)tok * a.n_heads + head) * hd + d] = from_f32<T>(o / l);
-    }
-}
-
-// The general kernel of portions: any type and head size, on mma.sync.  A block owns 32 rows, HB query heads of a kv head by 32 / HB
+// The general kernel: any type, head size and number of tokens, on mma.sync.  A block owns 32 rows, HB query heads of a kv head by 32 / HB
 // positions inside one 64-position block of a sequence, and walks the sequence's pages, whose numbers are widened once into shared memory
 // for all of them; a cluster's blocks take the pages in turn.  Four warps have 16 rows by 32 keys of a page each, with a maximum, sums and
 // a result of their own, which meet at the end.  The whole numbers of a page are exact in bfloat16; a float32 operand is the sum of three
@@ -555,16 +439,17 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
     };
     if (tid < 2) odd_keys[tid] = 0u;
     for (int i = tid; i < kTileRows * (hd / 8); i += kTileThreads) {
-        const int r = i % kTileRows, d = i / kTileRows * 8, pos = t0 + r % tb;
+        const int r = i % kTileRows, d = i / kTileRows * 8, pos = t0 + r / hb;
         float x[8] = {};
-        if (pos >= start && pos < end) load_n<8>(rows + ((size_t)(tok0 + pos - start) * width + head0 + r / tb) * hd + d, x);
+        if (pos >= start && pos < end) load_n<8>(rows + ((size_t)(tok0 + pos - start) * width + head0 + r % hb) * hd + d, x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] *= PIECES > 1 ? a.scale_log2e : 1.f;    // (a bfloat16 query stays as it is: its scores are multiplied)
         put(q + (size_t)r * row_of + d, (size_t)kTileRows * row_of, x);
     }
     // this warp's 16 rows and 32 keys of a page; a thread has rows g and g + 8 and columns 2 t, 2 t + 1 of every eight
     const int m0 = (warp & 1) * 16, half = warp >> 1, g = lane >> 2, t = lane & 3;
-    const int pos_of[2] = {t0 + (m0 + g) % tb, t0 + (m0 + g + 8) % tb}, lo_of[2] = {first_key(pos_of[0]), first_key(pos_of[1])};
+    const bool idle = t0 + m0 / hb >= end || t0 + (m0 + 15) / hb < start;        // (single tokens have 16 rows of the 32 at most)
+    const int pos_of[2] = {t0 + (m0 + g) / hb, t0 + (m0 + g + 8) / hb}, lo_of[2] = {first_key(pos_of[0]), first_key(pos_of[1])};
     // where a lane's row of the 8 x 8 matrices begins: of 16 rows by 16 numbers of q; of 16 keys by 16 numbers; turned, of 16 keys by 16 lanes
     const unsigned q_at = tc5::smem_u32(q + (size_t)(m0 + (lane & 15)) * row_of + (lane >> 4) * 8);
     const unsigned k_at = tc5::smem_u32(page + (size_t)(half * 32 + (lane & 7) + (lane >> 4) * 8) * row_of + (lane >> 3 & 1) * 8);
@@ -643,7 +528,7 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
         __syncthreads();
         float s[4][4] = {};                              // 16 rows by four times eight keys
 #pragma unroll 4
-        for (int k = 0; k < hd / 16; ++k) {
+        for (int k = 0; k < (idle ? 0 : hd / 16); ++k) {
             unsigned x[PIECES][4];
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) ldmatrix4(x[i], q_at + i * q_piece + k * 32);
@@ -717,7 +602,7 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
         const unsigned values_at = v_at + (own ? 0u : page_piece);
 #pragma unroll
         for (int d = 0; d < 4 * NL; ++d) {               // sixteen lanes at a time
-            if (d * 16 >= hd) break;
+            if (d * 16 >= hd || idle) break;
             float part[2][4] = {};
 #pragma unroll
             for (int j = 0; j < PIECES; ++j) {
@@ -774,7 +659,7 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
     }
     __syncthreads();
     for (int i = tid; i < share * (hd / 4); i += kTileThreads) {
-        const int here = i / (hd / 4), row = rank * share + here, d = i % (hd / 4) * 4, pos = t0 + row % tb;
+        const int here = i / (hd / 4), row = rank * share + here, d = i % (hd / 4) * 4, pos = t0 + row / hb;
         if (pos < start || pos >= end) continue;
         float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
@@ -785,7 +670,7 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
             o[0] = fmaf(v.x, by, o[0]); o[1] = fmaf(v.y, by, o[1]); o[2] = fmaf(v.z, by, o[2]); o[3] = fmaf(v.w, by, o[3]);
         }
         const int from = first_key(pos);
-        T* out = reinterpret_cast<T*>(a.out) + ((size_t)(tok0 + pos - start) * a.n_heads + head0 + row / tb) * hd + d;
+        T* out = reinterpret_cast<T*>(a.out) + ((size_t)(tok0 + pos - start) * a.n_heads + head0 + row % hb) * hd + d;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (odd != 0)
@@ -2026,13 +1911,8 @@ BLM_API int blm_attention_q8(const void* rotated, const void* pool, const void* 
         const PromptArgs pa{a, groups, (group + groups - 1) / groups, 1, status};
         return hd == 64 ? launch_prompt<64>(pa, max_q_len, touched, pages, stream) : launch_prompt<128>(pa, max_q_len, touched, pages, stream);
     }
-    if (max_q_len > 1 && n_seqs <= 65535 && max_q_len <= 500000) {
-        if (dtype == BLM_F32) return launch_tile<float>(a, n_tokens, max_q_len, max_kv_len, stream);
-        if (dtype == BLM_BF16) return launch_tile<__nv_bfloat16>(a, n_tokens, max_q_len, max_kv_len, stream);
-    }
-    const dim3 grid(n_heads * n_tokens);
-    if (dtype == BLM_F32) blm_launch_dependent(attend_general_kernel<float>, grid, dim3(kGeneralWarps * 32), 0, stream, a);
-    else if (dtype == BLM_BF16) blm_launch_dependent(attend_general_kernel<__nv_bfloat16>, grid, dim3(kGeneralWarps * 32), 0, stream, a);
-    else return blm_fail(BLM_BAD_ARGUMENT, "attention_q8: dtype %d", dtype);
-    return blm_check_launch("attention_q8");
+    BLM_REQUIRE(n_seqs <= 65535 && max_q_len <= 500000, "attention_q8: %d sequences (at most 65535), %d tokens (at most 500000)", n_seqs, max_q_len);
+    if (dtype == BLM_F32) return launch_tile<float>(a, n_tokens, max_q_len, max_kv_len, stream);
+    if (dtype == BLM_BF16) return launch_tile<__nv_bfloat16>(a, n_tokens, max_q_len, max_kv_len, stream);
+    return blm_fail(BLM_BAD_ARGUMENT, "attention_q8: dtype %d", dtype);
 }
