@@ -315,14 +315,17 @@ static int launch_few(const Args& a, int* status, cudaStream_t stream) {
 
 // ---- many tokens -----------------------------------------------------------------------------------------------------------
 // The tcgen05 product with the weight's rows as the 128 rows of the accumulator and N tokens (32 to 256) as its columns.  A stage holds
-// 64 places of K: one thread fetches the tokens (TMA, 128-byte swizzle, zeros beyond the last token and place), one issues the products,
-// and the other warps turn weights into bfloat16 in tensor memory, a row a lane, each group of four warps every kGroups-th tile of K: a
-// lane copies 16 bytes of each of the warp's two tiles of rows kAhead tiles ahead (cp.async), reads its row's four pieces (which hold
-// row g + 8 too), and a number is the whole number times its scale, exactly, in three instructions for two.  (Weights in shared memory instead, written and then read by the
-// products beside 256 tokens, took 100 KB of its traffic a tile, 780 cycles for 512 of the tensor core's.)  Where a weight has too few
-// rows to fill the SMs, K is cut over the blocks of a cluster.  The sums go from tensor memory to shared memory as they are, a row a
-// lane; then each token's results are read, four rows a thread (from all the cluster's blocks, in their order), finished, and written
-// as whole lines.  Waits are bounded.
+// 64 places of K: one thread fetches the tokens (TMA, 128-byte swizzle, zeros beyond the last token and place), one warp issues the
+// products, and the other warps turn weights into bfloat16 in tensor memory, a row a lane, each group of four warps every kGroups-th tile
+// of K: a lane copies 16 bytes of each of the warp's two tiles of rows, kAhead tiles ahead (cp.async), reads its row's four pieces (which
+// hold row g + 8 too), and makes two numbers in three instructions, each the whole number times its scale, exactly.  (Weights in shared
+// memory instead, written and then read by the products beside 256 tokens, took 100 KB of its traffic a tile, 780 cycles for 512 of the
+// tensor core's.)  Where a weight has too few rows to fill the SMs, K is cut over the blocks of a cluster.  The sums go from tensor memory
+// to shared memory as they are, a row a lane; then each token's results are read, four rows a thread (from all the cluster's blocks, in
+// their order), finished, and written as whole lines.  Waits are bounded.
+// Measured, with groups of 64: 512 tokens by 28,672 x 4,096 94 us (1,284 TFLOP/s), 2,048 by 16,384 x 2,048 117 us (1,180), 64 by
+// 28,672 x 4,096 30 us (2.2 TB/s of weights).  A tile of K with 256 tokens takes 0.34 us for 0.28 of products, a block's beginning and end
+// 7 us, which nothing hides; with few tokens it is the widening, 0.2 us a tile of 128 x 64 weights.
 enum { Q4_TIMEOUT_PRODUCT = 53 };
 
 // A grid that fills the SMs some times and leaves a few blocks is two launches: WAVES, whole times, then the REST with K cut over clusters.
@@ -602,7 +605,7 @@ static int launch_wide(const Args& a, int* status, cudaStream_t stream) {
         // blocks of a cluster: the number with the shortest time, that of so many turns of a share of K each and, about as long as 16
         // tiles of K, a block's beginning and end; no share below a stretch of 256 places
         int ranks = 1;
-        auto tiles = [&](int r) { return (long long)((blocks * r + at_once - 1) / at_once) * ((a.k_tiles + r - 1) / r + 16); };
+        auto tiles = [&](int r) { return ((long long)blocks * r + at_once - 1) / at_once * ((a.k_tiles + r - 1) / r + 16); };
         for (int r = 2; r <= 8 && a.k_tiles >= r * kBatch; r *= 2)
             if (tiles(r) < tiles(ranks)) ranks = r;
         const int share = (a.k_tiles + ranks - 1) / ranks;

@@ -2017,34 +2017,42 @@ def q8_pool(n_pages: int, n_kv: int, head_dim: int, device):
 
 
 def _q8_line(what, pool, scales, n_kv, head_dim):
-    line = q8_line_bytes(head_dim)
-    if (pool.dtype is not torch.int8 or pool.dim() != 3 or pool.shape[1] != n_kv or pool.shape[2] != line or scales.dtype is not torch.float32
-            or scales.shape != (pool.shape[0], n_kv, 2) or scales.data_ptr() != pool.data_ptr() + line - 16 or scales.stride() != (n_kv * line // 4, line // 4, 1)):
+    """The address of a line's pool."""
+    line = PAGE * (head_dim + (head_dim + 31) // 32 * 32) + 16
+    shape, at = pool.shape, pool.data_ptr()
+    if (len(shape) != 3 or shape[1] != n_kv or shape[2] != line or pool.dtype is not torch.int8 or scales.dtype is not torch.float32
+            or scales.data_ptr() != at + line - 16 or scales.shape != (shape[0], n_kv, 2) or scales.stride() != (n_kv * line // 4, line // 4, 1)):
         raise KernelError(f"{what}: pool int8 [pages, {n_kv}, {line}] and scales float32 [pages, {n_kv}, 2], as q8_pool gives them")
+    return at
 
 
 def _launch_ptrs(what, tensors, anywhere=()):
     """The addresses of the tensors (None: 0), which must be contiguous and lie on the current device (kernels are launched on its
     current stream); those of `tensors` begin at multiples of 16 bytes, those of `anywhere` where they like."""
-    now, out, odd = None, [], 15
-    for t in (*tensors, Ellipsis, *anywhere):
-        if t is Ellipsis:
-            odd = 0
-            continue
-        if t is None:
-            out.append(0)
-            continue
-        device, ptr = t.get_device(), t.data_ptr()
-        if device != now:
-            if device < 0:
-                raise KernelError("burn-lm_b200 kernels run on a CUDA device only; got a CPU tensor")
-            now = _current_device() if _current_device is not None else torch.cuda.current_device()
-            if device != now:
-                raise KernelError(f"{what}: a tensor on cuda:{device} while the current device is cuda:{now}")
-        if ptr & odd or not t.is_contiguous():
-            raise KernelError(f"{what}: tensors must be contiguous and begin at multiples of 16 bytes")
-        out.append(ptr)
+    now = tensors[0].get_device()
+    if now < 0 or now != (_current_device() if _current_device is not None else torch.cuda.current_device()):
+        _launch_refused(what, tensors[0])
+    out, odd = [], 15
+    for group in (tensors, anywhere):
+        for t in group:
+            if t is None:
+                out.append(0)
+                continue
+            ptr = t.data_ptr()
+            if t.get_device() != now or ptr & odd or not t.is_contiguous():
+                _launch_refused(what, t)
+            out.append(ptr)
+        odd = 0
     return out
+
+
+def _launch_refused(what, t):
+    device = t.get_device()
+    if device < 0:
+        raise KernelError("burn-lm_b200 kernels run on a CUDA device only; got a CPU tensor")
+    if device != torch.cuda.current_device():
+        raise KernelError(f"{what}: a tensor on cuda:{device} while the current device is cuda:{torch.cuda.current_device()}")
+    raise KernelError(f"{what}: tensors must be contiguous and begin at multiples of 16 bytes")
 
 
 _q8_places: dict = {}
@@ -2089,11 +2097,12 @@ def q8_values(pool, scales, pages, head_dim, dtype=torch.float32):
     (float32 or bfloat16, each rounded once) for `pages` int32 [P] on the device.  A page number outside the pool leaves its entry zero."""
     n_pages, n_kv = pool.shape[:2]
     _q8_line("q8_values", pool, scales, n_kv, head_dim)
-    if pages.dtype != torch.int32:
+    if pages.dtype is not torch.int32:
         raise KernelError("q8_values: pages must be int32")
     p_pool, p_pages = _launch_ptrs("q8_values", (pool,), (pages,))
-    out = torch.empty((pages.numel(), 2, n_kv, PAGE, head_dim), dtype=dtype, device=pool.device)
-    _call("attention_q8", "blm_q8_values", p_pool, p_pages, out.data_ptr(), _code(dtype), pages.numel(), n_kv, head_dim, n_pages, _stream())
+    n = pages.numel()
+    out = torch.empty((n, 2, n_kv, PAGE, head_dim), dtype=dtype, device=pool.device)
+    _call("attention_q8", "blm_q8_values", p_pool, p_pages, out.data_ptr(), _code(dtype), n, n_kv, head_dim, n_pages, _stream())
     return out
 
 
@@ -2132,22 +2141,26 @@ def rope_append_q8(qkv, out, step, pool, scales, tail, block_table, inv_freq, ro
     A step of one token a sequence may be run again with the same or another token before the sequence goes on; one of several
     tokens may not where it completes a block and leaves another unfinished.
     `pairs`, `table`, `turn_scale`: as for rope_append."""
-    if qkv.dim() != 2 or qkv.shape[1] != (n_heads + 2 * n_kv) * head_dim or out.shape != qkv.shape or out.dtype is not qkv.dtype:
+    shape, dtype = qkv.shape, qkv.dtype
+    if len(shape) != 2 or shape[1] != (n_heads + 2 * n_kv) * head_dim or out.shape != shape or out.dtype is not dtype:
         raise KernelError("rope_append_q8: qkv and out [N, (heads + 2 kv heads) * head_dim] of one dtype")
     _q8_line("rope_append_q8", pool, scales, n_kv, head_dim)
-    _q8_step("rope_append_q8", step, block_table, tail, n_kv, head_dim, qkv.dtype)
-    if rotary_dim and (inv_freq is None or inv_freq.dtype != torch.float64 or inv_freq.numel() != rotary_dim // 2):
+    _q8_step("rope_append_q8", step, block_table, tail, n_kv, head_dim, dtype)
+    if rotary_dim and (inv_freq is None or inv_freq.dtype is not torch.float64 or inv_freq.numel() != rotary_dim // 2):
         raise KernelError("rope_append_q8: inv_freq must be float64 [rotary_dim / 2]")
-    if table is not None and (table.dtype != torch.float32 or tuple(table.shape[1:]) != (rotary_dim // 2, 2)):
-        raise KernelError("rope_append_q8: table must be float32 [positions, rotary_dim / 2, 2]")
+    places = 0
+    if table is not None:
+        places = table.shape[0]
+        if table.dtype is not torch.float32 or table.shape != (places, rotary_dim // 2, 2):
+            raise KernelError("rope_append_q8: table must be float32 [positions, rotary_dim / 2, 2]")
     old = None
     if step.max_q_len > 1:
-        old = torch.empty((step.n_seqs, 2, n_kv, PAGE, head_dim), dtype=qkv.dtype, device=qkv.device)
+        old = torch.empty((step.n_seqs, 2, n_kv, PAGE, head_dim), dtype=dtype, device=qkv.device)
     p_qkv, p_out, p_pool, p_tail, p_table, p_old, p_block, p_freq = _launch_ptrs(
         "rope_append_q8", (qkv, out, pool, tail, table, old), (block_table, inv_freq if rotary_dim else None))
     p_cu, p_slot, p_start = _step_ptrs("rope_append_q8", step)
-    _call("attention_q8", "blm_rope_append_q8", p_qkv, p_out, _code(qkv.dtype), p_cu, p_slot, p_start, p_block, block_table.shape[1], p_freq,
-          rotary_dim, int(pairs), p_table, table.shape[0] if table is not None else 0, turn_scale, p_pool, p_tail, p_old, step.n_seqs,
+    _call("attention_q8", "blm_rope_append_q8", p_qkv, p_out, _code(dtype), p_cu, p_slot, p_start, p_block, block_table.shape[1], p_freq,
+          rotary_dim, int(pairs), p_table, places, turn_scale, p_pool, p_tail, p_old, step.n_seqs,
           step.max_q_len, n_heads, n_kv, head_dim, pool.shape[0], _stream())
     return old
 
@@ -2158,23 +2171,24 @@ def attention_q8(rotated, step, pool, scales, tail, old, block_table, out, n_hea
     sees the keys 0 .. p (the last `window` of them when window > 0): those of earlier blocks of PAGE positions in 8 bits, those of its
     own block unrounded, from the step's rows and, before them, from `old` (steps of one token a sequence: from `tail`).  So the result
     depends on the tokens, not on how they were cut into steps.  Scores, softmax and sums are fp32; out [N, n_heads * head_dim] in
-    rotated's dtype.  Rows of no sequence are left as they are.  bfloat16 steps of one token a sequence with heads of 64 or 128 lanes
-    stream the pages to the tensor cores (the probabilities, times the values' scale, are rounded to bfloat16) and may cut a sequence's
-    pages over several blocks: step.max_kv_len (the longest sequence after the step, or a bound) sizes that, step.workspace lends the
-    scratch."""
-    n = rotated.shape[0]
-    if rotated.dim() != 2 or rotated.shape[1] != (n_heads + 2 * n_kv) * head_dim or tuple(out.shape) != (n, n_heads * head_dim) or out.dtype != rotated.dtype:
+    rotated's dtype.  Rows of no sequence are left as they are.  In bfloat16 the probabilities, times the values' scale, are
+    rounded to bfloat16 (single tokens with heads of 64 or 128 lanes: to half precision); float32 steps keep 32 bits.  A sequence's pages may
+    be cut over several blocks: step.max_kv_len (the longest sequence after the step, or a bound) sizes that, step.workspace lends the
+    scratch that single tokens need for it.  At most 65,535 sequences and 500,000 tokens of one a step."""
+    shape, dtype = rotated.shape, rotated.dtype
+    n = shape[0]
+    if len(shape) != 2 or shape[1] != (n_heads + 2 * n_kv) * head_dim or out.shape != (n, n_heads * head_dim) or out.dtype is not dtype:
         raise KernelError("attention_q8: rotated [N, (heads + 2 kv heads) * head_dim] and out [N, heads * head_dim] of one dtype")
     _q8_line("attention_q8", pool, scales, n_kv, head_dim)
-    _q8_step("attention_q8", step, block_table, tail, n_kv, head_dim, rotated.dtype)
+    _q8_step("attention_q8", step, block_table, tail, n_kv, head_dim, dtype)
     if window < 0:
         raise KernelError(f"attention_q8: a window of {window} keys")
-    if step.max_q_len > 1 and (old is None or old.dtype != rotated.dtype or tuple(old.shape) != (step.n_seqs, 2, n_kv, PAGE, head_dim)):
+    if step.max_q_len > 1 and (old is None or old.dtype is not dtype or old.shape != (step.n_seqs, 2, n_kv, PAGE, head_dim)):
         raise KernelError("attention_q8: a step of several tokens a sequence needs what rope_append_q8 returned")
     found = tail if step.max_q_len <= 1 else old
     p_rot, p_pool, p_found, p_out, p_block = _launch_ptrs("attention_q8", (rotated, pool, found, out), (block_table,))
     p_cu, p_slot, p_start = _step_ptrs("attention_q8", step)
-    code, window = _code(rotated.dtype), int(window or 0)
+    code, window = _code(dtype), int(window or 0)
     splits = _ask("attention_q8", "blm_attention_q8_splits", code, step.n_seqs, step.max_q_len, step.max_kv_len, n_heads, n_kv, head_dim, window)
     scratch = None
     if splits > 1:
@@ -2308,35 +2322,41 @@ Q4_STORE, Q4_ADD, Q4_GATED = 0, 1, 2
 
 
 def product_q4(w, x, out=None, add_into=None, swiglu=False):
-    """x [N, K] (bfloat16) times a weight in 4 bits (Q4Weight) transposed: whole numbers on the tensor cores, scales on float32 sums.
+    """x [N, K] (bfloat16) times a weight in 4 bits (Q4Weight) transposed, on the tensor cores: every weight is a bfloat16 number exactly, sums
+    are float32.
 
     Ends, one at a time: `out` [N, M] bfloat16 or float32; `add_into` (float32 [N, M]) += the product; `swiglu`: the weight's rows
     come in tiles of GATE_TILE gate rows followed by the up rows of the same outputs and out [N, M / 2] = silu(gate) * up, in
     bfloat16 or float32.  x, out and add_into may be column ranges of wider tensors; x's rows begin at multiples of 16 bytes, or are
     copied first."""
-    n, k, m = x.shape[0], w.in_features, w.out_features
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] != k or (k > 1 and x.stride(1) != 1):
+    k, m, packed, shape, dtype = w.in_features, w.out_features, w.packed, x.shape, x.dtype
+    if len(shape) != 2 or dtype is not torch.bfloat16 or shape[1] != k or (k > 1 and x.stride(1) != 1):
         raise KernelError(f"product_q4: x is bfloat16 [N, {k}] with unit stride along its rows")
-    y = out if add_into is None else add_into
+    n, y, wide = shape[0], out, False
     if add_into is not None:
-        if out is not None or swiglu or add_into.dtype != torch.float32:
+        y, wide = add_into, True
+        if out is not None or swiglu or y.dtype is not torch.float32:
             raise KernelError("product_q4: add_into is float32 [N, M], alone")
-    elif out is None or out.dtype not in (torch.bfloat16, torch.float32):
-        raise KernelError("product_q4: out is bfloat16 or float32")
+    else:
+        wide = out is not None and out.dtype is torch.float32
+        if out is None or not wide and out.dtype is not torch.bfloat16:
+            raise KernelError("product_q4: out is bfloat16 or float32")
     if swiglu and m % (2 * GATE_TILE):
         raise KernelError(f"product_q4: gated rows come in tiles of {2 * GATE_TILE}, the weight has {m}")
-    if tuple(y.shape) != (n, m // 2 if swiglu else m) or (y.shape[1] > 1 and y.stride(1) != 1):
+    columns = m // 2 if swiglu else m
+    if y.shape != (n, columns) or (columns > 1 and y.stride(1) != 1):
         raise KernelError("product_q4: the result is [N, M] (gated: [N, M / 2]) with unit stride along its rows")
-    if not (x.is_cuda and y.is_cuda and w.packed.is_cuda):
-        raise KernelError("burn-lm_b200 kernels run on a CUDA device only; got a CPU tensor")
     now = x.get_device()
-    if y.get_device() != now or w.packed.get_device() != now or now != (_current_device() if _current_device is not None else torch.cuda.current_device()):
+    if now < 0 or y.get_device() != now or packed.get_device() != now or now != (_current_device() if _current_device is not None else torch.cuda.current_device()):
+        if not (x.is_cuda and y.is_cuda and packed.is_cuda):
+            raise KernelError("burn-lm_b200 kernels run on a CUDA device only; got a CPU tensor")
         raise KernelError("product_q4: x, the weight and the result lie on the current device")
-    if k % 8 or x.stride(0) % 8 or x.data_ptr() % 16:
-        wide = torch.zeros((n, -(-k // 64) * 64), dtype=torch.bfloat16, device=x.device)
-        wide[:, :k] = x
-        x, k = wide, wide.shape[1]
-    _call("gemm_q4", "blm_gemm_q4", _ptr(w.packed), w.packed.shape[1], w.group, _ptr(x), x.stride(0), _ptr(y), y.stride(0),
-          1 if y.dtype == torch.float32 else 0, Q4_ADD if add_into is not None else (Q4_GATED if swiglu else Q4_STORE), n, m, k,
-          status_word(x.device).data_ptr(), _stream())
+    p_x, apart = x.data_ptr(), x.stride(0)
+    if k % 8 or apart % 8 or p_x % 16:
+        rows = torch.zeros((n, -(-k // 64) * 64), dtype=dtype, device=x.device)
+        rows[:, :k] = x
+        x, k = rows, rows.shape[1]
+        p_x, apart = x.data_ptr(), k
+    _call("gemm_q4", "blm_gemm_q4", packed.data_ptr(), packed.shape[1], w.group, p_x, apart, y.data_ptr(), y.stride(0), wide,
+          Q4_ADD if add_into is not None else (Q4_GATED if swiglu else Q4_STORE), n, m, k, status_word(x.device).data_ptr(), _stream())
     return y
