@@ -526,7 +526,8 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
             }
         }
         __syncthreads();
-        float s[4][4] = {};                              // 16 rows by four times eight keys
+        // 16 rows by four times eight keys; the products of lower pieces by themselves, so that fewer sums of full size are cut off
+        float s[4][4] = {}, low[PIECES > 1 ? 4 : 1][4] = {};
 #pragma unroll 4
         for (int k = 0; k < (idle ? 0 : hd / 16); ++k) {
             unsigned x[PIECES][4];
@@ -541,12 +542,15 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
                     ldmatrix4(y, k_at + j * page_piece + c * 16 * row_of * 2 + k * 32);
 #pragma unroll
                     for (int i = 0; i < PIECES - j; ++i) {
-                        mma_bf16(s[2 * c], x[i], y[0], y[1]);
-                        mma_bf16(s[2 * c + 1], x[i], y[2], y[3]);
+                        mma_bf16(i + j == 0 ? s[2 * c] : low[PIECES > 1 ? 2 * c : 0], x[i], y[0], y[1]);
+                        mma_bf16(i + j == 0 ? s[2 * c + 1] : low[PIECES > 1 ? 2 * c + 1 : 0], x[i], y[2], y[3]);
                     }
                 }
             }
         }
+        if (PIECES > 1)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i / 4][i % 4] += low[PIECES > 1 ? i / 4 : 0][i % 4];
         float alpha[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -603,7 +607,7 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
 #pragma unroll
         for (int d = 0; d < 4 * NL; ++d) {               // sixteen lanes at a time
             if (d * 16 >= hd || idle) break;
-            float part[2][4] = {};
+            float part[2][4] = {}, less[2][4] = {};
 #pragma unroll
             for (int j = 0; j < PIECES; ++j) {
                 if (j > 0 && !own) break;
@@ -613,15 +617,15 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
                     ldmatrix4_turned(y, values_at + j * page_piece + c * 16 * row_of * 2 + d * 32);
 #pragma unroll
                     for (int i = 0; i < PIECES - j; ++i) {
-                        mma_bf16(part[0], p[c][i], y[0], y[1]);
-                        mma_bf16(part[1], p[c][i], y[2], y[3]);
+                        mma_bf16(i + j == 0 ? part[0] : less[0], p[c][i], y[0], y[1]);
+                        mma_bf16(i + j == 0 ? part[1] : less[1], p[c][i], y[2], y[3]);
                     }
                 }
             }
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[2 * d + x][e] = fmaf(acc[2 * d + x][e], alpha[e >> 1], part[x][e]);
+                for (int e = 0; e < 4; ++e) acc[2 * d + x][e] = fmaf(acc[2 * d + x][e], alpha[e >> 1], PIECES > 1 ? part[x][e] + less[x][e] : part[x][e]);
         }
     }
     __syncthreads();
