@@ -433,6 +433,13 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
     };
     // eight numbers as pieces, `apart` numbers between the pieces
     auto put = [&](__nv_bfloat16* to, size_t apart, float (&x)[8]) {
+        if (PIECES > 1) {                                // what would round to an infinity is cut off first: its last bits are nothing beside it
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const unsigned bits = __float_as_uint(x[e]), size = bits & 0x7fffffffu;
+                if (size >= 0x7f7f8000u && size < 0x7f800000u) x[e] = __uint_as_float(bits & 0xffff0000u);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < PIECES; ++i)
             *reinterpret_cast<uint4*>(to + i * apart) = make_uint4(take_two(x[0], x[1]), take_two(x[2], x[3]), take_two(x[4], x[5]), take_two(x[6], x[7]));
@@ -1228,7 +1235,7 @@ static bool tokens_take(int dtype, int hd, int max_q_len, int n_seqs, int n_kv, 
 //   warps 8 .. 11 turn a page into operands, once for both tiles: keys [64][D] and values transposed, [D][64], bfloat16 with the 128-byte
 //     swizzle, into rings of three each; a byte q + 128 in sixteen bits is the bfloat16 number (q + 128) 2^-133, and one subtraction makes
 //     it q 2^-133: two instructions for two numbers.  The values' rows stand in an order that keeps their eight-byte writes to two a bank;
-//   warp 12 (one thread) issues S = Q K^T and O += P V of both tiles.  Q lies in tensor memory (as a second operand in shared memory its
+//   warp 12 issues S = Q K^T and O += P V of both tiles.  Q lies in tensor memory (as a second operand in shared memory its
 //     reads, 32 KB a page and tile, would cost more than the products);
 //   warps 0 .. 7 are the softmax, a row a thread: Q times a power of two that brings the row's largest lane to 2^60 (the keys' 2^-133 has to
 //     meet ordinary numbers), scores times the keys' scale, a reference maximum that moves when a score exceeds it by 2^8, probabilities

@@ -582,3 +582,19 @@ def test_a_portion_captured_and_two_graphs_at_once():
         g.replay()
         assert torch.equal(o, plain)
     k.check_status(torch.device("cuda:0"))
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_the_largest_floats(which):
+    """Keys and values next to the largest float32 number, which no bfloat16 number reaches: later ones do not reach the queries before."""
+    outs = []
+    for with_it in (False, True):
+        b = Batch(1, 4, 1, 64, F32, 256, seed=6, scale=1e-3)
+        qkv = b.rows(90)
+        if with_it:
+            qkv.view(90, 6, 64)[70, 4 + which, 5] = torch.finfo(F32).max if which else 3.39e38
+        step, out, old = b.append([(0, 90)], qkv=qkv, rot=0, check=False)
+        outs.append(b.attend([(0, 90)], step, out, old, check=False).view(90, 4, 64))
+    assert torch.equal(outs[0][:70], outs[1][:70]) and torch.isfinite(outs[1][:70]).all()
+    if which == 1:
+        assert torch.isfinite(outs[1][70:]).all() and (outs[1][70:, :, 5] > 1e30).all()
