@@ -742,6 +742,7 @@ struct TokenArgs {
     float* part_acc;             // [N, n_heads, n_splits, hd]
     float* part_ml;              // [N, n_heads, n_splits, 2]: maximum (base 2) and sum
     int n_splits, head_tiles, heads_a_tile, pages_per_split;
+    int clustered;               // the shares of a sequence are the blocks of a cluster, and meet in it
     int* status;
 };
 enum { Q8_TIMEOUT_PAGE = 51, Q8_TIMEOUT_FREE = 52 };
@@ -853,6 +854,7 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
     constexpr int KS = HD / 16, PIECES = HD / 64;                        // PIECES: 16-byte pieces of a key row in a thread
     constexpr unsigned STAGE = line_bytes(HD);
     const AttendArgs& a = ta.a;
+    __shared__ float2 met[8];                                            // maximum and sum of this share's heads, for the cluster
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* ring = smem_raw;                                      // [S][keys, values, scales]
     float* sm_acc = reinterpret_cast<float*>(ring);                      // [WARPS][8][HD], when the ring has been read
@@ -876,7 +878,14 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
     const int key_lo = a.window > 0 ? max(0, pos + 1 - a.window) : 0, mine = pos / kPage;
     const int pg_first = key_lo / kPage, n_pg = max(0, mine - pg_first);          // blocks in 8 bits
     const int active = active_splits(n_pg, ta.n_splits, ta.pages_per_split);
-    if (next <= tok || split >= active) return;          // (the whole block; the kernel that merges computes the same number)
+    if (next <= tok) return;                             // (the whole cluster)
+    if (split >= active) {                               // (the whole block; the kernel that merges computes the same number)
+        if (ta.clustered && active > 1) {
+            cluster_sync();
+            cluster_sync();
+        }
+        return;
+    }
     const int per = (n_pg + active - 1) / active;
     const int pg_lo = pg_first + split * per, pg_hi = min(pg_first + n_pg, pg_lo + per);
     __syncthreads();
@@ -1108,6 +1117,7 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
     }
     if (warp == WARPS) asm volatile("bar.sync 1, %0;\n" ::"r"((WARPS + 1) * 32) : "memory");
     __syncthreads();
+    const bool meet = ta.clustered && active > 1;
     for (int i = tid; i < G * HD; i += blockDim.x) {
         const int h = i / HD, d = i % HD;
         float m = -INFINITY;
@@ -1124,12 +1134,48 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
         const size_t row = (size_t)tok * a.n_heads + head0 + h;
         if (active == 1) {
             reinterpret_cast<__nv_bfloat16*>(a.out)[row * HD + d] = __float2bfloat16_rn(o / l);
+        } else if (meet) {
+            sm_acc[h * HD + d] = o;                      // (no other thread reads or writes lane d of head h)
+            if (d == 0) met[h] = make_float2(m, l);
         } else {
             const size_t part = row * ta.n_splits + split;
             ta.part_acc[part * HD + d] = o;
             if (d == 0) { ta.part_ml[part * 2] = m; ta.part_ml[part * 2 + 1] = l; }
         }
     }
+    if (!meet) return;
+    // the cluster's shares: some of the heads each, four lanes a thread, all reads before the first use
+    cluster_sync();
+    const int heads = (G - split + active - 1) / active;
+    for (int i = tid; i < heads * (HD / 4); i += blockDim.x) {
+        const int h = split + i / (HD / 4) * active, d = i % (HD / 4) * 4;
+        float m[8], l[8];
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < active) {
+                m[k] = cluster_float(smem_u32(&met[h].x), k);
+                l[k] = cluster_float(smem_u32(&met[h].y), k);
+                v[k] = cluster_float4(smem_u32(sm_acc + h * HD + d), k);
+            }
+        float top = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < active) top = fmaxf(top, m[k]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < active) {
+                const float w = ex2(m[k] - ref);
+                total = fmaf(l[k], w, total);
+                o.x = fmaf(v[k].x, w, o.x); o.y = fmaf(v[k].y, w, o.y); o.z = fmaf(v[k].z, w, o.z); o.w = fmaf(v[k].w, w, o.w);
+            }
+        const float by = 1.f / total;
+        *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + ((size_t)tok * a.n_heads + head0 + h) * HD + d) =
+            make_uint2(pack_bf16(o.x * by, o.y * by), pack_bf16(o.z * by, o.w * by));
+    }
+    cluster_sync();                                      // what others read stays until they have
 }
 
 // Merges the shares: a block per (sequence, head); 512 / HD groups of threads take shares in turn, four lanes a thread.
@@ -1182,6 +1228,7 @@ __global__ void __launch_bounds__(128) merge_kernel(const TokenArgs ta) {
 
 // The plan of a step of single tokens, the same for the caller that provides the scratch and for the launch.
 struct TokenPlan { int splits, pages_per_split, wpp, head_tiles, heads_a_tile; };
+constexpr int kClusterShares = 8;        // so many shares, the blocks of a cluster, meet in it; more in a second kernel
 static TokenPlan plan_tokens(int n_seqs, int n_heads, int n_kv, int hd, int max_kv_len, int window) {
     TokenPlan p;
     const int group = n_heads / n_kv, sms = blm_sm_count();
@@ -1191,9 +1238,13 @@ static TokenPlan plan_tokens(int n_seqs, int n_heads, int n_kv, int hd, int max_
     if (window > 0 && pages > window / kPage + 2) pages = window / kPage + 2;
     if (pages < 1) pages = 1;
     const int rows = n_seqs * n_kv * p.head_tiles;       // blocks of an unsplit step
-    // Walks of more than 8 pages are cut, as far as that fills the SMs about twice (8 sequences of 2,000 tokens, heads of 128: 14.9 us in
-    // 4 shares, 18.6 in 8, 19.5 in one; one sequence of 32,000: 20.1 us in 37, 24.6 in 56).
-    const int by_length = (pages + 7) / 8, to_fill = (2 * sms + rows - 1) / rows;
+    // Walks are cut, as far as the shares' blocks are resident together (three of heads of 128 an SM, four of 64: one block more than that
+    // is a second turn): into up to eight of two pages or more, which meet in a cluster, and long ones into shares of eight pages, which
+    // meet in a second kernel.  Measured, heads of 128, 32 to 8: one sequence of 500, 2,000, 4,000 tokens 6.0, 7.0, 9.4 us (with shares of
+    // eight pages and the second kernel 6.9, 10.3, 11.4); 8 of 2,000 14.0 in five or six shares, 19.8 in seven, which are 448 blocks;
+    // 32 of 1,000 20.0 in one, 27 in two; one of 32,000 20.1 in 55 and 20.5 in 37.
+    const int eights = (pages + 7) / 8, twos = (pages + 1) / 2, to_fill = (hd == 128 ? 3 : 4) * sms / rows;
+    const int by_length = eights > kClusterShares ? eights : twos < kClusterShares ? twos : kClusterShares;
     p.splits = by_length < to_fill ? by_length : to_fill;
     if (p.splits > 64) p.splits = 64;
     if (p.splits < 1) p.splits = 1;
@@ -1218,8 +1269,8 @@ static int launch_tokens_as(const TokenArgs& ta, cudaStream_t stream) {
             return blm_fail(BLM_CUDA_ERROR, "attention_q8: %s", cudaGetErrorString(cudaGetLastError()));
         if (dev >= 0 && dev < 64) opted_in[dev] = true;
     }
-    blm_launch_dependent(attend_token_kernel<HD, WPP>, grid, dim3((kTokenWarps + 1) * 32), smem, stream, ta);
-    if (ta.n_splits > 1) blm_launch_dependent(merge_kernel<HD>, dim3(ta.a.n_heads, ta.a.n_seqs), dim3(128), 0, stream, ta);
+    blm_launch_cluster(attend_token_kernel<HD, WPP>, ta.clustered ? ta.n_splits : 1, grid, dim3((kTokenWarps + 1) * 32), smem, stream, ta);
+    if (ta.n_splits > 1 && !ta.clustered) blm_launch_dependent(merge_kernel<HD>, dim3(ta.a.n_heads, ta.a.n_seqs), dim3(128), 0, stream, ta);
     return blm_check_launch("attention_q8");
 }
 // bfloat16 steps of single tokens with heads of 64 or 128 lanes
@@ -1889,12 +1940,13 @@ BLM_API int blm_q8_values(const void* pool, const int* pages, void* out, int dty
     return blm_check_launch("q8_values");
 }
 
-// Over how many shares a step cuts its sequences: what the scratch holds is n_tokens * n_heads * shares * (hd + 2) float32 when there are
+// Over how many shares that meet in memory a step cuts its sequences: what the scratch holds is n_tokens * n_heads * shares * (hd + 2) float32 when there are
 // several, which a second kernel merges.
 BLM_API int blm_attention_q8_splits(int dtype, int n_seqs, int max_q_len, int max_kv_len, int n_heads, int n_kv, int hd, int window) {
     using namespace q8;
     if (n_seqs < 1 || n_kv < 1 || n_heads < n_kv || !tokens_take(dtype, hd, max_q_len, n_seqs, n_kv, n_heads)) return 1;
-    return plan_tokens(n_seqs, n_heads, n_kv, hd, max_kv_len, window).splits;
+    const int splits = plan_tokens(n_seqs, n_heads, n_kv, hd, max_kv_len, window).splits;
+    return splits > kClusterShares ? splits : 1;
 }
 
 BLM_API int blm_attention_q8(const void* rotated, const void* pool, const void* found, int found_by_slot, int dtype,
@@ -1910,9 +1962,10 @@ BLM_API int blm_attention_q8(const void* rotated, const void* pool, const void* 
                        out, n_seqs, n_heads, n_kv, hd, n_pages, window, scale * 1.4426950408889634f};
     if (tokens_take(dtype, hd, max_q_len, n_seqs, n_kv, n_heads)) {
         const TokenPlan p = plan_tokens(n_seqs, n_heads, n_kv, hd, max_kv_len, window);
-        BLM_REQUIRE(p.splits == splits && (splits == 1 || scratch != nullptr), "attention_q8: scratch for %d shares, the step has %d", splits, p.splits);
+        const bool clustered = p.splits > 1 && p.splits <= kClusterShares;
+        BLM_REQUIRE((clustered ? 1 : p.splits) == splits && (splits == 1 || scratch != nullptr), "attention_q8: scratch for %d shares, the step has %d", splits, p.splits);
         const TokenArgs ta{a, scratch, scratch ? scratch + (size_t)n_tokens * n_heads * splits * hd : nullptr, p.splits, p.head_tiles, p.heads_a_tile,
-                           p.pages_per_split, status};
+                           p.pages_per_split, clustered, status};
         if (hd == 64) return launch_tokens_as<64, 1>(ta, stream);
         return p.wpp == 1 ? launch_tokens_as<128, 1>(ta, stream) : launch_tokens_as<128, 2>(ta, stream);
     }
