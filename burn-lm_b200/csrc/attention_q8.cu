@@ -406,7 +406,7 @@ __device__ __forceinline__ unsigned take_two(float& x, float& y) {
 }
 
 template <typename T, int NL>
-__global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendArgs a, int hb, int ranks) {
+__global__ void __launch_bounds__(kTileThreads, NL == 1 ? 3 : 1) attend_tile_kernel(const AttendArgs a, int hb, int ranks) {
     constexpr int PIECES = Tile<T>::kPieces;
     extern __shared__ __align__(16) unsigned char tile_shared[];
     __shared__ unsigned odd_keys[2];                     // bits: keys of the own block whose values hold an infinity or a NaN
@@ -466,6 +466,16 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
 #pragma unroll
     for (int i = 0; i < 8 * NL; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
     const int pieces = 4 * hd, chunks = 4 * padded(hd), per = hd / 8;            // of sixteen bytes: of a page's keys, of its values
+    // where a thread's pieces lie in a page, and go (worked out once: it takes longer than their widening)
+    int k_from[2 * NL], k_to[2 * NL], v_to[2 * NL], v_lanes[2 * NL];
+#pragma unroll
+    for (int i = 0; i < 2 * NL; ++i) {
+        const int c = tid + i * kTileThreads, rem = c % padded(hd), piece = rem & 31, lanes0 = rem / 32 * 4;
+        k_from[i] = key_piece(c % kPage, c / kPage * 16, hd);
+        k_to[i] = c % kPage * row_of + c / kPage * 16;
+        v_to[i] = (kPage + c / padded(hd) * 16 + (piece & 3) * 4) * row_of + (piece >> 2) * per + lanes0;
+        v_lanes[i] = min(4, per - lanes0);               // (the last piece of a row may have fewer)
+    }
     uint4 next_k[2 * NL], next_v[2 * NL];
     float2 next_scale = make_float2(0.f, 0.f);
     bool next_there = false;
@@ -478,7 +488,7 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
 #pragma unroll
         for (int i = 0; i < 2 * NL; ++i) {
             const int c = tid + i * kTileThreads;
-            if (c < pieces) next_k[i] = *reinterpret_cast<const uint4*>(line + key_piece(c % kPage, c / kPage * 16, hd));
+            if (c < pieces) next_k[i] = *reinterpret_cast<const uint4*>(line + k_from[i]);
             if (c < chunks) next_v[i] = *reinterpret_cast<const uint4*>(line + kPage * hd + c * 16);
         }
     };
@@ -495,31 +505,29 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
                 if (b + ranks < mine) fetch(b + ranks);
                 continue;
             }
-            __nv_bfloat16* values = page + (size_t)kPage * row_of;
 #pragma unroll
             for (int i = 0; i < 2 * NL; ++i) {
                 const int c = tid + i * kTileThreads;
                 if (c < pieces) {
-                    uint4* to = reinterpret_cast<uint4*>(page + (size_t)(c % kPage) * row_of + c / kPage * 16);
+                    uint4* to = reinterpret_cast<uint4*>(page + k_to[i]);
                     auto four = [&](unsigned w) { return make_uint2(pack_bf16(wide(w, 0), wide(w, 1)), pack_bf16(wide(w, 2), wide(w, 3))); };
                     const uint2 x = four(next_k[i].x), y = four(next_k[i].y), z = four(next_k[i].z), w = four(next_k[i].w);
                     to[0] = make_uint4(x.x, x.y, y.x, y.y);
                     to[1] = make_uint4(z.x, z.y, w.x, w.y);
                 }
                 if (c < chunks) {                        // four lanes of four keys
-                    const int rem = c % padded(hd), piece = rem & 31, lanes0 = rem / 32 * 4, key = c / padded(hd) * 16 + (piece & 3) * 4;
-                    __nv_bfloat16* to = values + (size_t)key * row_of + (piece >> 2) * per + lanes0;
+                    __nv_bfloat16* to = page + v_to[i];
                     const unsigned w[4] = {next_v[i].x, next_v[i].y, next_v[i].z, next_v[i].w};
                     if (per % 4 == 0) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            *reinterpret_cast<uint2*>(to + (size_t)e * row_of) = make_uint2(pack_bf16(wide(w[0], e), wide(w[1], e)), pack_bf16(wide(w[2], e), wide(w[3], e)));
-                    } else {
+                            *reinterpret_cast<uint2*>(to + e * row_of) = make_uint2(pack_bf16(wide(w[0], e), wide(w[1], e)), pack_bf16(wide(w[2], e), wide(w[3], e)));
+                    } else {                             // (rows of an odd number of pairs of lanes)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            if (lanes0 + x < per)
+                        for (int x = 0; x < 4; x += 2)
+                            if (x < v_lanes[i])
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) to[(size_t)e * row_of + x] = __float2bfloat16(wide(w[x], e));
+                                for (int e = 0; e < 4; ++e) *reinterpret_cast<unsigned*>(to + e * row_of + x) = pack_bf16(wide(w[x], e), wide(w[x + 1], e));
                     }
                 }
             }
@@ -699,13 +707,16 @@ __global__ void __launch_bounds__(kTileThreads) attend_tile_kernel(const AttendA
 template <typename T, int NL>
 static int launch_tile(const AttendArgs& a, int n_tokens, int max_q_len, int max_kv_len, cudaStream_t stream) {
     const int group = a.n_heads / a.n_kv, hb = group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1, tb = kTileRows / hb;
-    // a walk of several pages is shared by the blocks of a cluster, as far as that gives an SM no more than four
+    // a walk of several pages is shared by the blocks of a cluster, as far as they are resident together: three an SM with heads of up to 64
+    // lanes, two of up to 128 (60 tokens behind 1,000 in float32, heads of 64: 26 us so, 35 with four; 8 single tokens behind 2,000 with
+    // heads of 80: 27 us with two blocks of all the registers they want, 35 with three)
+    const size_t smem = Tile<T>::smem(a.hd);
+    const int at_once = blm_sm_count() * (NL == 1 ? 3 : NL == 2 ? 2 : 1);
     const int tiles = a.n_kv * (group / hb) * ((n_tokens + tb - 1) / tb + a.n_seqs - 1);
     int pages = (max_kv_len + kPage - 1) / kPage, ranks = 1;
     if (a.window > 0 && pages > a.window / kPage + 2) pages = a.window / kPage + 2;
-    while (ranks < 8 && (long long)tiles * ranks * 2 <= 4ll * blm_sm_count() && pages >= 2 * ranks) ranks *= 2;
+    while (ranks < 8 && (long long)tiles * ranks * 2 <= at_once && pages >= 2 * ranks) ranks *= 2;
     const dim3 grid(a.n_kv * (group / hb) * ranks, (max_q_len + tb - 2) / tb + 1, a.n_seqs);
-    const size_t smem = Tile<T>::smem(a.hd);
     if (cudaFuncSetAttribute(attend_tile_kernel<T, NL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return blm_fail(BLM_CUDA_ERROR, "attention_q8: %s", cudaGetErrorString(cudaGetLastError()));
     blm_launch_cluster(attend_tile_kernel<T, NL>, ranks, grid, dim3(kTileThreads), smem, stream, a, hb, ranks);
