@@ -745,7 +745,8 @@ static int launch_tile(const AttendArgs& a, int n_tokens, int max_q_len, int max
 //   * the values' scale rides in the exponent: p' = 2^(score + log2 vs - m), with the maximum m taken of that sum, is at most 1, its
 //     product with the whole numbers needs no scale, and the sum of the probabilities gets p' / vs.  p' is rounded to half precision
 //     times 2^12 (11 bits from the largest down to 2^-26 of it).
-// Warps keep their own running maximum, sum and output and merge at the end; shares of a sequence meet in a second kernel.  The own
+// Warps keep their own running maximum, sum and output and merge at the end; up to eight shares of a sequence meet in their cluster, more in a
+// second kernel.  The own
 // block's keys, unrounded, are read straight from the tail and the step's rows by the four warps of the last share, in bfloat16,
 // while the first pages are on their way.  Waits are bounded; one that runs out leaves a code in the status word.
 struct TokenArgs {
@@ -1362,18 +1363,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int ranks = pa.ranks, rank = blockIdx.x % ranks, kv_group = blockIdx.x / ranks;
     const int kvh = kv_group / pa.head_groups, hg = kv_group % pa.head_groups, seq = blockIdx.z;
-    pdl_wait();
-    const int tok0 = a.cu_seqlens[seq], n = a.cu_seqlens[seq + 1] - tok0, start = a.start_pos[seq], slot = a.slot_of_seq[seq], end = start + n;
-    // the sequence's last blocks, which walk furthest, begin first
-    const int mine = (end - 1) / kPage - (int)blockIdx.y;
-    if (n <= 0 || mine < start / kPage) return;          // (the whole cluster)
-    const int p0 = mine * kPage, group = a.n_heads / a.n_kv, head0 = kvh * group + hg * pa.heads_a_group;
+    const int group = a.n_heads / a.n_kv, head0 = kvh * group + hg * pa.heads_a_group;
     const int G = min(pa.heads_a_group, group - hg * pa.heads_a_group), tiles = (G + 1) / 2;
-    auto first_key = [&](int pos) { return a.window > 0 ? max(0, pos + 1 - a.window) : 0; };
-    // this block's share of the walk (some may have none); the last step of the last is the own block
-    const int pg_first = first_key(max(start, p0)) / kPage, share = (mine - pg_first + ranks) / ranks;
-    const int pg_lo = pg_first + rank * share, steps = max(0, min(share, mine + 1 - pg_lo)), own_rank = (mine - pg_first) / share;
-    const int own_step = rank == own_rank ? steps - 1 : steps;
     if (threadIdx.x == 0) {
         for (int s = 0; s < KS; ++s) {
             mbar_init(raw_full + s, 1);
@@ -1392,11 +1383,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         odd_values[0] = odd_values[1] = 0u;
         tc5::mbar_init_fence();
     }
-    if (warp == 12) tc5::tmem_alloc(tmem_slot, 512);
+    if (warp == 12) tc5::tmem_alloc(tmem_slot, 512);      // (while the kernel before ends)
+    pdl_wait();
+    const int tok0 = a.cu_seqlens[seq], n = a.cu_seqlens[seq + 1] - tok0, start = a.start_pos[seq], slot = a.slot_of_seq[seq], end = start + n;
+    // the sequence's last blocks, which walk furthest, begin first
+    const int mine = (end - 1) / kPage - (int)blockIdx.y;
+    const bool none_here = n <= 0 || mine < start / kPage;                       // (the whole cluster)
+    const int p0 = mine * kPage;
+    auto first_key = [&](int pos) { return a.window > 0 ? max(0, pos + 1 - a.window) : 0; };
+    // this block's share of the walk (some may have none); the last step of the last is the own block
+    const int pg_first = first_key(max(start, p0)) / kPage, share = max(1, (mine - pg_first + ranks) / ranks);
+    const int pg_lo = pg_first + rank * share, steps = max(0, min(share, mine + 1 - pg_lo)), own_rank = (mine - pg_first) / share;
+    const int own_step = rank == own_rank ? steps - 1 : steps;
     tc5::fence_before();
     __syncthreads();
     tc5::fence_after();
     pdl_launch_dependents();                              // (not before this block has its tensor memory: the next kernel may take some too)
+    if (none_here) {
+        if (warp == 12) tc5::tmem_free(*tmem_slot, 512);
+        return;
+    }
     // a tile's columns: 64 of scores (and probabilities), HD of sums, HD / 2 of queries
     const unsigned tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);                 // (one number for a warp: what the products are issued with)
     constexpr unsigned kTileCols = 256, kOCol = 64, kQCol = 64 + HD;
