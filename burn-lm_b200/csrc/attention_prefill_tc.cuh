@@ -299,7 +299,6 @@ __global__ void __launch_bounds__(attn_tc::kThreads, attn_tc::blocks_an_sm(HDV))
             for (int d = threadIdx.x; d < a.dv; d += kThreads) a.out[(size_t)n * a.out_stride + (size_t)head * a.dv + d] = __float2bfloat16(0.f);
     }
     if (q0 >= q_len) return;                                      // the whole block: nothing was set up yet
-    pdl_launch_dependents();
     const int start = a.start_pos[seq];
     const int kv_total = start + q_len;                           // keys of this sequence in the cache after the step's append
     const int rows = min(BQ, q_len - q0);
@@ -338,6 +337,8 @@ __global__ void __launch_bounds__(attn_tc::kThreads, attn_tc::blocks_an_sm(HDV))
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     const unsigned tmem_base = *tmem_slot;
+    // not before this block has its tensor memory: the next kernel may take some while it waits for this one
+    pdl_launch_dependents();
 
     // Who waits for whom, step j (a page of 64 keys; t = j % kSRing, b = j & 1):
     //   scores warp:  pv_done[t] of step j - kSRing (its columns were read), k_full  ->  S(j)  ->  s_full[t], k_empty
