@@ -1308,7 +1308,7 @@ static bool tokens_take(int dtype, int hd, int max_q_len, int n_seqs, int n_kv, 
 // other, the two tiles half a page apart; products alone would take 1,024, exponentials as much.  (Two sets of columns for the scores, with
 // the queries in shared memory to make room, took as long: 2,100; sixteen softmax warps of half a row each 2,300.)  The products are issued
 // by a whole warp: behind `lane == 0`, where what an instruction needs is not known to be one number for the warp, each took 65 cycles to
-// issue and each wait 400, and a page 2,900.  2,048 tokens, 32 heads of 128 to 8: 49 us (695 TFLOP/s).
+// issue and each wait 400, and a page 2,900.  2,048 tokens, 32 heads of 128 to 8: 49 us (705 TFLOP/s).
 constexpr int kPromptThreads = 14 * 32, kPromptStages = 3;
 enum { Q8_TIMEOUT_PROMPT = 55 };
 struct PromptArgs {
@@ -1321,7 +1321,7 @@ template <int HD> struct Prompt {
     static constexpr int kTile = 64 * HD * 2;                                // bytes of a page's keys (or values) as operands
     static constexpr int kRaw = (line_bytes(HD) + 127) / 128 * 128;
     static constexpr int kRows = 256 * HD * 2;                               // queries on their way in, sums on their way out
-    static constexpr int kSmem = kPromptStages * (2 * kTile + kRaw) + kRows + 4 * 8 + 24 * 8 + 16 + 1024;
+    static constexpr int kSmem = kPromptStages * (2 * kTile + kRaw) + kRows + 4 * 16 + 24 * 8 + 16 + 1024;
 };
 // two bytes of a word as two bfloat16 numbers, (byte - 128) 2^-133
 template <int LO>
@@ -1347,7 +1347,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     unsigned char* values = keys + KS * P::kTile;                            // [KS][HD lanes][128 bytes: 64 keys]
     unsigned char* raw = values + KS * P::kTile;                             // [KS][page]
     unsigned char* staged = raw + KS * P::kRaw;                              // [8 warps][32 rows][HD], the 16-byte pieces of row r at c ^ (r & 7)
-    float2* scales = reinterpret_cast<float2*>(staged + P::kRows);           // [4] of the pages in the works
+    float4* scales = reinterpret_cast<float4*>(staged + P::kRows);           // [4] of the pages in the works: what the softmax makes of their scales
     unsigned long long* raw_full = reinterpret_cast<unsigned long long*>(scales + 4);
     unsigned long long* raw_free = raw_full + KS;
     unsigned long long* k_full = raw_free + KS;
@@ -1503,28 +1503,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             if (!own && !mbar_wait(raw_full + s, (j / KS) & 1)) { ok = false; break; }
             const float2 scale = own ? make_float2(1.f, 1.f) : *scales_of(page, HD);
             const bool none = scale.y < 0.f;
-            // a thread's pieces, all before the first use (each read waiting for the write before it would be the most of a page's time):
-            // of the keys sixteen lanes, four pieces of a 64-lane half by eight keys a warp; of the values four lanes of four keys
+            // a thread's pieces: of the keys sixteen lanes, four pieces of a 64-lane half by eight keys a warp; of the values four lanes of four keys
             constexpr int kPieces = HD / 32;
             auto key_at = [&](int i, int& half, int& r) {
                 const int at = i * 4 + cw;
                 half = HD == 128 ? at & 1 : 0;
                 r = (HD == 128 ? at >> 1 : at) * 8 + (lane >> 2);
             };
-            uint4 kv[kPieces], vv[kPieces];
-            if (!own && !none) {
-#pragma unroll
-                for (int i = 0; i < kPieces; ++i) {
-                    int half, r;
-                    key_at(i, half, r);
-                    kv[i] = *reinterpret_cast<const uint4*>(page + key_piece(r, (half * 4 + (lane & 3)) * 16, HD));
-                    vv[i] = *reinterpret_cast<const uint4*>(page + kPage * HD + cw * (16 * HD) + i * 512 + lane * 16);      // keys 16 cw .. 16 cw + 15
-                }
-            }
-            if (!own) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(raw_free + s);
-            }
             if (j >= KS && !mbar_wait(k_free + s, parity)) { ok = false; break; }
             if (own || none) {
                 constexpr int kEach = HD / 16;           // (all loads before the first use: one latency, not eight)
@@ -1545,14 +1530,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                 for (int i = 0; i < kPieces; ++i) {
                     int half, r;
                     key_at(i, half, r);
-                    const uint4 v = kv[i];
+                    const uint4 v = *reinterpret_cast<const uint4*>(page + key_piece(r, (half * 4 + (lane & 3)) * 16, HD));
                     unsigned char* to = kt + half * 8192 + r * 128;
                     const int c = (lane & 3) * 2;
                     *reinterpret_cast<uint4*>(to + ((c ^ (r & 7)) << 4)) = make_uint4(tiny_two<0>(v.x), tiny_two<2>(v.x), tiny_two<0>(v.y), tiny_two<2>(v.y));
                     *reinterpret_cast<uint4*>(to + (((c + 1) ^ (r & 7)) << 4)) = make_uint4(tiny_two<0>(v.z), tiny_two<2>(v.z), tiny_two<0>(v.w), tiny_two<2>(v.w));
                 }
             }
-            if (me == 0) scales[j & 3] = scale;
+            if (me == 0) {
+                // Scores are multiplied by the first number (times the row's own).  Probabilities leave times 2^ the third, the values' scale
+                // times 2^60 (the own block's: 2^-73), and their sum times the fourth takes it off again.  (A block whose values are all next
+                // to zero: any scale will do.)  The second is below zero for a page that is none.
+                const float vs = scale.y < 0x1p-100f ? 0x1p-100f : scale.y;
+                scales[j & 3] = own ? make_float4(0x1p-67f, 1.f, -73.f, 0x1p73f) : make_float4(0x1p66f * scale.x, scale.y, __log2f(vs) + 60.f, 0x1p-60f / vs);
+            }
             tc5::fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(k_full + s);
@@ -1593,7 +1584,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                 const int g = lane >> 2, t = lane & 3;
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) {
-                    const uint4 v = vv[i];
+                    const uint4 v = *reinterpret_cast<const uint4*>(page + kPage * HD + cw * (16 * HD) + i * 512 + lane * 16);      // keys 16 cw .. 16 cw + 15
                     const unsigned w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
@@ -1604,7 +1595,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             }
             tc5::fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(v_full + s);
+            if (lane == 0) {
+                mbar_arrive(v_full + s);
+                if (!own) mbar_arrive(raw_free + s);
+            }
         }
         if (!ok && lane == 0) gave_up();
     } else if (warp < 4 * tiles) {
@@ -1667,14 +1661,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             tc5::fence_after();
             const bool own = j == own_step;
             const int key0 = (pg_lo + j) * kPage;
-            const float2 scale = scales[j & 3];
-            // probabilities leave times 2^shift, the values' scale times 2^60 (the own block's: 2^-73), and their sum is divided by it again
-            // (a block whose values are all next to zero: any scale will do; of a page that the row sees nothing of, whatever its scale)
-            float f = own ? to_log2 * 0x1p-67f : to_log2 * (0x1p66f * scale.x);
-            // keys of zeros: their scores stay zeros, and a hidden key's minus infinity; of a page that the row sees nothing of, whatever its scale
-            if (f == 0.f || key0 + 63 < lo) f = 0x1p-126f;
-            const float vs = own ? 1.f : (key0 + 63 < lo || scale.y < 0x1p-100f ? 0x1p-100f : scale.y);
-            const float shift = own ? -73.f : __log2f(vs) + 60.f, to_sum = own ? 0x1p73f : 0x1p-60f / vs;
+            const float4 scale = scales[j & 3];
+            float f = to_log2 * scale.x, shift = scale.z, to_sum = scale.w;
             float x[64];
 #pragma unroll
             for (int c = 0; c < 64; c += 16) tc5::tmem_ld16(at + c, x + c);
@@ -1685,6 +1673,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
 #pragma unroll
                 for (int i = 0; i < 64; ++i)
                     if (i < from || i > to) x[i] = -INFINITY;
+                if (f == 0.f) f = 0x1p-126f;             // (keys of zeros: a hidden one's score stays minus infinity)
+                if (from > 63) {                         // of a page that the row sees nothing of, whatever its scales
+                    f = 0x1p-126f;
+                    shift = to_sum = 0.f;
+                }
             }
             float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
