@@ -55,6 +55,39 @@ __device__ __forceinline__ unsigned pack_bf16(float a, float b) {
     return *reinterpret_cast<const unsigned*>(&v);
 }
 
+// Steps of several tokens have a block of threads for every block of `unit` positions that a sequence touches.  The one with number `at`,
+// the sequences in turn, each one's from its last (which walk furthest): its sequence, -1 where there are fewer, and its number from the
+// sequence's last.  A warp asks together.  (With a grid of the longest sequence's blocks for every sequence, a prompt of 2,000 tokens
+// beside 63 single ones was 287 us of attention, most of it blocks that had nothing to do.)
+__device__ __forceinline__ int find_block(const int* cu_seqlens, const int* start_pos, int n_seqs, int unit, int at, int& from_last) {
+    const int lane = threadIdx.x & 31;
+    for (int base = 0; base < n_seqs; base += 32) {
+        const int s = base + lane;
+        int count = 0;
+        if (s < n_seqs) {
+            const int n = cu_seqlens[s + 1] - cu_seqlens[s], start = start_pos[s];
+            if (n > 0) count = (start + n - 1) / unit - start / unit + 1;
+        }
+        int sum = count;
+#pragma unroll
+        for (int w = 1; w < 32; w *= 2) {
+            const int below = __shfl_up_sync(0xffffffffu, sum, w);
+            if (lane >= w) sum += below;
+        }
+        const int total = __shfl_sync(0xffffffffu, sum, 31);
+        if (at < total) {
+            const int of = __ffs(__ballot_sync(0xffffffffu, at < sum)) - 1;
+            from_last = at - __shfl_sync(0xffffffffu, sum - count, of);
+            return base + of;
+        }
+        at -= total;
+    }
+    from_last = 0;
+    return -1;
+}
+// the most that sequences with n_tokens together touch
+static inline long long most_blocks(long long n_tokens, long long n_seqs, int unit) { return (n_tokens + n_seqs * (unit - 2)) / unit + n_seqs; }
+
 // sixteen bytes of T, as floats
 template <typename T> struct Vec { static constexpr int n = 16 / sizeof(T); };
 __device__ __forceinline__ void load_vec(const float* p, float* o) {
@@ -107,7 +140,7 @@ struct AppendArgs {
     signed char* pool;           // [pages][n_kv][line_bytes]
     void* tail;                  // [slots][2][n_kv][64][hd]
     void* old;                   // [n_seqs][2][n_kv][64][hd], or null when every sequence brings one token
-    int n_heads, n_kv, hd, n_pages;
+    int n_heads, n_kv, hd, n_pages, n_seqs;
 };
 
 __device__ __forceinline__ float2 turn_of(const AppendArgs& a, int pos, int pair) {
@@ -286,11 +319,12 @@ __global__ void __launch_bounds__(kAppendThreads) append_prompt_kernel(const App
     float* red = reinterpret_cast<float*>(rows + kPage * ld);
     pdl_launch_dependents();
     pdl_wait();
-    const int seq = blockIdx.z, head = blockIdx.y, tok0 = a.cu_seqlens[seq], n = a.cu_seqlens[seq + 1] - tok0;
-    if (n <= 0) return;
+    int from_last;
+    const int seq = find_block(a.cu_seqlens, a.start_pos, a.n_seqs, kPage, (int)blockIdx.x, from_last), head = blockIdx.y;
+    if (seq < 0) return;
+    const int tok0 = a.cu_seqlens[seq], n = a.cu_seqlens[seq + 1] - tok0;
     const int start = a.start_pos[seq], end = start + n, first = start / kPage, last = (end - 1) / kPage;
-    int b = first + (int)blockIdx.x;
-    if (b > last) return;
+    int b = last - from_last;
     const bool query = head < a.n_heads, value = head >= a.n_heads + a.n_kv;
     const bool last_open = end % kPage != 0;
     if (!query && b > first && b == last && last_open) return;         // the block x = 0 has it
@@ -406,7 +440,7 @@ __device__ __forceinline__ unsigned take_two(float& x, float& y) {
 }
 
 template <typename T, int NL>
-__global__ void __launch_bounds__(kTileThreads, NL == 1 ? 3 : 1) attend_tile_kernel(const AttendArgs a, int hb, int ranks) {
+__global__ void __launch_bounds__(kTileThreads, NL == 1 ? 3 : 1) attend_tile_kernel(const AttendArgs a, int hb, int ranks, int single) {
     constexpr int PIECES = Tile<T>::kPieces;
     extern __shared__ __align__(16) unsigned char tile_shared[];
     __shared__ unsigned odd_keys[2];                     // bits: keys of the own block whose values hold an infinity or a NaN
@@ -416,12 +450,16 @@ __global__ void __launch_bounds__(kTileThreads, NL == 1 ? 3 : 1) attend_tile_ker
     __nv_bfloat16* page = q + (size_t)PIECES * kTileRows * row_of;               // [slots][64 keys][hd + 8]
     float* met = reinterpret_cast<float*>(tile_shared);                          // [2 halves][32 rows][hd + 4], at the end
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = a.n_heads / a.n_kv, per_kv = group / hb, tb = kTileRows / hb;
-    const int rank = blockIdx.x % ranks, heads = blockIdx.x / ranks, kvh = heads / per_kv, head0 = kvh * group + heads % per_kv * hb, seq = blockIdx.z;
+    const int n_groups = a.n_kv * per_kv, rank = blockIdx.x % ranks, heads = blockIdx.x / ranks % n_groups, at = blockIdx.x / ranks / n_groups;
+    const int kvh = heads / per_kv, head0 = kvh * group + heads % per_kv * hb;
     pdl_wait();
     pdl_launch_dependents();
+    int from_last = 0;
+    const int seq = single ? at : find_block(a.cu_seqlens, a.start_pos, a.n_seqs, tb, at, from_last);
+    if (seq < 0) return;                                 // (the whole cluster)
     const int tok0 = a.cu_seqlens[seq], n = a.cu_seqlens[seq + 1] - tok0, start = a.start_pos[seq], slot = a.slot_of_seq[seq], end = start + n;
-    const int tile = (end - 1) / tb - (int)blockIdx.y;   // (the tiles that walk furthest begin first)
-    if (n <= 0 || tile < start / tb) return;             // (the whole cluster)
+    if (n <= 0) return;
+    const int tile = (end - 1) / tb - from_last;
     const int t0 = tile * tb, mine = t0 / kPage, p0 = mine * kPage, width = a.n_heads + 2 * a.n_kv;
     auto first_key = [&](int pos) { return a.window > 0 ? max(0, pos + 1 - a.window) : 0; };
     const int pg_lo = first_key(max(start, t0)) / kPage;
@@ -716,10 +754,11 @@ static int launch_tile(const AttendArgs& a, int n_tokens, int max_q_len, int max
     int pages = (max_kv_len + kPage - 1) / kPage, ranks = 1;
     if (a.window > 0 && pages > a.window / kPage + 2) pages = a.window / kPage + 2;
     while (ranks < 8 && (long long)tiles * ranks * 2 <= at_once && pages >= 2 * ranks) ranks *= 2;
-    const dim3 grid(a.n_kv * (group / hb) * ranks, (max_q_len + tb - 2) / tb + 1, a.n_seqs);
+    const long long blocks = (long long)a.n_kv * (group / hb) * ranks * (max_q_len <= 1 ? a.n_seqs : most_blocks(n_tokens, a.n_seqs, tb));
+    BLM_REQUIRE(blocks < 1ll << 31, "attention_q8: %d tokens of %d heads in one step", n_tokens, a.n_heads);
     if (cudaFuncSetAttribute(attend_tile_kernel<T, NL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return blm_fail(BLM_CUDA_ERROR, "attention_q8: %s", cudaGetErrorString(cudaGetLastError()));
-    blm_launch_cluster(attend_tile_kernel<T, NL>, ranks, grid, dim3(kTileThreads), smem, stream, a, hb, ranks);
+    blm_launch_cluster(attend_tile_kernel<T, NL>, ranks, dim3((unsigned)blocks), dim3(kTileThreads), smem, stream, a, hb, ranks, max_q_len <= 1);
     return blm_check_launch("attention_q8");
 }
 template <typename T>
@@ -1361,8 +1400,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(o_done + 1);
     unsigned* odd_values = tmem_slot + 1;                                    // [2] bits: keys of the own block whose values hold an infinity or a NaN
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int ranks = pa.ranks, rank = blockIdx.x % ranks, kv_group = blockIdx.x / ranks;
-    const int kvh = kv_group / pa.head_groups, hg = kv_group % pa.head_groups, seq = blockIdx.z;
+    const int ranks = pa.ranks, rank = blockIdx.x % ranks, n_groups = a.n_kv * pa.head_groups, kv_group = blockIdx.x / ranks % n_groups;
+    const int kvh = kv_group / pa.head_groups, hg = kv_group % pa.head_groups;
     const int group = a.n_heads / a.n_kv, head0 = kvh * group + hg * pa.heads_a_group;
     const int G = min(pa.heads_a_group, group - hg * pa.heads_a_group), tiles = (G + 1) / 2;
     if (threadIdx.x == 0) {
@@ -1385,10 +1424,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     }
     if (warp == 12) tc5::tmem_alloc(tmem_slot, 512);      // (while the kernel before ends)
     pdl_wait();
+    int from_last;
+    const int found = find_block(a.cu_seqlens, a.start_pos, a.n_seqs, kPage, blockIdx.x / ranks / n_groups, from_last), seq = max(found, 0);
+    const bool none_here = found < 0;                    // (the whole cluster)
     const int tok0 = a.cu_seqlens[seq], n = a.cu_seqlens[seq + 1] - tok0, start = a.start_pos[seq], slot = a.slot_of_seq[seq], end = start + n;
-    // the sequence's last blocks, which walk furthest, begin first
-    const int mine = (end - 1) / kPage - (int)blockIdx.y;
-    const bool none_here = n <= 0 || mine < start / kPage;                       // (the whole cluster)
+    const int mine = (end - 1) / kPage - from_last;
     const int p0 = mine * kPage;
     auto first_key = [&](int pos) { return a.window > 0 ? max(0, pos + 1 - a.window) : 0; };
     // this block's share of the walk (some may have none); the last step of the last is the own block
@@ -1859,7 +1899,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
 
 // `touched` 64-position blocks of all sequences, the longest walk of so many `pages`.
 template <int HD>
-static int launch_prompt(PromptArgs pa, int max_q_len, long long touched, int pages, cudaStream_t stream) {
+static int launch_prompt(PromptArgs pa, int n_tokens, long long touched, int pages, cudaStream_t stream) {
     static int resident[64][4] = {};                     // clusters of 1, 2, 4 and 8 blocks that the device holds at once
     int dev = 0;
     cudaGetDevice(&dev);
@@ -1897,13 +1937,14 @@ static int launch_prompt(PromptArgs pa, int max_q_len, long long touched, int pa
         const long long length = (walks + resident[dev][i] - 1) / resident[dev][i] * ((pages + (1 << i) - 1 >> i) + 11);
         if (length < best) { best = length; pa.ranks = 1 << i; }
     }
-    const dim3 grid(pa.a.n_kv * pa.head_groups * pa.ranks, (max_q_len + kPage - 2) / kPage + 1, pa.a.n_seqs);
-    blm_launch_cluster(attend_prompt_kernel<HD>, pa.ranks, grid, dim3(kPromptThreads), Prompt<HD>::kSmem, stream, pa);
+    const long long blocks = (long long)pa.a.n_kv * pa.head_groups * pa.ranks * most_blocks(n_tokens, pa.a.n_seqs, kPage);
+    BLM_REQUIRE(blocks < 1ll << 31, "attention_q8: %d tokens of %d heads in one step", n_tokens, pa.a.n_heads);
+    blm_launch_cluster(attend_prompt_kernel<HD>, pa.ranks, dim3((unsigned)blocks), dim3(kPromptThreads), Prompt<HD>::kSmem, stream, pa);
     return blm_check_launch("attention_q8");
 }
 
 template <typename T, bool VEC>
-static int launch_append(const AppendArgs& a, int n_seqs, int max_q_len, cudaStream_t stream) {
+static int launch_append(const AppendArgs& a, int n_tokens, int n_seqs, int max_q_len, cudaStream_t stream) {
     const size_t smem = (size_t)kPage * (a.hd + 16 / sizeof(T)) * sizeof(T) + kAppendThreads / 32 * sizeof(float);
     const void* kernel = max_q_len == 1 ? (const void*)append_token_kernel<T, VEC> : (const void*)append_prompt_kernel<T, VEC>;
     if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
@@ -1911,8 +1952,7 @@ static int launch_append(const AppendArgs& a, int n_seqs, int max_q_len, cudaStr
     if (max_q_len == 1) {
         blm_launch_dependent(append_token_kernel<T, VEC>, dim3(a.n_kv, n_seqs, 2), dim3(kAppendThreads), smem, stream, a);
     } else {
-        // a run of max_q_len tokens touches this many blocks at most, wherever it begins
-        const dim3 grid((max_q_len + kPage - 2) / kPage + 1, a.n_heads + 2 * a.n_kv, n_seqs);
+        const dim3 grid((unsigned)most_blocks(n_tokens, n_seqs, kPage), a.n_heads + 2 * a.n_kv);
         blm_launch_dependent(append_prompt_kernel<T, VEC>, grid, dim3(kAppendThreads), smem, stream, a);
     }
     return blm_check_launch("rope_append_q8");
@@ -1921,7 +1961,7 @@ static int launch_append(const AppendArgs& a, int n_seqs, int max_q_len, cudaStr
 
 BLM_API int blm_rope_append_q8(const void* qkv, void* out, int dtype, const int* cu_seqlens, const int* slot_of_seq, const int* start_pos,
                                const int* block_table, int table_stride, const double* inv_freq, int rot, int pairing, const float* table,
-                               int table_len, float turn_scale, void* pool, void* tail, void* old, int n_seqs, int max_q_len,
+                               int table_len, float turn_scale, void* pool, void* tail, void* old, int n_tokens, int n_seqs, int max_q_len,
                                int n_heads, int n_kv, int hd, int n_pages, cudaStream_t stream) {
     using namespace q8;
     if (n_seqs == 0 || max_q_len == 0) return BLM_OK;
@@ -1933,10 +1973,10 @@ BLM_API int blm_rope_append_q8(const void* qkv, void* out, int dtype, const int*
     BLM_REQUIRE(n_seqs <= 65535 && n_heads + 2 * n_kv <= 65535, "rope_append_q8: %d sequences, %d heads (at most 65535 of either)", n_seqs, n_heads + 2 * n_kv);
     BLM_REQUIRE(dtype == BLM_F32 || dtype == BLM_BF16, "rope_append_q8: dtype %d", dtype);
     const AppendArgs a{qkv, out, cu_seqlens, slot_of_seq, start_pos, block_table, table_stride, inv_freq, (const float2*)table, table ? table_len : 0,
-                       turn_scale, rot, pairing, (signed char*)pool, tail, old, n_heads, n_kv, hd, n_pages};
+                       turn_scale, rot, pairing, (signed char*)pool, tail, old, n_heads, n_kv, hd, n_pages, n_seqs};
     const bool vec = rot % 16 == 0;
-    if (dtype == BLM_F32) return vec ? launch_append<float, true>(a, n_seqs, max_q_len, stream) : launch_append<float, false>(a, n_seqs, max_q_len, stream);
-    return vec ? launch_append<__nv_bfloat16, true>(a, n_seqs, max_q_len, stream) : launch_append<__nv_bfloat16, false>(a, n_seqs, max_q_len, stream);
+    if (dtype == BLM_F32) return vec ? launch_append<float, true>(a, n_tokens, n_seqs, max_q_len, stream) : launch_append<float, false>(a, n_tokens, n_seqs, max_q_len, stream);
+    return vec ? launch_append<__nv_bfloat16, true>(a, n_tokens, n_seqs, max_q_len, stream) : launch_append<__nv_bfloat16, false>(a, n_tokens, n_seqs, max_q_len, stream);
 }
 
 BLM_API int blm_q8_values(const void* pool, const int* pages, void* out, int dtype, int n, int n_kv, int hd, int n_pages, cudaStream_t stream) {
@@ -1979,7 +2019,7 @@ BLM_API int blm_attention_q8(const void* rotated, const void* pool, const void* 
         if (hd == 64) return launch_tokens_as<64, 1>(ta, stream);
         return p.wpp == 1 ? launch_tokens_as<128, 1>(ta, stream) : launch_tokens_as<128, 2>(ta, stream);
     }
-    if (dtype == BLM_BF16 && (hd == 64 || hd == 128) && max_q_len > 1 && n_seqs <= 65535 && max_q_len <= 4000000) {
+    if (dtype == BLM_BF16 && (hd == 64 || hd == 128) && max_q_len > 1) {
         const int group = n_heads / n_kv, groups = (group + 3) / 4;
         int pages = (max_kv_len + kPage - 1) / kPage;
         if (window > 0 && pages > window / kPage + 2) pages = window / kPage + 2;
@@ -1987,9 +2027,8 @@ BLM_API int blm_attention_q8(const void* rotated, const void* pool, const void* 
         const int from = max_kv_len > max_q_len ? max_kv_len - max_q_len : 0;
         const long long touched = n_seqs == 1 ? (from + n_tokens - 1) / kPage - from / kPage + 1 : (n_tokens + 63ll * n_seqs + 63) / kPage;
         const PromptArgs pa{a, groups, (group + groups - 1) / groups, 1, status};
-        return hd == 64 ? launch_prompt<64>(pa, max_q_len, touched, pages, stream) : launch_prompt<128>(pa, max_q_len, touched, pages, stream);
+        return hd == 64 ? launch_prompt<64>(pa, n_tokens, touched, pages, stream) : launch_prompt<128>(pa, n_tokens, touched, pages, stream);
     }
-    BLM_REQUIRE(n_seqs <= 65535 && max_q_len <= 500000, "attention_q8: %d sequences (at most 65535), %d tokens (at most 500000)", n_seqs, max_q_len);
     if (dtype == BLM_F32) return launch_tile<float>(a, n_tokens, max_q_len, max_kv_len, stream);
     if (dtype == BLM_BF16) return launch_tile<__nv_bfloat16>(a, n_tokens, max_q_len, max_kv_len, stream);
     return blm_fail(BLM_BAD_ARGUMENT, "attention_q8: dtype %d", dtype);

@@ -201,7 +201,7 @@ _protos = {
     },
     "attention_q8": {
         "blm_rope_append_q8": [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p,
-                               c_int, c_float, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
+                               c_int, c_float, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
         "blm_q8_values": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
         "blm_attention_q8": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                              c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
@@ -2160,7 +2160,7 @@ def rope_append_q8(qkv, out, step, pool, scales, tail, block_table, inv_freq, ro
         "rope_append_q8", (qkv, out, pool, tail, table, old), (block_table, inv_freq if rotary_dim else None))
     p_cu, p_slot, p_start = _step_ptrs("rope_append_q8", step)
     _call("attention_q8", "blm_rope_append_q8", p_qkv, p_out, _code(dtype), p_cu, p_slot, p_start, p_block, block_table.shape[1], p_freq,
-          rotary_dim, int(pairs), p_table, places, turn_scale, p_pool, p_tail, p_old, step.n_seqs,
+          rotary_dim, int(pairs), p_table, places, turn_scale, p_pool, p_tail, p_old, shape[0], step.n_seqs,
           step.max_q_len, n_heads, n_kv, head_dim, pool.shape[0], _stream())
     return old
 
@@ -2174,7 +2174,7 @@ def attention_q8(rotated, step, pool, scales, tail, old, block_table, out, n_hea
     rotated's dtype.  Rows of no sequence are left as they are.  In bfloat16 the probabilities, times the values' scale, are
     rounded to bfloat16 (single tokens with heads of 64 or 128 lanes: to half precision); float32 steps keep 32 bits.  A sequence's pages may
     be cut over several blocks: step.max_kv_len (the longest sequence after the step, or a bound) sizes that, step.workspace lends the
-    scratch that single tokens need for it.  At most 65,535 sequences and 500,000 tokens of one a step."""
+    scratch that single tokens need for it."""
     shape, dtype = rotated.shape, rotated.dtype
     n = shape[0]
     if len(shape) != 2 or shape[1] != (n_heads + 2 * n_kv) * head_dim or out.shape != (n, n_heads * head_dim) or out.dtype is not dtype:

@@ -598,3 +598,13 @@ def test_the_largest_floats(which):
     assert torch.equal(outs[0][:70], outs[1][:70]) and torch.isfinite(outs[1][:70]).all()
     if which == 1:
         assert torch.isfinite(outs[1][70:]).all() and (outs[1][70:, :, 5] > 1e30).all()
+
+
+@pytest.mark.parametrize("heads,n_kv,dim,dtype", [(8, 2, 128, BF16), (4, 2, 80, BF16), (4, 1, 64, F32)])
+def test_a_prompt_beside_many_single_tokens(heads, n_kv, dim, dtype):
+    """More than 32 sequences of very unequal lengths in one step, some of them empty, the long one in the middle."""
+    b = Batch(40, heads, n_kv, dim, dtype, 300, seed=dim)
+    b.append([(s, 1 + 7 * s % 90) for s in range(40)], check=False)
+    entries = [(s, 150 if s == 37 else 2 if s == 3 else 65 if s == 20 else 1) for s in range(40) if s % 5 != 4]
+    b.go(entries, padding=3)
+    K().check_status(torch.device("cuda:0"))
