@@ -1425,10 +1425,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     if (warp == 12) tc5::tmem_alloc(tmem_slot, 512);      // (while the kernel before ends)
     pdl_wait();
     int from_last;
-    const int found = find_block(a.cu_seqlens, a.start_pos, a.n_seqs, kPage, blockIdx.x / ranks / n_groups, from_last), seq = max(found, 0);
+    const int found = find_block(a.cu_seqlens, a.start_pos, a.n_seqs, kPage, blockIdx.x / ranks / n_groups, from_last);
     const bool none_here = found < 0;                    // (the whole cluster)
-    const int tok0 = a.cu_seqlens[seq], n = a.cu_seqlens[seq + 1] - tok0, start = a.start_pos[seq], slot = a.slot_of_seq[seq], end = start + n;
-    const int mine = (end - 1) / kPage - from_last;
+    auto one = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };               // (one number for a warp: it need not have a register in each thread)
+    const int seq = one(max(found, 0)), tok0 = one(a.cu_seqlens[seq]), start = one(a.start_pos[seq]), slot = one(a.slot_of_seq[seq]);
+    const int end = start + one(a.cu_seqlens[seq + 1]) - tok0, mine = (end - 1) / kPage - one(from_last);
     const int p0 = mine * kPage;
     auto first_key = [&](int pos) { return a.window > 0 ? max(0, pos + 1 - a.window) : 0; };
     // this block's share of the walk (some may have none); the last step of the last is the own block
