@@ -61,6 +61,11 @@ __device__ __forceinline__ unsigned pack_bf16(float a, float b) {
 // beside 63 single ones was 287 us of attention, most of it blocks that had nothing to do.)
 __device__ __forceinline__ int find_block(const int* cu_seqlens, const int* start_pos, int n_seqs, int unit, int at, int& from_last) {
     const int lane = threadIdx.x & 31;
+    if (n_seqs == 1) {                                   // (a quarter of a microsecond sooner)
+        const int n = cu_seqlens[1] - cu_seqlens[0], start = start_pos[0];
+        from_last = at;
+        return n > 0 && at <= (start + n - 1) / unit - start / unit ? 0 : -1;
+    }
     for (int base = 0; base < n_seqs; base += 32) {
         const int s = base + lane;
         int count = 0;
