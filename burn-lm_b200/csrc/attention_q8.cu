@@ -789,10 +789,10 @@ static int launch_tile(const AttendArgs& a, int n_tokens, int max_q_len, int max
 //   * the values' scale rides in the exponent: p' = 2^(score + log2 vs - m), with the maximum m taken of that sum, is at most 1, its
 //     product with the whole numbers needs no scale, and the sum of the probabilities gets p' / vs.  p' is rounded to half precision
 //     times 2^12 (11 bits from the largest down to 2^-26 of it).
-// Warps keep their own running maximum, sum and output and merge at the end; up to eight shares of a sequence meet in their cluster, more in a
-// second kernel.  The own
-// block's keys, unrounded, are read straight from the tail and the step's rows by the four warps of the last share, in bfloat16,
-// while the first pages are on their way.  Waits are bounded; one that runs out leaves a code in the status word.
+// Warps keep their own running maximum, sum and output and merge at the end; up to eight shares of a sequence meet in their cluster, more
+// in a second kernel.  The own block's keys, unrounded, are read straight from the tail and the step's rows by the four warps of the last
+// share, while the first pages are on their way; their probabilities are bfloat16 numbers 2^(score - m), as large as 2^112 where a key's
+// values are small.  Waits are bounded; one that runs out leaves a code in the status word.
 struct TokenArgs {
     AttendArgs a;
     float* part_acc;             // [N, n_heads, n_splits, hd]
@@ -1010,40 +1010,71 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
             const bool seen0 = k0 <= own_hi && k0 >= own_lo, seen2 = k0 + 2 <= own_hi && k0 + 2 >= own_lo;
             const uint4* r0 = reinterpret_cast<const uint4*>(row(min(k0, own_hi), 0) + t * (HD / 4));
             const uint4* r2 = reinterpret_cast<const uint4*>(row(min(k0 + 2, own_hi), 0) + t * (HD / 4));
+            // all loads before the first use: one latency
+            uint4 k_of[2][KS / 2], v[HD / 64][4];        // (v: lanes g HD / 8 .. + HD / 8 of keys 4 t .. 4 t + 3)
+#pragma unroll
+            for (int j = 0; j < KS / 2; ++j) {
+                k_of[0][j] = r0[j];
+                k_of[1][j] = r2[j];
+            }
+            bool sees[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int key = quarter * 16 + 4 * t + e;
+                sees[e] = key <= own_hi && key >= own_lo;
+                const uint4* from = reinterpret_cast<const uint4*>(row(min(key, own_hi), 1) + g * (HD / 8));
+#pragma unroll
+                for (int j = 0; j < HD / 64; ++j) v[j][e] = from[j];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int j = 0; j < HD / 64; ++j)
+                    if (!sees[e]) v[j][e] = make_uint4(0u, 0u, 0u, 0u);
             float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < KS / 2; ++j) {
-                const uint4 x = seen0 ? r0[j] : make_uint4(0u, 0u, 0u, 0u), y = seen2 ? r2[j] : make_uint4(0u, 0u, 0u, 0u);
+                const uint4 x = seen0 ? k_of[0][j] : make_uint4(0u, 0u, 0u, 0u), y = seen2 ? k_of[1][j] : make_uint4(0u, 0u, 0u, 0u);
                 mma_sync<false>(c, x.x, y.x, x.y, y.y, qf[2 * j][0], qf[2 * j][1]);
                 mma_sync<false>(c, x.z, y.z, x.w, y.w, qf[2 * j + 1][0], qf[2 * j + 1][1]);
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) c[e] = (e < 2 ? seen0 : seen2) ? c[e] * a.scale_log2e : -INFINITY;
+            // what a key's values weigh, as log2 of 2^-7 of the largest magnitude among them: the reference is one of score times value here
+            // too, so that neither these rows nor the pages leave the range of the pages' half precision (with the scores alone, values of 1e-8
+            // behind pages were off by a tenth).  Two keys a word, their magnitudes' bits.
+            unsigned size[2] = {0u, 0u};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                unsigned top = 0;                        // of two magnitudes' bits at once
+#pragma unroll
+                for (int j = 0; j < HD / 64; ++j)
+                    top = __vmaxu2(__vmaxu2(top, v[j][e].x & 0x7fff7fffu), __vmaxu2(__vmaxu2(v[j][e].y & 0x7fff7fffu, v[j][e].z & 0x7fff7fffu), v[j][e].w & 0x7fff7fffu));
+                size[e >> 1] |= max(top & 0xffffu, top >> 16) << (16 * (e & 1));
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+#pragma unroll
+                for (int x = 4; x < 32; x *= 2) size[w] = __vmaxu2(size[w], __shfl_xor_sync(0xffffffffu, size[w], x));
+                size[w] = __shfl_sync(0xffffffffu, size[w], g >> 1) >> (16 * (g & 1)) & 0xffffu;      // of keys k0 and k0 + 2
+            }
+            const float lv0 = (float)max((int)(size[0] >> 7) - 134, -100), lv2 = (float)max((int)(size[1] >> 7) - 134, -100);
             float shift0, shift1;
-            st.refer(fmaxf(c[0], c[2]), fmaxf(c[1], c[3]), shift0, shift1);
+            st.refer(fmaxf(c[0] + lv0, c[2] + lv2), fmaxf(c[1] + lv0, c[3] + lv2), shift0, shift1);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 c[e] = ex2(c[e] + (e & 1 ? shift1 : shift0));
                 st.l[e & 1] += c[e];
             }
             const unsigned b0 = transposed(pack_bf16(c[0], c[1])), b1 = transposed(pack_bf16(c[2], c[3]));
-            // lanes g HD / 8 .. + HD / 8 of keys 4 t .. 4 t + 3
 #pragma unroll
-            for (int j = 0; j < HD / 64; ++j) {
-                uint4 v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int key = quarter * 16 + 4 * t + e;
-                    const bool seen = key <= own_hi && key >= own_lo;
-                    v[e] = seen ? reinterpret_cast<const uint4*>(row(min(key, own_hi), 1) + g * (HD / 8))[j] : make_uint4(0u, 0u, 0u, 0u);
-                }
+            for (int j = 0; j < HD / 64; ++j)
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
-                    const unsigned w0 = n == 0 ? v[0].x : n == 1 ? v[0].y : n == 2 ? v[0].z : v[0].w, w1 = n == 0 ? v[1].x : n == 1 ? v[1].y : n == 2 ? v[1].z : v[1].w;
-                    const unsigned w2 = n == 0 ? v[2].x : n == 1 ? v[2].y : n == 2 ? v[2].z : v[2].w, w3 = n == 0 ? v[3].x : n == 1 ? v[3].y : n == 2 ? v[3].z : v[3].w;
+                    auto word = [&](const uint4& u) { return n == 0 ? u.x : n == 1 ? u.y : n == 2 ? u.z : u.w; };
+                    const unsigned w0 = word(v[j][0]), w1 = word(v[j][1]), w2 = word(v[j][2]), w3 = word(v[j][3]);
                     mma_sync<false>(st.o[4 * j + n], __byte_perm(w0, w1, 0x5410), __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x5410), __byte_perm(w2, w3, 0x7632), b0, b1);
                 }
-            }
         }
 
         // the queries in half precision: times a power of two that brings the row's largest lane to 16 .. 32

@@ -1,0 +1,47 @@
+"""Attention over a cache line in 8 bits where its numbers are far from 1, or none."""
+import pytest
+import torch
+
+from test_gpu_q8 import BF16, Batch
+
+pytestmark = pytest.mark.gpu
+
+
+def sized(b, n, size):
+    """Rows of a step whose values are about `size`."""
+    x = b.rows(n).view(n, -1, b.dim)
+    x[:, b.heads + b.n_kv:] *= size
+    return x.view(n, -1)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("pages,own", [(1e-20, 1e-20), (1e-8, 1e-8), (1e8, 1e8), (1e20, 1e20), (1e30, 1e30), (1.0, 1e-8), (1e-8, 1.0), (0.0, 1.0), (1.0, 0.0)])
+def test_single_tokens_with_values_of_any_size(pages, own, dim):
+    """The rows of the own block and the pages weigh what they are worth, whatever the size of either's values."""
+    b = Batch(3, 16, 2, dim, BF16, 768, seed=dim)
+    b.append([(0, 576), (1, 300), (2, 64)], qkv=sized(b, 940, pages), check=False)
+    b.append([(0, 20), (1, 2), (2, 40)], qkv=sized(b, 62, own), check=False)
+    for _ in range(2):
+        step, out, old = b.append([(0, 1), (1, 1), (2, 1)], qkv=sized(b, 3, own), check=False)
+        b.attend([(0, 1), (1, 1), (2, 1)], step, out, old)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("times", [1.0, 2.5, 12.0])
+@pytest.mark.parametrize("single", [True, False])
+def test_a_tall_key_without_a_value(dim, times, single):
+    """A key of the own block far above all others, whose value is zero: what is left is the others', however small."""
+    heads, n_kv = 8, 2
+    b = Batch(1, heads, n_kv, dim, BF16, 700, seed=3)
+    b.append([(0, 576)], rot=0, check=False)
+    query = b.rows(1)
+    tall = b.rows(5)
+    rows = tall.view(5, -1, dim)
+    rows[1, heads: heads + n_kv] = times * query.view(1, -1, dim)[0, [0, heads // n_kv]]
+    rows[1, heads + n_kv:] = 0
+    rows[1:, :heads] = query.view(1, -1, dim)[0, [0] * (heads // n_kv) + [heads // n_kv] * (heads // n_kv)]
+    b.append([(0, 5)], qkv=tall, rot=0, check=False)
+    qkv = query if single else torch.cat([query, b.rows(2)])
+    qkv.view(len(qkv), -1, dim)[0, :heads] = rows[1, :heads]
+    step, out, old = b.append([(0, len(qkv))], qkv=qkv, rot=0, check=False)
+    b.attend([(0, len(qkv))], step, out, old)
