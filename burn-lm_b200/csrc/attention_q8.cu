@@ -1127,7 +1127,9 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
             const float2 scale = *scales_of(keys, HD);
             // (a block whose values are all next to zero: any scale will do; a NaN stays one)
             const float vs = scale.y < 0x1p-100f ? 0x1p-100f : scale.y, lv = __log2f(vs);
-            const float f0 = to_log2_0 * scale.x, f1 = to_log2_1 * scale.x;
+            // (a block of keys with an infinity: its numbers are zeros, whose score's sum need not come out as exactly 0 here; times an infinity it
+            // must be none all the same, not minus infinity)
+            const float ks = fmaf(scale.x, 0.f, scale.x), f0 = to_log2_0 * ks, f1 = to_log2_1 * ks;
             float sc[CH][4], top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
             for (int ch = 0; ch < CH; ++ch) {

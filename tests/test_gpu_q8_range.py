@@ -45,3 +45,19 @@ def test_a_tall_key_without_a_value(dim, times, single):
     qkv.view(len(qkv), -1, dim)[0, :heads] = rows[1, :heads]
     step, out, old = b.append([(0, len(qkv))], qkv=qkv, rot=0, check=False)
     b.attend([(0, len(qkv))], step, out, old)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 80])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_a_cached_key_that_is_none(dim, bad):
+    """A complete block with an infinite key reads as no number to every head of its kv head, and the other kv head is untouched."""
+    outs = []
+    for with_it in (False, True):
+        b = Batch(8, 32, 2, dim, BF16, 400, seed=1)
+        rows = b.rows(8 * 330)
+        if with_it:
+            rows.view(8, 330, -1, dim)[:, 100, 32, 3] = bad
+        b.append([(s, 330) for s in range(8)], qkv=rows, rot=0, check=False)
+        step, out, old = b.append([(s, 1) for s in range(8)], rot=0, check=False)
+        outs.append(b.attend([(s, 1) for s in range(8)], step, out, old, check=False).view(8, 2, 16, dim))
+    assert torch.isnan(outs[1][:, 0]).all() and torch.equal(outs[1][:, 1], outs[0][:, 1])
