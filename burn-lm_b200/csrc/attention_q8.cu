@@ -1378,8 +1378,10 @@ static bool tokens_take(int dtype, int hd, int max_q_len, int n_seqs, int n_kv, 
 //   warp 12 issues S = Q K^T and O += P V of both tiles.  Q lies in tensor memory (as a second operand in shared memory its
 //     reads, 32 KB a page and tile, would cost more than the products);
 //   warps 0 .. 7 are the softmax, a row a thread: Q times a power of two that brings the row's largest lane to 2^60 (the keys' 2^-133 has to
-//     meet ordinary numbers), scores times the keys' scale, a reference maximum that moves when a score exceeds it by 2^8, probabilities
-//     times the values' scale times 2^60, rounded to bfloat16, over the scores' columns.
+//     meet ordinary numbers), scores times the keys' scale, a reference maximum m of score + log2 vs (vs: the values' scale; 2^-21 of the own
+//     block) that moves when one exceeds it by 2^8, probabilities 2^(score + log2 vs - m + 112), of the own block 2^(score - 21 - m), rounded
+//     to bfloat16, over the scores' columns.  So they stay below 2^121 whatever the values' size, and their products with values of about
+//     1e-20 to 1e28 above 2^-126 down to probabilities of 2^-20.
 // A tile's scores of the next page are issued behind its product of this one, by the same warp, so one set of columns does.  Measured, a
 // page takes 2,200 cycles: a tile's softmax 1,400 (max, exponent and sum in pairs) and its product and next scores 730, one after the
 // other, the two tiles half a page apart; products alone would take 1,024, exponentials as much.  (Two sets of columns for the scores, with
@@ -1617,11 +1619,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                 }
             }
             if (me == 0) {
-                // Scores are multiplied by the first number (times the row's own).  Probabilities leave times 2^ the third, the values' scale
-                // times 2^60 (the own block's: 2^-73), and their sum times the fourth takes it off again.  (A block whose values are all next
-                // to zero: any scale will do.)  The second is below zero for a page that is none.
+                // Scores are multiplied by the first number (times the row's own).  The third is the log2 of the values' scale, which the reference
+                // is taken with; of the own block, whose values have none and whose probabilities leave 2^133 smaller, -21, so that they stay
+                // below 2^8 and that the block seldom moves the reference (0 for it: 2,048 tokens 49.5 us instead of 49.0).  Their sum, the
+                // pages' times 2^-112, counts the fourth times, in units of 2^10.  (A block whose values are all next to zero: any scale will
+                // do.)  The second is below zero for a page that is none.
                 const float vs = scale.y < 0x1p-100f ? 0x1p-100f : scale.y;
-                scales[j & 3] = own ? make_float4(0x1p-67f, 1.f, -73.f, 0x1p73f) : make_float4(0x1p66f * scale.x, scale.y, __log2f(vs) + 60.f, 0x1p-60f / vs);
+                scales[j & 3] = own ? make_float4(0x1p-67f, 1.f, -21.f, 0x1p11f) : make_float4(0x1p66f * scale.x, scale.y, __log2f(vs), 0x1p-10f / vs);
             }
             tc5::fence_async_smem();
             __syncwarp();
@@ -1741,7 +1745,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             const bool own = j == own_step;
             const int key0 = (pg_lo + j) * kPage;
             const float4 scale = scales[j & 3];
-            float f = to_log2 * scale.x, shift = scale.z, to_sum = scale.w;
+            float f = to_log2 * scale.x, lv = scale.z, to_sum = scale.w;
             float x[64];
 #pragma unroll
             for (int c = 0; c < 64; c += 16) tc5::tmem_ld16(at + c, x + c);
@@ -1755,7 +1759,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                 if (f == 0.f) f = 0x1p-126f;             // (keys of zeros: a hidden one's score stays minus infinity)
                 if (from > 63) {                         // of a page that the row sees nothing of, whatever its scales
                     f = 0x1p-126f;
-                    shift = to_sum = 0.f;
+                    lv = to_sum = 0.f;
                 }
             }
             float top[4] = {x[0], x[1], x[2], x[3]};
@@ -1765,7 +1769,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                 for (int k = 0; k < 4; ++k) top[k] = max3(top[k], x[i + k], x[i + k + 4]);
 #pragma unroll
             for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], x[60 + k]);
-            const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * f;
+            const float mx = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), f, lv);
             // (nothing seen: the product is minus infinity, or none where f is zero or none: neither moves the reference)
             const bool move = mx > m + 8.f;
             if (__any_sync(0xffffffffu, move)) {
@@ -1787,7 +1791,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                     }
                 }
             }
-            const float less = shift - (m == -INFINITY ? 0.f : m);
+            const float less = lv + (own ? 0.f : 112.f) - (m == -INFINITY ? 0.f : m);
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < 64; i += 2) {
@@ -1803,7 +1807,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                 for (int i = 0; i < 16; ++i) w[i] = pack_bf16(x[2 * (c + i)], x[2 * (c + i) + 1]);
                 tc5::tmem_st16(at + c, w);
             }
-            l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), to_sum, l);
+            l = fmaf(((sum[0] + sum[1]) + (sum[2] + sum[3])) * (own ? 1.f : 0x1p-112f), to_sum, l);
             tc5::wait_st();
             tc5::fence_before();
             __syncwarp();
@@ -1846,7 +1850,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
 #pragma unroll
                 for (int i = 0; i < 64; i += 16) tc5::tmem_ld16(at + kOCol + c * 64 + i, o + i);
                 tc5::wait_ld(o);
-                const float times = 0x1p73f * by;
+                const float times = 0x1p11f * by;                                // (units of 2^-133 2^112 over those of 2^-10)
 #pragma unroll
                 for (int g = 0; g < 8; ++g)
                     my_rows[lane * (HD / 8) + ((g * (HD / 64) + c) ^ (lane & 7))] =
@@ -1893,7 +1897,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             const float by = mk == top ? 1.f : ex2(mk - top);
             float l = lk * by;
             for (int w = 1; w < ranks; w *= 2) l += __shfl_xor_sync(0xffffffffu, l, w);
-            weights[threadIdx.x] = by * (0x1p73f / l);
+            weights[threadIdx.x] = by * (0x1p11f / l);
         }
         __syncthreads();
         for (int i = threadIdx.x; i < some * (HD / 4); i += kPromptThreads) {

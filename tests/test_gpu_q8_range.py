@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_q8 import BF16, Batch
+from test_gpu_q8 import BF16, F32, Batch, K
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +61,25 @@ def test_a_cached_key_that_is_none(dim, bad):
         step, out, old = b.append([(s, 1) for s in range(8)], rot=0, check=False)
         outs.append(b.attend([(s, 1) for s in range(8)], step, out, old, check=False).view(8, 2, 16, dim))
     assert torch.isnan(outs[1][:, 0]).all() and torch.equal(outs[1][:, 1], outs[0][:, 1])
+
+
+@pytest.mark.parametrize("heads,n_kv,dim,dtype", [(8, 2, 64, BF16), (6, 1, 128, BF16), (4, 2, 80, BF16), (4, 2, 64, F32)])
+@pytest.mark.parametrize("size", [1e-20, 1e-12, 1e-8, 1e8, 1e20, 1e25])
+def test_portions_with_values_of_any_size(heads, n_kv, dim, dtype, size):
+    """Whole prompts, and portions whose walk several blocks share."""
+    b = Batch(2, heads, n_kv, dim, dtype, 1500, seed=dim)
+    for entries in ([(0, 300), (1, 70)], [(0, 1000)], [(0, 40), (1, 5)]):
+        step, out, old = b.append(entries, qkv=sized(b, sum(n for _, n in entries), size), check=False)
+        b.attend(entries, step, out, old)
+    K().check_status(torch.device("cuda:0"))
+
+
+@pytest.mark.parametrize("heads,n_kv,dim,dtype", [(8, 2, 64, BF16), (8, 2, 128, BF16), (4, 2, 80, BF16), (4, 2, 64, F32)])
+@pytest.mark.parametrize("pages,own", [(1e-12, 1.0), (1.0, 1e-12), (1e12, 1.0), (1.0, 1e12), (0.0, 1.0), (1.0, 0.0)])
+def test_portions_with_pages_of_unlike_sizes(heads, n_kv, dim, dtype, pages, own):
+    """Pages and own block, and pages beside one another, whose values are of very different sizes."""
+    b = Batch(1, heads, n_kv, dim, dtype, 1500, seed=dim)
+    b.append([(0, 448)], qkv=sized(b, 448, pages), check=False)
+    b.append([(0, 448)], qkv=sized(b, 448, own), check=False)
+    step, out, old = b.append([(0, 90)], qkv=sized(b, 90, own), check=False)
+    b.attend([(0, 90)], step, out, old)
