@@ -448,7 +448,10 @@ template <typename T, int NL>
 __global__ void __launch_bounds__(kTileThreads, NL == 1 ? 3 : 1) attend_tile_kernel(const AttendArgs a, int hb, int ranks, int single) {
     constexpr int PIECES = Tile<T>::kPieces;
     extern __shared__ __align__(16) unsigned char tile_shared[];
-    __shared__ unsigned odd_keys[2];                     // bits: keys of the own block whose values hold an infinity or a NaN
+    // bits: keys of the own block whose values hold an infinity or a NaN; that hold one themselves (where a number is several pieces, which an
+    // infinity has not)
+    __shared__ __align__(16) unsigned odd_keys[4];
+    unsigned* odd_scores = odd_keys + 2;
     __shared__ float met_m[2][kTileRows], met_l[2][kTileRows], weights[2 * kTileRows];
     const int hd = a.hd, row_of = hd + 8;                // numbers between rows: eight rows' 16-byte pieces meet in no bank
     __nv_bfloat16* q = reinterpret_cast<__nv_bfloat16*>(tile_shared);            // [PIECES][32 rows][hd + 8]
@@ -487,7 +490,7 @@ __global__ void __launch_bounds__(kTileThreads, NL == 1 ? 3 : 1) attend_tile_ker
         for (int i = 0; i < PIECES; ++i)
             *reinterpret_cast<uint4*>(to + i * apart) = make_uint4(take_two(x[0], x[1]), take_two(x[2], x[3]), take_two(x[4], x[5]), take_two(x[6], x[7]));
     };
-    if (tid < 2) odd_keys[tid] = 0u;
+    if (tid < 4) odd_keys[tid] = 0u;
     for (int i = tid; i < kTileRows * (hd / 8); i += kTileThreads) {
         const int r = i % kTileRows, d = i / kTileRows * 8, pos = t0 + r / hb;
         float x[8] = {};
@@ -580,6 +583,16 @@ __global__ void __launch_bounds__(kTileThreads, NL == 1 ? 3 : 1) attend_tile_ker
                 const int key = c % kPage, d = c / kPage * 8;
                 float x[8] = {};
                 if (p0 + key < end) load_n<8>(own_row(p0 + key, 0) + d, x);
+                if (PIECES > 1) {
+                    unsigned top = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+                    if (top >= 0x7f800000u) {
+                        atomicOr(odd_scores + (key >> 5), 1u << (key & 31));
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = 0.f;
+                    }
+                }
                 put(page + (size_t)key * row_of + d, (size_t)kPage * row_of, x);
             }
         }
@@ -609,6 +622,13 @@ __global__ void __launch_bounds__(kTileThreads, NL == 1 ? 3 : 1) attend_tile_ker
         if (PIECES > 1)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i / 4][i % 4] += low[PIECES > 1 ? i / 4 : 0][i % 4];
+        if (PIECES > 1 && own) {                         // (left out here: at the end the rows that see such a key ask what its score is)
+            const unsigned hidden = odd_scores[half] >> (2 * t);
+            if (hidden != 0)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (hidden >> (i / 4 * 8 + (i & 1)) & 1) s[i / 4][i % 4] = -INFINITY;
+        }
         float alpha[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -706,8 +726,9 @@ __global__ void __launch_bounds__(kTileThreads, NL == 1 ? 3 : 1) attend_tile_ker
     if (ranks > 1) cluster_sync();
     else __syncthreads();
     const int parts = 2 * ranks, share = kTileRows / ranks, last = (mine - pg_lo) % ranks;       // (whose step was the own block)
-    unsigned long long odd = 0;
-    for (int w = 0; w < 2; ++w) odd |= (unsigned long long)(ranks > 1 ? __float_as_uint(cluster_float(tc5::smem_u32(odd_keys + w), last)) : odd_keys[w]) << (32 * w);
+    const float4 odd_bits = ranks > 1 ? cluster_float4(tc5::smem_u32(odd_keys), last) : *reinterpret_cast<const float4*>(odd_keys);
+    const unsigned long long odd = (unsigned long long)__float_as_uint(odd_bits.y) << 32 | __float_as_uint(odd_bits.x);
+    const unsigned long long odd_k = PIECES > 1 ? (unsigned long long)__float_as_uint(odd_bits.w) << 32 | __float_as_uint(odd_bits.z) : 0;
     if (tid < share * parts) {                           // the parts' weights, a thread each: a row's are neighbours
         const int row = rank * share + tid / parts, k = tid % parts;
         const float mk = cluster_float(tc5::smem_u32(&met_m[k & 1][row]), k >> 1), lk = cluster_float(tc5::smem_u32(&met_l[k & 1][row]), k >> 1);
@@ -731,19 +752,31 @@ __global__ void __launch_bounds__(kTileThreads, NL == 1 ? 3 : 1) attend_tile_ker
             const float by = weights[here * parts + k];
             o[0] = fmaf(v.x, by, o[0]); o[1] = fmaf(v.y, by, o[1]); o[2] = fmaf(v.z, by, o[2]); o[3] = fmaf(v.w, by, o[3]);
         }
-        const int from = first_key(pos);
         T* out = reinterpret_cast<T*>(a.out) + ((size_t)(tok0 + pos - start) * a.n_heads + head0 + row % hb) * hd + d;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (odd != 0)
-                for (int k = max(p0, from); k <= pos; ++k)
-                    if (odd >> (k - p0) & 1) {
-                        const float v = to_f32(own_row(k, 1)[d + e]);
-                        if (!(fabsf(v) < INFINITY)) o[e] += v;
-                    }
-            out[e] = from_f32<T>(o[e]);
-        }
+        for (int e = 0; e < 4; ++e) out[e] = from_f32<T>(o[e]);
     }
+    // infinities and NaN of the own block, by the rows that see them: of a value they join the result; a key's leave it only where its score is
+    // minus infinity (the thread that wrote a place looks at it again)
+    if ((odd | odd_k) != 0)
+        for (int i = tid; i < share * (hd / 4); i += kTileThreads) {
+            const int row = rank * share + i / (hd / 4), d = i % (hd / 4) * 4, pos = t0 + row / hb, head = head0 + row % hb;
+            if (pos < start || pos >= end) continue;
+            T* out = reinterpret_cast<T*>(a.out) + ((size_t)(tok0 + pos - start) * a.n_heads + head) * hd + d;
+            const T* q_row = rows + ((size_t)(tok0 + pos - start) * width + head) * hd;
+            for (int k = max(p0, first_key(pos)); k <= pos; ++k) {
+                float score = -INFINITY;
+                if (odd_k >> (k - p0) & 1) {
+                    score = 0.f;
+                    for (int x = 0; x < hd; ++x) score = fmaf(to_f32(q_row[x]) * a.scale_log2e, to_f32(own_row(k, 0)[x]), score);
+                }
+                for (int e = 0; e < 4; ++e) {
+                    const float v = to_f32(own_row(k, 1)[d + e]);
+                    if (!(score == -INFINITY)) out[e] = from_f32<T>(NAN);
+                    else if (odd >> (k - p0) & 1 && !(fabsf(v) < INFINITY)) out[e] = from_f32<T>(to_f32(out[e]) + v);
+                }
+            }
+        }
     if (ranks > 1) cluster_sync();                       // what others read stays until they have
 }
 
@@ -1621,7 +1654,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             if (me == 0) {
                 // Scores are multiplied by the first number (times the row's own).  The third is the log2 of the values' scale, which the reference
                 // is taken with; of the own block, whose values have none and whose probabilities leave 2^133 smaller, -21, so that they stay
-                // below 2^8 and that the block seldom moves the reference (0 for it: 2,048 tokens 49.5 us instead of 49.0).  Their sum, the
+                // below 2^8 and that the block seldom moves the reference (0 for it: 2,048 tokens 49.5 us instead of 48.9).  Their sum, the
                 // pages' times 2^-112, counts the fourth times, in units of 2^10.  (A block whose values are all next to zero: any scale will
                 // do.)  The second is below zero for a page that is none.
                 const float vs = scale.y < 0x1p-100f ? 0x1p-100f : scale.y;

@@ -2174,8 +2174,9 @@ def attention_q8(rotated, step, pool, scales, tail, old, block_table, out, n_hea
     rotated's dtype.  Rows of no sequence are left as they are.  In bfloat16 the probabilities, times the values' scale, are
     rounded to bfloat16 (single tokens with heads of 64 or 128 lanes: to half precision); float32 steps keep 32 bits.  Values may be as large
     as 1e28 (sums of probabilities times values are formed before they are divided) and, in bfloat16, as small as 1e-20 before their smaller
-    probabilities lose bits; keys as large as 1e18.  A sequence's pages may be cut over several blocks: step.max_kv_len (the longest sequence after the step, or a bound) sizes that, step.workspace lends the
-    scratch that single tokens need for it."""
+    probabilities lose bits; keys as large as 1e17.  An infinite key of the own block leaves the rows that see it no number, except where its
+    score is minus infinity.  A sequence's pages may be cut over several blocks: step.max_kv_len (the longest sequence after the step, or a
+    bound) sizes that, step.workspace lends the scratch that single tokens need for it."""
     shape, dtype = rotated.shape, rotated.dtype
     n = shape[0]
     if len(shape) != 2 or shape[1] != (n_heads + 2 * n_kv) * head_dim or out.shape != (n, n_heads * head_dim) or out.dtype is not dtype:

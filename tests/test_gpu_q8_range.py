@@ -1,4 +1,5 @@
 """Attention over a cache line in 8 bits where its numbers are far from 1, or none."""
+import numpy as np
 import pytest
 import torch
 
@@ -83,3 +84,49 @@ def test_portions_with_pages_of_unlike_sizes(heads, n_kv, dim, dtype, pages, own
     b.append([(0, 448)], qkv=sized(b, 448, own), check=False)
     step, out, old = b.append([(0, 90)], qkv=sized(b, 90, own), check=False)
     b.attend([(0, 90)], step, out, old)
+
+
+@pytest.mark.parametrize("heads,n_kv,dim,dtype", [(8, 1, 64, BF16), (8, 1, 128, BF16), (8, 1, 80, BF16), (8, 1, 64, F32), (6, 1, 128, F32)])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf")])
+def test_an_infinite_key_of_the_own_block(heads, n_kv, dim, dtype, bad):
+    """Rows that see an infinite key: no numbers where its score is plus infinity, the others' result where it is minus infinity.
+    The block with it, once it is in 8 bits, reads as none of them numbers."""
+    b = Batch(1, heads, n_kv, dim, dtype, 256, seed=6)
+    qkv = b.rows(130)
+    qkv.view(130, -1, dim)[100, heads, 5] = bad
+    step, out, old = b.append([(0, 130)], qkv=qkv, rot=0, check=False)
+    got = b.attend([(0, 130)], step, out, old, check=False).view(130, heads, dim).double().cpu().numpy()
+    q = out.view(130, -1, dim)[:, :heads].double().cpu().numpy()
+    rows = b.line.rows[0].copy()
+    b.line.rows[0] = rows[:128]
+    with np.errstate(invalid="ignore"):
+        want, weight, _ = b.line.attend(0, q[:128], 0, b.scale)
+    finite = rows[:128].copy()
+    finite[100, 0, 0, 5] = 0
+    b.line.rows[0] = finite
+    _, _, reach = b.line.attend(0, q[:128], 0, b.scale)
+    # as for finite numbers: rounded scores and sums, in bfloat16 a rounded probability and result
+    relative = (dim + 8) * 2.0 ** -24 * 2 * reach + 2.0 ** -21 + 80 * 2.0 ** -24
+    half = 2.0 ** -8 if dtype == BF16 else 2.0 ** -24
+    seen_up = np.sign(bad) * q[100:128, :, 5] > 0
+    assert np.isnan(want[100:][seen_up]).all() and np.isfinite(want[100:][~seen_up]).all() and seen_up.any() and not seen_up.all()
+    assert np.isnan(got[100:128][seen_up]).all()
+    there = np.isfinite(want)
+    bound = np.broadcast_to(weight * (2 * relative + (half if dtype == BF16 else 0.0)) + half * np.abs(want) + 1e-30, want.shape)
+    assert (np.abs(got[:128][there] - want[there]) <= bound[there]).all()
+    assert np.isnan(got[128:]).all()
+
+
+@pytest.mark.parametrize("heads,n_kv,dim,dtype", [(8, 2, 64, BF16), (6, 1, 128, BF16), (4, 2, 80, BF16), (4, 2, 64, F32)])
+@pytest.mark.parametrize("keys", [1e-17, 1e-8, 1e8, 1e17])
+def test_keys_of_any_size(heads, n_kv, dim, dtype, keys):
+    """Keys far from 1 against queries as far on the other side: prompts, portions and single tokens."""
+    def rows(b, n):
+        x = b.rows(n).view(n, -1, dim)
+        x[:, :heads] /= keys
+        x[:, heads: heads + n_kv] *= keys
+        return x.view(n, -1)
+    b = Batch(2, heads, n_kv, dim, dtype, 1000, seed=dim)
+    for entries in ([(0, 700), (1, 70)], [(0, 40), (1, 5)], [(0, 1), (1, 1)]):
+        step, out, old = b.append(entries, qkv=rows(b, sum(n for _, n in entries)), check=False)
+        b.attend(entries, step, out, old)
