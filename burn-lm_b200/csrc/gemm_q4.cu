@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kWarps * 32, Few::kBlocks) few_kernel(const Fe
             x[j][h] = g < n && k < a.K ? *reinterpret_cast<const uint4*>(a.x + (size_t)g * a.ldx + k) : make_uint4(0u, 0u, 0u, 0u);
         }
     // times a power of two: the largest of this stretch to 2^120 (zeros, infinities and NaN: as they are)
-    float back[2];                                   // of tokens 2 t and 2 t + 1: what takes that and the weights' 2^-133 off again, over 2^66
+    float back[2];                                   // of tokens 2 t and 2 t + 1: what takes that and the weights' 2^-133 off again, over 2^40
     {
         unsigned top = 0;                                // of two magnitudes' bits at once
 #pragma unroll
@@ -148,7 +148,8 @@ __global__ void __launch_bounds__(kWarps * 32, Few::kBlocks) few_kernel(const Fe
                 uint4& v = x[j][h];
                 v = make_uint4(times(v.x), times(v.y), times(v.z), times(v.w));
             }
-        const float mine = __uint_as_float((unsigned)(127 + 67 - by) << 23);      // 2^(133 - 66 - by), of token g
+        // 2^(133 - 40 - by), of token g: sums with scales of up to 2^80 stay floats times the 2^40, those of 2^-110 times the rest of it
+        const float mine = __uint_as_float((unsigned)(127 + 93 - by) << 23);
         back[0] = __shfl_sync(0xffffffffu, mine, 8 * t);
         back[1] = __shfl_sync(0xffffffffu, mine, 8 * t + 4);
     }
@@ -221,8 +222,8 @@ __global__ void __launch_bounds__(kWarps * 32, Few::kBlocks) few_kernel(const Fe
                         total[3] = fmaf(m8, part[3], total[3]);
                     }
             }
-            *reinterpret_cast<float2*>(to) = make_float2(total[0] * 0x1p66f * back[0], total[1] * 0x1p66f * back[1]);
-            *reinterpret_cast<float2*>(to + 8 * 8) = make_float2(total[2] * 0x1p62f * back[0], total[3] * 0x1p62f * back[1]);
+            *reinterpret_cast<float2*>(to) = make_float2(total[0] * 0x1p40f * back[0], total[1] * 0x1p40f * back[1]);
+            *reinterpret_cast<float2*>(to + 8 * 8) = make_float2(total[2] * 0x1p36f * back[0], total[3] * 0x1p36f * back[1]);
         }
         __syncthreads();
         for (int i = threadIdx.x; i < count * F::kSums; i += kWarps * 32) {

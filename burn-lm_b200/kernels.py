@@ -2205,6 +2205,7 @@ def attention_q8(rotated, step, pool, scales, tail, old, block_table, out, n_hea
 # -- weights in 4 bits -----------------------------------------------------------------------------------------------------------
 Q4_GROUPS = (32, 64, 128)     # places of K that share a scale
 _Q4_STRETCH = 256             # places of K that a warp of the product's kernels loads together
+_Q4_SCALES = (2.0 ** -110, 2.0 ** 80)          # between these, a scale times a whole number is no denormal number and the kernels' sums are floats
 
 
 class Q4Weight:
@@ -2247,7 +2248,8 @@ def _q4_order(device):
 
 def pack_q4(values, scales, group) -> Q4Weight:
     """A weight in 4 bits from its numbers: values [M, K] whole numbers of -8 .. 7 (any integer type), scales [M, ceil(K / group)] of
-    five significant bits at most; the weight is scales[m, k // group] * values[m, k].  Plain tensor operations, on any device."""
+    five significant bits at most, 0 or of magnitudes from 2^-110 to 2^80; the weight is scales[m, k // group] * values[m, k].  Plain tensor
+    operations, on any device."""
     if group not in Q4_GROUPS:
         raise KernelError(f"pack_q4: groups of {group} places; {Q4_GROUPS} are known")
     if values.dim() != 2 or values.is_floating_point() or values.numel() == 0 or tuple(scales.shape) != (values.shape[0], -(-values.shape[1] // group)):
@@ -2258,6 +2260,9 @@ def pack_q4(values, scales, group) -> Q4Weight:
     s = scales.to(torch.float32)
     if not torch.equal(_five_bits(s), s) or not torch.isfinite(s).all():
         raise KernelError("pack_q4: scales are finite and have five significant bits at most")
+    size = s.abs()
+    if not ((size == 0) | ((size >= _Q4_SCALES[0]) & (size <= _Q4_SCALES[1]))).all():
+        raise KernelError("pack_q4: scales are 0 or of magnitudes from 2^-110 to 2^80")
     tiles, stretches, per = -(-m // 16), -(-k // _Q4_STRETCH), _Q4_STRETCH // min(group, 64)
     wide = torch.zeros((tiles * 16, stretches * per), dtype=torch.bfloat16, device=values.device)
     if group == 128:                                     # a scale for every 64 places
@@ -2279,7 +2284,8 @@ def pack_q4(values, scales, group) -> Q4Weight:
 def quantize_q4(w, group=64) -> Q4Weight:
     """A weight [M, K] (float32 or bfloat16) rounded to 4 bits.  Of each row's groups of `group` places, the number of largest magnitude
     (the negative one on a tie) becomes -8 times the scale, rounded to five significant bits; the others the nearest whole numbers of
-    -8 .. 7 times it.  A group of zeros has scale 0.  Plain tensor operations, on any device."""
+    -8 .. 7 times it.  A group of zeros, or of numbers below 2^-107, has scale 0; numbers beyond 2^83 are refused.  Plain tensor operations, on
+    any device."""
     if group not in Q4_GROUPS:
         raise KernelError(f"quantize_q4: groups of {group} places; {Q4_GROUPS} are known")
     if w.dim() != 2 or w.dtype not in (torch.float32, torch.bfloat16) or w.numel() == 0:
@@ -2293,9 +2299,11 @@ def quantize_q4(w, group=64) -> Q4Weight:
         x = x.view(-1, groups, group)
         lo, hi = x.amin(dim=2), x.amax(dim=2)
         s = _five_bits(torch.where(hi > -lo, hi, lo) / -8.0)
-        s = torch.where(s.abs() < 2.0 ** -110, torch.zeros_like(s), s)          # (so that a scale times a whole number is no denormal number)
+        s = torch.where(s.abs() < _Q4_SCALES[0], torch.zeros_like(s), s)
         if not torch.isfinite(s).all():
             raise KernelError("quantize_q4: the weight holds an infinity or a NaN")
+        if float(s.abs().max()) > _Q4_SCALES[1]:
+            raise KernelError("quantize_q4: the weight holds numbers beyond 2^83")
         safe = torch.where(s == 0, torch.ones_like(s), s)
         v = torch.where((s == 0)[..., None], torch.zeros_like(x), torch.round(x / safe[..., None]).clamp(-8, 7))
         values[r: r + 4096] = v.to(torch.int8).view(x.shape[0], -1)[:, :k]

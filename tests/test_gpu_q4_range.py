@@ -1,0 +1,43 @@
+"""Products with 4-bit weights: scales at the ends of their range, long rows."""
+import pytest
+import torch
+
+from test_gpu_q4 import BF16, DEV, F32, K, check, tokens, weight
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("n", [1, 8, 9, 40])
+@pytest.mark.parametrize("exponent", [-110, 80])
+def test_scales_at_the_ends_of_their_range(exponent, n):
+    k_ = K()
+    m, k, group = 48, 512, 64
+    g = torch.Generator(device=DEV).manual_seed(3)
+    values = torch.randint(-8, 8, (m, k), device=DEV, generator=g, dtype=torch.int8)
+    scales = torch.full((m, k // group), 2.0 ** exponent, device=DEV)
+    scales[::3] *= -1
+    w = k_.pack_q4(values, scales, group)
+    dense = values.double() * scales.double().repeat_interleave(group, dim=1)
+    assert torch.equal(k_.q4_values(w).double(), dense)
+    x = (tokens(n, k, 2).float() * (2.0 ** -20 if exponent > 0 else 2.0 ** 20)).to(BF16)
+    out = torch.empty((n, m), dtype=F32, device=DEV)
+    k_.product_q4(w, x, out=out)
+    # (a scale that is a power of two changes exponents only)
+    check(out.double().mul(2.0 ** -exponent).float(), x, dense * 2.0 ** -exponent, k)
+
+
+@pytest.mark.parametrize("n", [1, 3, 8, 9])
+@pytest.mark.parametrize("m,k", [(40, 14336), (40, 14400), (200, 16384), (64, 16392), (40, 20000)])
+def test_long_rows(m, k, n):
+    """Rows of K cut over clusters of seven and eight blocks, and longer ones, which the other kernel takes."""
+    k_ = K()
+    w, dense = weight(m, k, 64)
+    x = tokens(n, k, n)
+    out = torch.full((n, m), float("nan"), dtype=F32, device=DEV)
+    k_.product_q4(w, x, out=out)
+    check(out, x, dense, k)
+    if m % 16 == 0:
+        gated = torch.full((n, m // 2), float("nan"), dtype=BF16, device=DEV)
+        k_.product_q4(w, x, out=gated, swiglu=True)
+        check(gated, x, dense, k, gated=True)
+    k_.check_status(torch.device("cuda:0"))
