@@ -80,6 +80,32 @@ struct FewArgs {
     int* status;
 };
 
+// An infinity or a NaN among a token's numbers makes all its sums none in the kernel (n = v + 8 times it, and -8 times it).  What they are is the sum
+// of weight times such a number, none where the weight is zero: for a row of a tile and the row 8 behind it, from memory, and seldom.
+template <bool TWO>
+__device__ __noinline__ float2 odd_sums(const unsigned char* w, const __nv_bfloat16* x, int K, int stretches, int unit_bytes, int tile, int row, float y, float behind) {
+    bool any = false;
+    float sum[2] = {0.f, 0.f};
+#pragma unroll 1
+    for (int k = 0; k < K; ++k) {
+        const float v = __bfloat162float(x[k]);
+        if (fabsf(v) < INFINITY) continue;
+        any = true;
+        const unsigned char* unit = w + ((size_t)tile * stretches + k / 256) * unit_bytes;
+        const int j = k / 64 % 4, h = k / 32 % 2, at = TWO ? 2 * j + h : j;
+        const unsigned word = *reinterpret_cast<const unsigned*>(unit + j * kTileBytes + ((row & 7) * 4 + k / 8 % 4) * 16 + (2 * h + k / 4 % 2) * 4);
+        const unsigned two = word >> (16 * (k & 1) + 8 * (k >> 1 & 1));
+        const __nv_bfloat16* scales = reinterpret_cast<const __nv_bfloat16*>(unit + kBatch * kTileBytes) + (row & 7) * (TWO ? 8 : 4) + at;
+        sum[0] += (float)((int)(two & 15) - 8) * __bfloat162float(scales[0]) * v;
+        sum[1] += (float)((int)(two >> 4 & 15) - 8) * __bfloat162float(scales[8 * (TWO ? 8 : 4)]) * v;
+    }
+    if (any) {
+        y = row < 8 ? sum[0] : sum[1];
+        behind = sum[1];
+    }
+    return make_float2(y, behind);
+}
+
 template <bool TWO>
 __global__ void __launch_bounds__(kWarps * 32, Few::kBlocks) few_kernel(const FewArgs fa) {
     using F = Few;
@@ -121,7 +147,7 @@ __global__ void __launch_bounds__(kWarps * 32, Few::kBlocks) few_kernel(const Fe
             const int k = (kt + j) * 64 + 32 * h + 8 * t;
             x[j][h] = g < n && k < a.K ? *reinterpret_cast<const uint4*>(a.x + (size_t)g * a.ldx + k) : make_uint4(0u, 0u, 0u, 0u);
         }
-    // times a power of two: the largest of this stretch to 2^120 (zeros, infinities and NaN: as they are)
+    // times a power of two: the largest of this stretch to 2^120 (zeros as they are; infinities and NaN too, whose sums odd_sums puts right)
     float back[2];                                   // of tokens 2 t and 2 t + 1: what takes that and the weights' 2^-133 off again, over 2^40
     {
         unsigned top = 0;                                // of two magnitudes' bits at once
@@ -246,6 +272,11 @@ __global__ void __launch_bounds__(kWarps * 32, Few::kBlocks) few_kernel(const Fe
             for (int r = 0; r < fa.chunks; ++r) {
                 y += cluster_float(at, r);
                 if (a.end == END_GATED) up += cluster_float(at + 8 * 8 * 4, r);
+            }
+            if (__builtin_expect(!(fabsf(y) < INFINITY && fabsf(up) < INFINITY), 0)) {
+                const float2 both = odd_sums<TWO>(a.w, a.x + (size_t)tok * a.ldx, a.K, a.stretches, a.unit, b0 + slot, row, y, up);
+                y = both.x;
+                up = both.y;
             }
             if (a.end == END_GATED) y = y / (1.0f + __expf(-y)) * up;
             const size_t to = (size_t)tok * a.ldy + out;

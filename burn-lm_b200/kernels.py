@@ -2338,7 +2338,7 @@ def product_q4(w, x, out=None, add_into=None, swiglu=False):
     Ends, one at a time: `out` [N, M] bfloat16 or float32; `add_into` (float32 [N, M]) += the product; `swiglu`: the weight's rows
     come in tiles of GATE_TILE gate rows followed by the up rows of the same outputs and out [N, M / 2] = silu(gate) * up, in
     bfloat16 or float32.  x, out and add_into may be column ranges of wider tensors; x's rows begin at multiples of 16 bytes, or are
-    copied first."""
+    copied first.  An infinite number of a token times a weight is an infinity, times a weight of zero none, for any number of tokens."""
     k, m, packed, shape, dtype = w.in_features, w.out_features, w.packed, x.shape, x.dtype
     if len(shape) != 2 or dtype is not torch.bfloat16 or shape[1] != k or (k > 1 and x.stride(1) != 1):
         raise KernelError(f"product_q4: x is bfloat16 [N, {k}] with unit stride along its rows")

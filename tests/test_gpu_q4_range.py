@@ -1,10 +1,39 @@
-"""Products with 4-bit weights: scales at the ends of their range, long rows."""
+"""Products with 4-bit weights: tokens that are no numbers, scales at the ends of their range, long rows."""
 import pytest
 import torch
 
 from test_gpu_q4 import BF16, DEV, F32, K, check, tokens, weight
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("n", [1, 2, 8, 9, 40])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,k", [(64, 192), (200, 72), (48, 4160)])
+def test_tokens_that_are_no_numbers(m, k, group, n):
+    """An infinite place gives every row the infinity of its weight's sign there, or no number where the weight is zero or infinities of both
+    signs meet, whatever the number of tokens; the other tokens' results are untouched."""
+    w, dense = weight(m, k, group)
+    x = tokens(n, k, 1)
+    inf = float("inf")
+    x[0, 5] = inf
+    if n > 1:
+        x[1, k - 1], x[1, 33] = -inf, -inf
+    if n > 2:
+        x[3, 64], x[4, k // 2], x[4, k // 2 + 1], x[6, 0] = -inf, inf, inf, float("nan")
+    want = torch.stack([(row * dense).sum(dim=1) for row in x.double()])
+    for dtype in (BF16, F32):
+        out = torch.full((n, m), 3.0, dtype=dtype, device=DEV)
+        K().product_q4(w, x, out=out)
+        odd = ~torch.isfinite(x).all(dim=1)
+        assert torch.equal(out[odd].double().nan_to_num(nan=7.0), want[odd].nan_to_num(nan=7.0))
+        check(out[~odd], x[~odd], dense, k)
+    if m % 16 == 0:
+        gated = torch.full((n, m // 2), 3.0, dtype=F32, device=DEV)
+        K().product_q4(w, x, out=gated, swiglu=True)
+        both = want.view(n, -1, 2, 8)
+        act = (both[:, :, 0] / (1 + torch.exp(-both[:, :, 0])) * both[:, :, 1]).reshape(n, -1)
+        assert torch.equal(gated[odd].double().nan_to_num(nan=7.0), act[odd].nan_to_num(nan=7.0))
 
 
 @pytest.mark.parametrize("n", [1, 8, 9, 40])
