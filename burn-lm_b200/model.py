@@ -91,8 +91,8 @@ class Model:
         self.bound = False
         if runtime.cache == "int8":
             self._check_eight_bits()
-        if runtime.weights == "int4" and not any(getattr(p, "four_bit", ()) for p in self.parts()):
-            raise ValueError("weights in 4 bits: none of this model's parts holds products that take them")
+        if runtime.weights == "int4":
+            self._check_four_bits()
 
     def _check_eight_bits(self) -> None:
         """Every run that keeps keys and values does so in 8 bits, and no run reads another's line (whose unfinished block it would need
@@ -108,6 +108,18 @@ class Model:
                 raise ValueError(f"a cache in 8 bits: run {run} of the schedule reads the cache line of run {e.cache_of}, which lines in 8 bits do not offer")
         if not some:
             raise ValueError("a cache in 8 bits: this model keeps no keys and values")
+
+    def _check_four_bits(self) -> None:
+        """Every part of the layers that multiplies by a matrix does so with 4-bit weights (the embedding and the output projection stay
+        as stored)."""
+        some = False
+        for where, parts in [("the stream", self.stream_parts)] + [(f"layer {i}", layer.parts()) for i, layer in enumerate(self.layers)]:
+            for p in parts:
+                some = some or bool(getattr(p, "four_bit", ()))
+                if not getattr(p, "four_bit", ()) and any(len(t.shape) >= 2 and min(t.shape[-2:]) >= 16 for t in p.tensor_specs()):
+                    raise ValueError(f"weights in 4 bits: {type(p).__name__} of {where} holds its weights as stored only")
+        if not some:
+            raise ValueError("weights in 4 bits: none of this model's parts holds products that take them")
 
     # -- weights ---------------------------------------------------------------------------------
     def parts(self):
@@ -254,7 +266,8 @@ def tensor_specs_of(config: dict):
 def load_model(folder: str, dtype="bfloat16", device="cuda", cache="compute", weights="stored") -> Model:
     """Build the model a folder's config.json names and bind its safetensors weights.  `cache` "int8": keys and values in 8 bits with a
     scale for every block of 64 positions and head; `weights` "int4": the weights of the layers' products rounded to 4 bits with a
-    scale for every 64 places (embeddings, norms and the output projection stay as stored)."""
+    scale for every 64 places (embeddings, norms and the output projection stay as stored).  A model with a part that has no such
+    form is refused, with the part's name."""
     config = read_config_json(folder)
     _, typed, plan = plan_of(config)
     runtime = make_runtime(dtype, device, cache, weights)
