@@ -106,6 +106,15 @@ class _StateGroup:
         self.state = torch.zeros((len(runs), max_seqs, *need.state_shape), dtype=dt, device=device)
 
 
+def default_slots(needs: list, n_pages: int) -> int:
+    """How many sequences a cache of `n_pages` pages has slots for where nobody says: as many as there are pages, 1,024 at most.  A line in 8
+    bits keeps a whole unrounded block for every slot beside its pages, two pages' bytes in bfloat16 and four in float32: with one for
+    every four pages it takes about three quarters of a bfloat16 line and half of a float32 one."""
+    flat = [one for need in needs if need is not None for one in (need if isinstance(need, tuple) else (need,))]
+    slots = n_pages // 4 if any(one.bits == 8 for one in flat) else n_pages
+    return max(1, min(slots, 1024))
+
+
 class Cache:
     def __init__(self, needs: list, schedule, max_tokens: int, max_seqs: int, max_seq_len: int, dtype, device, named=None):
         """needs[run]: CacheNeed of every run of the schedule (None where the run reads another's).  `named`: what parts

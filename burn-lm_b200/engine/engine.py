@@ -15,7 +15,7 @@ from typing import Optional, Sequence
 
 import torch
 
-from ..cache import Cache, CacheError
+from ..cache import Cache, CacheError, default_slots
 from ..model import Model, load_model
 from .. import kernels as K
 from ..parts.base import StepContext
@@ -50,7 +50,8 @@ class Engine:
 
     def __init__(self, model: Model, max_tokens: int, max_seqs: Optional[int] = None,
                  max_seq_len: Optional[int] = None, max_step_tokens: Optional[int] = None):
-        """`max_tokens`: token places of the cache (rounded up to pages); `max_seqs`: slots; `max_seq_len`: the most
+        """`max_tokens`: token places of the cache (rounded up to pages); `max_seqs`: slots (None: one a page, at most 1,024;
+        with a cache in 8 bits one for four pages, see cache.default_slots); `max_seq_len`: the most
         one sequence may hold; `max_step_tokens`: the most tokens one step may bring (its activations are
         sized by it); None: as many as the cache holds."""
         self.model = model
@@ -60,7 +61,7 @@ class Engine:
         page = K.PAGE
         pages = (max_tokens + page - 1) // page
         if max_seqs is None:
-            max_seqs = max(1, min(pages, 1024))
+            max_seqs = default_slots(model.cache_needs(), pages)
         if max_seq_len is None:
             max_seq_len = model.plan.max_positions
         max_seq_len = min(max_seq_len, pages * page)

@@ -64,6 +64,13 @@ def cache_tokens(max_tokens: int) -> int:
     return max_tokens + max(32 * PAGE, max_tokens // 4)
 
 
+def cache_slots(max_tokens: int, cache: str):
+    """Slots for as many requests as `cache_tokens` has pages for: a cache in the compute dtype has one a page anyway (None), one in 8 bits as
+    many as it is sized for, at least 32."""
+    from ..kernels import PAGE
+    return max(32, min(cache_tokens(max_tokens) // PAGE // 4, 1024)) if cache == "int8" else None
+
+
 def main(argv=None) -> int:
     import argparse
 
@@ -77,7 +84,8 @@ def main(argv=None) -> int:
     ap.add_argument("--cache", default="compute", choices=["compute", "int8"], help="what keys and values are kept in")
     ap.add_argument("--weights", default="stored", choices=["stored", "int4"], help="what the layers' weights are held in")
     args = ap.parse_args(argv)
-    engine = Engine.from_folder(args.model, dtype=args.dtype, max_tokens=cache_tokens(args.max_tokens), cache=args.cache, weights=args.weights)
+    engine = Engine.from_folder(args.model, dtype=args.dtype, max_tokens=cache_tokens(args.max_tokens),
+                                max_seqs=cache_slots(args.max_tokens, args.cache), cache=args.cache, weights=args.weights)
     rp = Replayer(engine, args.out)
     for line in sys.stdin:
         line = line.strip()
