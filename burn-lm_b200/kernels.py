@@ -2337,8 +2337,8 @@ def product_q4(w, x, out=None, add_into=None, swiglu=False):
 
     Ends, one at a time: `out` [N, M] bfloat16 or float32; `add_into` (float32 [N, M]) += the product; `swiglu`: the weight's rows
     come in tiles of GATE_TILE gate rows followed by the up rows of the same outputs and out [N, M / 2] = silu(gate) * up, in
-    bfloat16 or float32.  x, out and add_into may be column ranges of wider tensors; x's rows begin at multiples of 16 bytes, or are
-    copied first.  An infinite number of a token times a weight is an infinity, times a weight of zero none, for any number of tokens."""
+    bfloat16 or float32.  x, out and add_into may be column ranges of wider tensors; x's rows begin at multiples of 16 bytes and
+    do not overlap, or are copied first.  An infinite number of a token times a weight is an infinity, times a weight of zero none, for any number of tokens."""
     k, m, packed, shape, dtype = w.in_features, w.out_features, w.packed, x.shape, x.dtype
     if len(shape) != 2 or dtype is not torch.bfloat16 or shape[1] != k or (k > 1 and x.stride(1) != 1):
         raise KernelError(f"product_q4: x is bfloat16 [N, {k}] with unit stride along its rows")
@@ -2356,13 +2356,15 @@ def product_q4(w, x, out=None, add_into=None, swiglu=False):
     columns = m // 2 if swiglu else m
     if y.shape != (n, columns) or (columns > 1 and y.stride(1) != 1):
         raise KernelError("product_q4: the result is [N, M] (gated: [N, M / 2]) with unit stride along its rows")
+    if n > 1 and y.stride(0) < columns:
+        raise KernelError("product_q4: rows of the result overlap")
     now = x.get_device()
     if now < 0 or y.get_device() != now or packed.get_device() != now or now != (_current_device() if _current_device is not None else torch.cuda.current_device()):
         if not (x.is_cuda and y.is_cuda and packed.is_cuda):
             raise KernelError("burn-lm_b200 kernels run on a CUDA device only; got a CPU tensor")
         raise KernelError("product_q4: x, the weight and the result lie on the current device")
     p_x, apart = x.data_ptr(), x.stride(0)
-    if k % 8 or apart % 8 or p_x % 16:
+    if k % 8 or apart % 8 or p_x % 16 or apart < k:      # (a tensor map has no rows that overlap)
         rows = torch.zeros((n, -(-k // 64) * 64), dtype=dtype, device=x.device)
         rows[:, :k] = x
         x, k = rows, rows.shape[1]

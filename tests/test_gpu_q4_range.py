@@ -70,3 +70,19 @@ def test_long_rows(m, k, n):
         k_.product_q4(w, x, out=gated, swiglu=True)
         check(gated, x, dense, k, gated=True)
     k_.check_status(torch.device("cuda:0"))
+
+
+@pytest.mark.parametrize("n", [2, 8, 9, 40, 300])
+def test_the_same_row_many_times(n):
+    """A broadcast token, and rows that overlap: read as what they are."""
+    k_ = K()
+    m, k = 48, 512
+    w, dense = weight(m, k, 64)
+    x = tokens(1, k, 3).expand(n, k)
+    out = torch.full((n, m), float("nan"), dtype=F32, device=DEV)
+    k_.product_q4(w, x, out=out)
+    check(out, x, dense, k)
+    assert (out == out[0]).all()
+    x = tokens(1, k + 8 * n, 4)[0].as_strided((n, k), (8, 1))
+    k_.product_q4(w, x, out=out)
+    check(out, x, dense, k)

@@ -1,4 +1,4 @@
-"""The range of a 4-bit weight's scales, without a GPU."""
+"""The range of a 4-bit weight's scales and what a product refuses, without a GPU."""
 import pytest
 import torch
 
@@ -26,3 +26,14 @@ def test_weights_too_large_or_small():
         w[3, 5] = big
         with pytest.raises(K.KernelError, match="beyond 2.83"):
             K.quantize_q4(w, 64)
+
+
+def test_results_whose_rows_overlap_are_refused():
+    w = K.pack_q4(torch.zeros(16, 64, dtype=torch.int8), torch.ones(16, 1), 64)
+    x = torch.zeros(3, 64, dtype=torch.bfloat16)
+    for out in (torch.zeros(1, 16).expand(3, 16), torch.zeros(64).as_strided((3, 16), (8, 1))):
+        for end in (dict(out=out), dict(add_into=out)):
+            with pytest.raises(K.KernelError, match="rows of the result overlap"):
+                K.product_q4(w, x, **end)
+    with pytest.raises(K.KernelError, match="CUDA device"):      # (a single row overlaps nothing)
+        K.product_q4(w, x[:1], out=torch.zeros(64).as_strided((1, 16), (8, 1)))
