@@ -2117,11 +2117,11 @@ def _q8_step(what, step, block_table, tail, n_kv, head_dim, dtype):
 
 
 def _step_ptrs(what, step):
-    """The addresses of a step's bounds, slots and positions: int32, wherever they begin."""
+    """The addresses of a step's bounds, slots and positions: int32 on the current device, wherever they begin."""
     cu, slot, start = step.cu_seqlens, step.slot_of_seq, step.start_pos
     device = cu.get_device()
-    if device < 0 or slot.get_device() != device or start.get_device() != device or not (cu.is_contiguous() and slot.is_contiguous() and start.is_contiguous()):
-        raise KernelError(f"{what}: a step's tensors are contiguous and lie on the CUDA device")
+    if device < 0 or device != (_current_device() if _current_device is not None else torch.cuda.current_device()) or slot.get_device() != device or start.get_device() != device or not (cu.is_contiguous() and slot.is_contiguous() and start.is_contiguous()):
+        raise KernelError(f"{what}: a step's tensors are contiguous and lie on the current CUDA device")
     return cu.data_ptr(), slot.data_ptr(), start.data_ptr()
 
 

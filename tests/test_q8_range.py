@@ -1,0 +1,32 @@
+"""What the functions of a cache line in 8 bits refuse beside shapes and types, without a GPU."""
+import types
+
+import pytest
+
+from burn_lm_b200 import kernels as K
+
+
+class On:
+    """A tensor on a device, as far as an address is asked for."""
+
+    def __init__(self, device, contiguous=True):
+        self.device, self.contiguous = device, contiguous
+
+    def get_device(self):
+        return self.device
+
+    def is_contiguous(self):
+        return self.contiguous
+
+    def data_ptr(self):
+        return 64 + self.device
+
+
+def test_a_steps_tensors_lie_on_the_current_device(monkeypatch):
+    """Kernels run on the current device's stream: a step on another one is refused, as the other tensors are."""
+    monkeypatch.setattr(K, "_current_device", lambda: 1)
+    step = lambda *t: types.SimpleNamespace(cu_seqlens=t[0], slot_of_seq=t[1], start_pos=t[2])  # noqa: E731
+    assert K._step_ptrs("attention_q8", step(On(1), On(1), On(1))) == (65, 65, 65)
+    for bad in ((On(0), On(0), On(0)), (On(1), On(0), On(1)), (On(1), On(1), On(0)), (On(1), On(1), On(1, False)), (On(-1), On(-1), On(-1))):
+        with pytest.raises(K.KernelError, match="attention_q8: a step's tensors"):
+            K._step_ptrs("attention_q8", step(*bad))
