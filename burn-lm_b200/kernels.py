@@ -9,6 +9,7 @@ functions raise.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 from ctypes import c_float, c_int, c_longlong, c_size_t, c_uint, c_ulonglong, c_void_p
 
@@ -2185,6 +2186,8 @@ def attention_q8(rotated, step, pool, scales, tail, old, block_table, out, n_hea
     _q8_step("attention_q8", step, block_table, tail, n_kv, head_dim, dtype)
     if window < 0:
         raise KernelError(f"attention_q8: a window of {window} keys")
+    if not 0.0 <= scale < math.inf:                      # (a row's largest score is sought before it is multiplied)
+        raise KernelError(f"attention_q8: scores times {scale}")
     if step.max_q_len > 1 and (old is None or old.dtype is not dtype or old.shape != (step.n_seqs, 2, n_kv, PAGE, head_dim)):
         raise KernelError("attention_q8: a step of several tokens a sequence needs what rope_append_q8 returned")
     found = tail if step.max_q_len <= 1 else old

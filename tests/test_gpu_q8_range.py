@@ -130,3 +130,13 @@ def test_keys_of_any_size(heads, n_kv, dim, dtype, keys):
     for entries in ([(0, 700), (1, 70)], [(0, 40), (1, 5)], [(0, 1), (1, 1)]):
         step, out, old = b.append(entries, qkv=rows(b, sum(n for _, n in entries)), check=False)
         b.attend(entries, step, out, old)
+
+
+@pytest.mark.parametrize("heads,n_kv,dim,dtype", [(8, 2, 64, BF16), (8, 2, 128, BF16), (4, 2, 80, BF16), (4, 2, 64, F32)])
+@pytest.mark.parametrize("window", [0, 100])
+def test_scores_times_zero(heads, n_kv, dim, dtype, window):
+    """The mean of the values that a query sees."""
+    b = Batch(2, heads, n_kv, dim, dtype, 600, seed=dim)
+    b.scale = 0.0
+    for entries in ([(0, 300), (1, 70)], [(0, 40), (1, 5)], [(0, 1), (1, 1)]):
+        b.go(entries, window=window)

@@ -4,6 +4,7 @@ import types
 import pytest
 
 from burn_lm_b200 import kernels as K
+from test_q8 import arguments
 
 
 class On:
@@ -30,3 +31,14 @@ def test_a_steps_tensors_lie_on_the_current_device(monkeypatch):
     for bad in ((On(0), On(0), On(0)), (On(1), On(0), On(1)), (On(1), On(1), On(0)), (On(1), On(1), On(1, False)), (On(-1), On(-1), On(-1))):
         with pytest.raises(K.KernelError, match="attention_q8: a step's tensors"):
             K._step_ptrs("attention_q8", step(*bad))
+
+
+@pytest.mark.parametrize("scale", [-0.125, -1e-30, float("nan"), float("inf")])
+def test_scales_of_scores_that_are_refused(scale):
+    """The portions' kernel seeks the largest score before it multiplies: a negative scale would make it the smallest."""
+    a = arguments()
+    with pytest.raises(K.KernelError, match="attention_q8: scores times"):
+        K.attention_q8(a.out, a.step, a.pool, a.scales, a.tail, a.old, a.table, a.o, a.heads, a.kv, a.dim, scale)
+    for fine in (0.0, 1.0):
+        with pytest.raises(K.KernelError, match="CUDA device"):
+            K.attention_q8(a.out, a.step, a.pool, a.scales, a.tail, a.old, a.table, a.o, a.heads, a.kv, a.dim, fine)
