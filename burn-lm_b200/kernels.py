@@ -2075,12 +2075,16 @@ def _q8_value_places(head_dim: int, device):
 
 def q8_write(pool, scales, pages, keys, key_scales, values, value_scales) -> None:
     """Puts whole blocks into a cache line in 8 bits (a saved conversation, say): pages int [P]; keys and values int8
-    [P, n_kv, PAGE, head_dim]; their scales [P, n_kv].  Plain tensor operations, on any device."""
+    [P, n_kv, PAGE, head_dim]; their scales [P, n_kv], none below zero.  Plain tensor operations, on any device."""
     p, n_kv, page, head_dim = keys.shape
     _q8_line("q8_write", pool, scales, n_kv, head_dim)
     if (page != PAGE or keys.dtype != torch.int8 or values.dtype != torch.int8 or values.shape != keys.shape or pages.numel() != p
             or tuple(key_scales.shape) != (p, n_kv) or tuple(value_scales.shape) != (p, n_kv)):
         raise KernelError(f"q8_write: keys and values int8 [P, kv heads, {PAGE}, head_dim], scales [P, kv heads], a page for each")
+    if bool((key_scales < 0).any()) or bool((value_scales < 0).any()):         # (by a scale below zero the kernels know a page that is none)
+        raise KernelError("q8_write: scales are not below zero")
+    if p and not 0 <= int(pages.min()) <= int(pages.max()) < pool.shape[0]:
+        raise KernelError(f"q8_write: pages are numbers below {pool.shape[0]}")
     line = torch.full((p, n_kv, pool.shape[2]), -128, dtype=torch.int8, device=pool.device)      # a byte holds the number + 128
     k = (keys ^ -128).reshape(p, n_kv, PAGE // 2, 2, head_dim)
     if head_dim % 32 == 0:                               # the 16-byte pieces of odd rows are exchanged pairwise

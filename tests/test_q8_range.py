@@ -2,6 +2,7 @@
 import types
 
 import pytest
+import torch
 
 from burn_lm_b200 import kernels as K
 from test_q8 import arguments
@@ -42,3 +43,21 @@ def test_scales_of_scores_that_are_refused(scale):
     for fine in (0.0, 1.0):
         with pytest.raises(K.KernelError, match="CUDA device"):
             K.attention_q8(a.out, a.step, a.pool, a.scales, a.tail, a.old, a.table, a.o, a.heads, a.kv, a.dim, fine)
+
+
+def test_writing_refuses_scales_below_zero_and_pages_of_another_pool():
+    """A block with a negative scale would be taken for a page that is none, and its keys left out; page -1 would be the pool's last."""
+    pool, scales = K.q8_pool(3, 2, 32, "cpu")
+    eight, s, pages = torch.ones(2, 2, 64, 32, dtype=torch.int8), torch.ones(2, 2), torch.tensor([0, 2])
+    before = pool.clone()
+    down = s.clone()
+    down[1, 0] = -1.0
+    for ks, vs in ((down, s), (s, down)):
+        with pytest.raises(K.KernelError, match="below zero"):
+            K.q8_write(pool, scales, pages, eight, ks, eight, vs)
+    for wrong in ([-1, 0], [0, 3]):
+        with pytest.raises(K.KernelError, match="numbers below 3"):
+            K.q8_write(pool, scales, torch.tensor(wrong), eight, s, eight, s)
+    assert torch.equal(pool, before)
+    for fine in (s * 0, s * float("inf"), s * float("nan")):
+        K.q8_write(pool, scales, pages, eight, fine, eight, s)
