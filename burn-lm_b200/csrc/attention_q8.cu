@@ -1000,6 +1000,7 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
                 unsigned char* stage = ring + (size_t)s * STAGE;
                 if (page < 0) {                          // none of the pool's: the consumers know it by a scale below zero
                     *const_cast<float2*>(scales_of(stage, HD)) = make_float2(0.f, -1.f);
+                    tc5::fence_async_smem();             // (a copy may write the same place next)
                     mbar_arrive(full + s);
                     continue;
                 }
@@ -1545,6 +1546,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                 unsigned char* stage = raw + s * P::kRaw;
                 if (page < 0) {                          // none of the pool's: known by a scale below zero
                     *const_cast<float2*>(scales_of(stage, HD)) = make_float2(0.f, -1.f);
+                    tc5::fence_async_smem();             // (a copy may write the same place next)
                     mbar_arrive(raw_full + s);
                     continue;
                 }

@@ -140,3 +140,23 @@ def test_scores_times_zero(heads, n_kv, dim, dtype, window):
     b.scale = 0.0
     for entries in ([(0, 300), (1, 70)], [(0, 40), (1, 5)], [(0, 1), (1, 1)]):
         b.go(entries, window=window)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("every", [2, 3, 4, 5])
+def test_pages_that_are_none_between_others(dim, every):
+    """Every second to fifth page of a long walk outside the pool: each place of the ring holds a page, none, and a page again."""
+    from q8_reference import PAGE, Line
+    b = Batch(1, 8, 2, dim, BF16, 2200, seed=every)
+    b.append([(0, 2048)], rot=0, check=False)
+    b.table[0, :32:every] = -1
+    kept = [i for i in range(2048) if i // PAGE % every]
+    line = Line(1, 2, dim)
+    line.append(0, b.line.rows[0][kept])
+    b.line = line
+    for new in (70, 1):
+        step, out, old = b.append([(0, new)], rot=0, check=False)
+        o = b.attend([(0, new)], step, out, old, check=False)
+        step.start_pos = step.start_pos.cpu() - (2048 - len(kept))
+        b.check_attention([(0, new)], step, out, o, 0)
+    K().check_status(torch.device("cuda:0"))
