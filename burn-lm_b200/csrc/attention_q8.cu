@@ -2044,7 +2044,7 @@ BLM_API int blm_rope_append_q8(const void* qkv, void* out, int dtype, const int*
     using namespace q8;
     if (n_seqs == 0 || max_q_len == 0) return BLM_OK;
     BLM_REQUIRE(hd >= 16 && hd <= 256 && hd % 16 == 0, "rope_append_q8: heads of %d lanes (multiples of 16 from 16 to 256)", hd);
-    BLM_REQUIRE(n_kv > 0 && n_heads % n_kv == 0, "rope_append_q8: %d heads do not divide into %d kv heads", n_heads, n_kv);
+    BLM_REQUIRE(n_kv > 0 && n_heads > 0 && n_heads % n_kv == 0, "rope_append_q8: %d heads do not divide into %d kv heads", n_heads, n_kv);
     BLM_REQUIRE(rot >= 0 && rot <= hd && rot % 2 == 0, "rope_append_q8: %d rotated lanes of a head of %d", rot, hd);
     BLM_REQUIRE(rot == 0 || inv_freq != nullptr, "rope_append_q8: no frequencies");
     BLM_REQUIRE(pairing >= 0 && pairing <= 2 && (pairing != PAIRS_TILED || rot % 16 == 0), "rope_append_q8: pairing %d of %d lanes", pairing, rot);
@@ -2084,7 +2084,7 @@ BLM_API int blm_attention_q8(const void* rotated, const void* pool, const void* 
     using namespace q8;
     if (n_tokens == 0 || n_seqs == 0) return BLM_OK;
     BLM_REQUIRE(hd >= 16 && hd <= 256 && hd % 16 == 0, "attention_q8: heads of %d lanes (multiples of 16 from 16 to 256)", hd);
-    BLM_REQUIRE(n_kv > 0 && n_heads % n_kv == 0, "attention_q8: %d heads do not divide into %d kv heads", n_heads, n_kv);
+    BLM_REQUIRE(n_kv > 0 && n_heads > 0 && n_heads % n_kv == 0, "attention_q8: %d heads do not divide into %d kv heads", n_heads, n_kv);
     BLM_REQUIRE((long long)n_tokens * n_heads < (1ll << 31), "attention_q8: %d tokens of %d heads in one step", n_tokens, n_heads);
     const AttendArgs a{rotated, (const signed char*)pool, found, found_by_slot, block_table, table_stride, cu_seqlens, slot_of_seq, start_pos,
                        out, n_seqs, n_heads, n_kv, hd, n_pages, window, scale * 1.4426950408889634f};

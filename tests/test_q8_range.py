@@ -61,3 +61,14 @@ def test_writing_refuses_scales_below_zero_and_pages_of_another_pool():
     assert torch.equal(pool, before)
     for fine in (s * 0, s * float("inf"), s * float("nan")):
         K.q8_write(pool, scales, pages, eight, fine, eight, s)
+
+
+@pytest.mark.parametrize("heads,kv", [(0, 2), (-2, 2), (5, 2), (2, 0), (1, 2)])
+@pytest.mark.parametrize("dtype,dim,new", [(1, 64, 1), (1, 128, 5), (0, 64, 1), (1, 80, 7)])
+def test_numbers_of_heads_at_the_entry(heads, kv, dtype, dim, new):
+    """The entries refuse what cannot be planned (with no head at all, a division by zero ended the process); no pointer is looked at."""
+    with pytest.raises(K.KernelError, match="attention_q8: .* heads do not divide"):
+        K._call("attention_q8", "blm_attention_q8", 0, 0, 0, 1, dtype, 0, 4, 0, 0, 0, 0, new, 1, heads, kv, dim, 1, 0, 0.125, new, 64, 0, 1, 0, 0)
+    with pytest.raises(K.KernelError, match="rope_append_q8: .* heads do not divide"):
+        K._call("attention_q8", "blm_rope_append_q8", 0, 0, dtype, 0, 0, 0, 0, 4, 0, 0, 0, 0, 0, 1.0, 0, 0, 0, new, 1, new, heads, kv, dim, 1, 0)
+    assert K._ask("attention_q8", "blm_attention_q8_splits", dtype, 1, new, 5000, heads, kv, dim, 0) >= 1
