@@ -13,11 +13,11 @@
 // rows from the rotated projection and the rows before them from `old`.  Steps of one token a sequence read the tail itself.
 //
 // Layout of a kv head's part of a page: keys [64][D] bytes, where D is a multiple of 32 with the 16-byte pieces of odd rows exchanged
-// pairwise (so that the decode kernel's reads of neighbouring rows meet in no bank of shared memory); then values so that the decode kernel's tensor-core fragments are 16-byte
-// pieces: for keys 16 w + 4 t + e and lanes d = g (D / 8) + n the byte at
+// pairwise (so that the decode kernel's reads of neighbouring rows meet in no bank of shared memory); then the values, so that the decode
+// kernel's tensor-core fragments are 16-byte pieces: for keys 16 w + 4 t + e and lanes d = g (D / 8) + n the byte at
 //     w (16 Dp) + (n / 4) 512 + (4 g + t) 16 + (n % 4) 4 + e,     Dp = D rounded up to a multiple of 32:
 // thread (g, t) of a warp finds four lanes of four keys in 16 bytes; then 16 bytes whose first eight are the two scales, so that one
-// copy brings all a block needs.  A byte holds q + 128: behind the byte 0x64 it is the half-precision number 1024 + 128 + q, so that
+// copy brings all that a block needs.  A byte holds q + 128: behind the byte 0x64 it is the half-precision number 1024 + 128 + q, so that
 // one byte permutation makes two numbers.
 #include <cuda_fp16.h>
 #include <math.h>
@@ -312,10 +312,11 @@ __global__ void __launch_bounds__(kAppendThreads) append_token_kernel(const Appe
     store_block<T>(a, rows, ld, value, page, kvh, red);
 }
 
-// Steps of several tokens: a block is (64-position block x of the sequence's new tokens, head of q, k or v, sequence).  Bound by the
-// memory: every row is read once and written once (keys and values pass through shared memory on their way into 8 bits).  The rows
-// that the step found in the tail and the rows of its last, unfinished block belong to one thread block (x = 0), which reads the
-// tail before it writes it.
+// Steps of several tokens: a block is (64-position block that a sequence touches, head of q, k or v).  Every row is read once and written
+// once (keys and values pass through shared memory on their way into 8 bits, which is read twice: for the largest magnitude, then for the
+// numbers).  The rows that the step found in the tail and the rows of the sequence's last, unfinished block belong to the thread block of
+// the sequence's first, which reads the tail before it writes it.  2,048 tokens of 32 heads of 64 to 8: 18.8 us (float32 21.2), 4.3 of
+// them the memory's.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kAppendThreads) append_prompt_kernel(const AppendArgs a) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -332,7 +333,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_prompt_kernel(const App
     int b = last - from_last;
     const bool query = head < a.n_heads, value = head >= a.n_heads + a.n_kv;
     const bool last_open = end % kPage != 0;
-    if (!query && b > first && b == last && last_open) return;         // the block x = 0 has it
+    if (!query && b > first && b == last && last_open) return;         // the block of the sequence's first has it
     const int slot = a.slot_of_seq[seq], kvh = value ? head - a.n_heads - a.n_kv : head - a.n_heads;
     const T* qkv = reinterpret_cast<const T*>(a.qkv);
     T* out = reinterpret_cast<T*>(a.out);
@@ -2006,8 +2007,8 @@ static int launch_prompt(PromptArgs pa, int n_tokens, long long touched, int pag
     }
     // A walk is shared by as many blocks as make the step shortest: its turns, each a share of the longest walk's pages and, about as long
     // as six pages, a block's beginning and end, and five more where the shares have to meet.  Heads of 128, 32 to 8 kv heads, in 1, 2, 4
-    // and 8 blocks: 64 tokens alone 8.9, 14.1, 13.5, 14.8 us; 64 behind 1,000 25.8, 20.6, 16.3, 26.6; 64 behind 8,192 145, 82, 48, 32;
-    // 256 behind 8,192 149, 85, 50, 94.
+    // and 8 blocks: 64 tokens alone 8.5, 14.1, 13.5, 14.8 us; 64 behind 1,000 25.8, 20.6, 16.3, 26.6; 64 behind 8,192 145, 82, 48, 32; 256
+    // behind 8,192 149, 85, 50, 94.  (`pages` may be a bound far above what the step has, as in captured steps: 64 tokens alone then 14.1.)
     const long long walks = (long long)pa.a.n_kv * pa.head_groups * touched;
     long long best = (walks + resident[dev][0] - 1) / resident[dev][0] * (pages + 6);
     for (int i = 1; i < 4; ++i) {

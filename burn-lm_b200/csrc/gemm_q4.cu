@@ -355,7 +355,7 @@ static int launch_few(const Args& a, int* status, cudaStream_t stream) {
 // tensor core's.)  Where a weight has too few rows to fill the SMs, K is cut over the blocks of a cluster.  The sums go from tensor memory
 // to shared memory as they are, a row a lane; then each token's results are read, four rows a thread (from all the cluster's blocks, in
 // their order), finished, and written as whole lines.  Waits are bounded.
-// Measured, with groups of 64: 512 tokens by 28,672 x 4,096 94 us (1,284 TFLOP/s), 2,048 by 16,384 x 2,048 117 us (1,180), 64 by
+// Measured, with groups of 64: 512 tokens by 28,672 x 4,096 93 to 96 us (1,250 to 1,296 TFLOP/s), 2,048 by 16,384 x 2,048 117 us (1,180), 64 by
 // 28,672 x 4,096 30 us (2.2 TB/s of weights).  A tile of K with 256 tokens takes 0.34 us for 0.28 of products, a block's beginning and end
 // 7 us, which nothing hides; with few tokens it is the widening, 0.2 us a tile of 128 x 64 weights.
 enum { Q4_TIMEOUT_PRODUCT = 53 };
