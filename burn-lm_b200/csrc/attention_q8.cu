@@ -93,6 +93,11 @@ __device__ __forceinline__ int find_block(const int* cu_seqlens, const int* star
 // the most that sequences with n_tokens together touch
 static inline long long most_blocks(long long n_tokens, long long n_seqs, int unit) { return (n_tokens + n_seqs * (unit - 2)) / unit + n_seqs; }
 
+// the halves of two bfloat16 numbers that are infinities or NaN, as masks
+__device__ __forceinline__ unsigned odd_two(unsigned v) {
+    return ((v & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((v & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+}
+
 // sixteen bytes of T, as floats
 template <typename T> struct Vec { static constexpr int n = 16 / sizeof(T); };
 __device__ __forceinline__ void load_vec(const float* p, float* o) {
@@ -1078,15 +1083,23 @@ __global__ void __launch_bounds__((kTokenWarps + 1) * 32) attend_token_kernel(co
             // what a key's values weigh, as log2 of 2^-7 of the largest magnitude among them: the reference is one of score times value here
             // too, so that neither these rows nor the pages leave the range of the pages' half precision (with the scores alone, values of 1e-8
             // behind pages were off by a tenth).  Two keys a word, their magnitudes' bits.
-            unsigned size[2] = {0u, 0u};
+            unsigned size[2];
+            auto look = [&](bool all) {                  // (a value that is no number says nothing about the others)
+                size[0] = size[1] = 0u;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                unsigned top = 0;                        // of two magnitudes' bits at once
+                for (int e = 0; e < 4; ++e) {
+                    unsigned top = 0;                    // of two magnitudes' bits at once
 #pragma unroll
-                for (int j = 0; j < HD / 64; ++j)
-                    top = __vmaxu2(__vmaxu2(top, v[j][e].x & 0x7fff7fffu), __vmaxu2(__vmaxu2(v[j][e].y & 0x7fff7fffu, v[j][e].z & 0x7fff7fffu), v[j][e].w & 0x7fff7fffu));
-                size[e >> 1] |= max(top & 0xffffu, top >> 16) << (16 * (e & 1));
-            }
+                    for (int j = 0; j < HD / 64; ++j) {
+                        uint4 x = v[j][e];
+                        if (!all) x = make_uint4(x.x & ~odd_two(x.x), x.y & ~odd_two(x.y), x.z & ~odd_two(x.z), x.w & ~odd_two(x.w));
+                        top = __vmaxu2(__vmaxu2(top, x.x & 0x7fff7fffu), __vmaxu2(__vmaxu2(x.y & 0x7fff7fffu, x.z & 0x7fff7fffu), x.w & 0x7fff7fffu));
+                    }
+                    size[e >> 1] |= max(top & 0xffffu, top >> 16) << (16 * (e & 1));
+                }
+            };
+            look(true);
+            if (__any_sync(0xffffffffu, odd_two(size[0]) != 0 || odd_two(size[1]) != 0)) look(false);
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
 #pragma unroll
@@ -1443,11 +1456,6 @@ __device__ __forceinline__ unsigned tiny_two(unsigned word) {
     const unsigned p = __byte_perm(word, 0u, LO == 0 ? 0x4140 : 0x4342), less = 0x00800080u;
     const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&p), *reinterpret_cast<const __nv_bfloat162*>(&less));
     return *reinterpret_cast<const unsigned*>(&v);
-}
-
-// the halves of two bfloat16 numbers that are infinities or NaN, as masks
-__device__ __forceinline__ unsigned odd_two(unsigned v) {
-    return ((v & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((v & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
 }
 
 template <int HD>

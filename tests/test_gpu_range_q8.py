@@ -160,3 +160,47 @@ def test_pages_that_are_none_between_others(dim, every):
         step.start_pos = step.start_pos.cpu() - (2048 - len(kept))
         b.check_attention([(0, new)], step, out, o, 0)
     K().check_status(torch.device("cuda:0"))
+
+
+@pytest.mark.parametrize("heads,n_kv,dim,dtype", [(8, 2, 64, BF16), (8, 2, 128, BF16), (4, 2, 80, BF16), (4, 2, 64, F32)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("size", [1.0, 1e-12])
+@pytest.mark.parametrize("where", [0, 20, 33])
+def test_a_value_that_is_none_beside_single_tokens(heads, n_kv, dim, dtype, bad, size, where):
+    """One lane of one value of the own block, in the tail or the token's own: that lane shows it, the others are what they are without it."""
+    b = Batch(1, heads, n_kv, dim, dtype, 500, seed=dim)
+    b.append([(0, 384)], qkv=sized(b, 384, size), rot=0, check=False)
+    own, last = sized(b, 33, size), sized(b, 1, size)
+    rows = own.view(33, -1, dim)[where] if where < 33 else last.view(-1, dim)
+    rows[heads + n_kv, 5] = bad
+    b.append([(0, 33)], qkv=own, rot=0, check=False)
+    step, out, old = b.append([(0, 1)], qkv=last, rot=0, check=False)
+    o = b.attend([(0, 1)], step, out, old, check=False).view(heads, dim)
+    mine = o[: heads // n_kv, 5].clone()
+    assert torch.isnan(mine).all() if bad != bad else (mine == bad).all()
+    # without it: its lane taken out on both sides
+    b.line.rows[0][384 + where, 1, 0, 5] = 0
+    for h in range(heads // n_kv):
+        o[h, 5] = 0
+    b.line.rows[0][:, 1, 0, 5] = 0
+    b.check_attention([(0, 1)], step, out, o.view(1, -1), 0)
+
+
+
+@pytest.mark.parametrize("heads,n_kv,dim,dtype", [(8, 2, 64, BF16), (8, 2, 128, BF16), (4, 2, 80, BF16), (4, 2, 64, F32), (4, 2, 128, F32)])
+@pytest.mark.parametrize("cuts", [(130,), (90, 40), (100, 1, 1, 28)])
+def test_a_key_that_is_none_in_the_own_block(heads, n_kv, dim, dtype, cuts):
+    """A NaN among a key's lanes: every later query of its heads has no result, the others and those before are untouched by it."""
+    outs = []
+    for with_it in (False, True):
+        b = Batch(1, heads, n_kv, dim, dtype, 256, seed=6)
+        qkv, parts, at = b.rows(130), [], 0
+        if with_it:
+            qkv.view(130, -1, dim)[95, heads, 3] = float("nan")
+        for n in cuts:
+            step, out, old = b.append([(0, n)], qkv=qkv[at: at + n].clone(), rot=0, check=False)
+            parts.append(b.attend([(0, n)], step, out, old, check=False))
+            at += n
+        outs.append(torch.cat(parts).view(130, n_kv, heads // n_kv, dim))
+    assert torch.isnan(outs[1][95:, 0]).all()
+    assert torch.equal(outs[1][:95], outs[0][:95]) and torch.equal(outs[1][:, 1], outs[0][:, 1])
