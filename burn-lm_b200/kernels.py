@@ -2081,9 +2081,11 @@ def q8_write(pool, scales, pages, keys, key_scales, values, value_scales) -> Non
     if (page != PAGE or keys.dtype != torch.int8 or values.dtype != torch.int8 or values.shape != keys.shape or pages.numel() != p
             or tuple(key_scales.shape) != (p, n_kv) or tuple(value_scales.shape) != (p, n_kv)):
         raise KernelError(f"q8_write: keys and values int8 [P, kv heads, {PAGE}, head_dim], scales [P, kv heads], a page for each")
-    if bool((key_scales < 0).any()) or bool((value_scales < 0).any()):         # (by a scale below zero the kernels know a page that is none)
+    at = pages.to(device=pool.device, dtype=torch.int64)
+    down, outside = torch.stack([((key_scales < 0) | (value_scales < 0)).any(), ((at < 0) | (at >= pool.shape[0])).any()]).tolist()
+    if down:                                             # (by a scale below zero the kernels know a page that is none)
         raise KernelError("q8_write: scales are not below zero")
-    if p and not 0 <= int(pages.min()) <= int(pages.max()) < pool.shape[0]:
+    if outside:
         raise KernelError(f"q8_write: pages are numbers below {pool.shape[0]}")
     line = torch.full((p, n_kv, pool.shape[2]), -128, dtype=torch.int8, device=pool.device)      # a byte holds the number + 128
     k = (keys ^ -128).reshape(p, n_kv, PAGE // 2, 2, head_dim)
@@ -2092,7 +2094,6 @@ def q8_write(pool, scales, pages, keys, key_scales, values, value_scales) -> Non
         k = torch.stack([k[:, :, :, 0], odd.reshape(p, n_kv, PAGE // 2, head_dim)], dim=3)
     line[:, :, : PAGE * head_dim] = k.reshape(p, n_kv, PAGE * head_dim)
     line[:, :, PAGE * head_dim:][:, :, _q8_value_places(head_dim, pool.device).reshape(-1)] = (values ^ -128).reshape(p, n_kv, PAGE * head_dim)
-    at = pages.to(torch.int64)
     pool[at] = line
     scales[at] = torch.stack([key_scales, value_scales], dim=2).to(torch.float32)
 
@@ -2177,11 +2178,12 @@ def attention_q8(rotated, step, pool, scales, tail, old, block_table, out, n_hea
     own block unrounded, from the step's rows and, before them, from `old` (steps of one token a sequence: from `tail`).  So the result
     depends on the tokens, not on how they were cut into steps.  Scores, softmax and sums are fp32; out [N, n_heads * head_dim] in
     rotated's dtype.  Rows of no sequence are left as they are.  In bfloat16 the probabilities, times the values' scale, are
-    rounded to bfloat16 (single tokens with heads of 64 or 128 lanes: to half precision); float32 steps keep 32 bits.  Values may be as large
-    as 1e28 (sums of probabilities times values are formed before they are divided) and, in bfloat16, as small as 1e-20 before their smaller
-    probabilities lose bits; keys as large as 1e17.  An infinite key of the own block leaves the rows that see it no number, except where its
-    score is minus infinity.  A sequence's pages may be cut over several blocks: step.max_kv_len (the longest sequence after the step, or a
-    bound) sizes that, step.workspace lends the scratch that single tokens need for it."""
+    rounded to bfloat16 (single tokens with heads of 64 or 128 lanes: to half precision where they meet pages, as are queries, whose lanes
+    below 2^-18 of the row's largest lose bits); float32 steps keep 32 bits.  Values may be as large as 1e28 (sums of probabilities times
+    values are formed before they are divided) and, in bfloat16, as small as 1e-20 before their smaller probabilities lose bits; keys as
+    large as 1e17.  An infinite key of the own block leaves the rows that see it no number, except where its score is minus infinity.  A
+    sequence's pages may be cut over several blocks: step.max_kv_len (the longest sequence after the step, or a bound) sizes that,
+    step.workspace lends the scratch that single tokens need for it."""
     shape, dtype = rotated.shape, rotated.dtype
     n = shape[0]
     if len(shape) != 2 or shape[1] != (n_heads + 2 * n_kv) * head_dim or out.shape != (n, n_heads * head_dim) or out.dtype is not dtype:
